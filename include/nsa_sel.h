@@ -1,6 +1,7 @@
 /*
  * nsa_sel.h -- C ABI of the B200 (sm_100a) NSA selected-branch attention forward, with the
- * block selection that produces its index rows and the backward that the reference lacks.
+ * block selection that produces its index rows, and with the backward and the 4-bit KV cache
+ * (writing, reading back, attention of single tokens) that the reference lacks.
  *
  * This is the drop-in boundary for the one hot path of the nsa-hopper reference: the
  * selected-branch forward that its kernels expose through pybind as
@@ -73,6 +74,7 @@ typedef struct CUstream_st* nsa_stream_t;
 
 #define NSA_DTYPE_BF16 0
 #define NSA_DTYPE_F32 1
+#define NSA_DTYPE_F16 2 /* the cache functions only */
 
 #define NSA_KEYMAP_CAUSAL 0     /* key position p is visible to query t iff p <= t */
 #define NSA_KEYMAP_COMPRESSED 1 /* compressed key i is visible iff linspace(0, T-1, kv_len)[i] <= t */
@@ -256,6 +258,98 @@ int64_t nsa_sel_backward_workspace_bytes(const nsa_sel_bwd_desc* desc);
    sub-block) the tokens that attend to it) and the tcgen05 gradient kernel.  The sums are
    accumulated with atomic adds, so the last bits may differ between runs. */
 int nsa_sel_backward(const nsa_sel_bwd_desc* desc, nsa_stream_t stream);
+
+/* ------------------------------------------------------------------ 4-bit paged KV cache
+   The reference has no cache and no form for single tokens.  These functions keep a sequence's keys and
+   values in 4.5 bits a value and attend to them, one token (or a few) of a sequence at a time.
+
+   The cache is num_pages pages of 64 tokens.  Page p of KV head h is a record of nsa_cache_record_bytes(d_qk, d_v)
+   = 36 * (d_qk + d_v) bytes at cache + p * page_stride + h * record bytes:
+       K codes [64][d_qk / 2], K scales [64][d_qk / 16], V codes [64][d_v / 2], V scales [64][d_v / 16].
+   16 neighbouring values along d share a scale byte, 5 exponent bits (bias 15) over 3 mantissa bits, no sign: `byte << 7`
+   is the scale in half precision.  A code has 4 bits, sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6
+   and the same with the sign; the low nibble is the even index.  Writing takes the scale nearest to max|x| / 6 (at most
+   10240) and the codes nearest to x / scale, ties to even, and saturates (beyond 61440).  Groups whose largest |x| is
+   below 2.3e-5 become zeros; a group that holds a NaN or an infinity reads back as NaNs.  A value has at most 6
+   significant bits, so reading back into bf16, fp16 or fp32 is exact.
+
+   (d_qk, d_v) is (64, 64), (128, 128), (192, 128) or (128, 64), as in the forward.
+
+   The batch, the same for all three calls: sequence s has lens[s] tokens (the call's own included), token t of it is at
+   place t % 64 of page pages[s][t / 64].  The call has n_rows rows; row r of sequence s (cu_seqlens[s] <= r <
+   cu_seqlens[s + 1]) is the token at position lens[s] - (cu_seqlens[s + 1] - r), so a sequence's rows are its last tokens;
+   without cu_seqlens row r is the last token of sequence r, and n_rows == n_seqs.  The device arrays are trusted for
+   nothing: a token at a negative position, behind the page table's width or on a page outside [0, num_pages) is absent: it
+   is not written, reads back as zeros and is not attended to.  Two rows that name one place of the cache (two sequences
+   that write to a shared page) leave a mixture of both there. */
+typedef struct nsa_cache_batch {
+  void* cache;                /* see above; 16-byte aligned (only nsa_cache_write changes it) */
+  const int32_t* pages;       /* int32 [n_seqs, width] */
+  const int32_t* lens;        /* int32 [n_seqs] */
+  const int32_t* cu_seqlens;  /* optional int32 [n_seqs + 1] */
+  int64_t page_stride;        /* bytes from one page to the next; 0 = heads_kv records, else a multiple of 16 not below */
+  int64_t pages_stride;       /* entries from one row of `pages` to the next; 0 = width */
+  int32_t num_pages, n_seqs, width, n_rows, heads_kv, d_qk, d_v;
+  int32_t reserved;
+} nsa_cache_batch;
+
+/* Bytes of a record (one page of one KV head), -1 for a (d_qk, d_v) outside the built family. */
+int64_t nsa_cache_record_bytes(int32_t d_qk, int32_t d_v);
+
+/* Quantises the rows' K [n_rows, heads_kv, d_qk] and V [n_rows, heads_kv, d_v] into the cache; in_dtype NSA_DTYPE_BF16 or
+   NSA_DTYPE_F16.  Strides in elements (multiples of 8; d has unit stride), pointers 16-byte aligned.  One launch.  Rows
+   that must not meet: the call does not order itself against calls on other streams. */
+int nsa_cache_write(const nsa_cache_batch* batch, const void* k, const void* v, int64_t k_row_stride, int64_t k_head_stride,
+                    int64_t v_row_stride, int64_t v_head_stride, int32_t in_dtype, nsa_stream_t stream);
+
+/* Reads the rows back: k [heads_kv, n_rows, d_qk], v [heads_kv, n_rows, d_v] (the packed layout of the varlen forward),
+   contiguous, 16-byte aligned, dtype NSA_DTYPE_BF16, _F16 or _F32.  Absent tokens and rows of no sequence read as zeros.
+   One launch. */
+int nsa_cache_read(const nsa_cache_batch* batch, void* k, void* v, int32_t out_dtype, nsa_stream_t stream);
+
+/* Attention of the rows over the cache: row n at position t sees key p iff p <= t, and t - p < window (if window > 0),
+   and p lies in one of the blocks sel[n][kvh] (if sel is given; block_size keys each, a set as in the forward; entries < 0
+   or behind t select nothing).  A row that sees no key gets O = 0 and LSE = -inf.  Zero-initialise, then fill. */
+typedef struct nsa_cache_attend_desc {
+  nsa_cache_batch batch;
+  const void* q;              /* [n_rows, heads_q, d_qk], dtype q_dtype, d has unit stride, 16-byte aligned */
+  const int32_t* sel;         /* optional int32 [n_rows, heads_kv, n_sel] */
+  void* o;                    /* [n_rows, heads_q, d_v], dtype o_dtype, contiguous, 16-byte aligned */
+  float* lse;                 /* optional fp32 [n_rows, heads_q], natural log */
+  const float* o_weight;      /* optional device float w multiplying the result; NULL = 1 */
+  void* workspace;            /* nsa_cache_attend_workspace_bytes() bytes, 16-byte aligned, of this call alone */
+  int64_t q_row_stride;       /* elements, multiples of 8; 0 = heads_q * d_qk */
+  int64_t q_head_stride;      /* 0 = d_qk */
+  int32_t heads_q;            /* a multiple of heads_kv */
+  int32_t n_sel;
+  int32_t block_size;         /* l_prime of sel: 64, 128 or 256 */
+  int32_t window;             /* > 0: sliding window; 0: none */
+  int32_t q_dtype;            /* NSA_DTYPE_BF16 or NSA_DTYPE_F16 */
+  int32_t o_dtype;            /* q_dtype or NSA_DTYPE_F32 */
+  int32_t o_accumulate;       /* 1: O += w * result (fp32 O only) */
+  int32_t keep_rows;          /* 0: rows of no sequence get O = 0, LSE = -inf; 1: they are left as they were */
+  float scale;                /* softmax scale; <= 0 selects 1/sqrt(d_qk) */
+  int32_t reserved[5];
+} nsa_cache_attend_desc;
+
+/* How nsa_cache_attend would run on a device of sm_count SMs (<= 0: the current device). */
+typedef struct nsa_cache_attend_plan_info {
+  int64_t workspace_bytes;
+  int32_t workers;            /* warps that share the call's (row, KV head, page) slots evenly */
+  int32_t slots;              /* slots of every row and KV head; 0 = as many as it has pages */
+  int32_t share;              /* slots of a worker; 0 = worked out on the device */
+  int32_t grid, threads, smem_bytes;
+  int32_t merge;              /* warps that join a cut row's parts; 0 = no row is cut, one launch */
+  int32_t tiles;              /* 16-row tiles of a KV head's query heads */
+} nsa_cache_attend_plan_info;
+int nsa_cache_attend_plan(const nsa_cache_attend_desc* desc, int32_t sm_count, nsa_cache_attend_plan_info* out);
+
+/* Bytes of the workspace on the current device, or -1 if the description is invalid (see nsa_sel_last_error()). */
+int64_t nsa_cache_attend_workspace_bytes(const nsa_cache_attend_desc* desc);
+
+/* Queues the attention (one or two launches).  Results do not depend on timing: the parts of a row are joined in a
+   fixed order. */
+int nsa_cache_attend(const nsa_cache_attend_desc* desc, nsa_stream_t stream);
 
 /* Size in bytes of the static scratch used by nsa_sel_select_noalloc. */
 int64_t nsa_sel_select_static_scratch_bytes(void);

@@ -48,16 +48,23 @@ def _run(cmd: List[str]) -> None:
 
 
 def build_kernel_lib(force: bool = False, extra: List[str] = ()) -> str:
-    # the translation unit first, then every header it may include (staleness check)
-    srcs = [os.path.join(CSRC, "nsa_sel_api.cu")] + sorted(
-        os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh"))
-    srcs.append(os.path.join(INCLUDE, "nsa_sel.h"))
-    if not force and not _stale(LIB, srcs):
+    # one object for each translation unit: rebuilt when it or a header it may include is newer
+    units = {"nsa_sel_api.cu": sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh") and "cache" not in f)
+             + ["nsa_host.h"],
+             "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "nsa_host.h"]}
+    objects = []
+    for unit, headers in units.items():
+        obj = os.path.join(PKG, unit[:-3] + ".o")
+        objects.append(obj)
+        srcs = [os.path.join(CSRC, f) for f in [unit, *headers]] + [os.path.join(INCLUDE, "nsa_sel.h")]
+        if force or extra or _stale(obj, srcs):
+            _run([NVCC, *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", f"-I{INCLUDE}",
+                  f"-I{CSRC}", *extra, "-c", "-o", obj + ".tmp", srcs[0]])
+            os.replace(obj + ".tmp", obj)
+    if not force and not _stale(LIB, objects):
         return LIB
-    cmd = [NVCC, *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
-           "-cudart", "shared", f"-I{INCLUDE}", f"-I{CSRC}", "-Xlinker", f"-rpath={CUDA_HOME}/lib64",
-           *extra, "-o", LIB + ".tmp", srcs[0]]
-    _run(cmd)
+    _run([NVCC, *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-cudart", "shared", "-Xlinker",
+          f"-rpath={CUDA_HOME}/lib64", "-o", LIB + ".tmp", *objects])
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -30,6 +30,7 @@ NSA_DEBUG_NO_ROW_OWNER = 4
 NSA_DEBUG_RO_PAD128 = 8
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_F16 = 2
 KEYMAP_CAUSAL = 0
 KEYMAP_COMPRESSED = 1
 
@@ -94,6 +95,40 @@ class NsaSelBwdDesc(ctypes.Structure):
     ]
 
 
+class NsaCacheBatch(ctypes.Structure):
+    """Mirror of ``nsa_cache_batch``."""
+
+    _fields_ = [
+        ("cache", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64), ("pages_stride", ctypes.c_int64),
+        ("num_pages", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("width", ctypes.c_int32), ("n_rows", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32), ("d_qk", ctypes.c_int32), ("d_v", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class NsaCacheAttendDesc(ctypes.Structure):
+    """Mirror of ``nsa_cache_attend_desc``."""
+
+    _fields_ = [
+        ("batch", NsaCacheBatch), ("q", ctypes.c_void_p), ("sel", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p), ("o_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("heads_q", ctypes.c_int32), ("n_sel", ctypes.c_int32), ("block_size", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("q_dtype", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("o_accumulate", ctypes.c_int32),
+        ("keep_rows", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32 * 5),
+    ]
+
+
+class NsaCacheAttendPlanInfo(ctypes.Structure):
+    """Mirror of ``nsa_cache_attend_plan_info``."""
+
+    _fields_ = [
+        ("workspace_bytes", ctypes.c_int64), ("workers", ctypes.c_int32), ("slots", ctypes.c_int32),
+        ("share", ctypes.c_int32), ("grid", ctypes.c_int32), ("threads", ctypes.c_int32), ("smem_bytes", ctypes.c_int32),
+        ("merge", ctypes.c_int32), ("tiles", ctypes.c_int32),
+    ]
+
+
 class NsaSelError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"nsa_sel error {code}: {message}")
@@ -142,6 +177,20 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
     lib.nsa_sel_backward.restype = ctypes.c_int
     lib.nsa_sel_select_status.argtypes = []
     lib.nsa_sel_select_status.restype = ctypes.c_int32
+    if hasattr(lib, "nsa_cache_attend"):  # absent from builds that predate it
+        batch, i64 = ctypes.POINTER(NsaCacheBatch), ctypes.c_int64
+        lib.nsa_cache_record_bytes.argtypes = [i32, i32]
+        lib.nsa_cache_record_bytes.restype = i64
+        lib.nsa_cache_write.argtypes = [batch, vp, vp] + [i64] * 4 + [i32, vp]
+        lib.nsa_cache_write.restype = ctypes.c_int
+        lib.nsa_cache_read.argtypes = [batch, vp, vp, i32, vp]
+        lib.nsa_cache_read.restype = ctypes.c_int
+        lib.nsa_cache_attend.argtypes = [ctypes.POINTER(NsaCacheAttendDesc), vp]
+        lib.nsa_cache_attend.restype = ctypes.c_int
+        lib.nsa_cache_attend_workspace_bytes.argtypes = [ctypes.POINTER(NsaCacheAttendDesc)]
+        lib.nsa_cache_attend_workspace_bytes.restype = i64
+        lib.nsa_cache_attend_plan.argtypes = [ctypes.POINTER(NsaCacheAttendDesc), i32, ctypes.POINTER(NsaCacheAttendPlanInfo)]
+        lib.nsa_cache_attend_plan.restype = ctypes.c_int
     if path is None:
         _lib = lib
     return lib
@@ -243,3 +292,54 @@ def backward_workspace_bytes(desc: NsaSelBwdDesc) -> int:
 def backward(desc: NsaSelBwdDesc, stream: int = 0) -> None:
     """nsa_sel_backward: adds dQ, dK, dV of the selected branch (see include/nsa_sel.h)."""
     check(load().nsa_sel_backward(ctypes.byref(desc), ctypes.c_void_p(stream)))
+
+
+# ------------------------------------------------------------------ the 4-bit paged KV cache
+def _filled(obj, **kw):
+    for key, val in kw.items():
+        if not hasattr(obj, key):
+            raise KeyError(key)
+        setattr(obj, key, val)
+    return obj
+
+
+def make_cache_batch(**kw) -> NsaCacheBatch:
+    return _filled(NsaCacheBatch(), **kw)
+
+
+def make_cache_attend_desc(**kw) -> NsaCacheAttendDesc:
+    return _filled(NsaCacheAttendDesc(), **kw)
+
+
+def cache_record_bytes(d_qk: int, d_v: int) -> int:
+    """nsa_cache_record_bytes: bytes of one page of one KV head, -1 for dims outside the built family."""
+    return int(load().nsa_cache_record_bytes(d_qk, d_v))
+
+
+def cache_write(batch: NsaCacheBatch, k: int, v: int, k_strides, v_strides, in_dtype: int, stream: int = 0) -> None:
+    """nsa_cache_write; strides are (row, head) in elements."""
+    check(load().nsa_cache_write(ctypes.byref(batch), ctypes.c_void_p(k), ctypes.c_void_p(v), *k_strides, *v_strides,
+                                 in_dtype, ctypes.c_void_p(stream)))
+
+
+def cache_read(batch: NsaCacheBatch, k: int, v: int, out_dtype: int, stream: int = 0) -> None:
+    check(load().nsa_cache_read(ctypes.byref(batch), ctypes.c_void_p(k), ctypes.c_void_p(v), out_dtype,
+                                ctypes.c_void_p(stream)))
+
+
+def cache_attend_plan(desc: NsaCacheAttendDesc, sm_count: int = 148) -> Dict[str, int]:
+    info = NsaCacheAttendPlanInfo()
+    check(load().nsa_cache_attend_plan(ctypes.byref(desc), sm_count, ctypes.byref(info)))
+    return {name: getattr(info, name) for name, _ in NsaCacheAttendPlanInfo._fields_}
+
+
+def cache_attend_workspace_bytes(desc: NsaCacheAttendDesc) -> int:
+    """nsa_cache_attend_workspace_bytes (raises on an invalid description)."""
+    n = int(load().nsa_cache_attend_workspace_bytes(ctypes.byref(desc)))
+    if n < 0:
+        raise NsaSelError(NSA_ERR_INVALID_ARG, last_error())
+    return n
+
+
+def cache_attend(desc: NsaCacheAttendDesc, stream: int = 0) -> None:
+    check(load().nsa_cache_attend(ctypes.byref(desc), ctypes.c_void_p(stream)))

@@ -1,0 +1,99 @@
+// Where things are in the 4-bit paged KV cache: the record's layout, a row's sequence and position, a
+// token's page, and the share of one worker of the attention kernel.  Every index that the cache kernels
+// take from the caller's device tensors (page table, lengths, cu_seqlens, selection) is turned into an
+// address here and nowhere else, and each is checked against its range first: the host cannot see those
+// values, so a value out of range makes the token absent, never an access out of bounds.  Plain C++ on
+// purpose: the CPU tests compile this header and feed it broken tables.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define NSA_HD __host__ __device__ __forceinline__
+#else
+#define NSA_HD inline
+#endif
+
+namespace nsa {
+namespace cache {
+
+constexpr int kPage = 64;   // tokens of a page
+constexpr int kGroup = 16;  // neighbouring values that share a scale
+
+// A record (one page of one KV head): K codes, K scales, V codes, V scales, token after token.
+NSA_HD constexpr int record_bytes(int d_qk, int d_v) { return kPage * (d_qk + d_v) * 9 / 16; }
+NSA_HD constexpr int k_scale_at(int d_qk) { return kPage * d_qk / 2; }
+NSA_HD constexpr int v_code_at(int d_qk) { return kPage * d_qk * 9 / 16; }
+NSA_HD constexpr int v_scale_at(int d_qk, int d_v) { return v_code_at(d_qk) + kPage * d_v / 2; }
+
+// The batch that all three calls describe: page table [n_seqs, width], lengths, packed rows.
+struct Batch {
+  const int32_t* pages;
+  const int32_t* lens;
+  const int32_t* cu;      // nullptr: row r is the last token of sequence r
+  int64_t page_row;       // entries between two sequences' rows of `pages`
+  int32_t n_seqs, width;  // width: pages a sequence can have
+  int32_t num_pages;      // pages of the cache
+  int32_t n_rows;
+};
+
+// The sequence of a row, -1 for a row of none (before cu[0], behind cu[n_seqs], or in a cu_seqlens that
+// is not in order).
+NSA_HD int sequence_of(const Batch& b, int row) {
+  if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
+  if (b.n_seqs <= 0 || row < b.cu[0]) return -1;
+  int lo = 0, hi = b.n_seqs;  // the last s with cu[s] <= row is in [lo, hi)
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (b.cu[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  return row < b.cu[lo + 1] ? lo : -1;
+}
+
+// Position of a row in its sequence (from sequence_of, >= 0): the sequence's last rows are the call's.
+// Negative where the sequence has no such token.
+NSA_HD int position_of(const Batch& b, int seq, int row) {
+  const int len = b.lens[seq] > 0 ? b.lens[seq] : 0;
+  const int behind = b.cu == nullptr ? 1 : b.cu[seq + 1] - row;  // >= 1
+  return len - behind;
+}
+
+// Keys of a sequence that a row at `pos` may see at most: those up to itself that the page table can hold.
+NSA_HD int keys_up_to(const Batch& b, int pos) {
+  if (pos < 0) return 0;
+  const int64_t held = (int64_t)b.width * kPage;
+  return pos < held ? pos + 1 : (int)held;
+}
+
+// The cache page of 64-key sub-block `sub` of a sequence, -1 where there is none.
+NSA_HD int page_of(const Batch& b, int seq, int sub) {
+  if (sub < 0 || sub >= b.width) return -1;
+  const int p = b.pages[(int64_t)seq * b.page_row + sub];
+  return p >= 0 && p < b.num_pages ? p : -1;
+}
+
+// First and one-past-last visible key of a row (window <= 0: no window).
+NSA_HD int first_key(int pos, int window) { return window > 0 && pos + 1 > window ? pos + 1 - window : 0; }
+
+// The sub-block that slot j of a row stands for, -1 if it shows no key: entry j / per of the row's
+// selection (per = l' / 64), or the j-th sub-block from the window's first.
+NSA_HD int selected_sub(int entry, int part, int per, int first, int end) {
+  if (entry < 0 || end <= 0 || entry > (end - 1) / (per * kPage)) return -1;  // (before the product can overflow)
+  const int sub = entry * per + part;
+  return sub * kPage < end && (sub + 1) * kPage > first ? sub : -1;
+}
+NSA_HD int running_sub(int j, int first, int end) {
+  const int sub = first / kPage + j;
+  return end > first && sub * (int64_t)kPage < end ? sub : -1;
+}
+// Slots of a row that takes its sub-blocks one after the other; at least one, so that every row has an owner.
+NSA_HD int running_slots(int first, int end) { return end > first ? (end - 1) / kPage - first / kPage + 1 : 1; }
+
+// All slots of a call in one line are shared out evenly: worker w has [w * per, (w + 1) * per).
+NSA_HD uint32_t share(uint32_t total, uint32_t workers) {
+  const uint32_t per = (total + workers - 1) / workers;
+  return per > 0 ? per : 1;
+}
+
+}  // namespace cache
+}  // namespace nsa

@@ -19,6 +19,7 @@
 #include <string.h>
 
 #include "nsa_sel.h"
+#include "nsa_host.h"
 #include "nsa_sel_kernel.cuh"
 #include "nsa_ro_kernel.cuh"
 #include "nsa_select_kernel.cuh"
@@ -960,6 +961,23 @@ int backward(const nsa_sel_bwd_desc* d, nsa_stream_t stream) {
 }
 
 }  // namespace
+
+// What the other translation units of the library use of the above (nsa_host.h).
+namespace nsa {
+namespace host {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int current_sm_count(int* sm_count, int* device) { return ::current_sm_count(sm_count, device); }
+
+}  // namespace host
+}  // namespace nsa
 
 extern "C" {
 

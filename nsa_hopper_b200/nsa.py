@@ -242,6 +242,44 @@ def nsa_forward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, *, n_sel: int
     return O, sel
 
 
+def cache_compress(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: torch.Tensor, cmp_cache: torch.Tensor,
+                   cmp_pages: torch.Tensor, cmp_block: int = 32, cmp_stride: int = 16) -> torch.Tensor:
+    """One decode step of :func:`compress_kv` on 4-bit caches: where a sequence's newest token completes a
+    compressed key (``lens[s]`` = cmp_block + i * cmp_stride), the mean of its last ``cmp_block`` keys and
+    values, read back from ``cache``, is written to place i of ``cmp_cache``.  Returns the number of
+    compressed keys of each sequence, int32 [S].  Nothing is read on the host."""
+    from . import ops
+
+    S = lens.shape[0]
+    count = torch.where(lens >= cmp_block, (lens - cmp_block) // cmp_stride + 1, torch.zeros_like(lens))
+    complete = (lens >= cmp_block) & ((lens - cmp_block) % cmp_stride == 0)
+    cu = torch.arange(S + 1, device=lens.device, dtype=torch.int32) * cmp_block
+    K, V = ops.cache_read(cache, d_qk, pages, lens, cu, S * cmp_block, torch.float32)
+    Kc, Vc = (x[0].unflatten(1, (S, cmp_block)).mean(2).transpose(0, 1).to(torch.bfloat16) for x in (K, V))
+    ops.cache_write(cmp_cache, Kc.contiguous(), Vc.contiguous(), cmp_pages, torch.where(complete, count, torch.zeros_like(count)))
+    return count
+
+
+def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, sel: torch.Tensor, *,
+               l_prime: int = 64, window: int = 512, cmp_cache: Optional[torch.Tensor] = None,
+               cmp_pages: Optional[torch.Tensor] = None, cmp_lens: Optional[torch.Tensor] = None,
+               gate_w: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The three NSA branches and the gate of :func:`nsa_forward` for the newest token of every sequence of a
+    4-bit cache (``ops.cache_write`` has put its K and V there): Q [S, Hq, d_qk] bf16 or fp16, sel int32
+    [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  The compressed branch sees
+    every key of ``cmp_cache`` (kept by :func:`cache_compress`), as the newest token does in the forward;
+    without one it is left out.  Each branch adds its gated result into O."""
+    from . import ops
+
+    g = gate_weights(gate_w, Q.device)
+    O = torch.empty(Q.shape[0], Q.shape[1], cache.shape[2] // 36 - Q.shape[2], dtype=torch.float32, device=Q.device)
+    ops.cache_attend(Q, cache, pages, lens, sel=sel, l_prime=l_prime, out=O, weight=g[1:2], with_lse=False)
+    if cmp_cache is not None:
+        ops.cache_attend(Q, cmp_cache, cmp_pages, cmp_lens, out=O, weight=g[0:1], accumulate=True, with_lse=False)
+    ops.cache_attend(Q, cache, pages, lens, window=window, out=O, weight=g[2:3], accumulate=True, with_lse=False)
+    return O
+
+
 def validate_fn(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, sel: torch.Tensor, cfg: Dict) -> torch.Tensor:
     """The ``fn(Q, K, V, sel, cfg)`` that ``validate.check(fn, dtype)`` calls (validate.py:21)."""
     o, _ = nsa_forward(Q, K, V, n_sel=cfg["n_sel"], l_prime=cfg["l_prime"], window=cfg["window"], sel_override=sel)

@@ -110,5 +110,65 @@ class SelectedAttention(torch.autograd.Function):
         return dq.to(Q.dtype), dk.to(K.dtype), dv.to(V.dtype), None, None
 
 
+PAGE = 64  # tokens of a page of the 4-bit cache
+
+
+def cache_alloc(num_pages: int, heads_kv: int, d_qk: int, d_v: int, device="cuda") -> torch.Tensor:
+    """A 4-bit paged KV cache of zeros: uint8 [num_pages, heads_kv, 36 * (d_qk + d_v)], a page holding
+    64 tokens (4.5 bits a value; the layout of a record is described in include/nsa_sel.h)."""
+    return torch.zeros(num_pages, heads_kv, _C.cache_record_bytes(int(d_qk), int(d_v)), dtype=torch.uint8, device=device)
+
+
+def cache_write(cache: torch.Tensor, K: torch.Tensor, V: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
+                cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    """Quantises the newest tokens of a batch of sequences into the 4-bit cache (nsa_cache_write).
+
+    ``pages`` int32 [S, W] is the page table, ``lens`` int32 [S] the sequences' tokens, the new ones
+    included.  K [N, Hkv, d_qk] and V [N, Hkv, d_v] (bf16 or fp16, any row and head strides that are
+    multiples of 8) hold the rows: row r of sequence s, ``cu_seqlens[s] <= r < cu_seqlens[s + 1]``, is
+    its token ``lens[s] - (cu_seqlens[s + 1] - r)``; without ``cu_seqlens`` row s is the last token of
+    sequence s.  A prefill of one sequence in the forward's layout [1, Hkv, T, d] is
+    ``K[0].transpose(0, 1)`` with ``cu_seqlens = [0, T]``.  Tokens that the page table does not hold
+    (a page < 0, a position < 0 or behind the table) are not written, rows of no sequence neither."""
+    _C.cache_write(cache, K, V, pages, lens, cu_seqlens)
+
+
+def cache_read(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: torch.Tensor,
+               cu_seqlens: Optional[torch.Tensor] = None, n_tokens: Optional[int] = None,
+               dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Reads the batch's newest tokens back from the 4-bit cache (nsa_cache_read): K [1, Hkv, N, d_qk] and
+    V [1, Hkv, N, d_v], packed as ``forward_lse`` takes a varlen batch with the same ``cu_seqlens``.
+    ``n_tokens`` = N is needed with ``cu_seqlens`` (whose last entry the host cannot see); a whole
+    sequence is read where it has ``lens[s]`` rows.  The values are exact in every dtype; tokens that
+    the page table does not hold, and rows of no sequence, are zeros."""
+    if n_tokens is None:
+        if cu_seqlens is not None:
+            raise ValueError("n_tokens (the rows that cu_seqlens packs) is needed with cu_seqlens")
+        n_tokens = lens.shape[0]
+    k, v = _C.cache_read(cache, int(d_qk), pages, lens, cu_seqlens, int(n_tokens), dtype)
+    return k, v
+
+
+def cache_attend(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
+                 sel: Optional[torch.Tensor] = None, l_prime: int = 64, window: int = 0,
+                 cu_seqlens: Optional[torch.Tensor] = None, scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                 weight: Optional[torch.Tensor] = None, accumulate: bool = False,
+                 with_lse: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of the batch's newest tokens over the 4-bit cache (nsa_cache_attend): the decode step.
+
+    Q [N, Hq, d_qk] (bf16 or fp16) has the rows of :func:`cache_write`; the row at position t sees
+    the keys p <= t, with ``window`` > 0 those with t - p < window, and with ``sel`` int32
+    [N, Hkv, KSEL] those in its selected blocks of ``l_prime`` keys (a set; entries < 0 or behind t
+    select nothing).  Returns (O [N, Hq, d_v] of Q's dtype, LSE fp32 [N, Hq], natural log); a row that
+    sees no key, or of no sequence, has O = 0 and LSE = -inf.
+
+    ``out``, ``weight``, ``accumulate``: as in :func:`forward_ext`, the result times ``weight[0]`` is
+    written to ``out`` (fp32 or Q's dtype) or added into it (fp32); rows of no sequence are then left
+    as they were.  ``with_lse=False`` skips the LSE (an empty tensor is returned).  No gradients."""
+    o, lse = _C.cache_attend(Q, cache, pages, lens, sel, int(l_prime), int(window), cu_seqlens, float(scale), out, weight,
+                             bool(accumulate), bool(with_lse))
+    return o, lse
+
+
 def library_version() -> int:
     return int(_C.library_version())

@@ -1,0 +1,266 @@
+"""The 4-bit paged KV cache without a GPU: the index arithmetic that the kernels share (compiled for the
+host and fed broken tables), the plan, the checks of arguments, the number format."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from nsa_hopper_b200 import capi, ops
+from oracle import cache as oc
+
+CSRC = os.path.join(capi.PKG_DIR, "csrc")
+
+SHIM = r"""
+#include "nsa_cache_index.h"
+using namespace nsa::cache;
+extern "C" {
+static Batch make(const int32_t* pages, const int32_t* lens, const int32_t* cu, int n_seqs, int width, int num_pages, int n_rows) {
+  return {pages, lens, cu, width, n_seqs, width, num_pages, n_rows};
+}
+void locate(const int32_t* pages, const int32_t* lens, const int32_t* cu, int n_seqs, int width, int num_pages, int n_rows,
+            int32_t* out) {
+  const Batch b = make(pages, lens, cu, n_seqs, width, num_pages, n_rows);
+  for (int r = 0; r < n_rows; ++r) {
+    const int seq = sequence_of(b, r), pos = seq < 0 ? -1 : position_of(b, seq, r);
+    out[4 * r] = seq, out[4 * r + 1] = pos;
+    out[4 * r + 2] = pos < 0 ? -1 : page_of(b, seq, pos / kPage);
+    out[4 * r + 3] = keys_up_to(b, pos);
+  }
+}
+int selected(int entry, int part, int per, int first, int end) { return selected_sub(entry, part, per, first, end); }
+int running(int j, int first, int end) { return running_sub(j, first, end); }
+int slots(int first, int end) { return running_slots(first, end); }
+int first(int pos, int window) { return first_key(pos, window); }
+unsigned int sharing(unsigned int total, unsigned int workers) { return share(total, workers); }
+int record(int dqk, int dv) { return record_bytes(dqk, dv); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def index(tmp_path_factory):
+    d = tmp_path_factory.mktemp("index")
+    (d / "shim.cpp").write_text(SHIM)
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                    f"-I{CSRC}", "-o", str(d / "shim.so"), str(d / "shim.cpp")], check=True)
+    return ctypes.CDLL(str(d / "shim.so"))
+
+
+def _locate(lib, pages, lens, cu, num_pages, n_rows):
+    out = np.zeros((n_rows, 4), np.int32)
+    ptr = lambda a: None if a is None else a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    lib.locate(ptr(pages), ptr(lens), ptr(cu), len(lens), pages.shape[1], num_pages, n_rows, ptr(out))
+    return out
+
+
+BIG = 2**31 - 1
+
+
+@pytest.mark.parametrize("cu", [
+    None,
+    [0, 1, 1, 4, 9],                 # an empty sequence, rows behind the last
+    [0, 0, 0, 0, 0],                 # no rows at all
+    [2, 3, 5, 6, 11],                # rows before the first
+    [0, 7, 3, 5, 12],                # not in order
+    [0, BIG, BIG, BIG, BIG],         # behind every row
+    [-5, -3, 0, 2, 3],               # negative
+    [12, 9, 5, 2, 0],                # backwards
+])
+@pytest.mark.parametrize("lens", [[0, 1, 64, 130], [-7, 63, 65, BIG], [256, 257, 10**9, 128]])
+def test_rows_land_inside_the_cache_or_nowhere(index, cu, lens):
+    width, num_pages, n_rows = 4, 6, 4 if cu is None else 12
+    pages = np.array([[0, 5, 6, -1], [3, -2**31, BIG, 2], [1, 4, 0, 2], [5, 5, -1, 7]], np.int32)
+    lens, cu = np.array(lens, np.int32), None if cu is None else np.array(cu, np.int32)
+    got = _locate(index, pages, lens, cu, num_pages, n_rows)
+    for r, (seq, pos, page, keys) in enumerate(got.tolist()):
+        assert -1 <= seq < 4 and -1 <= page < num_pages and 0 <= keys <= width * 64
+        if seq >= 0:
+            assert cu is None or cu[seq] <= r < cu[seq + 1]
+            assert page == (-1 if pos < 0 or pos >= width * 64 or not 0 <= pages[seq, pos // 64] < num_pages
+                            else pages[seq, pos // 64])
+            assert keys == min(max(pos + 1, 0), width * 64)
+        if cu is None or (np.diff(cu) >= 0).all():
+            assert (seq, pos if seq >= 0 else -1, page) == oc.place(r, pages, lens, cu, num_pages)
+
+
+def test_sub_blocks(index):
+    # selection: nothing behind the visible keys or before the window, no overflow for any entry
+    for entry in (-2**31, -1, 0, 1, 2, 3, 7, 2**24, BIG):
+        for per in (1, 2, 4):
+            for part in range(per):
+                for first, end in ((0, 0), (0, 1), (0, 64), (0, 65), (100, 300), (255, 256), (0, BIG // 64 * 64)):
+                    sub = index.selected(entry, part, per, first, end)
+                    want = entry * per + part
+                    ok = entry >= 0 and want * 64 < end and (want + 1) * 64 > first
+                    assert sub == (want if ok else -1), (entry, per, part, first, end)
+    for first, end in ((0, 0), (0, 1), (63, 64), (63, 65), (64, 65), (100, 300), (0, 640)):
+        n = index.slots(first, end)
+        subs = [index.running(j, first, end) for j in range(n + 2)]
+        want = [s for s in range(11) if s * 64 < end and (s + 1) * 64 > first] if end > first else []
+        assert n == max(1, len(want)) and subs == want + [-1] * (n + 2 - len(want))
+    assert [index.first(p, w) for p, w in ((5, 0), (5, 1), (5, 6), (5, 7), (5, BIG), (BIG - 1, 3))] == [0, 5, 0, 0, 0, BIG - 3]
+
+
+@pytest.mark.parametrize("total,workers", [(1, 1), (5, 3), (64, 1184), (1185, 1184), (2**31 - 1, 1184), (2**31 - 1, 2368)])
+def test_shares_cover_the_line(index, total, workers):
+    per = index.sharing(total, workers)
+    assert per >= 1 and per * workers >= total and (per - 1) * workers < max(total, workers)
+
+
+def test_record_bytes():
+    for dqk, dv, want in ((64, 64, 4608), (128, 128, 9216), (192, 128, 11520), (128, 64, 6912)):
+        assert capi.cache_record_bytes(dqk, dv) == want
+    assert capi.cache_record_bytes(96, 96) == -1
+    assert capi.cache_record_bytes(64, 128) == -1
+
+
+# ------------------------------------------------------------------ number format
+def test_format_by_definition():
+    s = oc._SCALES
+    assert s[0] == 0 and s[1] == 2.0**-17 and s[8] == 2.0**-14 and s[-1] == 10240 and (np.diff(s) > 0).all()
+    assert (s.astype(np.float16) == s).all() and ((6 * s).astype(np.float16) == 6 * s).all()
+    every = (oc.LEVELS[:, None] * s).astype(np.float32)
+    assert (torch.from_numpy(every).to(torch.bfloat16).float().numpy() == every).all()
+    assert (every.astype(np.float16).astype(np.float32) == every).all()
+    x = np.zeros((1, 16))
+    x[0, :9] = [6, 0.25, 0.75, 1.25, -1.75, 2.5, 3.5, 5, -0.2]  # scale 1; ties go to the even code
+    code, byte = oc.quantise(x)
+    assert oc.scale_value(byte)[0, 0] == 1
+    assert (oc.values(code, byte)[0, :9] == [6, 0, 1, 1, -2, 2, 4, 4, 0]).all()
+    x[0, 3] = np.nan
+    assert np.isnan(oc.values(*oc.quantise(x))).all()
+    assert (oc.values(*oc.quantise(np.full((1, 16), 1e30))) == 61440).all()
+
+
+# ------------------------------------------------------------------ plan and refusals of the C ABI
+def _batch(**kw):
+    base = dict(cache=256, pages=256, lens=256, num_pages=1000, n_seqs=8, width=64, n_rows=8, heads_kv=4, d_qk=128, d_v=128)
+    base.update(kw)
+    return capi.make_cache_batch(**base)
+
+
+def _attend(batch=None, **kw):
+    base = dict(q=256, o=256, heads_q=64, q_dtype=capi.DTYPE_BF16, o_dtype=capi.DTYPE_BF16)
+    base.update(kw)
+    return capi.make_cache_attend_desc(batch=_batch(**(batch or {})), **base)
+
+
+def test_plan_shares_out_the_work():
+    p = capi.cache_attend_plan(_attend(sel=256, n_sel=16, block_size=64))     # 8 x 4 x 16 slots, a worker each
+    assert p["slots"] == 16 and p["share"] == 1 and p["workers"] == 512 and p["grid"] == 148 and p["merge"] == 1
+    assert p["smem_bytes"] <= 232448
+    p = capi.cache_attend_plan(_attend())                                      # every key: the ragged line
+    assert p["slots"] == 0 and p["share"] == 0 and p["merge"] >= 1
+    p = capi.cache_attend_plan(_attend(dict(n_rows=4096, n_seqs=4096)))        # many rows: whole ones
+    assert p["slots"] == 64 and p["share"] % 64 == 0 and p["merge"] == 0
+    p = capi.cache_attend_plan(_attend(window=1))
+    assert p["slots"] == 1
+    p = capi.cache_attend_plan(_attend(window=66, heads_q=4 * 17))
+    assert p["slots"] == 3 and p["tiles"] == 2
+    p = capi.cache_attend_plan(_attend(dict(n_rows=1, n_seqs=1, width=2048)))
+    assert p["merge"] == 8                                                     # one row over hundreds of workers
+    for d in ((64, 64), (192, 128), (128, 64)):
+        assert capi.cache_attend_plan(_attend(dict(d_qk=d[0], d_v=d[1])))["smem_bytes"] <= 232448
+    p = capi.cache_attend_plan(_attend(dict(n_rows=0, n_seqs=0)))
+    assert p["workers"] == 0 and p["workspace_bytes"] == 16
+
+
+BAD = [
+    (dict(d_qk=96), {}, capi.NSA_ERR_UNSUPPORTED),
+    (dict(heads_kv=0), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(n_rows=7), {}, capi.NSA_ERR_INVALID_ARG),               # no cu_seqlens: one row a sequence
+    (dict(cache=0), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(cache=264), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(pages=0), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(lens=258), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(page_stride=4 * 9216 - 16), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(page_stride=4 * 9216 + 8), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(pages_stride=63), {}, capi.NSA_ERR_INVALID_ARG),
+    (dict(n_rows=2**28, n_seqs=2**28), {}, capi.NSA_ERR_UNSUPPORTED),
+]
+BAD_ATTEND = BAD + [
+    ({}, dict(heads_q=63), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(q=0), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(q=264), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(q_row_stride=12), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(o=0), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(q_dtype=capi.DTYPE_F32), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(o_dtype=capi.DTYPE_F16), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(o_accumulate=1), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(window=-1), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(sel=256, n_sel=0, block_size=64), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(sel=256, n_sel=16, block_size=96), capi.NSA_ERR_UNSUPPORTED),
+    ({}, dict(sel=256, n_sel=1025, block_size=64), capi.NSA_ERR_UNSUPPORTED),
+    (dict(n_rows=2**20, n_seqs=2**20, width=2**10), {}, capi.NSA_ERR_UNSUPPORTED),  # 2^32 slots
+]
+
+
+@pytest.mark.parametrize("batch,kw,code", BAD_ATTEND)
+def test_attend_refusals(batch, kw, code):
+    with pytest.raises(capi.NsaSelError) as e:
+        capi.cache_attend_plan(_attend(batch, **kw))
+    assert e.value.code == code and capi.last_error() != ""
+    assert capi.load().nsa_cache_attend(ctypes.byref(_attend(batch, **kw)), None) == code
+
+
+@pytest.mark.parametrize("batch,kw,code", BAD + [
+    ({}, dict(k=0), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(v=264), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(strides=(512, 128, 513, 128)), capi.NSA_ERR_INVALID_ARG),
+    ({}, dict(dtype=capi.DTYPE_F32), capi.NSA_ERR_INVALID_ARG),
+])
+def test_write_and_read_refusals(batch, kw, code):
+    a = dict(k=256, v=256, strides=(512, 128, 512, 128), dtype=capi.DTYPE_BF16)
+    a.update(kw)
+    b = _batch(**batch)
+    lib = capi.load()
+    ptr = ctypes.c_void_p
+    assert lib.nsa_cache_write(ctypes.byref(b), ptr(a["k"]), ptr(a["v"]), *a["strides"], a["dtype"], None) == code
+    if "strides" not in kw and "dtype" not in kw:
+        assert lib.nsa_cache_read(ctypes.byref(b), ptr(a["k"]), ptr(a["v"]), a["dtype"], None) == code
+    assert lib.nsa_cache_read(ctypes.byref(_batch()), ptr(256), ptr(256), 7, None) == capi.NSA_ERR_INVALID_ARG
+
+
+def test_struct_layout_matches_header(tmp_path):
+    mirrors = {"nsa_cache_batch": capi.NsaCacheBatch, "nsa_cache_attend_desc": capi.NsaCacheAttendDesc,
+               "nsa_cache_attend_plan_info": capi.NsaCacheAttendPlanInfo}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{capi.HEADER_PATH}"', "int main(void) {"]
+    want = []
+    for name, cls in mirrors.items():
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append(ctypes.sizeof(cls))
+        for f, _ in cls._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({name}, {f}));')
+            want.append(getattr(cls, f).offset)
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-o", str(tmp_path / "layout"), str(src)], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
+    assert [int(x) for x in out.split()] == want
+
+
+# ------------------------------------------------------------------ the torch ops refuse before any device call
+def test_torch_ops_refuse_host_tensors():
+    cache = ops.cache_alloc(4, 2, 128, 128, device="cpu")
+    assert cache.shape == (4, 2, 9216) and cache.dtype == torch.uint8
+    pages, lens = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    k = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="cache must be a CUDA tensor"):
+        ops.cache_write(cache, k, k, pages, lens)
+    with pytest.raises(RuntimeError, match="cache must be a CUDA tensor"):
+        ops.cache_read(cache, 128, pages, lens)
+    with pytest.raises(RuntimeError, match="cache must be a CUDA tensor"):
+        ops.cache_attend(torch.zeros(3, 8, 128, dtype=torch.bfloat16), cache, pages, lens)
+    with pytest.raises(RuntimeError, match="must be bfloat16 or float16"):
+        ops.cache_write(cache, k.float(), k.float(), pages, lens)
+    with pytest.raises(RuntimeError, match="one dtype"):
+        ops.cache_write(cache, k, k.half(), pages, lens)
+    with pytest.raises(RuntimeError, match="dtype must be"):
+        ops.cache_read(cache, 128, pages, lens, dtype=torch.float64)
+    with pytest.raises(ValueError, match="n_tokens"):
+        ops.cache_read(cache, 128, pages, lens, cu_seqlens=lens)
+    with pytest.raises(RuntimeError, match="not one of"):
+        ops.cache_alloc(4, 2, 96, 96, device="cpu")
