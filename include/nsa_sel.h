@@ -318,6 +318,8 @@ typedef struct nsa_cache_attend_desc {
   float* lse;                 /* optional fp32 [n_rows, heads_q], natural log */
   const float* o_weight;      /* optional device float w multiplying the result; NULL = 1 */
   void* workspace;            /* nsa_cache_attend_workspace_bytes() bytes, 16-byte aligned, of this call alone */
+  int32_t* err;               /* optional device int32; NSA_DEVERR_* bits are ORed into it (after a wait that ran out the
+                                 rows it concerns are NaN) */
   int64_t q_row_stride;       /* elements, multiples of 8; 0 = heads_q * d_qk */
   int64_t q_head_stride;      /* 0 = d_qk */
   int32_t heads_q;            /* a multiple of heads_kv */
@@ -329,17 +331,20 @@ typedef struct nsa_cache_attend_desc {
   int32_t o_accumulate;       /* 1: O += w * result (fp32 O only) */
   int32_t keep_rows;          /* 0: rows of no sequence get O = 0, LSE = -inf; 1: they are left as they were */
   float scale;                /* softmax scale; <= 0 selects 1/sqrt(d_qk) */
+  int32_t timeout_ms;         /* bound on every in-kernel wait; 0 = default (2000 ms) */
+  int32_t debug_flags;        /* NSA_DEBUG_STALL: nothing is copied, so that the waits run out; 0 in normal use */
   int32_t reserved[5];
 } nsa_cache_attend_desc;
 
 /* How nsa_cache_attend would run on a device of sm_count SMs (<= 0: the current device). */
 typedef struct nsa_cache_attend_plan_info {
   int64_t workspace_bytes;
-  int32_t workers;            /* warps that share the call's (row, KV head, page) slots evenly */
-  int32_t slots;              /* slots of every row and KV head; 0 = as many as it has pages */
-  int32_t share;              /* slots of a worker; 0 = worked out on the device */
+  int32_t slots;              /* (row, KV head) x page slots of a row; 0 = as many as it has pages, and then the next two are
+                                 worked out on the device (0) */
+  int32_t team;               /* warps that take turns at a row's slots */
+  int32_t share;              /* whole rows of a team, or its slots where rows are cut (merge != 0) */
   int32_t grid, threads, smem_bytes;
-  int32_t merge;              /* warps that join a cut row's parts; 0 = no row is cut, one launch */
+  int32_t merge;              /* warps that join the parts of a cut row's head; 0 = no row is cut, one launch */
   int32_t tiles;              /* 16-row tiles of a KV head's query heads */
 } nsa_cache_attend_plan_info;
 int nsa_cache_attend_plan(const nsa_cache_attend_desc* desc, int32_t sm_count, nsa_cache_attend_plan_info* out);

@@ -51,7 +51,7 @@ def build_kernel_lib(force: bool = False, extra: List[str] = ()) -> str:
     # one object for each translation unit: rebuilt when it or a header it may include is newer
     units = {"nsa_sel_api.cu": sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh") and "cache" not in f)
              + ["nsa_host.h"],
-             "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "nsa_host.h"]}
+             "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "ptx.cuh", "nsa_host.h"]}
     objects = []
     for unit, headers in units.items():
         obj = os.path.join(PKG, unit[:-3] + ".o")

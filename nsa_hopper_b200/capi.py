@@ -111,11 +111,12 @@ class NsaCacheAttendDesc(ctypes.Structure):
 
     _fields_ = [
         ("batch", NsaCacheBatch), ("q", ctypes.c_void_p), ("sel", ctypes.c_void_p), ("o", ctypes.c_void_p),
-        ("lse", ctypes.c_void_p), ("o_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p), ("o_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("err", ctypes.c_void_p),
         ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
         ("heads_q", ctypes.c_int32), ("n_sel", ctypes.c_int32), ("block_size", ctypes.c_int32), ("window", ctypes.c_int32),
         ("q_dtype", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("o_accumulate", ctypes.c_int32),
-        ("keep_rows", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32 * 5),
+        ("keep_rows", ctypes.c_int32), ("scale", ctypes.c_float), ("timeout_ms", ctypes.c_int32),
+        ("debug_flags", ctypes.c_int32), ("reserved", ctypes.c_int32 * 5),
     ]
 
 
@@ -123,7 +124,7 @@ class NsaCacheAttendPlanInfo(ctypes.Structure):
     """Mirror of ``nsa_cache_attend_plan_info``."""
 
     _fields_ = [
-        ("workspace_bytes", ctypes.c_int64), ("workers", ctypes.c_int32), ("slots", ctypes.c_int32),
+        ("workspace_bytes", ctypes.c_int64), ("slots", ctypes.c_int32), ("team", ctypes.c_int32),
         ("share", ctypes.c_int32), ("grid", ctypes.c_int32), ("threads", ctypes.c_int32), ("smem_bytes", ctypes.c_int32),
         ("merge", ctypes.c_int32), ("tiles", ctypes.c_int32),
     ]

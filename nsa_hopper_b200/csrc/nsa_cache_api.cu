@@ -109,8 +109,8 @@ int check_attend(const nsa_cache_attend_desc* d) {
   if (d->q == nullptr || d->o == nullptr) return fail(NSA_ERR_INVALID_ARG, "q and o must be non-NULL");
   if (misaligned(d->q, 16) || misaligned(d->o, 16) || d->q_row_stride % 8 != 0 || d->q_head_stride % 8 != 0)
     return fail(NSA_ERR_INVALID_ARG, "q and o must be 16-byte aligned and q's strides multiples of 8");
-  if (misaligned(d->sel, 4) || misaligned(d->lse, 4) || misaligned(d->o_weight, 4))
-    return fail(NSA_ERR_INVALID_ARG, "sel, lse and o_weight must be aligned to their element size");
+  if (misaligned(d->sel, 4) || misaligned(d->lse, 4) || misaligned(d->o_weight, 4) || misaligned(d->err, 4))
+    return fail(NSA_ERR_INVALID_ARG, "sel, lse, o_weight and err must be aligned to their element size");
   return NSA_OK;
 }
 
@@ -120,25 +120,28 @@ int plan_attend(const nsa_cache_attend_desc* d, int sm_count, nsa_cache_attend_p
   const nsa_cache_batch& b = d->batch;
   const int group = d->heads_q / b.heads_kv;
   p->tiles = (group + 15) / 16;
-  const int64_t most = most_slots(d), rows = (int64_t)b.n_rows * b.heads_kv * p->tiles, bound = rows * most;
-  const int64_t blocks = (int64_t)sm_count * C::CTAS, cap = blocks * C::NW;
-  const bool running = d->sel == nullptr && d->window == 0;
-  p->workers = (int32_t)std::min(cap, bound);
-  p->slots = running && b.n_rows <= C::kMaxRagged ? 0 : (int32_t)most;
-  if (p->slots != 0) {
-    int64_t share = (bound + p->workers - 1) / p->workers;
-    // Rows are left whole where there are many for each worker: what the last of them costs more is less than the joins.
-    if (rows >= 8 * cap || running) share = (share + most - 1) / most * most;
-    p->share = (int32_t)std::min(share, kMaxIndex);
-    p->workers = (int32_t)((bound + share - 1) / share);
+  const uint32_t most = (uint32_t)most_slots(d), rows = (uint32_t)b.n_rows * b.heads_kv * p->tiles;
+  const uint32_t warps = (uint32_t)sm_count * C::NW;
+  const bool ragged = d->sel == nullptr && d->window == 0 && b.n_rows <= C::kMaxRagged;
+  const nsa::cache::Split s = nsa::cache::split_line(rows, rows * most, most, warps);
+  p->slots = ragged ? 0 : (int32_t)most;
+  bool cut = s.cut != 0;
+  uint32_t teams;  // with a share of their own, at most
+  if (ragged) {
+    cut = nsa::cache::may_cut(rows, most, warps);
+    teams = (uint32_t)std::min<uint64_t>(warps, (uint64_t)rows * most);
+    p->grid = (int32_t)std::min<uint32_t>(sm_count, teams);
+  } else {
+    p->team = (int32_t)s.team;
+    p->share = (int32_t)s.share;
+    teams = nsa::cache::ceil_div(s.cut ? rows * most : rows, s.share);
+    p->grid = (int32_t)std::min<uint32_t>(sm_count, teams);
   }
-  p->grid = (int32_t)std::min<int64_t>(blocks, p->workers);
   p->threads = C::NW * 32;
   p->smem_bytes = C::kSmem;
-  const bool cut = p->slots == 0 ? p->workers > 1 : p->share % p->slots != 0;
-  const int64_t parts = most / std::max<int64_t>(1, bound / p->workers) + 1;
-  p->merge = !cut ? 0 : parts <= 32 ? 1 : 8;
-  p->workspace_bytes = cut ? ((int64_t)(b.n_rows + 1) * 4 + 15) / 16 * 16 + (int64_t)p->workers * 2 * C::kPart * 4 : 16;
+  // (a team that shares a row of one query alone with many: eight warps join each query head's parts)
+  p->merge = !cut ? 0 : (uint64_t)most * warps / C::NW > (uint64_t)rows * most * 4 ? 8 : 1;
+  p->workspace_bytes = cut ? ((int64_t)(b.n_rows + 2) * 4 + 15) / 16 * 16 + (int64_t)teams * 2 * C::kPart * 4 : 16;
   return NSA_OK;
 }
 
@@ -206,7 +209,7 @@ int attend(const nsa_cache_attend_desc* d, cudaStream_t st) {
   a.weight = d->o_weight;
   a.starts = static_cast<uint32_t*>(d->workspace);
   a.part = p.merge == 0 ? nullptr
-                        : reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + ((int64_t)(b.n_rows + 1) * 4 + 15) / 16 * 16);
+                        : reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + ((int64_t)(b.n_rows + 2) * 4 + 15) / 16 * 16);
   a.hq = d->heads_q;
   a.hkv = b.heads_kv;
   a.group = d->heads_q / b.heads_kv;
@@ -215,13 +218,16 @@ int attend(const nsa_cache_attend_desc* d, cudaStream_t st) {
   a.per = d->sel != nullptr ? d->block_size / 64 : 1;
   a.window = d->window;
   a.slots = p.slots;
-  a.workers = (uint32_t)p.workers;
-  a.share = (uint32_t)p.share;
+  a.warps = (uint32_t)sm * (uint32_t)(p.threads / 32);
+  a.split = {(uint32_t)p.team, (uint32_t)p.share, p.merge != 0};
   a.q_half = d->q_dtype == NSA_DTYPE_F16;
   a.o_dtype = d->o_dtype;
   a.accumulate = d->o_accumulate != 0;
   a.fill = d->keep_rows == 0;
   a.scale_log2 = (float)((d->scale > 0.0f ? (double)d->scale : 1.0 / sqrt((double)b.d_qk)) * 1.4426950408889634074);
+  a.err = d->err;
+  a.wait_ns = (uint64_t)(d->timeout_ms > 0 ? d->timeout_ms : 2000) * 1000000u;
+  a.stall = (d->debug_flags & NSA_DEBUG_STALL) != 0;
   return for_dims(b.d_qk, b.d_v, [&](auto dqk, auto dv) {
     return launch_attend<CfgFor<decltype(dqk)::value, decltype(dv)::value>>(a, p, dev, st);
   });

@@ -89,10 +89,34 @@ NSA_HD int running_sub(int j, int first, int end) {
 // Slots of a row that takes its sub-blocks one after the other; at least one, so that every row has an owner.
 NSA_HD int running_slots(int first, int end) { return end > first ? (end - 1) / kPage - first / kPage + 1 : 1; }
 
-// All slots of a call in one line are shared out evenly: worker w has [w * per, (w + 1) * per).
-NSA_HD uint32_t share(uint32_t total, uint32_t workers) {
-  const uint32_t per = (total + workers - 1) / workers;
-  return per > 0 ? per : 1;
+// How the slots of a call (rows x slots, standing in one line) are shared out among the device's warps.  `team` warps (a
+// power of two, neighbours of a block) take turns at a row's slots and join their results; a team has `share` whole rows, or,
+// where rows are cut, `share` slots, whose parts a second kernel joins.
+struct Split {
+  uint32_t team, share, cut;
+};
+constexpr uint32_t kTeam = 8;    // largest team
+constexpr uint32_t kJoins = 4;   // what the second kernel costs, in slots of a warp
+
+NSA_HD uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
+// `longest`: slots of the longest row (>= 1), `total` < 2^31: of all rows; `warps`: a multiple of kTeam.
+NSA_HD Split split_line(uint32_t rows, uint32_t total, uint32_t longest, uint32_t warps) {
+  Split s;
+  s.team = kTeam;
+  while (s.team > 1 && ((uint64_t)rows * s.team > warps || longest <= s.team / 2)) s.team /= 2;
+  const uint32_t teams = warps / s.team, whole = ceil_div(rows, teams);
+  const uint64_t uncut = (uint64_t)whole * ceil_div(longest, s.team);
+  const uint32_t even = ceil_div(total, teams);
+  s.cut = ceil_div(even, s.team) + kJoins < uncut;
+  s.share = s.cut ? even : whole;
+  return s;
+}
+// Whether split_line can cut rows of at most `longest` slots at all.
+NSA_HD bool may_cut(uint32_t rows, uint32_t longest, uint32_t warps) {
+  uint32_t team = kTeam;
+  while (team > 1 && (uint64_t)rows * team > warps) team /= 2;
+  return (uint64_t)ceil_div(rows, warps / team) * ceil_div(longest, team) > kJoins + 1;
 }
 
 }  // namespace cache

@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "nsa_cache_index.h"
+#include "ptx.cuh"
 
 namespace nsa {
 namespace cache {
@@ -216,16 +217,17 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 // reads (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  For that
 //   * the d axis of QK is permuted so that a thread's K fragments are d_qk / 4 consecutive codes of one key: one
 //     wide shared load, one conversion and one product with the scale for each pair, exact in fp16;
-//   * the key axis is permuted (key 16t + c + 4i is k index 2c, 2c+1, 2c+8, 2c+9 for i = 0..3) so that a thread's V
-//     fragments are d_v / 8 consecutive codes of four keys, which are interleaved two and two; P needs no
-//     exchange, its score registers are the A fragment.
+//   * a thread's V fragments are d_v / 8 consecutive codes of four keys, which are interleaved two and two; P needs no
+//     exchange, its score registers are the A fragment.  The key axis is permuted (k index 2c, 2c + 1 of a tile of 8 is key
+//     c, 4 + (c ^ 1)) so that neither K's nor V's shared loads collide more than two ways on the record as it is.
 // Q has up to 8 (bf16) or 11 significant bits, so a power of two per row puts it into fp16 (below 2^-14 of the row's
 // largest to within 2^-25 of it).  P is rounded to fp16 (at most 2^-11 of each term): the sum of
 // its fp32 values is the divisor.  Scores, statistics and O are fp32.
 //
-// All (row, page) slots of the call stand in one line that is cut evenly among the workers; a row that is cut
-// leaves partial (m, sum, O) in the workspace, and merge_kernel joins them in the order of the line: results do not
-// depend on timing.
+// All (row, page) slots of the call stand in one line that is shared out evenly (split_line): teams of 1 to 8 warps of a
+// block take turns at a row's pages and join their (m, sum, O) in shared memory; a row that is cut between teams leaves
+// partial results in the workspace, and merge_kernel joins them in the order of the line.  Results do not depend on
+// timing.
 struct AttendArgs {
   Batch b;
   const void* q;                 // [n_rows, Hq, DQK], bf16 or fp16, unit stride along d
@@ -236,46 +238,67 @@ struct AttendArgs {
   void* o;                       // [n_rows, Hq, DV]
   float* lse;                    // [n_rows, Hq] or nullptr
   const float* weight;
-  float* part;                   // partial results, 2 per worker
-  uint32_t* starts;              // slots before every row's, n_rows + 1 (ragged line only; the first block writes them)
+  float* part;                   // partial results, 2 for each team
+  uint32_t* starts;              // ragged line: slots before every row's (n_rows + 1), then the share of a team or 0 if no
+                                 // row is cut; written by the first block for merge_kernel
   int32_t hq, hkv, group, tiles; // tiles: 16-row tiles of a KV head's G query heads
   int32_t n_sel, per, window;    // per: sub-blocks of a selection block
   int32_t slots;                 // slots of every row; 0: as many as it has sub-blocks (the ragged line)
-  uint32_t workers, share;       // share: slots of a worker (0: from the line's length, on the device)
+  uint32_t warps;                // of the device
+  Split split;                   // (a ragged line's is worked out on the device)
   int32_t q_half, o_dtype, accumulate, fill;  // fill: rows of no sequence get O = 0, LSE = -inf; else they are left
   float scale_log2;
+  int32_t* err;                  // optional: NSA_DEVERR_TIMEOUT (1) if a copy did not come
+  uint64_t wait_ns;              // bound of every wait for a copy
+  int32_t stall;                 // (test) no copy is made, so that the waits run out
 };
 
-template <int DQK_, int DV_, int NW_, int STAGES_, int CTAS_>
+template <int DQK_, int DV_, int STAGES_, int ROUNDS_>
 struct AttendCfg {
-  static constexpr int DQK = DQK_, DV = DV_, NW = NW_, STAGES = STAGES_, CTAS = CTAS_;
+  static constexpr int DQK = DQK_, DV = DV_, NW = 8, STAGES = STAGES_, ROUNDS = ROUNDS_;
   static constexpr int kRecord = record_bytes(DQK, DV);
-  static constexpr int kQueue = 64;        // resolved slots of a warp
-  static constexpr int kMaxRagged = 512;   // rows of a ragged line
+  static constexpr int kQueue = 40;           // resolved slots of a warp
+  static constexpr int kMaxRagged = 512;      // rows of a ragged line
   static constexpr int kPart = 16 * DV + 32;  // floats of a partial result: O, m, sum
-  static constexpr int kSmem = NW * (STAGES * kRecord + kQueue * 16) + (kMaxRagged + 1) * 4;
+  static constexpr int kJoin = 16 * DV / ROUNDS + 64;  // floats of a warp in a team's join: O of a round, m, sum
+  static constexpr int kWarp = STAGES * (kRecord + 8) + kQueue * 16 + kJoin * 4;
+  static constexpr int kSmem = NW * kWarp + (kMaxRagged + 1) * 4;
+  static_assert(kSmem <= 232448, "227 KB of shared memory a block");
 };
 
-// Warps of a block, ring depth and blocks of an SM for each head dim: what fits 227 KB of shared memory and the
-// registers (a warp holds O and Q of a 16-row tile).
+// Ring depth and rounds of the join for each head dim.  A warp holds O and Q of a 16-row tile and a page's scores in up to
+// 255 registers, so a block has 8 warps and an SM one block.
 template <int DQK, int DV>
 struct CfgFor;
 template <>
-struct CfgFor<64, 64> : AttendCfg<64, 64, 8, 3, 1> {};
+struct CfgFor<64, 64> : AttendCfg<64, 64, 3, 1> {};
 template <>
-struct CfgFor<128, 64> : AttendCfg<128, 64, 8, 4, 1> {};
+struct CfgFor<128, 64> : AttendCfg<128, 64, 3, 1> {};
 template <>
-struct CfgFor<128, 128> : AttendCfg<128, 128, 8, 3, 1> {};
+struct CfgFor<128, 128> : AttendCfg<128, 128, 2, 1> {};
 template <>
-struct CfgFor<192, 128> : AttendCfg<192, 128, 6, 3, 1> {};
+struct CfgFor<192, 128> : AttendCfg<192, 128, 2, 2> {};
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// A record's copy into shared memory, by one thread: the barrier's phase ends when all bytes are there.
+__device__ __forceinline__ void copy_record(void* dst, const uint8_t* src, int bytes, uint64_t* bar) {
+  ptx::mbar_arrive_expect_tx(bar, bytes);
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   ptx::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
+               : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Waits for a phase, `ns` at most; false if that runs out.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t ns) {
+  const uint64_t t0 = ptx::globaltimer();
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (ptx::globaltimer() - t0 > ns) return false;
+  return true;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t ns) {
+  return ptx::mbar_try_wait(bar, parity) || wait_long(bar, parity, ns);
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -283,10 +306,33 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+__device__ __forceinline__ float exp2_fast(float x) { return ptx::ex2(x); }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -309,22 +355,26 @@ __device__ __forceinline__ int sequence_of_warp(const Batch& b, int row, int lan
   return b.n_seqs > 0 && b.cu[lo] <= row && row < b.cu[lo + 1] ? lo : -1;
 }
 
+// 2N consecutive values of one row of Q: as they are in memory, and as fp16 pairs; `factor` undoes the row's power of two.
 template <int N>
-__device__ __forceinline__ void load_q(uint32_t (&q)[N], const uint16_t* src, bool half, float& factor) {
-  // N fp16 pairs of consecutive d of one row; `factor` undoes the row's power of two
-  uint32_t raw[N];
+__device__ __forceinline__ void load_q(uint32_t (&q)[N], const uint16_t* src) {
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
     const uint4 x = src ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-    raw[4 * i] = x.x, raw[4 * i + 1] = x.y, raw[4 * i + 2] = x.z, raw[4 * i + 3] = x.w;
+    q[4 * i] = x.x, q[4 * i + 1] = x.y, q[4 * i + 2] = x.z, q[4 * i + 3] = x.w;
   }
-  float2 f[N];
+}
+template <int N>
+__device__ __forceinline__ void scale_q(uint32_t (&q)[N], bool half, float& factor) {
+  auto pair = [&](uint32_t x) {
+    return half ? __half22float2(*reinterpret_cast<__half2*>(&x))
+                : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+  };
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    f[i] = half ? __half22float2(*reinterpret_cast<__half2*>(&raw[i]))
-                : make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xFFFF0000u));
-    top = max(top, max(__float_as_uint(f[i].x) & 0x7FFFFFFFu, __float_as_uint(f[i].y) & 0x7FFFFFFFu));
+    const float2 f = pair(q[i]);
+    top = max(top, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
   }
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -334,7 +384,36 @@ __device__ __forceinline__ void load_q(uint32_t (&q)[N], const uint16_t* src, bo
   const float down = scaled ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
   factor = scaled ? __uint_as_float((uint32_t)e << 23) : 1.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = pack_half(f[i].x * down, f[i].y * down);
+  for (int i = 0; i < N; ++i) {
+    const float2 f = pair(q[i]);
+    q[i] = pack_half(f.x * down, f.y * down);
+  }
+}
+
+// Four neighbouring values of the result of (row, query head) `at`, times k.
+template <int DV>
+__device__ __forceinline__ void store4(const AttendArgs& a, int64_t at, int d, float4 v, float k) {
+  v.x *= k, v.y *= k, v.z *= k, v.w *= k;
+  if (a.o_dtype == kF32) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.o) + at * DV + d);
+    if (a.accumulate) {
+      const float4 x = *p;
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    }
+    *p = v;
+    return;
+  }
+  uint2 w;
+  if (a.o_dtype == kF16) {
+    w = make_uint2(pack_half(v.x, v.y), pack_half(v.z, v.w));
+  } else {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at * DV + d) = w;
+}
+__device__ __forceinline__ void store_lse(const AttendArgs& a, int64_t at, float m, float l) {
+  if (a.lse != nullptr) a.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
 }
 
 template <class C>
@@ -343,120 +422,129 @@ struct Worker {
   static constexpr int NT = DV / 8;     // 8-wide output tiles
   static constexpr int KS = DQK / 16;   // k steps of QK
 
-  // ---- the producer's side: rows and slots of the worker's share, one after the other
+  // ---- the producer's side: rows and slots of the team's share, one after the other
   struct Cursor {
-    uint32_t next, end;  // slots of the line still to resolve
-    int n, hm, j, len;   // row, KV head and tile in it, next slot, slots of the row
+    uint32_t next, end;    // slots of the line still to resolve
+    int n, hm, j, len;     // row, KV head and tile in it, next slot, slots of the row
     int seq, first, last;  // first and one-past-last visible key
+    int entry;             // lane i: entry i of the row's selection (n_sel <= 32)
+    unsigned twice;        // bit i: entry i stands before (a selection is a set)
   };
 
-  static __device__ __forceinline__ void enter_row(const AttendArgs& a, Cursor& c, const uint32_t* starts, int lane) {
-    c.seq = sequence_of_warp(a.b, c.n, lane);
-    const int pos = c.seq < 0 ? -1 : position_of(a.b, c.seq, c.n);
-    c.last = keys_up_to(a.b, pos);
-    c.first = pos < 0 ? 0 : first_key(pos, a.window);
-    c.len = a.slots ? a.slots : starts[c.n + 1] - starts[c.n];
+  // Called for every KV head and tile of a row; what depends on the row alone is worked out at the first.
+  static __device__ __forceinline__ void enter_row(const AttendArgs& a, Cursor& c, const uint32_t* starts, bool same_row,
+                                                   int lane) {
+    const int h = c.hm / a.tiles, g0 = c.hm % a.tiles * 16;
+    if (a.sel != nullptr && a.n_sel <= 32)
+      c.entry = lane < a.n_sel ? a.sel[((int64_t)c.n * a.hkv + h) * a.n_sel + lane] : -1;
+    // the row's queries on their way into L2 (begin() loads them when its turn comes)
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)c.n * a.q_row + (int64_t)(h * a.group + g0) * a.q_head;
+    constexpr int kLines = DQK / 64;
+    for (int i = lane; i < min(16, a.group - g0) * kLines; i += 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i / kLines * a.q_head + i % kLines * 64));
+    if (!same_row) {
+      c.seq = sequence_of_warp(a.b, c.n, lane);
+      const int pos = c.seq < 0 ? -1 : position_of(a.b, c.seq, c.n);
+      c.last = keys_up_to(a.b, pos);
+      c.first = pos < 0 ? 0 : first_key(pos, a.window);
+      c.len = a.slots ? a.slots : starts[c.n + 1] - starts[c.n];
+    }
+    if (a.sel != nullptr && a.n_sel <= 32)
+      c.twice = __ballot_sync(0xFFFFFFFFu, (__match_any_sync(0xFFFFFFFFu, c.entry) & ((1u << lane) - 1)) != 0);
   }
 
-  // Up to 32 more slots into the queue, those that show no key left out but for the last of a row's slots here (its
-  // owner has to leave the row's result).  An entry: page (-1: none), one past the last and the first visible key of
-  // the sub-block, and the row (times 2, + 1 if it is its last entry here).
+  // This warp's part (every team-th) of the next 32 * team slots of the row into the queue, those that show no key left out
+  // but for the warp's last entry of the row's slots here (its owners have to leave the row's result; one without a slot
+  // of its own gets an empty entry).  An entry: the record's address (0: none), the first and one past the last visible key
+  // of the sub-block (8 bits each), and the row (times 2, + 1 if it is the warp's last entry of it).
   static __device__ __forceinline__ int resolve(const AttendArgs& a, Cursor& c, const uint32_t* starts, int4* queue, int tail,
-                                                int lane) {
+                                                int team, int turn, int lane) {
     const int rows_h = a.hkv * a.tiles;
-    const int count = min(32u, min((uint32_t)(c.len - c.j), c.end - c.next));
-    const int j = c.j + lane;
+    const int count = min((uint32_t)(32 * team), min((uint32_t)(c.len - c.j), c.end - c.next));
+    const int own = (count - turn + team - 1) / team;  // (0 where count <= turn)
+    const int j = c.j + lane * team + turn;
     int sub = -1;
-    if (lane < count) {
-      if (a.sel != nullptr) {
-        const int32_t* row = a.sel + ((int64_t)c.n * a.hkv + c.hm / a.tiles) * a.n_sel;
-        const int at = j / a.per, entry = row[at];
-        sub = selected_sub(entry, j - at * a.per, a.per, c.first, c.last);
-        if (sub >= 0)
-          for (int i = 0; i < at; ++i)
-            if (row[i] == entry) sub = -1;  // a selection is a set
-      } else {
-        sub = running_sub(j, c.first, c.last);
-      }
+    if (a.sel == nullptr) {
+      if (lane < own) sub = running_sub(j, c.first, c.last);
+    } else if (a.n_sel <= 32) {
+      const int at = min(j / a.per, 31), entry = __shfl_sync(0xFFFFFFFFu, c.entry, at);
+      if (lane < own && !(c.twice >> at & 1)) sub = selected_sub(entry, j - at * a.per, a.per, c.first, c.last);
+    } else if (lane < own) {
+      const int32_t* row = a.sel + ((int64_t)c.n * a.hkv + c.hm / a.tiles) * a.n_sel;
+      const int at = j / a.per, entry = row[at];
+      sub = selected_sub(entry, j - at * a.per, a.per, c.first, c.last);
+      if (sub >= 0)
+        for (int i = 0; i < at; ++i)
+          if (row[i] == entry) sub = -1;
     }
     const int page = sub < 0 || c.seq < 0 ? -1 : page_of(a.b, c.seq, sub);
-    const bool final = lane == count - 1 && (c.j + count == c.len || c.next + count == c.end);
-    const bool keep = lane < count && (page >= 0 || final);
+    const bool over = c.j + count == c.len || c.next + count == c.end;
+    const bool final = over && lane == max(own - 1, 0);
+    const bool keep = page >= 0 || final;
     const unsigned kept = __ballot_sync(0xFFFFFFFFu, keep);
     if (keep) {
       const int base = sub * kPage;
+      const uint64_t at = page < 0 ? 0 : reinterpret_cast<uint64_t>(a.cache) + (int64_t)page * a.page_stride +
+                                             (int64_t)(c.hm / a.tiles) * C::kRecord;
       queue[(tail + __popc(kept & ((1u << lane) - 1))) % C::kQueue] =
-          make_int4(page, page < 0 ? 0 : min(kPage, c.last - base), page < 0 ? 0 : max(0, c.first - base),
-                    (c.n * rows_h + c.hm) * 2 + final);
+          make_int4((int)(uint32_t)at, (int)(uint32_t)(at >> 32),
+                    page < 0 ? 0 : max(0, c.first - base) | min(kPage, c.last - base) << 8, (c.n * rows_h + c.hm) * 2 + final);
     }
     __syncwarp();
     c.next += count;
     c.j += count;
     if (c.j == c.len && c.next < c.end) {  // the next row
       c.j = 0;
-      if (++c.hm == rows_h) {
-        c.hm = 0, ++c.n;
-        enter_row(a, c, starts, lane);
-      }
+      const bool same_row = ++c.hm < rows_h;
+      if (!same_row) c.hm = 0, ++c.n;
+      enter_row(a, c, starts, same_row, lane);
     }
     return tail + __popc(kept);
   }
 
-  static __device__ __forceinline__ void copy_record(const AttendArgs& a, const int4& e, uint32_t dst, int lane) {
-    if (e.x < 0) return;
-    const int h = (e.w >> 1) % (a.hkv * a.tiles) / a.tiles;
-    const uint8_t* src = a.cache + (int64_t)e.x * a.page_stride + (int64_t)h * C::kRecord;
-    constexpr int KC = DQK / 32, VC = DV / 32;  // 16-byte pieces of a token's codes
-#pragma unroll
-    for (int i = 0; i < 2 * KC; ++i) {  // K codes; in every 8 tokens, token u stands at place 2 (u % 4) + u / 4
-      const int x = lane + 32 * i, row = x / KC, piece = x - row * KC;
-      const int place = (row & ~7) | ((row & 3) << 1) | ((row >> 2) & 1);
-      cp_async16(dst + place * (DQK / 2) + piece * 16, src + x * 16);
-    }
-#pragma unroll
-    for (int i = 0; i < (DQK / 4 + 31) / 32; ++i)
-      if (lane + 32 * i < DQK / 4) cp_async16(dst + k_scale_at(DQK) + (lane + 32 * i) * 16, src + k_scale_at(DQK) + (lane + 32 * i) * 16);
-#pragma unroll
-    for (int i = 0; i < 2 * VC; ++i) {  // V codes; with 64-byte rows every other pair of tokens has its halves exchanged
-      const int x = lane + 32 * i, row = x / VC, piece = x - row * VC;
-      const int place = DV == 128 ? piece ^ (((row >> 1) & 1) << 1) : piece;
-      cp_async16(dst + v_code_at(DQK) + row * (DV / 2) + place * 16, src + v_code_at(DQK) + x * 16);
-    }
-#pragma unroll
-    for (int i = 0; i < (DV / 4 + 31) / 32; ++i)
-      if (lane + 32 * i < DV / 4)
-        cp_async16(dst + v_scale_at(DQK, DV) + (lane + 32 * i) * 16, src + v_scale_at(DQK, DV) + (lane + 32 * i) * 16);
+  static __device__ __forceinline__ const uint8_t* record_of(const int4& e) {
+    return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)e.y << 32 | (uint32_t)e.x);
   }
-
   // ---- the consumer's side
   float o[NT][4];
   uint32_t q0[KS * 2], q1[KS * 2];  // Q of rows r and r + 8: d = c * DQK / 4 + 2i, + 1
-  float f0, f1, m0, m1, l0, l1;
+  float f0, f1, m0, m1;
+  float2 l0, l1;  // each thread's share of the sums
 
-  __device__ __forceinline__ void begin(const AttendArgs& a, uint32_t row, int lane) {
+  // A new row: its queries are asked for, then (when the copies of the first pages are under way) made ready.
+  __device__ __forceinline__ void ask(const AttendArgs& a, uint32_t row, int lane) {
     const int rows_h = a.hkv * a.tiles, r = lane >> 2, c = lane & 3;
     const int n = row / rows_h, hm = row % rows_h, h = hm / a.tiles, g = hm % a.tiles * 16 + r;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)n * a.q_row + (int64_t)(h * a.group + g) * a.q_head +
                           c * (DQK / 4);
-    load_q(q0, g < a.group ? src : nullptr, a.q_half, f0);
-    load_q(q1, g + 8 < a.group ? src + 8 * a.q_head : nullptr, a.q_half, f1);
-    f0 *= a.scale_log2, f1 *= a.scale_log2;
+    load_q(q0, g < a.group ? src : nullptr);
+    load_q(q1, g + 8 < a.group ? src + 8 * a.q_head : nullptr);
+  }
+  __device__ __forceinline__ void begin(const AttendArgs& a) {
+    scale_q(q0, a.q_half, f0);
+    scale_q(q1, a.q_half, f1);
+    // (finite and not 0, so that -inf stays -inf)
+    f0 = fminf(fmaxf(f0 * a.scale_log2, 1e-38f), 3e38f), f1 = fminf(fmaxf(f1 * a.scale_log2, 1e-38f), 3e38f);
     m0 = m1 = -INFINITY;
-    l0 = l1 = 0.0f;
+    l0 = l1 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   }
 
   // One page: keys [lo, lim) of its 64 are visible.
-  __device__ __forceinline__ void page(const uint8_t* rec, int lim, int lo, int lane) {
+  __device__ __forceinline__ void page(uint8_t* rec, int lim, int lo, int lane) {
     const int r = lane >> 2, c = lane & 3;
     const bool whole = lim >= kPage && lo <= 0;
+    const int odd = 4 + (c ^ 1);                              // keys of this thread's columns in a tile of 8: c and odd
+    const int row = r & 1 ? 4 + (r >> 1 ^ 1) : r >> 1;        // key of K's fragment
+    const uint8_t* krec = rec + row * (DQK / 2) + c * (DQK / 8);
+    const uint8_t* kscales = rec + k_scale_at(DQK) + row * (DQK / kGroup) + c * (DQK / 64);
     float s[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-      const uint8_t* codes = rec + (8 * i + r) * (DQK / 2) + c * (DQK / 8);
-      const uint8_t* scales = rec + k_scale_at(DQK) + (8 * i + (r >> 1) + 4 * (r & 1)) * (DQK / kGroup) + c * (DQK / 64);
+      const uint8_t* codes = krec + 8 * i * (DQK / 2);
+      const uint8_t* scales = kscales + 8 * i * (DQK / kGroup);
       uint32_t w[DQK / 32];
       uint32_t sc[DQK / 64];
       if constexpr (DQK == 128) {
@@ -481,58 +569,67 @@ struct Worker {
         mma(s[i], q0[4 * j + 2], q1[4 * j + 2], q0[4 * j + 3], q1[4 * j + 3], b2, b3);
       }
     }
-    // softmax; score i, element e is key 16 (i / 2) + 8 (i % 2) + c + 4 (e % 2) of row r + 8 (e / 2)
-    float t0 = m0, t1 = m1;
+    // score i, element e is key 8 i + (c or odd, by e % 2) of row r + 8 (e / 2)
+    if (!whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[i][e] *= f0, s[i][e + 2] *= f1;
-        if (!whole) {
-          const int key = 8 * i + c + 4 * e;
+        for (int e = 0; e < 2; ++e) {
+          const int key = 8 * i + (e ? odd : c);
           if (key < lo || key >= lim) s[i][e] = s[i][e + 2] = -INFINITY;
         }
-        t0 = fmaxf(t0, s[i][e]), t1 = fmaxf(t1, s[i][e + 2]);
-      }
+      // what stands in the other keys' places may be anything, NaN too: with a scale of 0 their values are 0
+#pragma unroll
+      for (int key = lane; key < kPage; key += 32)
+        if (key < lo || key >= lim) {
+          uint8_t* z = rec + v_scale_at(DQK, DV) + key * (DV / kGroup);
+          if constexpr (DV == 128) *reinterpret_cast<uint2*>(z) = make_uint2(0, 0);
+          else *reinterpret_cast<uint32_t*>(z) = 0;
+        }
+      ptx::fence_proxy_async_smem();  // (before the record that is copied here next)
+      __syncwarp();
     }
+    // softmax: the maximum m of the unscaled scores, f > 0 turns them into powers of two
+    float t0 = m0, t1 = m1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t0 = max3(t0, s[i][0], s[i][1]), t1 = max3(t1, s[i][2], s[i][3]);
     t0 = fmaxf(t0, __shfl_xor_sync(0xFFFFFFFFu, t0, 1)), t1 = fmaxf(t1, __shfl_xor_sync(0xFFFFFFFFu, t1, 1));
     t0 = fmaxf(t0, __shfl_xor_sync(0xFFFFFFFFu, t0, 2)), t1 = fmaxf(t1, __shfl_xor_sync(0xFFFFFFFFu, t1, 2));
-    const float u0 = t0 == -INFINITY ? 0.0f : t0, u1 = t1 == -INFINITY ? 0.0f : t1;
+    const float u0 = t0 == -INFINITY ? 0.0f : t0 * f0, u1 = t1 == -INFINITY ? 0.0f : t1 * f1;
     if (__any_sync(0xFFFFFFFFu, t0 > m0 || t1 > m1)) {
-      const float a0 = exp2_fast(m0 - u0), a1 = exp2_fast(m1 - u1);
-      l0 *= a0, l1 *= a1;
+      const float a0 = exp2_fast(m0 * f0 - u0), a1 = exp2_fast(m1 * f1 - u1);
+      l0.x *= a0, l0.y *= a0, l1.x *= a1, l1.y *= a1;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] *= a0, o[i][1] *= a0, o[i][2] *= a1, o[i][3] *= a1;
       m0 = t0, m1 = t1;
     }
+    uint32_t p[8][2];  // fp16: rows r and r + 8
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s[i][0] = exp2_fast(s[i][0] - u0), s[i][1] = exp2_fast(s[i][1] - u0);
-      s[i][2] = exp2_fast(s[i][2] - u1), s[i][3] = exp2_fast(s[i][3] - u1);
-      l0 += s[i][0] + s[i][1], l1 += s[i][2] + s[i][3];
+      float2 x = fma2(make_float2(s[i][0], s[i][1]), make_float2(f0, f0), make_float2(-u0, -u0));
+      float2 y = fma2(make_float2(s[i][2], s[i][3]), make_float2(f1, f1), make_float2(-u1, -u1));
+      x = make_float2(exp2_fast(x.x), exp2_fast(x.y)), y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+      l0 = add2(l0, x), l1 = add2(l1, y);
+      p[i][0] = pack_half(x.x, x.y), p[i][1] = pack_half(y.x, y.y);
     }
     // PV; output tile j, element e is d = (2c + e % 2) * NT + j of row r + 8 (e / 2)
-    const uint8_t* vcodes = rec + v_code_at(DQK) + c * (DV / 2) + (DV == 128 ? (r * 8) ^ (((c >> 1) & 1) << 5) : r * 4);
-    const uint8_t* vscales = rec + v_scale_at(DQK, DV) + c * (DV / kGroup) + (DV == 128 ? r : r >> 1);
+    const uint8_t* vrec = rec + v_code_at(DQK) + r * (DV / 16);
+    const uint8_t* vscales = rec + v_scale_at(DQK, DV) + (DV == 128 ? r : r >> 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const uint32_t a0 = pack_half(s[2 * t][0], s[2 * t][1]), a1 = pack_half(s[2 * t][2], s[2 * t][3]);
-      const uint32_t a2 = pack_half(s[2 * t + 1][0], s[2 * t + 1][1]), a3 = pack_half(s[2 * t + 1][2], s[2 * t + 1][3]);
+      const uint32_t a0 = p[2 * t][0], a1 = p[2 * t][1], a2 = p[2 * t + 1][0], a3 = p[2 * t + 1][1];
       uint32_t w[4][DV / 64], z[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* at = vcodes + (16 * t + 4 * i) * (DV / 2);
+        const int key = 16 * t + 8 * (i / 2) + (i % 2 ? odd : c);
+        const uint8_t* at = vrec + key * (DV / 2);
         if constexpr (DV == 128) {
           const uint2 x = *reinterpret_cast<const uint2*>(at);
           w[i][0] = x.x, w[i][1] = x.y;
         } else {
           w[i][0] = *reinterpret_cast<const uint32_t*>(at);
         }
-        z[i] = vscales[(16 * t + 4 * i) * (DV / kGroup)];
-        if (!whole) {  // what stands behind the visible keys may be anything: 0 times a code is 0
-          const int key = 16 * t + 4 * i + c;
-          if (key < lo || key >= lim) z[i] = 0;
-        }
+        z[i] = vscales[key * (DV / kGroup)];
       }
       const uint32_t z0 = z[0] * 128u + (z[1] << 23), z1 = z[2] * 128u + (z[3] << 23);
 #pragma unroll
@@ -553,60 +650,96 @@ struct Worker {
     }
   }
 
-  // The row's result: whole, or this worker's part of it (`part` not null).
-  __device__ __forceinline__ void finish(const AttendArgs& a, uint32_t row, float* part, int lane) {
+  // The row's result: whole, or this team's part of it (`part` not null).  `join`: the team's warps' join buffers.
+  __device__ __forceinline__ void finish(const AttendArgs& a, uint32_t row, float* part, float* join, int team, int turn,
+                                         int barrier, int lane) {
     const int rows_h = a.hkv * a.tiles, r = lane >> 2, c = lane & 3;
-    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1), l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 1);
-    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2), l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
-    if (part != nullptr) {
-      if (c == 0) {
-        part[16 * DV + r] = m0, part[16 * DV + r + 8] = m1;
-        part[16 * DV + 16 + r] = l0, part[16 * DV + 16 + r + 8] = l1;
+    float n0 = l0.x + l0.y, n1 = l1.x + l1.y;
+    n0 += __shfl_xor_sync(0xFFFFFFFFu, n0, 1), n1 += __shfl_xor_sync(0xFFFFFFFFu, n1, 1);
+    n0 += __shfl_xor_sync(0xFFFFFFFFu, n0, 2), n1 += __shfl_xor_sync(0xFFFFFFFFu, n1, 2);
+    float e0 = m0 == -INFINITY ? m0 : m0 * f0, e1 = m1 == -INFINITY ? m1 : m1 * f1;  // as powers of two
+    const int n = row / rows_h, hm = row % rows_h, g0 = hm % a.tiles * 16;
+    const int64_t at0 = (int64_t)n * a.hq + hm / a.tiles * a.group + g0;  // the tile's first query head
+    const int used = min(16, a.group - g0);
+    const bool left = part == nullptr && !a.fill && sequence_of_warp(a.b, n, lane) < 0;  // a row to leave as it was
+    if (team == 1) {
+      if (part != nullptr) {
+        if (c == 0) {
+          part[16 * DV + r] = e0, part[16 * DV + r + 8] = e1;
+          part[16 * DV + 16 + r] = n0, part[16 * DV + 16 + r + 8] = n1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float4* to = reinterpret_cast<float4*>(part + (r + 8 * (e / 2)) * DV + (2 * c + e % 2) * NT);
+#pragma unroll
+          for (int j = 0; j < NT / 4; ++j) to[j] = make_float4(o[4 * j][e], o[4 * j + 1][e], o[4 * j + 2][e], o[4 * j + 3][e]);
+        }
+        return;
       }
+      if (left) return;
+      const float w = a.weight ? *a.weight : 1.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float4* to = reinterpret_cast<float4*>(part + (r + 8 * (e / 2)) * DV + (2 * c + e % 2) * NT);
+      for (int half = 0; half < 2; ++half) {
+        if (r + 8 * half >= used) continue;
+        const float l = half ? n1 : n0, k = l != 0.0f ? w / l : 0.0f;
+        const int64_t at = at0 + r + 8 * half;
+        if (c == 0) store_lse(a, at, half ? e1 : e0, l);
 #pragma unroll
-        for (int j = 0; j < NT / 4; ++j) to[j] = make_float4(o[4 * j][e], o[4 * j + 1][e], o[4 * j + 2][e], o[4 * j + 3][e]);
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < NT / 4; ++j)
+            store4<DV>(a, at, (2 * c + e) * NT + 4 * j,
+                       make_float4(o[4 * j][2 * half + e], o[4 * j + 1][2 * half + e], o[4 * j + 2][2 * half + e],
+                                   o[4 * j + 3][2 * half + e]), k);
       }
       return;
     }
-    const int n = row / rows_h, hm = row % rows_h, h = hm / a.tiles, g = hm % a.tiles * 16 + r;
-    if (!a.fill && sequence_of_warp(a.b, n, lane) < 0) return;
-    const float w = a.weight ? *a.weight : 1.0f;
+    // Join: maxima, then every warp's O against the common maximum, some columns a round.  The 16-byte pieces of a row
+    // are exchanged so that neither side meets bank conflicts.
+    constexpr int NTR = NT / C::ROUNDS, CS = NTR / 4, kMl = 16 * DV / C::ROUNDS;
+    float* mine = join + turn * C::kJoin;
+    if (c == 0) mine[kMl + r] = e0, mine[kMl + r + 8] = e1;
+    named_barrier(barrier, team * 32);
+    float t0 = -INFINITY, t1 = -INFINITY;
+    for (int w = 0; w < team; ++w)
+      t0 = fmaxf(t0, join[w * C::kJoin + kMl + r]), t1 = fmaxf(t1, join[w * C::kJoin + kMl + r + 8]);
+    e0 = exp2_fast(e0 - (t0 == -INFINITY ? 0.0f : t0)), e1 = exp2_fast(e1 - (t1 == -INFINITY ? 0.0f : t1));
+    if (c == 0) mine[kMl + 16 + r] = n0 * e0, mine[kMl + 16 + r + 8] = n1 * e1, mine[kMl + 32 + r] = t0, mine[kMl + 40 + r] = t1;
+    const float weight = a.weight && part == nullptr ? *a.weight : 1.0f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (g + 8 * half >= a.group) continue;
-      const float l = half ? l1 : l0, m = half ? m1 : m0, k = l != 0.0f ? w / l : 0.0f;
-      const int64_t at = (int64_t)n * a.hq + h * a.group + g + 8 * half;
-      if (a.lse != nullptr && c == 0) a.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+    for (int q = 0; q < C::ROUNDS; ++q) {
+      if (q > 0) named_barrier(barrier, team * 32);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t to = at * DV + (2 * c + e) * NT;
-        if (a.o_dtype == kF32) {
-          float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.o) + to);
+      for (int e = 0; e < 4; ++e) {
+        const float k = e < 2 ? e0 : e1;
+        float4* to = reinterpret_cast<float4*>(mine) + (r + 8 * (e / 2)) * (8 * CS);
 #pragma unroll
-          for (int j = 0; j < NT / 4; ++j) {
-            float4 v = a.accumulate ? p[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            v.x += o[4 * j][2 * half + e] * k, v.y += o[4 * j + 1][2 * half + e] * k;
-            v.z += o[4 * j + 2][2 * half + e] * k, v.w += o[4 * j + 3][2 * half + e] * k;
-            p[j] = v;
-          }
+        for (int j = 0; j < CS; ++j) {
+          const int t = q * NTR + 4 * j;
+          to[((2 * c + e % 2) * CS + j) ^ (((r & 1) << 2) + c)] =
+              make_float4(o[t][e] * k, o[t + 1][e] * k, o[t + 2][e] * k, o[t + 3][e] * k);
+        }
+      }
+      named_barrier(barrier, team * 32);
+      for (int i = turn * 32 + lane; i < 16 * 8 * CS; i += team * 32) {
+        const int x = i / (8 * CS), k = i % (8 * CS), d = k / CS * NT + q * NTR + k % CS * 4;
+        if (x >= used || left) continue;
+        const int place = x * (8 * CS) + (k ^ (((x & 1) << 2) + k / (2 * CS)));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (int w = 0; w < team; ++w) {
+          const float* from = join + w * C::kJoin;
+          const float4 y = reinterpret_cast<const float4*>(from)[place];
+          v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+          l += from[kMl + 16 + x];
+        }
+        const float m = mine[kMl + 32 + x];
+        if (part != nullptr) {
+          *reinterpret_cast<float4*>(part + x * DV + d) = v;
+          if (k == 0 && q == 0) part[16 * DV + x] = m, part[16 * DV + 16 + x] = l;
         } else {
-          uint32_t v[NT / 2];
-#pragma unroll
-          for (int j = 0; j < NT / 2; ++j) {
-            const float x = o[2 * j][2 * half + e] * k, y = o[2 * j + 1][2 * half + e] * k;
-            if (a.o_dtype == kF16) {
-              v[j] = pack_half(x, y);
-            } else {
-              const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
-              v[j] = *reinterpret_cast<const uint32_t*>(&p);
-            }
-          }
-          uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + to);
-#pragma unroll
-          for (int j = 0; j < NT / 8; ++j) p[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          store4<DV>(a, at0 + x, d, v, l != 0.0f ? weight / l : 0.0f);
+          if (k == 0 && q == 0) store_lse(a, at0 + x, m, l);
         }
       }
     }
@@ -614,14 +747,18 @@ struct Worker {
 };
 
 template <class C>
-__global__ void __launch_bounds__(C::NW * 32, C::CTAS) attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t line[2];  // of a ragged line: slots, the longest row's
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   uint8_t* ring = smem + warp * (C::STAGES * C::kRecord);
-  int4* queue = reinterpret_cast<int4*>(smem + C::NW * C::STAGES * C::kRecord) + warp * C::kQueue;
-  uint32_t* starts = reinterpret_cast<uint32_t*>(smem + C::NW * (C::STAGES * C::kRecord + C::kQueue * 16));
-  const uint32_t rows_h = a.hkv * a.tiles;
-  uint32_t total = (uint32_t)a.b.n_rows * rows_h * a.slots;
+  float* join = reinterpret_cast<float*>(smem + C::NW * C::STAGES * C::kRecord);
+  int4* queue = reinterpret_cast<int4*>(join + C::NW * C::kJoin) + warp * C::kQueue;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(queue + (C::NW - warp) * C::kQueue) + warp * C::STAGES;
+  uint32_t* starts = reinterpret_cast<uint32_t*>(smem + C::NW * C::kWarp);
+  const uint32_t rows_h = a.hkv * a.tiles, rows = a.b.n_rows * rows_h;
+  uint32_t total = rows * a.slots;
+  Split split = a.split;
   if (a.slots == 0) {  // the ragged line: every block counts the slots before each row (n_rows <= kMaxRagged)
     for (int n = threadIdx.x; n < a.b.n_rows; n += C::NW * 32) {
       const int seq = sequence_of(a.b, n), pos = seq < 0 ? -1 : position_of(a.b, seq, n);
@@ -629,10 +766,11 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) attend_kernel(const Atten
     }
     __syncthreads();
     if (warp == 0) {
-      uint32_t sum = 0;
+      uint32_t sum = 0, longest = 0;
       if (lane == 0) starts[0] = 0;
       for (int n0 = 0; n0 < a.b.n_rows; n0 += 32) {
         uint32_t x = n0 + lane < a.b.n_rows ? starts[n0 + lane + 1] : 0;
+        longest = max(longest, x);
 #pragma unroll
         for (int k = 1; k < 32; k *= 2) {
           const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, k);
@@ -641,75 +779,112 @@ __global__ void __launch_bounds__(C::NW * 32, C::CTAS) attend_kernel(const Atten
         if (n0 + lane < a.b.n_rows) starts[n0 + lane + 1] = sum + x;
         sum += __shfl_sync(0xFFFFFFFFu, x, 31);
       }
+#pragma unroll
+      for (int k = 16; k > 0; k /= 2) longest = max(longest, __shfl_xor_sync(0xFFFFFFFFu, longest, k));
+      if (lane == 0) line[0] = sum * rows_h, line[1] = longest;
     }
     __syncthreads();
-    if (blockIdx.x == 0 && a.part != nullptr)
+    total = line[0];
+    split = split_line(rows, total, line[1], a.warps);
+    if (blockIdx.x == 0 && a.part != nullptr) {
       for (int n = threadIdx.x; n <= a.b.n_rows; n += C::NW * 32) a.starts[n] = starts[n];
-    total = starts[a.b.n_rows] * rows_h;
+      if (threadIdx.x == 0) a.starts[a.b.n_rows + 1] = split.cut ? split.share : 0;
+    }
   }
-  const uint32_t per = a.share ? a.share : share(total, a.workers);
-  // neighbouring shares are on different SMs, so that a short line uses many of them
-  const uint32_t me = warp * gridDim.x + blockIdx.x;
-  if (me >= a.workers || (uint64_t)me * per >= total) return;
+  // neighbouring teams are on different SMs, so that a few of them use many
+  const int team = split.team, turn = warp % team, sub_team = warp / team;
+  const uint32_t me = sub_team * gridDim.x + blockIdx.x;
 
   typename Worker<C>::Cursor cur;
-  cur.next = me * per;
-  cur.end = min(total, cur.next + per);
-  uint32_t before;  // the line's slots before the row
-  if (a.slots) {
-    const uint32_t row = cur.next / a.slots;
-    cur.n = row / rows_h, cur.hm = row % rows_h, cur.j = cur.next % a.slots;
-    before = row * a.slots;
-  } else {
-    int lo = 0, hi = a.b.n_rows;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (starts[mid] * rows_h <= cur.next) lo = mid;
-      else hi = mid;
+  auto start_of = [&](uint32_t row) {  // the line's slots before a row
+    if (a.slots) return row * a.slots;
+    const uint32_t n = row / rows_h, s0 = starts[n];
+    return n == a.b.n_rows ? total : s0 * rows_h + row % rows_h * (starts[n + 1] - s0);
+  };
+  uint32_t row = 0;
+  if (split.cut) {
+    if ((uint64_t)me * split.share >= total) return;
+    cur.next = me * split.share;
+    cur.end = total - cur.next < split.share ? total : cur.next + split.share;
+    if (a.slots) {
+      row = cur.next / a.slots;
+    } else {
+      int lo = 0, hi = a.b.n_rows;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (starts[mid] * rows_h <= cur.next) lo = mid;
+        else hi = mid;
+      }
+      row = lo * rows_h + (cur.next - starts[lo] * rows_h) / (starts[lo + 1] - starts[lo]);
     }
-    const uint32_t len = starts[lo + 1] - starts[lo], into = cur.next - starts[lo] * rows_h;
-    cur.n = lo, cur.hm = into / len, cur.j = into % len;
-    before = cur.next - cur.j;
+  } else {
+    if ((uint64_t)me * split.share >= rows) return;
+    row = me * split.share;
+    cur.next = start_of(row);
+    cur.end = start_of(min(rows - row, split.share) + row);
   }
-  const bool cut_before = before < cur.next;  // the first row's earlier slots are another worker's
-  Worker<C>::enter_row(a, cur, starts, lane);
+  cur.n = row / rows_h, cur.hm = row % rows_h, cur.j = cur.next - start_of(row);
+  const bool cut_before = cur.j != 0;  // the first row's earlier slots are another team's
+  Worker<C>::enter_row(a, cur, starts, false, lane);
 
+  if (lane < C::STAGES) ptx::mbar_init(bars + lane, 1);
+  ptx::fence_mbar_init();
+  __syncwarp();
   Worker<C> w;
+  w.ask(a, row, lane);
   int head = 0, tail = 0, issued = 0;
-  bool fresh = true, first_row = true;
-  // the ring holds STAGES records: STAGES - 1 in flight while one is worked on; one (maybe empty) copy group each
+  uint32_t phases = 0, flying = 0;  // each stage's parity of the next phase; copies on their way
+  bool lost = false;                // a copy did not come: rows from here on are NaN
   auto issue = [&] {
     while (tail - issued < C::STAGES && tail - head <= C::kQueue - 32 && cur.next < cur.end)
-      tail = Worker<C>::resolve(a, cur, starts, queue, tail, lane);
+      tail = Worker<C>::resolve(a, cur, starts, queue, tail, team, turn, lane);
     if (issued < tail) {
-      const int4 e = queue[issued % C::kQueue];
-      Worker<C>::copy_record(a, e, (uint32_t)__cvta_generic_to_shared(ring + (issued % C::STAGES) * C::kRecord), lane);
-      ++issued;
+      const uint8_t* src = Worker<C>::record_of(queue[issued % C::kQueue]);
+      const int stage = issued++ % C::STAGES;
+      if (src != nullptr && !lost && !a.stall) {
+        if (lane == 0) copy_record(ring + stage * C::kRecord, src, C::kRecord, bars + stage);
+        flying |= 1u << stage;
+      }
     }
-    cp_commit();
   };
+  // the ring holds STAGES records: STAGES - 1 on their way while one is worked on
   for (int i = 0; i < C::STAGES - 1; ++i) issue();
+  w.begin(a);
+  bool fresh = false, first_row = true;
   while (head < issued) {
+    issue();
     const int4 e = queue[head % C::kQueue];
-    cp_wait<C::STAGES - 2>();
-    __syncwarp();
-    const uint32_t row = (uint32_t)e.w >> 1;
-    if (fresh) w.begin(a, row, lane);
+    const int stage = head % C::STAGES;
+    if (fresh) {
+      w.ask(a, (uint32_t)e.w >> 1, lane);
+      w.begin(a);
+    }
     fresh = e.w & 1;
-    if (e.x >= 0) w.page(ring + (head % C::STAGES) * C::kRecord, e.y, e.z, lane);
+    if (Worker<C>::record_of(e) != nullptr) {
+      lost = lost || !__all_sync(0xFFFFFFFFu, wait_for(bars + stage, phases >> stage & 1, a.wait_ns));
+      if (!lost) {
+        phases ^= 1u << stage, flying &= ~(1u << stage);
+        w.page(ring + stage * C::kRecord, e.z >> 8, e.z & 255, lane);
+      } else {
+        w.l0.x = w.l1.x = __int_as_float(0x7FFFFFFF);
+      }
+    }
     if (fresh) {
       // a row is whole here unless it began before this share, or goes on behind it
       const bool head_cut = first_row && cut_before;
       const bool tail_cut = head + 1 == tail && cur.next == cur.end && cur.j < cur.len;
       float* part = head_cut || tail_cut ? a.part + ((size_t)me * 2 + (head_cut ? 0 : 1)) * C::kPart : nullptr;
-      w.finish(a, row, part, lane);
+      w.finish(a, (uint32_t)e.w >> 1, part, join + sub_team * team * C::kJoin, team, turn, 1 + sub_team, lane);
       first_row = false;
     }
     __syncwarp();
     ++head;
-    issue();
   }
-  cp_wait<0>();
+  if (lost) {  // the block's memory is not given up under a copy (bounded, too)
+    if (a.err != nullptr && lane == 0) atomicOr(a.err, 1);
+    for (int i = 0; i < C::STAGES; ++i)
+      if (flying >> i & 1) wait_for(bars + i, phases >> i & 1, a.wait_ns);
+  }
 }
 
 // Joins the parts of the rows that were cut, in the order of the line.  WPH warps share a row's query head:
@@ -725,18 +900,19 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
   if (unit >= (int64_t)a.b.n_rows * a.hq) return;
   const int n = unit / a.hq, hq = unit % a.hq, h = hq / a.group, g = hq % a.group;
   const uint32_t hm = h * a.tiles + g / 16;
-  uint32_t start, len, total;
+  uint32_t start, len, per = a.split.share;
   if (a.slots) {
-    len = a.slots, start = ((uint32_t)n * rows_h + hm) * len, total = (uint32_t)a.b.n_rows * rows_h * a.slots;
+    len = a.slots, start = ((uint32_t)n * rows_h + hm) * len;
   } else {
     const uint32_t s0 = a.starts[n];
-    len = a.starts[n + 1] - s0, start = s0 * rows_h + hm * len, total = a.starts[a.b.n_rows] * rows_h;
+    len = a.starts[n + 1] - s0, start = s0 * rows_h + hm * len;
+    per = a.starts[a.b.n_rows + 1];
   }
-  const uint32_t per = a.share ? a.share : share(total, a.workers);
+  if (per == 0) return;
   const uint32_t w0 = start / per, w1 = (start + len - 1) / per;
   if (w0 == w1) return;  // the row was not cut
   if (!a.fill && sequence_of(a.b, n) < 0) return;
-  // the first worker has the row as its last, the others as their first
+  // the first team has the row as its last, the others as their first
   auto part_of = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 ? 1 : 0)) * C::kPart; };
   const int mine = WPH == 1 ? 0 : warp;
   float m = -INFINITY;
@@ -789,26 +965,10 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
     }
   }
   const float k = l != 0.0f ? (a.weight ? *a.weight : 1.0f) / l : 0.0f;
-  if (a.lse != nullptr && lane == 0) a.lse[unit] = l != 0.0f ? (top + log2f(l)) * 0.693147180559945309f : -INFINITY;
+  if (lane == 0) store_lse(a, unit, top, l);
 #pragma unroll
-  for (int i = 0; i < (V4 + 31) / 32; ++i) {
-    if (lane + 32 * i >= V4) continue;
-    float4 v = make_float4(acc[i].x * k, acc[i].y * k, acc[i].z * k, acc[i].w * k);
-    const int64_t at = unit * V4 + lane + 32 * i;
-    if (a.o_dtype == kF32) {
-      float4* p = static_cast<float4*>(a.o) + at;
-      if (a.accumulate) {
-        const float4 x = *p;
-        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-      }
-      *p = v;
-    } else if (a.o_dtype == kF16) {
-      static_cast<uint2*>(a.o)[at] = make_uint2(pack_half(v.x, v.y), pack_half(v.z, v.w));
-    } else {
-      const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-      static_cast<uint2*>(a.o)[at] = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    }
-  }
+  for (int i = 0; i < (V4 + 31) / 32; ++i)
+    if (lane + 32 * i < V4) store4<DV>(a, unit, 4 * (lane + 32 * i), acc[i], k);
 }
 
 }  // namespace cache

@@ -34,7 +34,10 @@ int selected(int entry, int part, int per, int first, int end) { return selected
 int running(int j, int first, int end) { return running_sub(j, first, end); }
 int slots(int first, int end) { return running_slots(first, end); }
 int first(int pos, int window) { return first_key(pos, window); }
-unsigned int sharing(unsigned int total, unsigned int workers) { return share(total, workers); }
+void split(uint32_t rows, uint32_t total, uint32_t longest, uint32_t warps, uint32_t* out) {
+  const Split s = split_line(rows, total, longest, warps);
+  out[0] = s.team, out[1] = s.share, out[2] = s.cut, out[3] = may_cut(rows, longest, warps);
+}
 int record(int dqk, int dv) { return record_bytes(dqk, dv); }
 }
 """
@@ -104,10 +107,30 @@ def test_sub_blocks(index):
     assert [index.first(p, w) for p, w in ((5, 0), (5, 1), (5, 6), (5, 7), (5, BIG), (BIG - 1, 3))] == [0, 5, 0, 0, 0, BIG - 3]
 
 
-@pytest.mark.parametrize("total,workers", [(1, 1), (5, 3), (64, 1184), (1185, 1184), (2**31 - 1, 1184), (2**31 - 1, 2368)])
-def test_shares_cover_the_line(index, total, workers):
-    per = index.sharing(total, workers)
-    assert per >= 1 and per * workers >= total and (per - 1) * workers < max(total, workers)
+def test_shares_cover_the_line(index):
+    rng = np.random.default_rng(0)
+    warps = 148 * 8
+    for i in range(4000):
+        rows = int(np.exp(rng.uniform(0, np.log(5000))))
+        longest = int(np.exp(rng.uniform(0, np.log(min(40000, (2**31 - 1) // rows)))))
+        total = rows * longest if i % 2 else int(rng.integers(rows + longest - 1, rows * longest + 1))
+        out = (ctypes.c_uint32 * 4)()
+        index.split(rows, total, longest, warps, out)
+        team, share, cut, may = out
+        assert team in (1, 2, 4, 8) and share >= 1
+        teams = warps // team
+        if cut:
+            assert may and share * teams >= total
+        else:
+            assert share * teams >= rows
+        # a shorter longest row of the same rows is never cut where the host has said that none is
+        if not may:
+            for shorter in (x for x in {1, 2, 3, 5, longest // 2, longest - 1} if 0 < x < longest):
+                index.split(rows, min(total, rows * shorter), shorter, warps, out)
+                assert not out[2]
+        # what the split costs is at most what either way costs
+        slots = -(-share // team) + 4 if cut else share * -(-longest // team)
+        assert slots <= -(-rows // teams) * -(-longest // team)
 
 
 def test_record_bytes():
@@ -149,23 +172,27 @@ def _attend(batch=None, **kw):
 
 
 def test_plan_shares_out_the_work():
-    p = capi.cache_attend_plan(_attend(sel=256, n_sel=16, block_size=64))     # 8 x 4 x 16 slots, a worker each
-    assert p["slots"] == 16 and p["share"] == 1 and p["workers"] == 512 and p["grid"] == 148 and p["merge"] == 1
+    p = capi.cache_attend_plan(_attend(sel=256, n_sel=16, block_size=64))     # 32 rows, 8 warps each take 2 pages
+    assert (p["slots"], p["team"], p["share"], p["grid"], p["merge"], p["workspace_bytes"]) == (16, 8, 1, 32, 0, 16)
     assert p["smem_bytes"] <= 232448
+    p = capi.cache_attend_plan(_attend(dict(n_rows=256, n_seqs=256), sel=256, n_sel=16, block_size=64))
+    assert (p["team"], p["share"], p["grid"], p["merge"]) == (1, 1, 148, 0)    # a warp for each row
     p = capi.cache_attend_plan(_attend())                                      # every key: the ragged line
-    assert p["slots"] == 0 and p["share"] == 0 and p["merge"] >= 1
-    p = capi.cache_attend_plan(_attend(dict(n_rows=4096, n_seqs=4096)))        # many rows: whole ones
-    assert p["slots"] == 64 and p["share"] % 64 == 0 and p["merge"] == 0
+    assert p["slots"] == 0 and p["share"] == 0 and p["merge"] >= 1 and p["workspace_bytes"] > 16
+    p = capi.cache_attend_plan(_attend(dict(width=40)))                        # short rows are not cut
+    assert p["slots"] == 0 and p["merge"] == 0
+    p = capi.cache_attend_plan(_attend(dict(n_rows=4096, n_seqs=4096)))        # too many rows for it
+    assert p["slots"] == 64
     p = capi.cache_attend_plan(_attend(window=1))
-    assert p["slots"] == 1
+    assert p["slots"] == 1 and p["team"] == 1
     p = capi.cache_attend_plan(_attend(window=66, heads_q=4 * 17))
-    assert p["slots"] == 3 and p["tiles"] == 2
+    assert p["slots"] == 3 and p["tiles"] == 2 and p["team"] == 4
     p = capi.cache_attend_plan(_attend(dict(n_rows=1, n_seqs=1, width=2048)))
-    assert p["merge"] == 8                                                     # one row over hundreds of workers
+    assert p["merge"] == 8                                                     # one row over many blocks
     for d in ((64, 64), (192, 128), (128, 64)):
         assert capi.cache_attend_plan(_attend(dict(d_qk=d[0], d_v=d[1])))["smem_bytes"] <= 232448
     p = capi.cache_attend_plan(_attend(dict(n_rows=0, n_seqs=0)))
-    assert p["workers"] == 0 and p["workspace_bytes"] == 16
+    assert p["grid"] == 0 and p["workspace_bytes"] == 16
 
 
 BAD = [

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from nsa_hopper_b200 import nsa, ops
+from nsa_hopper_b200 import capi, nsa, ops
 from oracle import cache as oc
 
 pytestmark = pytest.mark.gpu
@@ -461,6 +461,27 @@ def test_two_graphs_and_eager_calls_at_once():
         back, _ = ops.cache_read(c2, 128, pages2, l2)
         np.testing.assert_array_equal(back[0].double().cpu().numpy().transpose(1, 0, 2),
                                       oc.values(*oc.quantise(k.double().cpu().numpy())))
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_waits_are_bounded(n):
+    """A launch whose copies never come ends by itself: the error word is set, the rows are NaN, the next call is right."""
+    q, cache, pages, lens = _small(24, n)
+    want = ops.cache_attend(q, cache, pages, lens)
+    o, lse, err = torch.zeros_like(want[0]), torch.zeros_like(want[1]), torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = capi.make_cache_batch(cache=cache.data_ptr(), pages=pages.data_ptr(), lens=lens.data_ptr(), num_pages=64, n_seqs=n,
+                                  width=pages.shape[1], n_rows=n, heads_kv=2, d_qk=128, d_v=128)
+    desc = capi.make_cache_attend_desc(batch=batch, q=q.data_ptr(), o=o.data_ptr(), lse=lse.data_ptr(), heads_q=16,
+                                       err=err.data_ptr(), timeout_ms=20, debug_flags=capi.NSA_DEBUG_STALL)
+    work = torch.empty(capi.cache_attend_workspace_bytes(desc), dtype=torch.uint8, device="cuda")
+    desc.workspace = work.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.cache_attend(desc, stream)
+    assert err.item() == capi.NSA_DEVERR_TIMEOUT and o.isnan().all() and lse.isnan().all()
+    err.zero_()
+    desc.debug_flags = 0
+    capi.cache_attend(desc, stream)
+    assert err.item() == 0 and torch.equal(o, want[0]) and torch.equal(lse, want[1])
 
 
 def test_side_stream():
