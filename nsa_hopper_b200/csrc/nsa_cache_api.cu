@@ -76,6 +76,18 @@ int done(cudaError_t e, const char* what) {
 }
 
 // ------------------------------------------------------------------ attention
+// A KV head's G query heads: one tile of 8, or tiles of 16.
+int tiles_of(int group) { return group <= 8 ? 1 : (group + 15) / 16; }
+
+// Calls f with the attention's configuration for a checked description.
+template <class F>
+int for_config(const nsa_cache_attend_desc* d, F&& f) {
+  return for_dims(d->batch.d_qk, d->batch.d_v, [&](auto dqk, auto dv) {
+    constexpr int kQk = decltype(dqk)::value, kV = decltype(dv)::value;
+    return d->heads_q / d->batch.heads_kv <= 8 ? f(CfgFor<kQk, kV, 1>()) : f(CfgFor<kQk, kV, 2>());
+  });
+}
+
 // Slots (64-key sub-blocks) of a row and KV head, at most.
 int64_t most_slots(const nsa_cache_attend_desc* d) {
   if (d->sel != nullptr) return (int64_t)d->n_sel * (d->block_size / 64);
@@ -103,7 +115,7 @@ int check_attend(const nsa_cache_attend_desc* d) {
     if (d->n_sel > 1024) return fail(NSA_ERR_UNSUPPORTED, "n_sel must be at most 1024");
   }
   if (b.n_rows == 0) return NSA_OK;
-  const int64_t rows = (int64_t)b.n_rows * b.heads_kv * ((d->heads_q / b.heads_kv + 15) / 16);
+  const int64_t rows = (int64_t)b.n_rows * b.heads_kv * tiles_of(d->heads_q / b.heads_kv);
   if (rows > kMaxIndex / 2 || rows * most_slots(d) > kMaxIndex)
     return fail(NSA_ERR_UNSUPPORTED, "n_rows * heads_kv * (pages that a row can see) must be below 2^31");
   if (d->q == nullptr || d->o == nullptr) return fail(NSA_ERR_INVALID_ARG, "q and o must be non-NULL");
@@ -119,7 +131,7 @@ template <class C>
 int plan_attend(const nsa_cache_attend_desc* d, int sm_count, nsa_cache_attend_plan_info* p) {
   const nsa_cache_batch& b = d->batch;
   const int group = d->heads_q / b.heads_kv;
-  p->tiles = (group + 15) / 16;
+  p->tiles = tiles_of(group);
   const uint32_t most = (uint32_t)most_slots(d), rows = (uint32_t)b.n_rows * b.heads_kv * p->tiles;
   const uint32_t warps = (uint32_t)sm_count * C::NW;
   const bool ragged = d->sel == nullptr && d->window == 0 && b.n_rows <= C::kMaxRagged;
@@ -139,8 +151,9 @@ int plan_attend(const nsa_cache_attend_desc* d, int sm_count, nsa_cache_attend_p
   }
   p->threads = C::NW * 32;
   p->smem_bytes = C::kSmem;
-  // (a team that shares a row of one query alone with many: eight warps join each query head's parts)
-  p->merge = !cut ? 0 : (uint64_t)most * warps / C::NW > (uint64_t)rows * most * 4 ? 8 : 1;
+  // Eight warps for each query head while the device has room for them at once (8 blocks an SM), else one: rows that are
+  // few have many parts.
+  p->merge = !cut ? 0 : (int64_t)b.n_rows * d->heads_q <= 8ll * sm_count ? 8 : 1;
   p->workspace_bytes = cut ? ((int64_t)(b.n_rows + 2) * 4 + 15) / 16 * 16 + (int64_t)teams * 2 * C::kPart * 4 : 16;
   return NSA_OK;
 }
@@ -153,19 +166,17 @@ int plan(const nsa_cache_attend_desc* d, int sm_count, nsa_cache_attend_plan_inf
     p->workspace_bytes = 16;
     return NSA_OK;
   }
-  return for_dims(d->batch.d_qk, d->batch.d_v, [&](auto dqk, auto dv) {
-    return plan_attend<CfgFor<decltype(dqk)::value, decltype(dv)::value>>(d, sm_count, p);
-  });
+  return for_config(d, [&](auto cfg) { return plan_attend<decltype(cfg)>(d, sm_count, p); });
 }
 
 std::mutex g_mu;
-uint32_t g_attr_done[nsa::host::kMaxDevices] = {};  // one bit for each head dim's attention kernel
+uint32_t g_attr_done[nsa::host::kMaxDevices] = {};  // one bit for each attention kernel
 
 template <class C>
 int launch_attend(const AttendArgs& a, const nsa_cache_attend_plan_info& p, int dev, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> lk(g_mu);
-    const uint32_t bit = 1u << ((C::DQK + C::DV) / 64);
+    const uint32_t bit = 1u << ((C::DQK + C::DV) / 64 * 2 + C::NH);
     if ((g_attr_done[dev] & bit) == 0) {
       const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&nsa::cache::attend_kernel<C>),
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
@@ -177,9 +188,20 @@ int launch_attend(const AttendArgs& a, const nsa_cache_attend_plan_info& p, int 
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.merge == 0) return done(e, "cache attention launch");
   const int64_t units = (int64_t)a.b.n_rows * a.hq;
-  if (p.merge == 1) nsa::cache::merge_kernel<C, 1><<<(unsigned)((units + 7) / 8), 256, 0, st>>>(a);
-  else nsa::cache::merge_kernel<C, 8><<<(unsigned)units, 256, 0, st>>>(a);
-  return done(cudaGetLastError(), "cache attention's merge launch");
+  cudaLaunchAttribute early;
+  memset(&early, 0, sizeof(early));
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(p.merge == 1 ? (units + 7) / 8 : units));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  e = p.merge == 1 ? cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 1>, a)
+                   : cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 8>, a);
+  return done(e, "cache attention's merge launch");
 }
 
 int attend(const nsa_cache_attend_desc* d, cudaStream_t st) {
@@ -228,9 +250,7 @@ int attend(const nsa_cache_attend_desc* d, cudaStream_t st) {
   a.err = d->err;
   a.wait_ns = (uint64_t)(d->timeout_ms > 0 ? d->timeout_ms : 2000) * 1000000u;
   a.stall = (d->debug_flags & NSA_DEBUG_STALL) != 0;
-  return for_dims(b.d_qk, b.d_v, [&](auto dqk, auto dv) {
-    return launch_attend<CfgFor<decltype(dqk)::value, decltype(dv)::value>>(a, p, dev, st);
-  });
+  return for_config(d, [&](auto cfg) { return launch_attend<decltype(cfg)>(a, p, dev, st); });
 }
 
 }  // namespace

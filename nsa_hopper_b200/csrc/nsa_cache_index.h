@@ -97,6 +97,7 @@ struct Split {
 };
 constexpr uint32_t kTeam = 8;    // largest team
 constexpr uint32_t kJoins = 4;   // what the second kernel costs, in slots of a warp
+constexpr uint32_t kLong = 16;   // slots of a warp from which on warps of their own are better than teams where rows are cut
 
 NSA_HD uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -105,11 +106,11 @@ NSA_HD Split split_line(uint32_t rows, uint32_t total, uint32_t longest, uint32_
   Split s;
   s.team = kTeam;
   while (s.team > 1 && ((uint64_t)rows * s.team > warps || longest <= s.team / 2)) s.team /= 2;
-  const uint32_t teams = warps / s.team, whole = ceil_div(rows, teams);
+  const uint32_t whole = ceil_div(rows, warps / s.team);
   const uint64_t uncut = (uint64_t)whole * ceil_div(longest, s.team);
-  const uint32_t even = ceil_div(total, teams);
-  s.cut = ceil_div(even, s.team) + kJoins < uncut;
-  s.share = s.cut ? even : whole;
+  s.cut = ceil_div(ceil_div(total, warps / s.team), s.team) + kJoins < uncut;
+  if (s.cut && total / warps >= kLong) s.team = 1;
+  s.share = s.cut ? ceil_div(total, warps / s.team) : whole;
   return s;
 }
 // Whether split_line can cut rows of at most `longest` slots at all.

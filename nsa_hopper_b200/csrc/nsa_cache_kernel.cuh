@@ -213,13 +213,15 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 // A key costs 9/16 (d_qk + d_v) bytes and 2 G (d_qk + d_v) operations: at d = 128 and G = 16 57 operations a
 // byte, so the floor is the cache's bytes from DRAM, provided that turning 4 bits into tensor-core operands keeps
 // up.  Hence the layout of the work: every warp is a worker of its own with a ring of page records in shared
-// memory (asynchronous copies), and codes go from there straight into the registers that the tensor core
-// reads (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  For that
+// memory (bulk copies), and codes go from there straight into the registers that the tensor core reads
+// (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  The cache is the A operand, S^T = K Q^T and
+// O^T = V^T P^T, so that 8 query heads (n) cost half of what 16 cost, and a decoded fragment serves both halves.  For that
 //   * the d axis of QK is permuted so that a thread's K fragments are d_qk / 4 consecutive codes of one key: one
 //     wide shared load, one conversion and one product with the scale for each pair, exact in fp16;
-//   * a thread's V fragments are d_v / 8 consecutive codes of four keys, which are interleaved two and two; P needs no
-//     exchange, its score registers are the A fragment.  The key axis is permuted (k index 2c, 2c + 1 of a tile of 8 is key
-//     c, 4 + (c ^ 1)) so that neither K's nor V's shared loads collide more than two ways on the record as it is.
+//   * a thread's V fragments are d_v / 8 consecutive codes of four keys, which are interleaved two and two; P^T takes
+//     its place by transposing 8 x 8 tiles between registers;
+//   * the key axis is permuted (rows 2q, 2q + 1 of a tile of 8 are keys q, 4 + (q ^ 1)) so that neither K's nor V's
+//     shared loads collide more than two ways on the record as it is.
 // Q has up to 8 (bf16) or 11 significant bits, so a power of two per row puts it into fp16 (below 2^-14 of the row's
 // largest to within 2^-25 of it).  P is rounded to fp16 (at most 2^-11 of each term): the sum of
 // its fp32 values is the divisor.  Scores, statistics and O are fp32.
@@ -241,7 +243,7 @@ struct AttendArgs {
   float* part;                   // partial results, 2 for each team
   uint32_t* starts;              // ragged line: slots before every row's (n_rows + 1), then the share of a team or 0 if no
                                  // row is cut; written by the first block for merge_kernel
-  int32_t hq, hkv, group, tiles; // tiles: 16-row tiles of a KV head's G query heads
+  int32_t hq, hkv, group, tiles; // tiles: of a KV head's G query heads
   int32_t n_sel, per, window;    // per: sub-blocks of a selection block
   int32_t slots;                 // slots of every row; 0: as many as it has sub-blocks (the ragged line)
   uint32_t warps;                // of the device
@@ -253,31 +255,32 @@ struct AttendArgs {
   int32_t stall;                 // (test) no copy is made, so that the waits run out
 };
 
-template <int DQK_, int DV_, int STAGES_, int ROUNDS_>
+template <int DQK_, int DV_, int NH_, int STAGES_, int ROUNDS_>
 struct AttendCfg {
-  static constexpr int DQK = DQK_, DV = DV_, NW = 8, STAGES = STAGES_, ROUNDS = ROUNDS_;
+  static constexpr int DQK = DQK_, DV = DV_, NH = NH_, NW = 8, STAGES = STAGES_, ROUNDS = ROUNDS_;
+  static constexpr int kHeads = 8 * NH;       // query heads of a tile
   static constexpr int kRecord = record_bytes(DQK, DV);
   static constexpr int kQueue = 40;           // resolved slots of a warp
   static constexpr int kMaxRagged = 512;      // rows of a ragged line
-  static constexpr int kPart = 16 * DV + 32;  // floats of a partial result: O, m, sum
-  static constexpr int kJoin = 16 * DV / ROUNDS + 64;  // floats of a warp in a team's join: O of a round, m, sum
+  static constexpr int kPart = kHeads * (DV + 2);              // floats of a partial result: O, m, sum
+  static constexpr int kJoin = kHeads * (DV / ROUNDS + 4);     // floats of a warp in a team's join: O of a round, m, sum, max
   static constexpr int kWarp = STAGES * (kRecord + 8) + kQueue * 16 + kJoin * 4;
   static constexpr int kSmem = NW * kWarp + (kMaxRagged + 1) * 4;
   static_assert(kSmem <= 232448, "227 KB of shared memory a block");
 };
 
-// Ring depth and rounds of the join for each head dim.  A warp holds O and Q of a 16-row tile and a page's scores in up to
-// 255 registers, so a block has 8 warps and an SM one block.
-template <int DQK, int DV>
+// Ring depth and rounds of the join for each head dim and tile (NH = 1: up to 8 query heads, 2: 16).  A warp holds O and Q
+// of a tile and a page's scores in up to 255 registers, so a block has 8 warps and an SM one block.
+template <int DQK, int DV, int NH>
 struct CfgFor;
-template <>
-struct CfgFor<64, 64> : AttendCfg<64, 64, 3, 1> {};
-template <>
-struct CfgFor<128, 64> : AttendCfg<128, 64, 3, 1> {};
-template <>
-struct CfgFor<128, 128> : AttendCfg<128, 128, 2, 1> {};
-template <>
-struct CfgFor<192, 128> : AttendCfg<192, 128, 2, 2> {};
+template <int NH>
+struct CfgFor<64, 64, NH> : AttendCfg<64, 64, NH, 3, 1> {};
+template <int NH>
+struct CfgFor<128, 64, NH> : AttendCfg<128, 64, NH, 3, 1> {};
+template <int NH>
+struct CfgFor<128, 128, NH> : AttendCfg<128, 128, NH, 2, 1> {};
+template <int NH>
+struct CfgFor<192, 128, NH> : AttendCfg<192, 128, NH, 2, NH> {};
 
 // A record's copy into shared memory, by one thread: the barrier's phase ends when all bytes are there.
 __device__ __forceinline__ void copy_record(void* dst, const uint8_t* src, int bytes, uint64_t* bar) {
@@ -419,7 +422,8 @@ __device__ __forceinline__ void store_lse(const AttendArgs& a, int64_t at, float
 template <class C>
 struct Worker {
   static constexpr int DQK = C::DQK, DV = C::DV;
-  static constexpr int NT = DV / 8;     // 8-wide output tiles
+  static constexpr int NH = C::NH;      // 8-wide tiles of query heads
+  static constexpr int MT = DV / 16;    // 16-high tiles of O^T
   static constexpr int KS = DQK / 16;   // k steps of QK
 
   // ---- the producer's side: rows and slots of the team's share, one after the other
@@ -434,13 +438,13 @@ struct Worker {
   // Called for every KV head and tile of a row; what depends on the row alone is worked out at the first.
   static __device__ __forceinline__ void enter_row(const AttendArgs& a, Cursor& c, const uint32_t* starts, bool same_row,
                                                    int lane) {
-    const int h = c.hm / a.tiles, g0 = c.hm % a.tiles * 16;
+    const int h = c.hm / a.tiles, g0 = c.hm % a.tiles * C::kHeads;
     if (a.sel != nullptr && a.n_sel <= 32)
       c.entry = lane < a.n_sel ? a.sel[((int64_t)c.n * a.hkv + h) * a.n_sel + lane] : -1;
     // the row's queries on their way into L2 (begin() loads them when its turn comes)
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)c.n * a.q_row + (int64_t)(h * a.group + g0) * a.q_head;
     constexpr int kLines = DQK / 64;
-    for (int i = lane; i < min(16, a.group - g0) * kLines; i += 32)
+    for (int i = lane; i < min(C::kHeads, a.group - g0) * kLines; i += 32)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i / kLines * a.q_head + i % kLines * 64));
     if (!same_row) {
       c.seq = sequence_of_warp(a.b, c.n, lane);
@@ -505,78 +509,91 @@ struct Worker {
   static __device__ __forceinline__ const uint8_t* record_of(const int4& e) {
     return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)e.y << 32 | (uint32_t)e.x);
   }
-  // ---- the consumer's side
-  float o[NT][4];
-  uint32_t q0[KS * 2], q1[KS * 2];  // Q of rows r and r + 8: d = c * DQK / 4 + 2i, + 1
-  float f0, f1, m0, m1;
-  float2 l0, l1;  // each thread's share of the sums
+  // ---- the consumer's side.  The thread's heads in tile h are 8 h + 2 c and 8 h + 2 c + 1 (c = lane % 4).
+  float o[MT][NH][4];      // O^T: d = (DV / 8) r + 2 j + e / 2 (r = lane / 4) of head 8 h + 2 c + e % 2
+  uint32_t q[NH][KS * 2];  // Q of head 8 h + r: d = c * DQK / 4 + 2 i, + 1
+  float2 f[NH], m[NH], l[NH];  // of the thread's heads: factor, maximum of the unscaled scores, the thread's share of the sum
 
   // A new row: its queries are asked for, then (when the copies of the first pages are under way) made ready.
   __device__ __forceinline__ void ask(const AttendArgs& a, uint32_t row, int lane) {
     const int rows_h = a.hkv * a.tiles, r = lane >> 2, c = lane & 3;
-    const int n = row / rows_h, hm = row % rows_h, h = hm / a.tiles, g = hm % a.tiles * 16 + r;
+    const int n = row / rows_h, hm = row % rows_h, h = hm / a.tiles, g = hm % a.tiles * C::kHeads + r;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)n * a.q_row + (int64_t)(h * a.group + g) * a.q_head +
                           c * (DQK / 4);
-    load_q(q0, g < a.group ? src : nullptr);
-    load_q(q1, g + 8 < a.group ? src + 8 * a.q_head : nullptr);
-  }
-  __device__ __forceinline__ void begin(const AttendArgs& a) {
-    scale_q(q0, a.q_half, f0);
-    scale_q(q1, a.q_half, f1);
-    // (finite and not 0, so that -inf stays -inf)
-    f0 = fminf(fmaxf(f0 * a.scale_log2, 1e-38f), 3e38f), f1 = fminf(fmaxf(f1 * a.scale_log2, 1e-38f), 3e38f);
-    m0 = m1 = -INFINITY;
-    l0 = l1 = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    for (int i = 0; i < NH; ++i) load_q(q[i], g + 8 * i < a.group ? src + 8 * i * a.q_head : nullptr);
+  }
+  __device__ __forceinline__ void begin(const AttendArgs& a, int lane) {
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      float factor;
+      scale_q(q[i], a.q_half, factor);
+      // (finite and not 0, so that -inf stays -inf)
+      factor = fminf(fmaxf(factor * a.scale_log2, 1e-38f), 3e38f);
+      const int from = (lane & 3) * 8;  // row r = 2 c
+      f[i] = make_float2(__shfl_sync(0xFFFFFFFFu, factor, from), __shfl_sync(0xFFFFFFFFu, factor, from + 4));
+      m[i] = make_float2(-INFINITY, -INFINITY);
+      l[i] = make_float2(0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < NH; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.0f;
   }
 
   // One page: keys [lo, lim) of its 64 are visible.
   __device__ __forceinline__ void page(uint8_t* rec, int lim, int lo, int lane) {
     const int r = lane >> 2, c = lane & 3;
     const bool whole = lim >= kPage && lo <= 0;
-    const int odd = 4 + (c ^ 1);                              // keys of this thread's columns in a tile of 8: c and odd
-    const int row = r & 1 ? 4 + (r >> 1 ^ 1) : r >> 1;        // key of K's fragment
+    const int row = r & 1 ? 4 + (r >> 1 ^ 1) : r >> 1;  // key of the tile's row r
     const uint8_t* krec = rec + row * (DQK / 2) + c * (DQK / 8);
     const uint8_t* kscales = rec + k_scale_at(DQK) + row * (DQK / kGroup) + c * (DQK / 64);
-    float s[8][4];
+    float s[4][NH][4];  // S^T: element e is key 16 t + row + 8 (e / 2) of head 8 h + 2 c + e % 2
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-      const uint8_t* codes = krec + 8 * i * (DQK / 2);
-      const uint8_t* scales = kscales + 8 * i * (DQK / kGroup);
-      uint32_t w[DQK / 32];
-      uint32_t sc[DQK / 64];
-      if constexpr (DQK == 128) {
-        const uint4 x = *reinterpret_cast<const uint4*>(codes);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-        const uint32_t both = *reinterpret_cast<const uint16_t*>(scales);
-        sc[0] = scale2(both & 0xFFu), sc[1] = scale2(both >> 8);
-      } else {
+    for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int g = 0; g < DQK / 64; ++g) {
-          const uint2 x = *reinterpret_cast<const uint2*>(codes + 8 * g);
-          w[2 * g] = x.x, w[2 * g + 1] = x.y;
-          sc[g] = scale2(scales[g]);
+      for (int h = 0; h < NH; ++h) s[t][h][0] = s[t][h][1] = s[t][h][2] = s[t][h][3] = 0.0f;
+      uint32_t w[2][DQK / 32], sc[2][DQK / 64];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint8_t* codes = krec + (16 * t + 8 * x) * (DQK / 2);
+        const uint8_t* scales = kscales + (16 * t + 8 * x) * (DQK / kGroup);
+        if constexpr (DQK == 128) {
+          const uint4 y = *reinterpret_cast<const uint4*>(codes);
+          w[x][0] = y.x, w[x][1] = y.y, w[x][2] = y.z, w[x][3] = y.w;
+          const uint32_t both = *reinterpret_cast<const uint16_t*>(scales);
+          sc[x][0] = scale2(both & 0xFFu), sc[x][1] = scale2(both >> 8);
+        } else {
+#pragma unroll
+          for (int g = 0; g < DQK / 64; ++g) {
+            const uint2 y = *reinterpret_cast<const uint2*>(codes + 8 * g);
+            w[x][2 * g] = y.x, w[x][2 * g + 1] = y.y;
+            sc[x][g] = scale2(scales[g]);
+          }
         }
       }
 #pragma unroll
       for (int j = 0; j < DQK / 32; ++j) {
-        const uint32_t z = sc[j / 2];
-        const uint32_t b0 = mul2(decode_byte<0>(w[j]), z), b1 = mul2(decode_byte<1>(w[j]), z);
-        const uint32_t b2 = mul2(decode_byte<2>(w[j]), z), b3 = mul2(decode_byte<3>(w[j]), z);
-        mma(s[i], q0[4 * j], q1[4 * j], q0[4 * j + 1], q1[4 * j + 1], b0, b1);
-        mma(s[i], q0[4 * j + 2], q1[4 * j + 2], q0[4 * j + 3], q1[4 * j + 3], b2, b3);
+        const uint32_t z0 = sc[0][j / 2], z1 = sc[1][j / 2];
+        const uint32_t a0 = mul2(decode_byte<0>(w[0][j]), z0), a1 = mul2(decode_byte<0>(w[1][j]), z1);
+        const uint32_t a2 = mul2(decode_byte<1>(w[0][j]), z0), a3 = mul2(decode_byte<1>(w[1][j]), z1);
+        const uint32_t b0 = mul2(decode_byte<2>(w[0][j]), z0), b1 = mul2(decode_byte<2>(w[1][j]), z1);
+        const uint32_t b2 = mul2(decode_byte<3>(w[0][j]), z0), b3 = mul2(decode_byte<3>(w[1][j]), z1);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) mma(s[t][h], a0, a1, a2, a3, q[h][4 * j], q[h][4 * j + 1]);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) mma(s[t][h], b0, b1, b2, b3, q[h][4 * j + 2], q[h][4 * j + 3]);
       }
     }
-    // score i, element e is key 8 i + (c or odd, by e % 2) of row r + 8 (e / 2)
     if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = 8 * i + (e ? odd : c);
-          if (key < lo || key >= lim) s[i][e] = s[i][e + 2] = -INFINITY;
+        for (int x = 0; x < 2; ++x) {
+          const int key = 16 * t + 8 * x + row;
+          if (key < lo || key >= lim)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) s[t][h][2 * x] = s[t][h][2 * x + 1] = -INFINITY;
         }
       // what stands in the other keys' places may be anything, NaN too: with a scale of 0 their values are 0
 #pragma unroll
@@ -589,35 +606,60 @@ struct Worker {
       ptx::fence_proxy_async_smem();  // (before the record that is copied here next)
       __syncwarp();
     }
-    // softmax: the maximum m of the unscaled scores, f > 0 turns them into powers of two
-    float t0 = m0, t1 = m1;
+    // Softmax against m, a maximum of the unscaled scores so far (f > 0 turns them into powers of two).  It is raised, and O
+    // and the sums with it, when a score is more than 2^kSlack above it: until then P is at most 2^kSlack, and neither its
+    // roundings nor the result depend on m.  So most pages need no exchange between the threads that share a head.
+    constexpr float kSlack = 8.0f;
+    uint32_t p[4][NH][2];  // P^T as the tensor core takes it: fp16 pairs of keys (of rows 2c, 2c + 1, and 8 more) of head 8 h + r
+    float2 top[NH], u[NH];
+    bool grown = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t0 = max3(t0, s[i][0], s[i][1]), t1 = max3(t1, s[i][2], s[i][3]);
-    t0 = fmaxf(t0, __shfl_xor_sync(0xFFFFFFFFu, t0, 1)), t1 = fmaxf(t1, __shfl_xor_sync(0xFFFFFFFFu, t1, 1));
-    t0 = fmaxf(t0, __shfl_xor_sync(0xFFFFFFFFu, t0, 2)), t1 = fmaxf(t1, __shfl_xor_sync(0xFFFFFFFFu, t1, 2));
-    const float u0 = t0 == -INFINITY ? 0.0f : t0 * f0, u1 = t1 == -INFINITY ? 0.0f : t1 * f1;
-    if (__any_sync(0xFFFFFFFFu, t0 > m0 || t1 > m1)) {
-      const float a0 = exp2_fast(m0 * f0 - u0), a1 = exp2_fast(m1 * f1 - u1);
-      l0.x *= a0, l0.y *= a0, l1.x *= a1, l1.y *= a1;
+    for (int h = 0; h < NH; ++h) {
+      top[h] = make_float2(fmaxf(s[0][h][0], s[0][h][2]), fmaxf(s[0][h][1], s[0][h][3]));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) o[i][0] *= a0, o[i][1] *= a0, o[i][2] *= a1, o[i][3] *= a1;
-      m0 = t0, m1 = t1;
+      for (int t = 1; t < 4; ++t)
+        top[h].x = max3(top[h].x, s[t][h][0], s[t][h][2]), top[h].y = max3(top[h].y, s[t][h][1], s[t][h][3]);
+      // (also where m still is -inf and a score is not; -inf - -inf is NaN, which is not greater)
+      grown = grown || (top[h].x - m[h].x) * f[h].x > kSlack || (top[h].y - m[h].y) * f[h].y > kSlack;
     }
-    uint32_t p[8][2];  // fp16: rows r and r + 8
+    if (__any_sync(0xFFFFFFFFu, grown)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float2 x = fma2(make_float2(s[i][0], s[i][1]), make_float2(f0, f0), make_float2(-u0, -u0));
-      float2 y = fma2(make_float2(s[i][2], s[i][3]), make_float2(f1, f1), make_float2(-u1, -u1));
-      x = make_float2(exp2_fast(x.x), exp2_fast(x.y)), y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-      l0 = add2(l0, x), l1 = add2(l1, y);
-      p[i][0] = pack_half(x.x, x.y), p[i][1] = pack_half(y.x, y.y);
+      for (int h = 0; h < NH; ++h) {
+        top[h] = make_float2(fmaxf(top[h].x, m[h].x), fmaxf(top[h].y, m[h].y));
+#pragma unroll
+        for (int k = 4; k < 32; k *= 2) {
+          top[h].x = fmaxf(top[h].x, __shfl_xor_sync(0xFFFFFFFFu, top[h].x, k));
+          top[h].y = fmaxf(top[h].y, __shfl_xor_sync(0xFFFFFFFFu, top[h].y, k));
+        }
+        // (where m is -inf, O and the sums are zeros or NaN, and stay)
+        const float2 k = make_float2(m[h].x == -INFINITY ? 1.0f : exp2_fast((m[h].x - top[h].x) * f[h].x),
+                                     m[h].y == -INFINITY ? 1.0f : exp2_fast((m[h].y - top[h].y) * f[h].y));
+        l[h] = mul2(l[h], k);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) o[j][h][0] *= k.x, o[j][h][1] *= k.y, o[j][h][2] *= k.x, o[j][h][3] *= k.y;
+        m[h] = top[h];
+      }
     }
-    // PV; output tile j, element e is d = (2c + e % 2) * NT + j of row r + 8 (e / 2)
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+      u[h] = make_float2(m[h].x == -INFINITY ? 0.0f : m[h].x * f[h].x, m[h].y == -INFINITY ? 0.0f : m[h].y * f[h].y);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float2 y = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-u[h].x, -u[h].y));
+          y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+          l[h] = add2(l[h], y);
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[t][h][x]) : "r"(pack_half(y.x, y.y)));
+        }
+    // PV
+    const int odd = 4 + (c ^ 1);  // keys of the tile's rows 2c and 2c + 1: c and odd
     const uint8_t* vrec = rec + v_code_at(DQK) + r * (DV / 16);
     const uint8_t* vscales = rec + v_scale_at(DQK, DV) + (DV == 128 ? r : r >> 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const uint32_t a0 = p[2 * t][0], a1 = p[2 * t][1], a2 = p[2 * t + 1][0], a3 = p[2 * t + 1][1];
       uint32_t w[4][DV / 64], z[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -638,108 +680,123 @@ struct Worker {
         constexpr uint32_t kLow = 0x0F0F0F0Fu;
         const uint32_t x0 = (w[0][j] & kLow) | ((w[1][j] << 4) & ~kLow), x1 = (w[2][j] & kLow) | ((w[3][j] << 4) & ~kLow);
         const uint32_t y0 = ((w[0][j] >> 4) & kLow) | (w[1][j] & ~kLow), y1 = ((w[2][j] >> 4) & kLow) | (w[3][j] & ~kLow);
-        mma(o[8 * j + 0], a0, a1, a2, a3, mul2(decode_byte<0>(x0), z0), mul2(decode_byte<0>(x1), z1));
-        mma(o[8 * j + 1], a0, a1, a2, a3, mul2(decode_byte<0>(y0), z0), mul2(decode_byte<0>(y1), z1));
-        mma(o[8 * j + 2], a0, a1, a2, a3, mul2(decode_byte<1>(x0), z0), mul2(decode_byte<1>(x1), z1));
-        mma(o[8 * j + 3], a0, a1, a2, a3, mul2(decode_byte<1>(y0), z0), mul2(decode_byte<1>(y1), z1));
-        mma(o[8 * j + 4], a0, a1, a2, a3, mul2(decode_byte<2>(x0), z0), mul2(decode_byte<2>(x1), z1));
-        mma(o[8 * j + 5], a0, a1, a2, a3, mul2(decode_byte<2>(y0), z0), mul2(decode_byte<2>(y1), z1));
-        mma(o[8 * j + 6], a0, a1, a2, a3, mul2(decode_byte<3>(x0), z0), mul2(decode_byte<3>(x1), z1));
-        mma(o[8 * j + 7], a0, a1, a2, a3, mul2(decode_byte<3>(y0), z0), mul2(decode_byte<3>(y1), z1));
+        pv<0>(o[4 * j + 0], x0, y0, x1, y1, z0, z1, p[t]);
+        pv<1>(o[4 * j + 1], x0, y0, x1, y1, z0, z1, p[t]);
+        pv<2>(o[4 * j + 2], x0, y0, x1, y1, z0, z1, p[t]);
+        pv<3>(o[4 * j + 3], x0, y0, x1, y1, z0, z1, p[t]);
       }
     }
+  }
+  template <int I>
+  static __device__ __forceinline__ void pv(float (&acc)[NH][4], uint32_t x0, uint32_t y0, uint32_t x1, uint32_t y1, uint32_t z0,
+                                            uint32_t z1, const uint32_t (&p)[NH][2]) {
+    const uint32_t a0 = mul2(decode_byte<I>(x0), z0), a1 = mul2(decode_byte<I>(y0), z0);
+    const uint32_t a2 = mul2(decode_byte<I>(x1), z1), a3 = mul2(decode_byte<I>(y1), z1);
+#pragma unroll
+    for (int h = 0; h < NH; ++h) mma(acc[h], a0, a1, a2, a3, p[h][0], p[h][1]);
+  }
+
+  // Four neighbouring values of d (from (DV / 8) r + 4 i on) of the thread's head 8 h + 2 c + e.
+  __device__ __forceinline__ float4 piece(int h, int e, int i) const {
+    return make_float4(o[2 * i][h][e], o[2 * i][h][2 + e], o[2 * i + 1][h][e], o[2 * i + 1][h][2 + e]);
   }
 
   // The row's result: whole, or this team's part of it (`part` not null).  `join`: the team's warps' join buffers.
   __device__ __forceinline__ void finish(const AttendArgs& a, uint32_t row, float* part, float* join, int team, int turn,
                                          int barrier, int lane) {
+    constexpr int kHeads = C::kHeads, PIECES = DV / 32;  // pieces of a thread and head
     const int rows_h = a.hkv * a.tiles, r = lane >> 2, c = lane & 3;
-    float n0 = l0.x + l0.y, n1 = l1.x + l1.y;
-    n0 += __shfl_xor_sync(0xFFFFFFFFu, n0, 1), n1 += __shfl_xor_sync(0xFFFFFFFFu, n1, 1);
-    n0 += __shfl_xor_sync(0xFFFFFFFFu, n0, 2), n1 += __shfl_xor_sync(0xFFFFFFFFu, n1, 2);
-    float e0 = m0 == -INFINITY ? m0 : m0 * f0, e1 = m1 == -INFINITY ? m1 : m1 * f1;  // as powers of two
-    const int n = row / rows_h, hm = row % rows_h, g0 = hm % a.tiles * 16;
+    const int n = row / rows_h, hm = row % rows_h, g0 = hm % a.tiles * kHeads;
     const int64_t at0 = (int64_t)n * a.hq + hm / a.tiles * a.group + g0;  // the tile's first query head
-    const int used = min(16, a.group - g0);
+    const int used = min(kHeads, a.group - g0);
     const bool left = part == nullptr && !a.fill && sequence_of_warp(a.b, n, lane) < 0;  // a row to leave as it was
+    const float weight = a.weight != nullptr && part == nullptr ? *a.weight : 1.0f;
+    float sum[NH][2], top[NH][2];  // top: as a power of two
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      sum[h][0] = l[h].x, sum[h][1] = l[h].y;
+      top[h][0] = m[h].x == -INFINITY ? m[h].x : m[h].x * f[h].x, top[h][1] = m[h].y == -INFINITY ? m[h].y : m[h].y * f[h].y;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 4; k < 32; k *= 2) sum[h][e] += __shfl_xor_sync(0xFFFFFFFFu, sum[h][e], k);
+    }
     if (team == 1) {
-      if (part != nullptr) {
-        if (c == 0) {
-          part[16 * DV + r] = e0, part[16 * DV + r + 8] = e1;
-          part[16 * DV + 16 + r] = n0, part[16 * DV + 16 + r + 8] = n1;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float4* to = reinterpret_cast<float4*>(part + (r + 8 * (e / 2)) * DV + (2 * c + e % 2) * NT);
-#pragma unroll
-          for (int j = 0; j < NT / 4; ++j) to[j] = make_float4(o[4 * j][e], o[4 * j + 1][e], o[4 * j + 2][e], o[4 * j + 3][e]);
-        }
-        return;
-      }
       if (left) return;
-      const float w = a.weight ? *a.weight : 1.0f;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (r + 8 * half >= used) continue;
-        const float l = half ? n1 : n0, k = l != 0.0f ? w / l : 0.0f;
-        const int64_t at = at0 + r + 8 * half;
-        if (c == 0) store_lse(a, at, half ? e1 : e0, l);
+      for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+          const int x = 8 * h + 2 * c + e;
+          if (x >= used) continue;
+          if (part != nullptr) {
+            if (r == 0) part[kHeads * DV + x] = top[h][e], part[kHeads * (DV + 1) + x] = sum[h][e];
 #pragma unroll
-          for (int j = 0; j < NT / 4; ++j)
-            store4<DV>(a, at, (2 * c + e) * NT + 4 * j,
-                       make_float4(o[4 * j][2 * half + e], o[4 * j + 1][2 * half + e], o[4 * j + 2][2 * half + e],
-                                   o[4 * j + 3][2 * half + e]), k);
-      }
+            for (int i = 0; i < PIECES; ++i) reinterpret_cast<float4*>(part + x * DV + r * (DV / 8))[i] = piece(h, e, i);
+          } else {
+            if (r == 0) store_lse(a, at0 + x, top[h][e], sum[h][e]);
+            const float k = sum[h][e] != 0.0f ? weight / sum[h][e] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) store4<DV>(a, at0 + x, r * (DV / 8) + 4 * i, piece(h, e, i), k);
+          }
+        }
       return;
     }
     // Join: maxima, then every warp's O against the common maximum, some columns a round.  The 16-byte pieces of a row
     // are exchanged so that neither side meets bank conflicts.
-    constexpr int NTR = NT / C::ROUNDS, CS = NTR / 4, kMl = 16 * DV / C::ROUNDS;
+    constexpr int CS = PIECES / C::ROUNDS, kMl = kHeads * DV / C::ROUNDS;
     float* mine = join + turn * C::kJoin;
-    if (c == 0) mine[kMl + r] = e0, mine[kMl + r + 8] = e1;
+    if (r == 0)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) mine[kMl + 8 * h + 2 * c] = top[h][0], mine[kMl + 8 * h + 2 * c + 1] = top[h][1];
     named_barrier(barrier, team * 32);
-    float t0 = -INFINITY, t1 = -INFINITY;
-    for (int w = 0; w < team; ++w)
-      t0 = fmaxf(t0, join[w * C::kJoin + kMl + r]), t1 = fmaxf(t1, join[w * C::kJoin + kMl + r + 8]);
-    e0 = exp2_fast(e0 - (t0 == -INFINITY ? 0.0f : t0)), e1 = exp2_fast(e1 - (t1 == -INFINITY ? 0.0f : t1));
-    if (c == 0) mine[kMl + 16 + r] = n0 * e0, mine[kMl + 16 + r + 8] = n1 * e1, mine[kMl + 32 + r] = t0, mine[kMl + 40 + r] = t1;
-    const float weight = a.weight && part == nullptr ? *a.weight : 1.0f;
+    float k[NH][2];
 #pragma unroll
-    for (int q = 0; q < C::ROUNDS; ++q) {
-      if (q > 0) named_barrier(barrier, team * 32);
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float k = e < 2 ? e0 : e1;
-        float4* to = reinterpret_cast<float4*>(mine) + (r + 8 * (e / 2)) * (8 * CS);
-#pragma unroll
-        for (int j = 0; j < CS; ++j) {
-          const int t = q * NTR + 4 * j;
-          to[((2 * c + e % 2) * CS + j) ^ (((r & 1) << 2) + c)] =
-              make_float4(o[t][e] * k, o[t + 1][e] * k, o[t + 2][e] * k, o[t + 3][e] * k);
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int x = 8 * h + 2 * c + e;
+        float common = -INFINITY;
+        for (int w = 0; w < team; ++w) common = fmaxf(common, join[w * C::kJoin + kMl + x]);
+        k[h][e] = exp2_fast(top[h][e] - (common == -INFINITY ? 0.0f : common));
+        if (r == 0) mine[kMl + kHeads + x] = sum[h][e] * k[h][e], mine[kMl + 2 * kHeads + x] = common;
       }
+    const int swap = CS == 4 ? c : (c & 1) | (c & 2) << 1;
+#pragma unroll
+    for (int t = 0; t < C::ROUNDS; ++t) {
+      if (t > 0) named_barrier(barrier, team * 32);
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float4* to = reinterpret_cast<float4*>(mine) + (8 * h + 2 * c + e) * (8 * CS);
+#pragma unroll
+          for (int i = 0; i < CS; ++i) {
+            float4 v = piece(h, e, t * CS + i);
+            v.x *= k[h][e], v.y *= k[h][e], v.z *= k[h][e], v.w *= k[h][e];
+            to[(r * CS + i) ^ swap] = v;
+          }
+        }
       named_barrier(barrier, team * 32);
-      for (int i = turn * 32 + lane; i < 16 * 8 * CS; i += team * 32) {
-        const int x = i / (8 * CS), k = i % (8 * CS), d = k / CS * NT + q * NTR + k % CS * 4;
+      for (int i = turn * 32 + lane; i < kHeads * 8 * CS; i += team * 32) {
+        const int x = i / (8 * CS), at = i % (8 * CS), d = at / CS * (DV / 8) + (t * CS + at % CS) * 4;
         if (x >= used || left) continue;
-        const int place = x * (8 * CS) + (k ^ (((x & 1) << 2) + k / (2 * CS)));
+        const int y = x >> 1 & 3, place = x * (8 * CS) + (at ^ (CS == 4 ? y : (y & 1) | (y & 2) << 1));
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
+        float all = 0.0f;
         for (int w = 0; w < team; ++w) {
           const float* from = join + w * C::kJoin;
-          const float4 y = reinterpret_cast<const float4*>(from)[place];
-          v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-          l += from[kMl + 16 + x];
+          const float4 z = reinterpret_cast<const float4*>(from)[place];
+          v.x += z.x, v.y += z.y, v.z += z.z, v.w += z.w;
+          all += from[kMl + kHeads + x];
         }
-        const float m = mine[kMl + 32 + x];
+        const float common = mine[kMl + 2 * kHeads + x];
         if (part != nullptr) {
           *reinterpret_cast<float4*>(part + x * DV + d) = v;
-          if (k == 0 && q == 0) part[16 * DV + x] = m, part[16 * DV + 16 + x] = l;
+          if (at == 0 && t == 0) part[kHeads * DV + x] = common, part[kHeads * (DV + 1) + x] = all;
         } else {
-          store4<DV>(a, at0 + x, d, v, l != 0.0f ? weight / l : 0.0f);
-          if (k == 0 && q == 0) store_lse(a, at0 + x, m, l);
+          store4<DV>(a, at0 + x, d, v, all != 0.0f ? weight / all : 0.0f);
+          if (at == 0 && t == 0) store_lse(a, at0 + x, common, all);
         }
       }
     }
@@ -756,10 +813,16 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   int4* queue = reinterpret_cast<int4*>(join + C::NW * C::kJoin) + warp * C::kQueue;
   uint64_t* bars = reinterpret_cast<uint64_t*>(queue + (C::NW - warp) * C::kQueue) + warp * C::STAGES;
   uint32_t* starts = reinterpret_cast<uint32_t*>(smem + C::NW * C::kWarp);
+  asm volatile("griddepcontrol.launch_dependents;");  // (merge_kernel, whose blocks then wait for the end of this one)
   const uint32_t rows_h = a.hkv * a.tiles, rows = a.b.n_rows * rows_h;
   uint32_t total = rows * a.slots;
   Split split = a.split;
-  if (a.slots == 0) {  // the ragged line: every block counts the slots before each row (n_rows <= kMaxRagged)
+  if (a.slots == 0) {
+    // the page table on its way into L2 (128 bytes a thread: all of an ordinary one)
+    const int64_t line128 = ((int64_t)blockIdx.x * (C::NW * 32) + threadIdx.x) * 32;
+    if (line128 < (int64_t)(a.b.n_seqs - 1) * a.b.page_row + a.b.width)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b.pages + line128));
+    // the ragged line: every block counts the slots before each row (n_rows <= kMaxRagged)
     for (int n = threadIdx.x; n < a.b.n_rows; n += C::NW * 32) {
       const int seq = sequence_of(a.b, n), pos = seq < 0 ? -1 : position_of(a.b, seq, n);
       starts[n + 1] = running_slots(pos < 0 ? 0 : first_key(pos, a.window), keys_up_to(a.b, pos));
@@ -849,7 +912,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   };
   // the ring holds STAGES records: STAGES - 1 on their way while one is worked on
   for (int i = 0; i < C::STAGES - 1; ++i) issue();
-  w.begin(a);
+  w.begin(a, lane);
   bool fresh = false, first_row = true;
   while (head < issued) {
     issue();
@@ -857,7 +920,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     const int stage = head % C::STAGES;
     if (fresh) {
       w.ask(a, (uint32_t)e.w >> 1, lane);
-      w.begin(a);
+      w.begin(a, lane);
     }
     fresh = e.w & 1;
     if (Worker<C>::record_of(e) != nullptr) {
@@ -866,7 +929,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
         phases ^= 1u << stage, flying &= ~(1u << stage);
         w.page(ring + stage * C::kRecord, e.z >> 8, e.z & 255, lane);
       } else {
-        w.l0.x = w.l1.x = __int_as_float(0x7FFFFFFF);
+        for (int i = 0; i < C::NH; ++i) w.l[i].x = w.l[i].y = __int_as_float(0x7FFFFFFF);
       }
     }
     if (fresh) {
@@ -888,18 +951,20 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
 }
 
 // Joins the parts of the rows that were cut, in the order of the line.  WPH warps share a row's query head:
-// 1 where a row has a few parts, 8 where one row is cut over hundreds of workers.
+// 1 where a row has a few parts, 8 where one row is cut over many teams.  Starts while attend_kernel still runs
+// (programmatic launch) and waits for its end before it reads anything.
 template <class C, int WPH>
 __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
   constexpr int DV = C::DV, V4 = DV / 4;
   __shared__ float shared_o[8][DV];
   __shared__ float shared_ml[8][2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rows_h = a.hkv * a.tiles;
   const int64_t unit = WPH == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;  // (row, query head)
   if (unit >= (int64_t)a.b.n_rows * a.hq) return;
-  const int n = unit / a.hq, hq = unit % a.hq, h = hq / a.group, g = hq % a.group;
-  const uint32_t hm = h * a.tiles + g / 16;
+  const int n = unit / a.hq, hq = unit % a.hq, h = hq / a.group, g = hq % a.group, x = g % C::kHeads;
+  const uint32_t hm = h * a.tiles + g / C::kHeads;
   uint32_t start, len, per = a.split.share;
   if (a.slots) {
     len = a.slots, start = ((uint32_t)n * rows_h + hm) * len;
@@ -909,66 +974,59 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
     per = a.starts[a.b.n_rows + 1];
   }
   if (per == 0) return;
-  const uint32_t w0 = start / per, w1 = (start + len - 1) / per;
-  if (w0 == w1) return;  // the row was not cut
+  const uint32_t w0 = start / per, parts = (start + len - 1) / per - w0 + 1;
+  if (parts == 1) return;  // the row was not cut
   if (!a.fill && sequence_of(a.b, n) < 0) return;
-  // the first team has the row as its last, the others as their first
-  auto part_of = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 ? 1 : 0)) * C::kPart; };
-  const int mine = WPH == 1 ? 0 : warp;
-  float m = -INFINITY;
-  for (uint32_t w = w0 + mine * 32 + lane; w <= w1; w += 32 * WPH) m = fmaxf(m, part_of(w)[16 * DV + g % 16]);
+  // the first team has the row as its last, the others as their first; this warp has every WPH-th part
+  auto part_of = [&](uint32_t i) { return a.part + ((size_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * C::kPart; };
+  const uint32_t mine = WPH == 1 ? 0 : warp;
+  float m = -INFINITY, l = 0.0f;  // (a maximum is never NaN: fmaxf leaves NaN out; where it is -inf the sums are zeros, or
+                                  // NaN, which stays)
+  for (uint32_t i = mine + WPH * lane; i < parts; i += WPH * 32) m = fmaxf(m, part_of(i)[C::kHeads * DV + x]);
 #pragma unroll
   for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, k));
-  const float u = m == -INFINITY ? 0.0f : m;  // (of this warp's parts)
-  float l = 0.0f;
-  float4 acc[(V4 + 31) / 32];
-#pragma unroll
-  for (int i = 0; i < (V4 + 31) / 32; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (uint32_t w = w0 + mine * 32; w <= w1; w += 32 * WPH)
-#pragma unroll 4
-    for (uint32_t x = w; x < min(w + 32, w1 + 1); ++x) {
-      const float* p = part_of(x);
-      const float f = exp2_fast(p[16 * DV + g % 16] - u);
-      l += p[16 * DV + 16 + g % 16] * f;
-#pragma unroll
-      for (int i = 0; i < (V4 + 31) / 32; ++i)
-        if (lane + 32 * i < V4) {
-          const float4 v = reinterpret_cast<const float4*>(p + g % 16 * DV)[lane + 32 * i];
-          acc[i].x += v.x * f, acc[i].y += v.y * f, acc[i].z += v.z * f, acc[i].w += v.w * f;
-        }
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // values 4 lane to 4 lane + 3 (lane < V4)
+  for (uint32_t i0 = mine; i0 < parts; i0 += WPH * 32) {
+    const uint32_t own = i0 + WPH * lane;
+    float factor = 0.0f;
+    if (own < parts) {
+      const float* p = part_of(own) + C::kHeads * DV + x;
+      factor = exp2_fast(p[0] - (m == -INFINITY ? 0.0f : m));
+      l += p[C::kHeads] * factor;
     }
-  float top = m;
-  if (WPH > 1) {
+    const int count = min(32u, (parts - i0 + WPH - 1) / WPH);
+#pragma unroll 8
+    for (int k = 0; k < count; ++k) {
+      const float f = __shfl_sync(0xFFFFFFFFu, factor, k);
+      if (lane < V4) {
+        const float4 v = reinterpret_cast<const float4*>(part_of(i0 + WPH * k) + x * DV)[lane];
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
+    }
+  }
 #pragma unroll
-    for (int i = 0; i < (V4 + 31) / 32; ++i)
-      if (lane + 32 * i < V4) reinterpret_cast<float4*>(shared_o[warp])[lane + 32 * i] = acc[i];
+  for (int k = 16; k > 0; k /= 2) l += __shfl_xor_sync(0xFFFFFFFFu, l, k);
+  if (WPH > 1) {
+    if (lane < V4) reinterpret_cast<float4*>(shared_o[warp])[lane] = acc;
     if (lane == 0) shared_ml[warp][0] = m, shared_ml[warp][1] = l;
     __syncthreads();
     if (warp != 0) return;
 #pragma unroll
-    for (int k = 0; k < WPH; ++k) top = fmaxf(top, shared_ml[k][0]);
-    const float v = top == -INFINITY ? 0.0f : top;
+    for (int k = 0; k < WPH; ++k) m = fmaxf(m, shared_ml[k][0]);
     l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < (V4 + 31) / 32; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < WPH; ++k) {
-      // (a maximum is never NaN: fmaxf leaves NaN out; where it is -inf the sums are zeros, or NaN, which stays)
-      const float mk = shared_ml[k][0], f = mk == -INFINITY ? 1.0f : exp2_fast(mk - v);
+      const float f = shared_ml[k][0] == -INFINITY ? 1.0f : exp2_fast(shared_ml[k][0] - m);
       l += shared_ml[k][1] * f;
-#pragma unroll
-      for (int i = 0; i < (V4 + 31) / 32; ++i)
-        if (lane + 32 * i < V4) {
-          const float4 x = reinterpret_cast<const float4*>(shared_o[k])[lane + 32 * i];
-          acc[i].x += x.x * f, acc[i].y += x.y * f, acc[i].z += x.z * f, acc[i].w += x.w * f;
-        }
+      if (lane < V4) {
+        const float4 v = reinterpret_cast<const float4*>(shared_o[k])[lane];
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
     }
   }
-  const float k = l != 0.0f ? (a.weight ? *a.weight : 1.0f) / l : 0.0f;
-  if (lane == 0) store_lse(a, unit, top, l);
-#pragma unroll
-  for (int i = 0; i < (V4 + 31) / 32; ++i)
-    if (lane + 32 * i < V4) store4<DV>(a, unit, 4 * (lane + 32 * i), acc[i], k);
+  if (lane == 0) store_lse(a, unit, m, l);
+  if (lane < V4) store4<DV>(a, unit, 4 * lane, acc, l != 0.0f ? (a.weight ? *a.weight : 1.0f) / l : 0.0f);
 }
 
 }  // namespace cache

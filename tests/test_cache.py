@@ -128,9 +128,9 @@ def test_shares_cover_the_line(index):
             for shorter in (x for x in {1, 2, 3, 5, longest // 2, longest - 1} if 0 < x < longest):
                 index.split(rows, min(total, rows * shorter), shorter, warps, out)
                 assert not out[2]
-        # what the split costs is at most what either way costs
-        slots = -(-share // team) + 4 if cut else share * -(-longest // team)
-        assert slots <= -(-rows // teams) * -(-longest // team)
+        # a warp never gets more than it would with whole rows
+        whole = min(-(-rows // (warps // t)) * -(-longest // t) for t in (1, 2, 4, 8) if rows * t <= warps or t == 1)
+        assert (-(-share // team) if cut else share * -(-longest // team)) <= max(whole, 1)
 
 
 def test_record_bytes():
