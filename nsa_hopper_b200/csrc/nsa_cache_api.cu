@@ -277,10 +277,10 @@ int nsa_cache_write(const nsa_cache_batch* b, const void* k, const void* v, int6
   if (rc != NSA_OK) return rc;
   const nsa::cache::WriteArgs a = {device_batch(b), {k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride},
                                    static_cast<uint8_t*>(b->cache), page_stride_of(b), b->heads_kv, in_dtype == NSA_DTYPE_F16};
-  const int64_t groups = (int64_t)b->n_rows * b->heads_kv * std::max(b->d_qk, b->d_v) / nsa::cache::kGroup;
+  const int64_t threads = (int64_t)b->n_rows * b->heads_kv * std::max(b->d_qk, b->d_v) / (2 * nsa::cache::kGroup);
   return for_dims(b->d_qk, b->d_v, [&](auto dqk, auto dv) {
     nsa::cache::write_kernel<decltype(dqk)::value, decltype(dv)::value>
-        <<<dim3((unsigned)((groups + 255) / 256), 2), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+        <<<dim3((unsigned)((threads + 255) / 256), 2), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     return done(cudaGetLastError(), "cache write launch");
   });
 }

@@ -22,6 +22,33 @@ namespace cache {
 
 enum : int { kBf16 = 0, kF32 = 1, kF16 = 2 };
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // ------------------------------------------------------------------ 4-bit conversions
 // Two codes of byte I of `w` as fp16 pair (low nibble in the low half).
 template <int I>
@@ -58,8 +85,11 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 // A scale byte in both halves of an fp16 pair.
 __device__ __forceinline__ uint32_t scale2(uint32_t byte) { return byte * 0x00800080u; }
 
-// The scale byte of a group from max|x| / 6: nearest, ties to even, at most 10240 (0xE2).
-__device__ __forceinline__ uint32_t scale_byte(float raw) {
+// The scale byte of a group with the largest value amax: the scale nearest to amax / 6, ties to even, at most 10240 (0xE2).
+// The product with 1/6 is off by 2^-23 of itself; rounded to 17 bits it is the quotient again where that has few bits (the
+// ties), and amax's 8 or 11 bits keep every other quotient 2^-12 of itself away from a tie.
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+  const float raw = __uint_as_float((__float_as_uint(amax * 0.16666667f) + 0x40u) & ~0x7Fu);
   if (raw >= 6.103515625e-05f) {  // 2^-14, the smallest normal scale
     const uint32_t b = __float_as_uint(raw);
     return min(((b + 0x7FFFFu + ((b >> 20) & 1u)) >> 20) - 896u, 226u);
@@ -68,12 +98,13 @@ __device__ __forceinline__ uint32_t scale_byte(float raw) {
 }
 
 // ------------------------------------------------------------------ writing
-// One thread quantises one group: 32 bytes in, 8 bytes of codes and a byte of scale out, so the kernel is
-// bound by memory (2.56 bytes a value).  x / s must fall on the right side of the borders between codes (0.25,
-// 0.75, ... 5), and exactly on one where it is one, for ties to go to the even code.  x (1 / s) has an error of
-// 2^-24 and would miss some of the ties; fma(x, 1 / s, 192) - 192 rounds the quotient to a multiple of 2^-16
-// instead.  A border is such a multiple, and with the 8 or 11 significant bits of x no other quotient is nearer
-// to a border t than t 2^-11, so the codes are those of a true division.
+// One thread quantises two neighbouring groups of a row and head: 64 bytes in, 16 bytes of codes and two of scales out, 2.56
+// bytes a value, and few enough instructions (with one group a thread the look-up of the row's place took as many as the
+// arithmetic, and the kernel 41 us where it now takes 35, for 65536 tokens of 4 heads with d = 128) to be bound by memory.
+// x / s must fall on the right side of the borders between codes (0.25, 0.75, ... 5), and exactly on one where it is one, for
+// ties to go to the even code.  x (1 / s) has an error of 2^-22 and would miss some of the ties; fma(x, 1 / s, 192) - 192
+// rounds the quotient to a multiple of 2^-16 instead.  A border is such a multiple, and with the 8 or 11 significant bits of x
+// no other quotient is nearer to a border t than t 2^-11, so the codes are those of a true division.
 struct WriteArgs {
   Batch b;
   const void* x[2];               // K, V [n_rows, Hkv, d], unit stride along d
@@ -83,68 +114,60 @@ struct WriteArgs {
   int32_t hkv, half;              // half: inputs are fp16, else bf16
 };
 
-template <int DQK, int DV, int WHICH>
-__device__ __forceinline__ void write_group(const WriteArgs& a, uint32_t i) {
-  constexpr int D = WHICH == 0 ? DQK : DV, GR = D / kGroup;
-  const uint32_t total = (uint32_t)a.b.n_rows * a.hkv * GR;
-  if ((i & ~31u) >= total) return;  // (whole warps)
-  const bool in = i < total;
-  const uint32_t g = i % GR, rh = (in ? i : total - 1) / GR, row = rh / a.hkv, h = rh % a.hkv;
-  const uint16_t* src = static_cast<const uint16_t*>(a.x[WHICH]) + (int64_t)row * a.row_stride[WHICH] +
-                        (int64_t)h * a.head_stride[WHICH] + g * kGroup;
-  const uint4 lo = *reinterpret_cast<const uint4*>(src), hi = *reinterpret_cast<const uint4*>(src + 8);
+// Codes of 16 values (as they are in memory); `scale`: their byte.
+__device__ __forceinline__ uint2 quantise(const uint4& lo, const uint4& hi, bool half, uint32_t& scale) {
   const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   uint32_t top = 0;  // |x| as integers: a NaN is above an infinity, an infinity above every number
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
   top = max(top & 0xFFFFu, top >> 16);
-  float amax;
-  bool fine;
-  if (a.half) {
-    fine = top < 0x7C00u;
-    amax = __half2float(__ushort_as_half((unsigned short)top));
-  } else {
-    fine = top < 0x7F80u;
-    amax = __uint_as_float(top << 16);
-  }
-  uint32_t sb = fine ? scale_byte(__fdiv_rn(amax, 6.0f)) : 255u;
-  const float s = __half2float(__ushort_as_half((unsigned short)(sb << 7)));
-  uint32_t code[2] = {0, 0};
-  if (fine && sb != 0) {
-    const float inv = __frcp_rn(s);
-    float y[16];
+  const bool fine = top < (half ? 0x7C00u : 0x7F80u);
+  scale = fine ? scale_byte(half ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16)) : 255u;
+  if (!fine || scale == 0) return make_uint2(0, 0);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__half2float(__ushort_as_half((unsigned short)(scale << 7)))));
+  float y[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 f = a.half ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
-                              : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-      y[2 * j] = __fadd_rn(__fmaf_rn(f.x, inv, 192.0f), -192.0f);
-      y[2 * j + 1] = __fadd_rn(__fmaf_rn(f.y, inv, 192.0f), -192.0f);
-    }
-    code[0] = encode8(y), code[1] = encode8(y + 8);
+  for (int j = 0; j < 8; ++j) {
+    float2 f = half ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                    : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+    f = add2(fma2(f, make_float2(inv, inv), make_float2(192.0f, 192.0f)), make_float2(-192.0f, -192.0f));
+    y[2 * j] = f.x, y[2 * j + 1] = f.y;
   }
-  // the scales of four neighbouring groups (of one token: GR is a multiple of 4) go out together
-  sb |= __shfl_down_sync(0xFFFFFFFFu, sb, 1) << 8;
-  sb |= __shfl_down_sync(0xFFFFFFFFu, sb, 2) << 16;
+  return make_uint2(encode8(y), encode8(y + 8));
+}
+
+template <int DQK, int DV, int WHICH>
+__device__ __forceinline__ void write_groups(const WriteArgs& a, uint32_t i) {
+  constexpr int D = WHICH == 0 ? DQK : DV, PAIRS = D / 32;
+  const uint32_t total = (uint32_t)a.b.n_rows * a.hkv * PAIRS;
+  if ((i & ~31u) >= total) return;  // (whole warps)
+  const bool in = i < total;
+  const uint32_t g = i % PAIRS, rh = (in ? i : total - 1) / PAIRS, row = rh / a.hkv, h = rh - row * a.hkv;
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x[WHICH]) + (int64_t)row * a.row_stride[WHICH] +
+                                                    (int64_t)h * a.head_stride[WHICH] + g * 32);
+  const uint4 x0 = src[0], x1 = src[1], x2 = src[2], x3 = src[3];
+  uint32_t s0, s1;
+  const uint2 c0 = quantise(x0, x1, a.half, s0), c1 = quantise(x2, x3, a.half, s1);
+  // the scales of two neighbouring threads (of one token: PAIRS is even) go out together
+  uint32_t scales = s0 | s1 << 8;
+  scales |= __shfl_down_sync(0xFFFFFFFFu, scales, 1) << 16;
   const int seq = in ? sequence_of(a.b, row) : -1;
   if (seq < 0) return;
   const int pos = position_of(a.b, seq, row);
   const int page = pos < 0 ? -1 : page_of(a.b, seq, pos / kPage);
   if (page < 0) return;
-  uint8_t* rec = a.cache + (int64_t)page * a.page_stride + (int64_t)h * record_bytes(DQK, DV);
-  const int t = pos % kPage;
-  uint8_t* codes = rec + (WHICH == 0 ? 0 : v_code_at(DQK)) + t * (D / 2) + g * 8;
-  *reinterpret_cast<uint2*>(codes) = make_uint2(code[0], code[1]);
-  if (g % 4 == 0) {
-    uint8_t* scales = rec + (WHICH == 0 ? k_scale_at(DQK) : v_scale_at(DQK, DV)) + t * GR + g;
-    *reinterpret_cast<uint32_t*>(scales) = sb;
-  }
+  uint8_t* rec = a.cache + (int64_t)page * a.page_stride + (int64_t)h * record_bytes(DQK, DV) + (WHICH == 0 ? 0 : v_code_at(DQK));
+  const uint32_t at = pos % kPage * PAIRS + g;
+  reinterpret_cast<uint4*>(rec)[at] = make_uint4(c0.x, c0.y, c1.x, c1.y);
+  if (g % 2 == 0) reinterpret_cast<uint32_t*>(rec + kPage * D / 2)[at / 2] = scales;
 }
 
 template <int DQK, int DV>
 __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-  if (blockIdx.y == 0) write_group<DQK, DV, 0>(a, i);
-  else write_group<DQK, DV, 1>(a, i);
+  if (blockIdx.y == 0) write_groups<DQK, DV, 0>(a, i);
+  else write_groups<DQK, DV, 1>(a, i);
 }
 
 // ------------------------------------------------------------------ reading back
@@ -310,33 +333,6 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float exp2_fast(float x) { return ptx::ex2(x); }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
