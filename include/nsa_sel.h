@@ -318,8 +318,7 @@ typedef struct nsa_cache_attend_desc {
   float* lse;                 /* optional fp32 [n_rows, heads_q], natural log */
   const float* o_weight;      /* optional device float w multiplying the result; NULL = 1 */
   void* workspace;            /* nsa_cache_attend_workspace_bytes() bytes, 16-byte aligned, of this call alone */
-  int32_t* err;               /* optional device int32; NSA_DEVERR_* bits are ORed into it (after a wait that ran out the
-                                 rows it concerns are NaN) */
+  int32_t* err;               /* optional device int32; NSA_DEVERR_* bits are ORed into it */
   int64_t q_row_stride;       /* elements, multiples of 8; 0 = heads_q * d_qk */
   int64_t q_head_stride;      /* 0 = d_qk */
   int32_t heads_q;            /* a multiple of heads_kv */
@@ -341,7 +340,8 @@ typedef struct nsa_cache_attend_plan_info {
   int64_t workspace_bytes;
   int32_t slots;              /* (row, KV head) x page slots of a row; 0 = as many as it has pages, and then the next two are
                                  worked out on the device (0) */
-  int32_t team;               /* warps that take turns at a row's slots */
+  int32_t team;               /* warps of a block that take turns at a row's slots */
+  int32_t cluster;            /* blocks of a cluster that share each row; 1 = none */
   int32_t share;              /* whole rows of a team, or its slots where rows are cut (merge != 0) */
   int32_t grid, threads, smem_bytes;
   int32_t merge;              /* warps that join the parts of a cut row's head; 0 = no row is cut, one launch */

@@ -125,7 +125,7 @@ class NsaCacheAttendPlanInfo(ctypes.Structure):
 
     _fields_ = [
         ("workspace_bytes", ctypes.c_int64), ("slots", ctypes.c_int32), ("team", ctypes.c_int32),
-        ("share", ctypes.c_int32), ("grid", ctypes.c_int32), ("threads", ctypes.c_int32), ("smem_bytes", ctypes.c_int32),
+        ("cluster", ctypes.c_int32), ("share", ctypes.c_int32), ("grid", ctypes.c_int32), ("threads", ctypes.c_int32), ("smem_bytes", ctypes.c_int32),
         ("merge", ctypes.c_int32), ("tiles", ctypes.c_int32),
     ]
 

@@ -134,21 +134,27 @@ int plan_attend(const nsa_cache_attend_desc* d, int sm_count, nsa_cache_attend_p
   p->tiles = tiles_of(group);
   const uint32_t most = (uint32_t)most_slots(d), rows = (uint32_t)b.n_rows * b.heads_kv * p->tiles;
   const uint32_t warps = (uint32_t)sm_count * C::NW;
-  const bool ragged = d->sel == nullptr && d->window == 0 && b.n_rows <= C::kMaxRagged;
+  p->cluster = (int32_t)nsa::cache::cluster_of(rows, most, warps);
+  // The ragged line is for rows that may have to be cut by their real lengths.
+  const bool ragged = d->sel == nullptr && d->window == 0 && b.n_rows <= C::kMaxRagged && p->cluster == 1 &&
+                      nsa::cache::may_cut(rows, most, warps);
   const nsa::cache::Split s = nsa::cache::split_line(rows, rows * most, most, warps);
   p->slots = ragged ? 0 : (int32_t)most;
-  bool cut = s.cut != 0;
+  bool cut = ragged;
   uint32_t teams;  // with a share of their own, at most
   if (ragged) {
-    cut = nsa::cache::may_cut(rows, most, warps);
     teams = (uint32_t)std::min<uint64_t>(warps, (uint64_t)rows * most);
-    p->grid = (int32_t)std::min<uint32_t>(sm_count, teams);
+  } else if (p->cluster > 1) {
+    p->team = nsa::cache::kTeam;
+    p->share = 1;
+    teams = rows;
   } else {
+    cut = s.cut != 0;
     p->team = (int32_t)s.team;
     p->share = (int32_t)s.share;
-    teams = nsa::cache::ceil_div(s.cut ? rows * most : rows, s.share);
-    p->grid = (int32_t)std::min<uint32_t>(sm_count, teams);
+    teams = nsa::cache::ceil_div(cut ? rows * most : rows, s.share);
   }
+  p->grid = p->cluster > 1 ? (int32_t)(rows * p->cluster) : (int32_t)std::min<uint32_t>(sm_count, teams);
   p->threads = C::NW * 32;
   p->smem_bytes = C::kSmem;
   // Eight warps for each query head while the device has room for them at once (8 blocks an SM), else one: rows that are
@@ -184,20 +190,28 @@ int launch_attend(const AttendArgs& a, const nsa_cache_attend_plan_info& p, int 
       g_attr_done[dev] |= bit;
     }
   }
-  nsa::cache::attend_kernel<C><<<p.grid, p.threads, C::kSmem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || p.merge == 0) return done(e, "cache attention launch");
-  const int64_t units = (int64_t)a.b.n_rows * a.hq;
-  cudaLaunchAttribute early;
-  memset(&early, 0, sizeof(early));
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)p.grid);
+  cfg.blockDim = dim3((unsigned)p.threads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)p.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, nsa::cache::attend_kernel<C>, a);
+  if (e != cudaSuccess || p.merge == 0) return done(e, "cache attention launch");
+  const int64_t units = (int64_t)a.b.n_rows * a.hq;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)(p.merge == 1 ? (units + 7) / 8 : units));
   cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = &early;
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   e = p.merge == 1 ? cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 1>, a)
                    : cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 8>, a);
@@ -242,6 +256,7 @@ int attend(const nsa_cache_attend_desc* d, cudaStream_t st) {
   a.slots = p.slots;
   a.warps = (uint32_t)sm * (uint32_t)(p.threads / 32);
   a.split = {(uint32_t)p.team, (uint32_t)p.share, p.merge != 0};
+  a.cluster = (uint32_t)p.cluster;
   a.q_half = d->q_dtype == NSA_DTYPE_F16;
   a.o_dtype = d->o_dtype;
   a.accumulate = d->o_accumulate != 0;

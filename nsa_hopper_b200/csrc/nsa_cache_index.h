@@ -89,17 +89,18 @@ NSA_HD int running_sub(int j, int first, int end) {
 // Slots of a row that takes its sub-blocks one after the other; at least one, so that every row has an owner.
 NSA_HD int running_slots(int first, int end) { return end > first ? (end - 1) / kPage - first / kPage + 1 : 1; }
 
+NSA_HD uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
 // How the slots of a call (rows x slots, standing in one line) are shared out among the device's warps.  `team` warps (a
 // power of two, neighbours of a block) take turns at a row's slots and join their results; a team has `share` whole rows, or,
 // where rows are cut, `share` slots, whose parts a second kernel joins.
 struct Split {
   uint32_t team, share, cut;
 };
-constexpr uint32_t kTeam = 8;    // largest team
-constexpr uint32_t kJoins = 4;   // what the second kernel costs, in slots of a warp
-constexpr uint32_t kLong = 16;   // slots of a warp from which on warps of their own are better than teams where rows are cut
-
-NSA_HD uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+constexpr uint32_t kTeam = 8;     // largest team: a block
+constexpr uint32_t kCluster = 8;  // largest cluster of blocks
+constexpr uint32_t kJoins = 4;    // what the second kernel costs, in slots of a warp
+constexpr uint32_t kLong = 16;    // slots of a warp from which on warps of their own are better than teams where rows are cut
 
 // `longest`: slots of the longest row (>= 1), `total` < 2^31: of all rows; `warps`: a multiple of kTeam.
 NSA_HD Split split_line(uint32_t rows, uint32_t total, uint32_t longest, uint32_t warps) {
@@ -118,6 +119,13 @@ NSA_HD bool may_cut(uint32_t rows, uint32_t longest, uint32_t warps) {
   uint32_t team = kTeam;
   while (team > 1 && (uint64_t)rows * team > warps) team /= 2;
   return (uint64_t)ceil_div(rows, warps / team) * ceil_div(longest, team) > kJoins + 1;
+}
+// Blocks that share each row, in a cluster, where rows are so few that most SMs would have none: at most as many as leave
+// each a slot for every second warp, and only where no warp gets more than cutting the rows would cost.  1: no clusters.
+NSA_HD uint32_t cluster_of(uint32_t rows, uint32_t longest, uint32_t warps) {
+  uint32_t n = kCluster;
+  while (n > 1 && ((uint64_t)rows * kTeam * n > warps || longest < kTeam * n / 2)) n /= 2;
+  return ceil_div(longest, kTeam * n) <= kJoins + 1 ? n : 1;
 }
 
 }  // namespace cache

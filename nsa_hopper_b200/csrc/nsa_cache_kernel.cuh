@@ -270,6 +270,7 @@ struct AttendArgs {
   int32_t n_sel, per, window;    // per: sub-blocks of a selection block
   int32_t slots;                 // slots of every row; 0: as many as it has sub-blocks (the ragged line)
   uint32_t warps;                // of the device
+  uint32_t cluster;              // blocks that share each row (1: none do); then rows are whole and a cluster has one
   Split split;                   // (a ragged line's is worked out on the device)
   int32_t q_half, o_dtype, accumulate, fill;  // fill: rows of no sequence get O = 0, LSE = -inf; else they are left
   float scale_log2;
@@ -453,8 +454,8 @@ struct Worker {
       c.twice = __ballot_sync(0xFFFFFFFFu, (__match_any_sync(0xFFFFFFFFu, c.entry) & ((1u << lane) - 1)) != 0);
   }
 
-  // This warp's part (every team-th) of the next 32 * team slots of the row into the queue, those that show no key left out
-  // but for the warp's last entry of the row's slots here (its owners have to leave the row's result; one without a slot
+  // This warp's part (every team-th, from `turn` on) of the next 32 * team slots of the row into the queue, those that show no
+  // key left out but for the warp's last entry of the row's slots here (its owners have to leave the row's result; one without a slot
   // of its own gets an empty entry).  An entry: the record's address (0: none), the first and one past the last visible key
   // of the sub-block (8 bits each), and the row (times 2, + 1 if it is the warp's last entry of it).
   static __device__ __forceinline__ int resolve(const AttendArgs& a, Cursor& c, const uint32_t* starts, int4* queue, int tail,
@@ -799,6 +800,41 @@ struct Worker {
   }
 };
 
+// Joins what the blocks of a cluster have of a row (`mine`: this block's part, in shared memory), each of them some columns.
+template <class C>
+__device__ __forceinline__ void join_cluster(const AttendArgs& a, uint32_t row, const float* mine, uint32_t rank) {
+  constexpr int kHeads = C::kHeads, DV = C::DV;
+  ptx::cluster_sync();  // all parts are there
+  const uint32_t rows_h = a.hkv * a.tiles;
+  const int n = row / rows_h, hm = row % rows_h, g0 = hm % a.tiles * kHeads;
+  const int64_t at0 = (int64_t)n * a.hq + hm / a.tiles * a.group + g0;
+  const int i = rank * (C::NW * 32) + threadIdx.x, x = i / (DV / 4), d = i % (DV / 4) * 4;
+  if (x < min(kHeads, a.group - g0) && (a.fill || sequence_of(a.b, n) >= 0)) {
+    float m[kCluster], l[kCluster], top = -INFINITY, sum = 0.0f;
+    float4 v[kCluster], acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < (int)kCluster; ++k) {
+      m[k] = -INFINITY, l[k] = 0.0f, v[k] = acc;
+      if (k < (int)a.cluster) {
+        const float* part = ptx::of_rank(mine, k);
+        m[k] = part[kHeads * DV + x], l[k] = part[kHeads * (DV + 1) + x];
+        v[k] = *reinterpret_cast<const float4*>(part + x * DV + d);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (int)kCluster; ++k) top = fmaxf(top, m[k]);
+#pragma unroll
+    for (int k = 0; k < (int)kCluster; ++k) {  // (where m is -inf the sums are zeros, or NaN, which stays)
+      const float f = m[k] == -INFINITY ? 1.0f : exp2_fast(m[k] - top);
+      sum += l[k] * f;
+      acc.x += v[k].x * f, acc.y += v[k].y * f, acc.z += v[k].z * f, acc.w += v[k].w * f;
+    }
+    if (d == 0) store_lse(a, at0 + x, top, sum);
+    store4<DV>(a, at0 + x, d, acc, sum != 0.0f ? (a.weight ? *a.weight : 1.0f) / sum : 0.0f);
+  }
+  ptx::cluster_sync();  // nobody leaves while its part is read
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -852,7 +888,9 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   }
   // neighbouring teams are on different SMs, so that a few of them use many
   const int team = split.team, turn = warp % team, sub_team = warp / team;
-  const uint32_t me = sub_team * gridDim.x + blockIdx.x;
+  const uint32_t rank = blockIdx.x % a.cluster;
+  const uint32_t me = a.cluster > 1 ? blockIdx.x / a.cluster : sub_team * gridDim.x + blockIdx.x;
+  const int every = team * a.cluster, first_slot = a.cluster > 1 ? warp * a.cluster + rank : turn;
 
   typename Worker<C>::Cursor cur;
   auto start_of = [&](uint32_t row) {  // the line's slots before a row
@@ -896,7 +934,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   bool lost = false;                // a copy did not come: rows from here on are NaN
   auto issue = [&] {
     while (tail - issued < C::STAGES && tail - head <= C::kQueue - 32 && cur.next < cur.end)
-      tail = Worker<C>::resolve(a, cur, starts, queue, tail, team, turn, lane);
+      tail = Worker<C>::resolve(a, cur, starts, queue, tail, every, first_slot, lane);
     if (issued < tail) {
       const uint8_t* src = Worker<C>::record_of(queue[issued % C::kQueue]);
       const int stage = issued++ % C::STAGES;
@@ -933,12 +971,14 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
       const bool head_cut = first_row && cut_before;
       const bool tail_cut = head + 1 == tail && cur.next == cur.end && cur.j < cur.len;
       float* part = head_cut || tail_cut ? a.part + ((size_t)me * 2 + (head_cut ? 0 : 1)) * C::kPart : nullptr;
+      if (a.cluster > 1) part = reinterpret_cast<float*>(smem);  // (the first warp's ring: a cluster has one row)
       w.finish(a, (uint32_t)e.w >> 1, part, join + sub_team * team * C::kJoin, team, turn, 1 + sub_team, lane);
       first_row = false;
     }
     __syncwarp();
     ++head;
   }
+  if (a.cluster > 1) join_cluster<C>(a, row, reinterpret_cast<const float*>(smem), rank);
   if (lost) {  // the block's memory is not given up under a copy (bounded, too)
     if (a.err != nullptr && lane == 0) atomicOr(a.err, 1);
     for (int i = 0; i < C::STAGES; ++i)

@@ -451,8 +451,11 @@ std::vector<torch::Tensor> cache_attend(torch::Tensor Q, torch::Tensor cache, to
   const Api& a = api();
   const int64_t ws = a.cache_attend_ws(&d);
   if (ws < 0) TORCH_CHECK(false, format_msg("nsa_cache_attend failed: %s", a.last_error()));
-  auto work = torch::empty({ws}, Q.options().dtype(torch::kByte));
-  d.workspace = work.data_ptr();
+  torch::Tensor work;
+  if (ws > 16) {  // (16: no row is cut, nothing is kept)
+    work = torch::empty({ws}, Q.options().dtype(torch::kByte));
+    d.workspace = work.data_ptr();
+  }
   const int rc = a.cache_attend(&d, current_stream());
   if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_cache_attend failed (%d): %s", rc, a.last_error()));
   return {O, L};

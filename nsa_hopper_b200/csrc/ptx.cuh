@@ -80,6 +80,19 @@ __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, boo
   return out != 0;
 }
 
+// ---------------------------------------------------------------- clusters
+// Barrier over all threads of the cluster: what they wrote to shared memory before it is seen after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same place in the shared memory of another block of the cluster.
+template <class T>
+__device__ __forceinline__ T* of_rank(T* p, uint32_t rank) {
+  uint64_t r;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<T*>(r);
+}
+
 // ---------------------------------------------------------------- L2 cache policies
 __device__ __forceinline__ uint64_t policy_evict_last() {
   uint64_t p;

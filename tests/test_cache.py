@@ -36,7 +36,7 @@ int slots(int first, int end) { return running_slots(first, end); }
 int first(int pos, int window) { return first_key(pos, window); }
 void split(uint32_t rows, uint32_t total, uint32_t longest, uint32_t warps, uint32_t* out) {
   const Split s = split_line(rows, total, longest, warps);
-  out[0] = s.team, out[1] = s.share, out[2] = s.cut, out[3] = may_cut(rows, longest, warps);
+  out[0] = s.team, out[1] = s.share, out[2] = s.cut, out[3] = may_cut(rows, longest, warps), out[4] = cluster_of(rows, longest, warps);
 }
 int record(int dqk, int dv) { return record_bytes(dqk, dv); }
 }
@@ -114,9 +114,12 @@ def test_shares_cover_the_line(index):
         rows = int(np.exp(rng.uniform(0, np.log(5000))))
         longest = int(np.exp(rng.uniform(0, np.log(min(40000, (2**31 - 1) // rows)))))
         total = rows * longest if i % 2 else int(rng.integers(rows + longest - 1, rows * longest + 1))
-        out = (ctypes.c_uint32 * 4)()
+        out = (ctypes.c_uint32 * 5)()
         index.split(rows, total, longest, warps, out)
-        team, share, cut, may = out
+        team, share, cut, may, cluster = out
+        assert cluster in (1, 2, 4, 8)
+        if cluster > 1:
+            assert rows * cluster <= 148 and cluster * 4 <= longest <= 5 * 8 * cluster
         assert team in (1, 2, 4, 8) and share >= 1
         teams = warps // team
         if cut:
@@ -172,15 +175,19 @@ def _attend(batch=None, **kw):
 
 
 def test_plan_shares_out_the_work():
-    p = capi.cache_attend_plan(_attend(sel=256, n_sel=16, block_size=64))     # 32 rows, 8 warps each take 2 pages
-    assert (p["slots"], p["team"], p["share"], p["grid"], p["merge"], p["workspace_bytes"]) == (16, 8, 1, 32, 0, 16)
+    p = capi.cache_attend_plan(_attend(sel=256, n_sel=16, block_size=64))     # 32 rows, a cluster of 4 blocks for each
+    assert (p["slots"], p["team"], p["cluster"], p["share"], p["grid"], p["merge"], p["workspace_bytes"]) == (16, 8, 4, 1, 128, 0, 16)
+    p = capi.cache_attend_plan(_attend(dict(n_rows=32, n_seqs=32), sel=256, n_sel=16, block_size=64))
+    assert (p["team"], p["cluster"], p["share"], p["grid"]) == (8, 1, 1, 128)  # 128 rows, a block for each
     assert p["smem_bytes"] <= 232448
     p = capi.cache_attend_plan(_attend(dict(n_rows=256, n_seqs=256), sel=256, n_sel=16, block_size=64))
     assert (p["team"], p["share"], p["grid"], p["merge"]) == (1, 1, 148, 0)    # a warp for each row
-    p = capi.cache_attend_plan(_attend())                                      # every key: the ragged line
+    p = capi.cache_attend_plan(_attend())                                      # every key, 64 pages
+    assert (p["slots"], p["cluster"], p["grid"], p["merge"]) == (64, 4, 128, 0)
+    p = capi.cache_attend_plan(_attend(dict(width=1500)))
     assert p["slots"] == 0 and p["share"] == 0 and p["merge"] >= 1 and p["workspace_bytes"] > 16
-    p = capi.cache_attend_plan(_attend(dict(width=40)))                        # short rows are not cut
-    assert p["slots"] == 0 and p["merge"] == 0
+    p = capi.cache_attend_plan(_attend(dict(n_rows=30, n_seqs=30, width=40)))  # short rows are not cut
+    assert p["slots"] == 40 and p["merge"] == 0 and p["cluster"] == 1
     p = capi.cache_attend_plan(_attend(dict(n_rows=4096, n_seqs=4096)))        # too many rows for it
     assert p["slots"] == 64
     p = capi.cache_attend_plan(_attend(window=1))
