@@ -82,6 +82,16 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t low2(uint32_t x) {  // (an operand's modifier, not an instruction)
+  uint32_t r;
+  asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {l, l};}" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t high2(uint32_t x) {
+  uint32_t r;
+  asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {h, h};}" : "=r"(r) : "r"(x));
+  return r;
+}
 // A scale byte in both halves of an fp16 pair.
 __device__ __forceinline__ uint32_t scale2(uint32_t byte) { return byte * 0x00800080u; }
 
@@ -506,10 +516,12 @@ struct Worker {
   static __device__ __forceinline__ const uint8_t* record_of(const int4& e) {
     return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)e.y << 32 | (uint32_t)e.x);
   }
+  static constexpr float kNone = -3e38f;  // a maximum of no scores
+
   // ---- the consumer's side.  The thread's heads in tile h are 8 h + 2 c and 8 h + 2 c + 1 (c = lane % 4).
   float o[MT][NH][4];      // O^T: d = (DV / 8) r + 2 j + e / 2 (r = lane / 4) of head 8 h + 2 c + e % 2
   uint32_t q[NH][KS * 2];  // Q of head 8 h + r: d = c * DQK / 4 + 2 i, + 1
-  float2 f[NH], m[NH], l[NH];  // of the thread's heads: factor, maximum of the unscaled scores, the thread's share of the sum
+  float2 f[NH], m[NH], l[NH];  // of the thread's heads: factor, maximum (a power of two), the thread's share of the sum
 
   // A new row: its queries are asked for, then (when the copies of the first pages are under way) made ready.
   __device__ __forceinline__ void ask(const AttendArgs& a, uint32_t row, int lane) {
@@ -529,7 +541,7 @@ struct Worker {
       factor = fminf(fmaxf(factor * a.scale_log2, 1e-38f), 3e38f);
       const int from = (lane & 3) * 8;  // row r = 2 c
       f[i] = make_float2(__shfl_sync(0xFFFFFFFFu, factor, from), __shfl_sync(0xFFFFFFFFu, factor, from + 4));
-      m[i] = make_float2(-INFINITY, -INFINITY);
+      m[i] = make_float2(kNone, kNone);
       l[i] = make_float2(0.0f, 0.0f);
     }
 #pragma unroll
@@ -558,8 +570,8 @@ struct Worker {
         if constexpr (DQK == 128) {
           const uint4 y = *reinterpret_cast<const uint4*>(codes);
           w[x][0] = y.x, w[x][1] = y.y, w[x][2] = y.z, w[x][3] = y.w;
-          const uint32_t both = *reinterpret_cast<const uint16_t*>(scales);
-          sc[x][0] = scale2(both & 0xFFu), sc[x][1] = scale2(both >> 8);
+          const uint32_t both = __byte_perm(*reinterpret_cast<const uint16_t*>(scales), 0, 0x4140) << 7;
+          sc[x][0] = low2(both), sc[x][1] = high2(both);
         } else {
 #pragma unroll
           for (int g = 0; g < DQK / 64; ++g) {
@@ -603,53 +615,57 @@ struct Worker {
       ptx::fence_proxy_async_smem();  // (before the record that is copied here next)
       __syncwarp();
     }
-    // Softmax against m, a maximum of the unscaled scores so far (f > 0 turns them into powers of two).  It is raised, and O
-    // and the sums with it, when a score is more than 2^kSlack above it: until then P is at most 2^kSlack, and neither its
-    // roundings nor the result depend on m.  So most pages need no exchange between the threads that share a head.
+    // Softmax, in powers of two, against a maximum m of the scores so far.  m is raised, and O and the sums with it, when a
+    // score is more than 2^kSlack above it: until then P is at most 2^kSlack, and neither its roundings nor the result depend
+    // on m.  So most pages need no exchange between the threads that share a head.  (The first m is so low that every number
+    // is above it, and it scales zeros, or NaN, which stays.)
     constexpr float kSlack = 8.0f;
     uint32_t p[4][NH][2];  // P^T as the tensor core takes it: fp16 pairs of keys (of rows 2c, 2c + 1, and 8 more) of head 8 h + r
-    float2 top[NH], u[NH];
-    bool grown = false;
+    float2 y[4][NH][2];
+    float most = -INFINITY;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      top[h] = make_float2(fmaxf(s[0][h][0], s[0][h][2]), fmaxf(s[0][h][1], s[0][h][3]));
-#pragma unroll
-      for (int t = 1; t < 4; ++t)
-        top[h].x = max3(top[h].x, s[t][h][0], s[t][h][2]), top[h].y = max3(top[h].y, s[t][h][1], s[t][h][3]);
-      // (also where m still is -inf and a score is not; -inf - -inf is NaN, which is not greater)
-      grown = grown || (top[h].x - m[h].x) * f[h].x > kSlack || (top[h].y - m[h].y) * f[h].y > kSlack;
-    }
-    if (__any_sync(0xFFFFFFFFu, grown)) {
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        top[h] = make_float2(fmaxf(top[h].x, m[h].x), fmaxf(top[h].y, m[h].y));
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          y[t][h][x] = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-m[h].x, -m[h].y));
+        most = max3(max3(most, y[t][h][0].x, y[t][h][0].y), y[t][h][1].x, y[t][h][1].y);
+      }
+    if (__any_sync(0xFFFFFFFFu, most > kSlack)) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        float2 top = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          top.x = max3(top.x, s[t][h][0], s[t][h][2]), top.y = max3(top.y, s[t][h][1], s[t][h][3]);
 #pragma unroll
         for (int k = 4; k < 32; k *= 2) {
-          top[h].x = fmaxf(top[h].x, __shfl_xor_sync(0xFFFFFFFFu, top[h].x, k));
-          top[h].y = fmaxf(top[h].y, __shfl_xor_sync(0xFFFFFFFFu, top[h].y, k));
+          top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, k));
+          top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, k));
         }
-        // (where m is -inf, O and the sums are zeros or NaN, and stay)
-        const float2 k = make_float2(m[h].x == -INFINITY ? 1.0f : exp2_fast((m[h].x - top[h].x) * f[h].x),
-                                     m[h].y == -INFINITY ? 1.0f : exp2_fast((m[h].y - top[h].y) * f[h].y));
+        top = make_float2(fmaxf(m[h].x, top.x * f[h].x), fmaxf(m[h].y, top.y * f[h].y));
+        const float2 k = make_float2(exp2_fast(m[h].x - top.x), exp2_fast(m[h].y - top.y));
         l[h] = mul2(l[h], k);
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][h][0] *= k.x, o[j][h][1] *= k.y, o[j][h][2] *= k.x, o[j][h][3] *= k.y;
-        m[h] = top[h];
+        m[h] = top;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            y[t][h][x] = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-top.x, -top.y));
       }
     }
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-      u[h] = make_float2(m[h].x == -INFINITY ? 0.0f : m[h].x * f[h].x, m[h].y == -INFINITY ? 0.0f : m[h].y * f[h].y);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float2 y = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-u[h].x, -u[h].y));
-          y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-          l[h] = add2(l[h], y);
-          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[t][h][x]) : "r"(pack_half(y.x, y.y)));
+          const float2 e = make_float2(exp2_fast(y[t][h][x].x), exp2_fast(y[t][h][x].y));
+          l[h] = add2(l[h], e);
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[t][h][x]) : "r"(pack_half(e.x, e.y)));
         }
     // PV
     const int odd = 4 + (c ^ 1);  // keys of the tile's rows 2c and 2c + 1: c and odd
@@ -708,11 +724,11 @@ struct Worker {
     const int used = min(kHeads, a.group - g0);
     const bool left = part == nullptr && !a.fill && sequence_of_warp(a.b, n, lane) < 0;  // a row to leave as it was
     const float weight = a.weight != nullptr && part == nullptr ? *a.weight : 1.0f;
-    float sum[NH][2], top[NH][2];  // top: as a power of two
+    float sum[NH][2], top[NH][2];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       sum[h][0] = l[h].x, sum[h][1] = l[h].y;
-      top[h][0] = m[h].x == -INFINITY ? m[h].x : m[h].x * f[h].x, top[h][1] = m[h].y == -INFINITY ? m[h].y : m[h].y * f[h].y;
+      top[h][0] = m[h].x, top[h][1] = m[h].y;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -753,9 +769,9 @@ struct Worker {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int x = 8 * h + 2 * c + e;
-        float common = -INFINITY;
+        float common = kNone;
         for (int w = 0; w < team; ++w) common = fmaxf(common, join[w * C::kJoin + kMl + x]);
-        k[h][e] = exp2_fast(top[h][e] - (common == -INFINITY ? 0.0f : common));
+        k[h][e] = exp2_fast(top[h][e] - common);
         if (r == 0) mine[kMl + kHeads + x] = sum[h][e] * k[h][e], mine[kMl + 2 * kHeads + x] = common;
       }
     const int swap = CS == 4 ? c : (c & 1) | (c & 2) << 1;
@@ -810,11 +826,11 @@ __device__ __forceinline__ void join_cluster(const AttendArgs& a, uint32_t row, 
   const int64_t at0 = (int64_t)n * a.hq + hm / a.tiles * a.group + g0;
   const int i = rank * (C::NW * 32) + threadIdx.x, x = i / (DV / 4), d = i % (DV / 4) * 4;
   if (x < min(kHeads, a.group - g0) && (a.fill || sequence_of(a.b, n) >= 0)) {
-    float m[kCluster], l[kCluster], top = -INFINITY, sum = 0.0f;
+    float m[kCluster], l[kCluster], top = Worker<C>::kNone, sum = 0.0f;
     float4 v[kCluster], acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < (int)kCluster; ++k) {
-      m[k] = -INFINITY, l[k] = 0.0f, v[k] = acc;
+      m[k] = Worker<C>::kNone, l[k] = 0.0f, v[k] = acc;
       if (k < (int)a.cluster) {
         const float* part = ptx::of_rank(mine, k);
         m[k] = part[kHeads * DV + x], l[k] = part[kHeads * (DV + 1) + x];
@@ -824,8 +840,8 @@ __device__ __forceinline__ void join_cluster(const AttendArgs& a, uint32_t row, 
 #pragma unroll
     for (int k = 0; k < (int)kCluster; ++k) top = fmaxf(top, m[k]);
 #pragma unroll
-    for (int k = 0; k < (int)kCluster; ++k) {  // (where m is -inf the sums are zeros, or NaN, which stays)
-      const float f = m[k] == -INFINITY ? 1.0f : exp2_fast(m[k] - top);
+    for (int k = 0; k < (int)kCluster; ++k) {
+      const float f = exp2_fast(m[k] - top);
       sum += l[k] * f;
       acc.x += v[k].x * f, acc.y += v[k].y * f, acc.z += v[k].z * f, acc.w += v[k].w * f;
     }
@@ -1016,8 +1032,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
   // the first team has the row as its last, the others as their first; this warp has every WPH-th part
   auto part_of = [&](uint32_t i) { return a.part + ((size_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * C::kPart; };
   const uint32_t mine = WPH == 1 ? 0 : warp;
-  float m = -INFINITY, l = 0.0f;  // (a maximum is never NaN: fmaxf leaves NaN out; where it is -inf the sums are zeros, or
-                                  // NaN, which stays)
+  float m = Worker<C>::kNone, l = 0.0f;  // (a maximum is never NaN: fmaxf leaves it out; the NaN is in the sums)
   for (uint32_t i = mine + WPH * lane; i < parts; i += WPH * 32) m = fmaxf(m, part_of(i)[C::kHeads * DV + x]);
 #pragma unroll
   for (int k = 16; k > 0; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, k));
@@ -1027,7 +1042,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
     float factor = 0.0f;
     if (own < parts) {
       const float* p = part_of(own) + C::kHeads * DV + x;
-      factor = exp2_fast(p[0] - (m == -INFINITY ? 0.0f : m));
+      factor = exp2_fast(p[0] - m);
       l += p[C::kHeads] * factor;
     }
     const int count = min(32u, (parts - i0 + WPH - 1) / WPH);
@@ -1053,7 +1068,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
     acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < WPH; ++k) {
-      const float f = shared_ml[k][0] == -INFINITY ? 1.0f : exp2_fast(shared_ml[k][0] - m);
+      const float f = exp2_fast(shared_ml[k][0] - m);
       l += shared_ml[k][1] * f;
       if (lane < V4) {
         const float4 v = reinterpret_cast<const float4*>(shared_o[k])[lane];
