@@ -295,12 +295,12 @@ struct AttendCfg {
   static constexpr int kHeads = 8 * NH;       // query heads of a tile
   static constexpr int kRecord = record_bytes(DQK, DV);
   static constexpr int kQueue = 40;           // resolved slots of a warp
-  static constexpr int kMaxRagged = 512;      // rows of a ragged line
+  static constexpr int kMaxRagged = 1920;     // rows of a ragged line
   static constexpr int kPart = kHeads * (DV + 2);              // floats of a partial result: O, m, sum
   static constexpr int kJoin = kHeads * (DV / ROUNDS + 4);     // floats of a warp in a team's join: O of a round, m, sum, max
   static constexpr int kWarp = STAGES * (kRecord + 8) + kQueue * 16 + kJoin * 4;
   static constexpr int kSmem = NW * kWarp + (kMaxRagged + 1) * 4;
-  static_assert(kSmem <= 232448, "227 KB of shared memory a block");
+  static_assert(kSmem + 128 <= 232448, "227 KB of shared memory a block, the static variables included");
 };
 
 // Ring depth and rounds of the join for each head dim and tile (NH = 1: up to 8 query heads, 2: 16).  A warp holds O and Q

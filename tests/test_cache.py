@@ -161,6 +161,27 @@ def test_format_by_definition():
     assert (oc.values(*oc.quantise(np.full((1, 16), 1e30))) == 61440).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantising_without_divisions_is_exact(dtype):
+    """The kernel's arithmetic, restated in numpy's fp32, against the definition: every finite value of the type as a
+    group's largest, and every value below each scale's saturation, with the approximate reciprocal off either way."""
+    every = torch.arange(0x7F80 if dtype == torch.bfloat16 else 0x7C00, dtype=torch.int16).view(dtype).float().numpy()
+    raw = ((every * np.float32(0.16666667)).view(np.uint32) + np.uint32(0x40)) & np.uint32(0xFFFFFF80)
+    big = raw.view(np.float32) >= np.float32(2.0**-14)
+    normal = np.minimum(((raw + np.uint32(0x7FFFF) + ((raw >> 20) & 1)) >> 20).astype(np.int64) - 896, 226)
+    byte = np.where(big, normal, np.rint(np.where(big, 0, raw.view(np.float32)).astype(np.float64) * 2.0**17).astype(np.int64))
+    want = oc._nearest_even(every.astype(np.float64) / 6.0, oc._SCALES)
+    np.testing.assert_array_equal(byte, want)
+    for b in range(1, 0xE3):
+        s = oc._SCALES[b]
+        x = every[(every <= 6.8 * s) & (every >= 0.2 * s)].astype(np.float64)
+        want = oc._nearest_even(x / s, oc.LEVELS)
+        for off in (-1, 0, 1):  # 2^-22: the reciprocal's error and the input's
+            inv = float(np.float32((1 / s) * (1 + off * 2.0**-22)))
+            y = ((x * inv + 192).astype(np.float32) - np.float32(192)).astype(np.float64)
+            np.testing.assert_array_equal(oc._nearest_even(np.maximum(y, 0), oc.LEVELS), want)
+
+
 # ------------------------------------------------------------------ plan and refusals of the C ABI
 def _batch(**kw):
     base = dict(cache=256, pages=256, lens=256, num_pages=1000, n_seqs=8, width=64, n_rows=8, heads_kv=4, d_qk=128, d_v=128)

@@ -269,15 +269,99 @@ def test_attend_long_selections(n_sel, l_prime):
     _attend_case((64, 64), 8, 2, [3000, 900], None, torch.bfloat16, 8, n_sel=n_sel, l_prime=l_prime)
 
 
-def test_attend_long_context_is_cut_and_joined():
-    _attend_case((128, 128), 16, 1, [20000], None, torch.bfloat16, 9)
-    _attend_case((128, 128), 8, 2, [20000, 1, 0, 64, 9999], None, torch.bfloat16, 10)
+def _random_cache(num_pages, hkv, dims, gen):
+    """Records of random codes, with scales between 0.04 and 0.6."""
+    parts = []
+    for d in dims:
+        parts.append(torch.randint(0, 256, (num_pages, hkv, 32 * d), generator=gen, dtype=torch.uint8))
+        parts.append(torch.randint(0x52, 0x72, (num_pages, hkv, 4 * d), generator=gen, dtype=torch.uint8))
+    return torch.cat(parts, -1)
 
 
-def test_attend_many_rows_are_left_whole():
-    lens = [(37 * i) % 200 for i in range(700)]
-    _attend_case((64, 64), 2, 1, lens, None, torch.float16, 11)
-    _attend_case((64, 64), 2, 1, lens, None, torch.float16, 12, n_sel=2)
+def _plan(n, hq, hkv, dims, width, n_sel, l_prime, window):
+    batch = capi.make_cache_batch(cache=256, pages=256, lens=256, num_pages=1, n_seqs=n, width=width, n_rows=n, heads_kv=hkv,
+                                  d_qk=dims[0], d_v=dims[1])
+    return capi.cache_attend_plan(capi.make_cache_attend_desc(batch=batch, q=256, o=256, heads_q=hq, sel=256 if n_sel else 0,
+                                                              n_sel=n_sel, block_size=l_prime, window=window), 0)
+
+
+# lengths, width of the page table, selection, head dims, heads; what the plan has to be for the case to be what it stands for
+SHARING = [
+    ([2100], 33, 0, (128, 128), (16, 1), dict(cluster=8, merge=0)),
+    ([2100, 3, 0, 64], 33, 0, (64, 64), (4, 1), dict(cluster=8, merge=0)),
+    ([1500] * 6, 24, 0, (128, 128), (24, 4), dict(cluster=4, merge=0)),
+    ([700, 1, 650], 16, 9, (192, 128), (64, 8), dict(cluster=2, merge=0)),
+    ([900] * 30, 40, 16, (128, 64), (8, 4), dict(cluster=1, team=8, merge=0)),
+    ([500] * 60, 8, 16, (128, 128), (32, 4), dict(cluster=1, team=4, merge=0)),
+    ([300] * 120, 8, 5, (64, 64), (32, 4), dict(cluster=1, team=2, merge=0)),
+    ([300] * 600, 6, 3, (64, 64), (4, 2), dict(cluster=1, team=1, merge=0)),
+    ([130, 70, 0, 200] * 500, 60, 0, (64, 64), (2, 1), dict(slots=60, cluster=1)),    # more rows than a ragged line takes
+    ([25000], 391, 0, (128, 128), (16, 1), dict(slots=0, merge=8)),                   # cut, eight warps join
+    ([20000, 1, 0, 64, 9999], 2000, 0, (192, 128), (6, 2), dict(slots=0, merge=8)),
+    ([5000] * 40 + [0, 1, 64], 200, 0, (128, 64), (48, 1), dict(slots=0, merge=1)),   # cut, one warp joins
+    ([30000] * 20 + [1] * 20, 480, 0, (64, 64), (8, 2), dict(slots=0)),               # long enough for warps of their own
+    ([40000] * 2, 630, 600, (64, 64), (17, 1), dict(slots=600, merge=8)),             # long selections are cut, too
+]
+
+
+@pytest.mark.parametrize("lens,width,n_sel,dims,heads,want", SHARING, ids=[str(i) for i in range(len(SHARING))])
+def test_attend_however_the_work_is_shared(lens, width, n_sel, dims, heads, want):
+    (hq, hkv), n = heads, len(lens)
+    plan = _plan(n, hq, hkv, dims, width, n_sel, 64, 0)
+    assert {k: plan[k] for k in want} == want
+    gen = _gen(40 + n)
+    num_pages = sum((x + 63) // 64 for x in lens)
+    pages, lens, _ = _batch(lens, None, num_pages, gen, width)
+    cache = _random_cache(num_pages, hkv, dims, gen)
+    q = torch.randn(n, hq, dims[0], generator=gen).bfloat16()
+    sel = None
+    if n_sel:
+        sel = torch.randint(-1, width, (n, hkv, n_sel), generator=gen, dtype=torch.int32)
+        sel[:, :, 0] = torch.clamp(lens - 1, min=0).view(-1, 1) // 64
+    args = _cuda(q, cache, pages, lens)
+    got = ops.cache_attend(*args, sel=None if sel is None else sel.cuda())
+    ref = oc.attend(q.double().numpy(), cache.numpy(), pages.numpy(), lens.numpy(), None if sel is None else sel.numpy())
+    _check(got, ref, dims[0], torch.bfloat16)
+    again = ops.cache_attend(*args, sel=None if sel is None else sel.cuda())
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    # the same rows through `out`, with cu_seqlens, and one row of no sequence behind, which stays
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    q1 = torch.cat((args[0], args[0][:1]))
+    s1 = None if sel is None else torch.cat((sel, sel[:1])).cuda()
+    out = torch.full((n + 1, hq, dims[1]), 3.0, device="cuda")
+    o, lse = ops.cache_attend(q1, *args[1:], sel=s1, cu_seqlens=cu, out=out, accumulate=True)
+    assert (o[n] == 3).all() and torch.isneginf(lse[n]).all()
+    tol = _tolerances(*ref, dims[0], torch.float32)[0]
+    assert (np.abs(o[:n].double().cpu().numpy() - 3 - ref[0]) <= tol + 2.0**-21).all()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attend_random_calls(seed):
+    """Shapes, tables and lengths at random, broken ones among them."""
+    rng = np.random.default_rng(100 + seed)
+    gen = _gen(100 + seed)
+    dims, dtype = DIMS[rng.integers(4)], DTYPES[rng.integers(2)]
+    hkv = int(rng.integers(1, 5))
+    hq = hkv * int(rng.choice([1, 3, 8, 9, 16, 20]))
+    S, width, P = int(rng.integers(1, 12)), int(rng.integers(1, 24)), 64
+    lens = np.where(rng.random(S) < 0.2, rng.choice([0, -3, width * 64, width * 64 + 5]), rng.integers(1, width * 64 + 1, S))
+    pages = rng.permutation(np.tile(np.arange(P), S * width // P + 1))[:S * width].reshape(S, width).astype(np.int32)
+    pages[rng.random((S, width)) < 0.1] = rng.choice([-1, P, P + 7, -2**31])
+    rows = None if rng.random() < 0.4 else rng.integers(0, 5, S)
+    n = S if rows is None else int(rows.sum()) + int(rng.integers(0, 3))
+    cu = None if rows is None else np.concatenate(([0], rows.cumsum())).astype(np.int32)
+    n = max(n, 1) if rows is not None else n
+    n_sel = int(rng.choice([0, 0, 1, 7, 40]))
+    l_prime = int(rng.choice([64, 128, 256]))
+    window = int(rng.choice([0, 0, 1, 63, 200, 5000]))
+    cache = _random_cache(P, hkv, dims, gen)
+    q = torch.randn(n, hq, dims[0], generator=gen).to(dtype)
+    sel = rng.integers(-2, width * 64 // l_prime + 2, (n, hkv, n_sel)).astype(np.int32) if n_sel else None
+    t = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+    lens = lens.astype(np.int32)
+    got = ops.cache_attend(q.cuda(), cache.cuda(), t(pages), t(lens), sel=t(sel), l_prime=l_prime, window=window, cu_seqlens=t(cu))
+    ref = oc.attend(q.double().numpy(), cache.numpy(), pages, lens, sel, l_prime, window, cu)
+    _check(got, ref, dims[0], dtype, f"seed {seed}")
 
 
 def test_attend_scale_and_large_queries():
