@@ -99,33 +99,44 @@ struct Split {
 };
 constexpr uint32_t kTeam = 8;     // largest team: a block
 constexpr uint32_t kCluster = 8;  // largest cluster of blocks
-constexpr uint32_t kJoins = 4;    // what the second kernel costs, in slots of a warp
 constexpr uint32_t kLong = 16;    // slots of a warp from which on warps of their own are better than teams where rows are cut
+// What things take, in quarters of the time that a warp needs for a slot while it has its quarter of the SM for itself
+// (2000 cycles): a slot beside another warp, a team's join, the second kernel.
+constexpr uint32_t kSlotAlone = 4, kSlotShared = 7, kJoin = 5, kMerge = 18;
+
+// Time of whole rows of at most `longest` slots with teams of `team` warps.
+NSA_HD uint64_t whole_rows(uint32_t rows, uint32_t longest, uint32_t warps, uint32_t team) {
+  const uint32_t slot = (uint64_t)rows * team * 2 > warps ? kSlotShared : kSlotAlone;
+  return (uint64_t)ceil_div(rows, warps / team) * ((uint64_t)ceil_div(longest, team) * slot + (team > 1 ? kJoin : 0));
+}
+NSA_HD uint32_t best_team(uint32_t rows, uint32_t longest, uint32_t warps) {
+  uint32_t best = 1;
+  for (uint32_t team = 2; team <= kTeam; team *= 2)
+    if (whole_rows(rows, longest, warps, team) < whole_rows(rows, longest, warps, best)) best = team;
+  return best;
+}
 
 // `longest`: slots of the longest row (>= 1), `total` < 2^31: of all rows; `warps`: a multiple of kTeam.
 NSA_HD Split split_line(uint32_t rows, uint32_t total, uint32_t longest, uint32_t warps) {
   Split s;
-  s.team = kTeam;
-  while (s.team > 1 && ((uint64_t)rows * s.team > warps || longest <= s.team / 2)) s.team /= 2;
-  const uint32_t whole = ceil_div(rows, warps / s.team);
-  const uint64_t uncut = (uint64_t)whole * ceil_div(longest, s.team);
-  s.cut = ceil_div(ceil_div(total, warps / s.team), s.team) + kJoins < uncut;
-  if (s.cut && total / warps >= kLong) s.team = 1;
-  s.share = s.cut ? ceil_div(total, warps / s.team) : whole;
+  s.team = best_team(rows, longest, warps);
+  const uint32_t cutting = total / warps >= kLong ? 1 : kTeam, share = ceil_div(total, warps / cutting);
+  const uint64_t cut = (uint64_t)ceil_div(share, cutting) * kSlotShared + (cutting > 1 ? kJoin : 0) + kMerge;
+  s.cut = cut < whole_rows(rows, longest, warps, s.team);
+  if (s.cut) s.team = cutting;
+  s.share = s.cut ? share : ceil_div(rows, warps / s.team);
   return s;
 }
 // Whether split_line can cut rows of at most `longest` slots at all.
 NSA_HD bool may_cut(uint32_t rows, uint32_t longest, uint32_t warps) {
-  uint32_t team = kTeam;
-  while (team > 1 && (uint64_t)rows * team > warps) team /= 2;
-  return (uint64_t)ceil_div(rows, warps / team) * ceil_div(longest, team) > kJoins + 1;
+  return whole_rows(rows, longest, warps, best_team(rows, longest, warps)) > kSlotShared + kMerge;
 }
 // Blocks that share each row, in a cluster, where rows are so few that most SMs would have none: at most as many as leave
-// each a slot for every second warp, and only where no warp gets more than cutting the rows would cost.  1: no clusters.
+// each a slot for every second warp, and only where no warp gets many.  1: no clusters.
 NSA_HD uint32_t cluster_of(uint32_t rows, uint32_t longest, uint32_t warps) {
   uint32_t n = kCluster;
   while (n > 1 && ((uint64_t)rows * kTeam * n > warps || longest < kTeam * n / 2)) n /= 2;
-  return ceil_div(longest, kTeam * n) <= kJoins + 1 ? n : 1;
+  return ceil_div(longest, kTeam * n) <= 5 ? n : 1;
 }
 
 }  // namespace cache

@@ -400,6 +400,10 @@ __device__ __forceinline__ void scale_q(uint32_t (&q)[N], bool half, float& fact
   }
 }
 
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool half) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return half ? pack_half(lo, hi) : *reinterpret_cast<const uint32_t*>(&b);
+}
 // Four neighbouring values of the result of (row, query head) `at`, times k.
 template <int DV>
 __device__ __forceinline__ void store4(const AttendArgs& a, int64_t at, int d, float4 v, float k) {
@@ -413,14 +417,8 @@ __device__ __forceinline__ void store4(const AttendArgs& a, int64_t at, int d, f
     *p = v;
     return;
   }
-  uint2 w;
-  if (a.o_dtype == kF16) {
-    w = make_uint2(pack_half(v.x, v.y), pack_half(v.z, v.w));
-  } else {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-    w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at * DV + d) = w;
+  const bool half = a.o_dtype == kF16;
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at * DV + d) = make_uint2(pack16(v.x, v.y, half), pack16(v.z, v.w, half));
 }
 __device__ __forceinline__ void store_lse(const AttendArgs& a, int64_t at, float m, float l) {
   if (a.lse != nullptr) a.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
@@ -952,7 +950,8 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     while (tail - issued < C::STAGES && tail - head <= C::kQueue - 32 && cur.next < cur.end)
       tail = Worker<C>::resolve(a, cur, starts, queue, tail, every, first_slot, lane);
     if (issued < tail) {
-      const uint8_t* src = Worker<C>::record_of(queue[issued % C::kQueue]);
+      const int4 e = queue[issued % C::kQueue];
+      const uint8_t* src = Worker<C>::record_of(e);
       const int stage = issued++ % C::STAGES;
       if (src != nullptr && !lost && !a.stall) {
         if (lane == 0) copy_record(ring + stage * C::kRecord, src, C::kRecord, bars + stage);

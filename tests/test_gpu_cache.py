@@ -293,7 +293,7 @@ SHARING = [
     ([700, 1, 650], 16, 9, (192, 128), (64, 8), dict(cluster=2, merge=0)),
     ([900] * 30, 40, 16, (128, 64), (8, 4), dict(cluster=1, team=8, merge=0)),
     ([500] * 60, 8, 16, (128, 128), (32, 4), dict(cluster=1, team=4, merge=0)),
-    ([300] * 120, 8, 5, (64, 64), (32, 4), dict(cluster=1, team=2, merge=0)),
+    ([900] * 120, 16, 16, (64, 64), (32, 4), dict(cluster=1, team=2, merge=0)),
     ([300] * 600, 6, 3, (64, 64), (4, 2), dict(cluster=1, team=1, merge=0)),
     ([130, 70, 0, 200] * 500, 60, 0, (64, 64), (2, 1), dict(slots=60, cluster=1)),    # more rows than a ragged line takes
     ([25000], 391, 0, (128, 128), (16, 1), dict(slots=0, merge=8)),                   # cut, eight warps join
