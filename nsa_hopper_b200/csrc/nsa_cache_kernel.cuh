@@ -353,6 +353,7 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 __device__ __forceinline__ int sequence_of_warp(const Batch& b, int row, int lane) {
   if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
   int lo = 0, hi = b.n_seqs;  // the last s with cu[s] <= row, if there is one, is in [lo, hi)
+#pragma unroll 1
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32;
     const int at = lo + lane * step;
@@ -421,7 +422,7 @@ __device__ __forceinline__ void store4(const AttendArgs& a, int64_t at, int d, f
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at * DV + d) = make_uint2(pack16(v.x, v.y, half), pack16(v.z, v.w, half));
 }
 __device__ __forceinline__ void store_lse(const AttendArgs& a, int64_t at, float m, float l) {
-  if (a.lse != nullptr) a.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
+  if (a.lse != nullptr) a.lse[at] = l != 0.0f ? (m + __log2f(l)) * 0.693147180559945309f : -INFINITY;
 }
 
 template <class C>
@@ -438,28 +439,27 @@ struct Worker {
     int seq, first, last;  // first and one-past-last visible key
     int entry;             // lane i: entry i of the row's selection (n_sel <= 32)
     unsigned twice;        // bit i: entry i stands before (a selection is a set)
+    bool entered;          // seq to twice are those of (n, hm)
   };
 
-  // Called for every KV head and tile of a row; what depends on the row alone is worked out at the first.
-  static __device__ __forceinline__ void enter_row(const AttendArgs& a, Cursor& c, const uint32_t* starts, bool same_row,
-                                                   int lane) {
+  static __device__ __forceinline__ void enter_row(const AttendArgs& a, Cursor& c, const uint32_t* starts, int lane) {
     const int h = c.hm / a.tiles, g0 = c.hm % a.tiles * C::kHeads;
     if (a.sel != nullptr && a.n_sel <= 32)
       c.entry = lane < a.n_sel ? a.sel[((int64_t)c.n * a.hkv + h) * a.n_sel + lane] : -1;
     // the row's queries on their way into L2 (begin() loads them when its turn comes)
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)c.n * a.q_row + (int64_t)(h * a.group + g0) * a.q_head;
     constexpr int kLines = DQK / 64;
+#pragma unroll 1
     for (int i = lane; i < min(C::kHeads, a.group - g0) * kLines; i += 32)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i / kLines * a.q_head + i % kLines * 64));
-    if (!same_row) {
-      c.seq = sequence_of_warp(a.b, c.n, lane);
-      const int pos = c.seq < 0 ? -1 : position_of(a.b, c.seq, c.n);
-      c.last = keys_up_to(a.b, pos);
-      c.first = pos < 0 ? 0 : first_key(pos, a.window);
-      c.len = a.slots ? a.slots : starts[c.n + 1] - starts[c.n];
-    }
+    c.seq = sequence_of_warp(a.b, c.n, lane);
+    const int pos = c.seq < 0 ? -1 : position_of(a.b, c.seq, c.n);
+    c.last = keys_up_to(a.b, pos);
+    c.first = pos < 0 ? 0 : first_key(pos, a.window);
+    c.len = a.slots ? a.slots : starts[c.n + 1] - starts[c.n];
     if (a.sel != nullptr && a.n_sel <= 32)
       c.twice = __ballot_sync(0xFFFFFFFFu, (__match_any_sync(0xFFFFFFFFu, c.entry) & ((1u << lane) - 1)) != 0);
+    c.entered = true;
   }
 
   // This warp's part (every team-th, from `turn` on) of the next 32 * team slots of the row into the queue, those that show no
@@ -469,6 +469,7 @@ struct Worker {
   static __device__ __forceinline__ int resolve(const AttendArgs& a, Cursor& c, const uint32_t* starts, int4* queue, int tail,
                                                 int team, int turn, int lane) {
     const int rows_h = a.hkv * a.tiles;
+    if (!c.entered) enter_row(a, c, starts, lane);
     const int count = min((uint32_t)(32 * team), min((uint32_t)(c.len - c.j), c.end - c.next));
     const int own = (count - turn + team - 1) / team;  // (0 where count <= turn)
     const int j = c.j + lane * team + turn;
@@ -482,9 +483,9 @@ struct Worker {
       const int32_t* row = a.sel + ((int64_t)c.n * a.hkv + c.hm / a.tiles) * a.n_sel;
       const int at = j / a.per, entry = row[at];
       sub = selected_sub(entry, j - at * a.per, a.per, c.first, c.last);
-      if (sub >= 0)
-        for (int i = 0; i < at; ++i)
-          if (row[i] == entry) sub = -1;
+#pragma unroll 1
+      for (int i = 0; i < at && sub >= 0; ++i)
+        if (row[i] == entry) sub = -1;
     }
     const int page = sub < 0 || c.seq < 0 ? -1 : page_of(a.b, c.seq, sub);
     const bool over = c.j + count == c.len || c.next + count == c.end;
@@ -504,9 +505,8 @@ struct Worker {
     c.j += count;
     if (c.j == c.len && c.next < c.end) {  // the next row
       c.j = 0;
-      const bool same_row = ++c.hm < rows_h;
-      if (!same_row) c.hm = 0, ++c.n;
-      enter_row(a, c, starts, same_row, lane);
+      if (++c.hm == rows_h) c.hm = 0, ++c.n;
+      c.entered = false;
     }
     return tail + __popc(kept);
   }
@@ -734,21 +734,36 @@ struct Worker {
     }
     if (team == 1) {
       if (left) return;
+      const bool whole = part == nullptr, wide = !whole || a.o_dtype == kF32;
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int x = 8 * h + 2 * c + e;
           if (x >= used) continue;
-          if (part != nullptr) {
-            if (r == 0) part[kHeads * DV + x] = top[h][e], part[kHeads * (DV + 1) + x] = sum[h][e];
+          if (r == 0) {
+            if (whole) store_lse(a, at0 + x, top[h][e], sum[h][e]);
+            else part[kHeads * DV + x] = top[h][e], part[kHeads * (DV + 1) + x] = sum[h][e];
+          }
+          const float k = !whole ? 1.0f : sum[h][e] != 0.0f ? __fdividef(weight, sum[h][e]) : 0.0f;
+          if (wide) {
+            float4* to = reinterpret_cast<float4*>((whole ? static_cast<float*>(a.o) + at0 * DV : part) + x * DV + r * (DV / 8));
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) reinterpret_cast<float4*>(part + x * DV + r * (DV / 8))[i] = piece(h, e, i);
-          } else {
-            if (r == 0) store_lse(a, at0 + x, top[h][e], sum[h][e]);
-            const float k = sum[h][e] != 0.0f ? weight / sum[h][e] : 0.0f;
+            for (int i = 0; i < PIECES; ++i) {
+              float4 v = whole && a.accumulate ? to[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              const float4 y = piece(h, e, i);
+              v.x += y.x * k, v.y += y.y * k, v.z += y.z * k, v.w += y.w * k;
+              to[i] = v;
+            }
+          } else {  // 16 bytes at once
+            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + (at0 + x) * DV + r * (DV / 8));
+            const bool half = a.o_dtype == kF16;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) store4<DV>(a, at0 + x, r * (DV / 8) + 4 * i, piece(h, e, i), k);
+            for (int i = 0; i < PIECES; i += 2) {
+              const float4 y = piece(h, e, i), z = piece(h, e, i + 1);
+              to[i / 2] = make_uint4(pack16(y.x * k, y.y * k, half), pack16(y.z * k, y.w * k, half),
+                                     pack16(z.x * k, z.y * k, half), pack16(z.z * k, z.w * k, half));
+            }
           }
         }
       return;
@@ -767,8 +782,9 @@ struct Worker {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int x = 8 * h + 2 * c + e;
-        float common = kNone;
-        for (int w = 0; w < team; ++w) common = fmaxf(common, join[w * C::kJoin + kMl + x]);
+        float common = r < team ? join[r * C::kJoin + kMl + x] : kNone;
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) common = fmaxf(common, __shfl_xor_sync(0xFFFFFFFFu, common, w));
         k[h][e] = exp2_fast(top[h][e] - common);
         if (r == 0) mine[kMl + kHeads + x] = sum[h][e] * k[h][e], mine[kMl + 2 * kHeads + x] = common;
       }
@@ -789,24 +805,26 @@ struct Worker {
           }
         }
       named_barrier(barrier, team * 32);
+#pragma unroll 1
       for (int i = turn * 32 + lane; i < kHeads * 8 * CS; i += team * 32) {
         const int x = i / (8 * CS), at = i % (8 * CS), d = at / CS * (DV / 8) + (t * CS + at % CS) * 4;
         if (x >= used || left) continue;
-        const int y = x >> 1 & 3, place = x * (8 * CS) + (at ^ (CS == 4 ? y : (y & 1) | (y & 2) << 1));
+        const int q = x >> 1 & 3, place = x * (8 * CS) + (at ^ (CS == 4 ? q : (q & 1) | (q & 2) << 1));
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float all = 0.0f;
-        for (int w = 0; w < team; ++w) {
-          const float* from = join + w * C::kJoin;
-          const float4 z = reinterpret_cast<const float4*>(from)[place];
-          v.x += z.x, v.y += z.y, v.z += z.z, v.w += z.w;
-          all += from[kMl + kHeads + x];
+#pragma unroll 1
+        for (int w = 0; w < team; w += 2) {
+          const float *from = join + w * C::kJoin, *next = from + C::kJoin;
+          const float4 y = reinterpret_cast<const float4*>(from)[place], z = reinterpret_cast<const float4*>(next)[place];
+          v.x += y.x + z.x, v.y += y.y + z.y, v.z += y.z + z.z, v.w += y.w + z.w;
+          all += from[kMl + kHeads + x] + next[kMl + kHeads + x];
         }
         const float common = mine[kMl + 2 * kHeads + x];
         if (part != nullptr) {
           *reinterpret_cast<float4*>(part + x * DV + d) = v;
           if (at == 0 && t == 0) part[kHeads * DV + x] = common, part[kHeads * (DV + 1) + x] = all;
         } else {
-          store4<DV>(a, at0 + x, d, v, all != 0.0f ? weight / all : 0.0f);
+          store4<DV>(a, at0 + x, d, v, all != 0.0f ? __fdividef(weight, all) : 0.0f);
           if (at == 0 && t == 0) store_lse(a, at0 + x, common, all);
         }
       }
@@ -869,6 +887,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     if (line128 < (int64_t)(a.b.n_seqs - 1) * a.b.page_row + a.b.width)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(a.b.pages + line128));
     // the ragged line: every block counts the slots before each row (n_rows <= kMaxRagged)
+#pragma unroll 1
     for (int n = threadIdx.x; n < a.b.n_rows; n += C::NW * 32) {
       const int seq = sequence_of(a.b, n), pos = seq < 0 ? -1 : position_of(a.b, seq, n);
       starts[n + 1] = running_slots(pos < 0 ? 0 : first_key(pos, a.window), keys_up_to(a.b, pos));
@@ -877,6 +896,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     if (warp == 0) {
       uint32_t sum = 0, longest = 0;
       if (lane == 0) starts[0] = 0;
+#pragma unroll 1
       for (int n0 = 0; n0 < a.b.n_rows; n0 += 32) {
         uint32_t x = n0 + lane < a.b.n_rows ? starts[n0 + lane + 1] : 0;
         longest = max(longest, x);
@@ -896,6 +916,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     total = line[0];
     split = split_line(rows, total, line[1], a.warps);
     if (blockIdx.x == 0 && a.part != nullptr) {
+#pragma unroll 1
       for (int n = threadIdx.x; n <= a.b.n_rows; n += C::NW * 32) a.starts[n] = starts[n];
       if (threadIdx.x == 0) a.starts[a.b.n_rows + 1] = split.cut ? split.share : 0;
     }
@@ -921,6 +942,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
       row = cur.next / a.slots;
     } else {
       int lo = 0, hi = a.b.n_rows;
+#pragma unroll 1
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (starts[mid] * rows_h <= cur.next) lo = mid;
@@ -936,39 +958,38 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   }
   cur.n = row / rows_h, cur.hm = row % rows_h, cur.j = cur.next - start_of(row);
   const bool cut_before = cur.j != 0;  // the first row's earlier slots are another team's
-  Worker<C>::enter_row(a, cur, starts, false, lane);
+  cur.entered = false;
 
   if (lane < C::STAGES) ptx::mbar_init(bars + lane, 1);
   ptx::fence_mbar_init();
   __syncwarp();
   Worker<C> w;
-  w.ask(a, row, lane);
-  int head = 0, tail = 0, issued = 0;
+  int head, tail = 0, issued = 0;
   uint32_t phases = 0, flying = 0;  // each stage's parity of the next phase; copies on their way
   bool lost = false;                // a copy did not come: rows from here on are NaN
-  auto issue = [&] {
+  bool fresh = true, first_row = true;
+  // the ring holds STAGES records: STAGES - 1 on their way (the first of them before the loop's first page) while one is
+  // worked on
+#pragma unroll 1
+  for (head = 1 - C::STAGES;; ++head) {
+#pragma unroll 1
     while (tail - issued < C::STAGES && tail - head <= C::kQueue - 32 && cur.next < cur.end)
       tail = Worker<C>::resolve(a, cur, starts, queue, tail, every, first_slot, lane);
+    if (head == 1 - C::STAGES) w.ask(a, row, lane);  // (before the pages: they would be ahead of it in the memory's queue)
     if (issued < tail) {
-      const int4 e = queue[issued % C::kQueue];
-      const uint8_t* src = Worker<C>::record_of(e);
+      const uint8_t* src = Worker<C>::record_of(queue[issued % C::kQueue]);
       const int stage = issued++ % C::STAGES;
       if (src != nullptr && !lost && !a.stall) {
         if (lane == 0) copy_record(ring + stage * C::kRecord, src, C::kRecord, bars + stage);
         flying |= 1u << stage;
       }
     }
-  };
-  // the ring holds STAGES records: STAGES - 1 on their way while one is worked on
-  for (int i = 0; i < C::STAGES - 1; ++i) issue();
-  w.begin(a, lane);
-  bool fresh = false, first_row = true;
-  while (head < issued) {
-    issue();
+    if (head < 0) continue;
+    if (head == issued) break;
     const int4 e = queue[head % C::kQueue];
     const int stage = head % C::STAGES;
     if (fresh) {
-      w.ask(a, (uint32_t)e.w >> 1, lane);
+      if (!first_row) w.ask(a, (uint32_t)e.w >> 1, lane);
       w.begin(a, lane);
     }
     fresh = e.w & 1;
@@ -991,7 +1012,6 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
       first_row = false;
     }
     __syncwarp();
-    ++head;
   }
   if (a.cluster > 1) join_cluster<C>(a, row, reinterpret_cast<const float*>(smem), rank);
   if (lost) {  // the block's memory is not given up under a copy (bounded, too)
