@@ -299,7 +299,7 @@ struct AttendCfg {
   static constexpr int kPart = kHeads * (DV + 2);              // floats of a partial result: O, m, sum
   static constexpr int kJoin = kHeads * (DV / ROUNDS + 4);     // floats of a warp in a team's join: O of a round, m, sum, max
   static constexpr int kWarp = STAGES * (kRecord + 8) + kQueue * 16 + kJoin * 4;
-  static constexpr int kSmem = NW * kWarp + (kMaxRagged + 1) * 4;
+  static constexpr int kSmem = NW * kWarp + (kMaxRagged + 2) * 4;
   static_assert(kSmem + 128 <= 232448, "227 KB of shared memory a block, the static variables included");
 };
 
@@ -463,15 +463,17 @@ struct Worker {
   }
 
   // This warp's part (every team-th, from `turn` on) of the next 32 * team slots of the row into the queue, those that show no
-  // key left out but for the warp's last entry of the row's slots here (its owners have to leave the row's result; one without a slot
-  // of its own gets an empty entry).  An entry: the record's address (0: none), the first and one past the last visible key
-  // of the sub-block (8 bits each), and the row (times 2, + 1 if it is the warp's last entry of it).
+  // key left out but for the warp's last entry of the row's slots here (its owners have to leave the row's result; one
+  // without a slot of its own gets an empty entry).  An entry: the record's address (0: none), the first and one past the
+  // last visible key of the sub-block (8 bits each), and the row (times 2, + 1 if it is the warp's last entry of it).
   static __device__ __forceinline__ int resolve(const AttendArgs& a, Cursor& c, const uint32_t* starts, int4* queue, int tail,
                                                 int team, int turn, int lane) {
     const int rows_h = a.hkv * a.tiles;
     if (!c.entered) enter_row(a, c, starts, lane);
-    const int count = min((uint32_t)(32 * team), min((uint32_t)(c.len - c.j), c.end - c.next));
-    const int own = (count - turn + team - 1) / team;  // (0 where count <= turn)
+    // (behind the last key of a row that takes its sub-blocks one after the other there is nothing to look for)
+    const bool behind = a.sel == nullptr && c.j >= running_slots(c.first, c.last);
+    const int left = min((uint32_t)(c.len - c.j), c.end - c.next), count = behind ? left : min(32 * team, left);
+    const int own = behind ? 0 : (count - turn + team - 1) / team;  // (0 where count <= turn)
     const int j = c.j + lane * team + turn;
     int sub = -1;
     if (a.sel == nullptr) {

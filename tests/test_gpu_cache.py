@@ -296,6 +296,7 @@ SHARING = [
     ([900] * 120, 16, 16, (64, 64), (32, 4), dict(cluster=1, team=2, merge=0)),
     ([300] * 600, 6, 3, (64, 64), (4, 2), dict(cluster=1, team=1, merge=0)),
     ([130, 70, 0, 200] * 500, 60, 0, (64, 64), (2, 1), dict(slots=60, cluster=1)),    # more rows than a ragged line takes
+    ([130, 70, 0, 6000] + [200] * 2000, 900, 0, (64, 64), (2, 1), dict(slots=900, cluster=1)),  # and a wide table
     ([25000], 391, 0, (128, 128), (16, 1), dict(slots=0, merge=8)),                   # cut, eight warps join
     ([20000, 1, 0, 64, 9999], 2000, 0, (192, 128), (6, 2), dict(slots=0, merge=8)),
     ([5000] * 40 + [0, 1, 64], 200, 0, (128, 64), (48, 1), dict(slots=0, merge=1)),   # cut, one warp joins
