@@ -75,6 +75,27 @@ int done(cudaError_t e, const char* what) {
   return fail(NSA_OK, "%s", "");
 }
 
+// A programmatic launch (see start_in_order), in clusters of `cluster` blocks.
+template <class Args>
+cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const Args& a) {
+  cudaLaunchAttribute attr[2];
+  memset(attr, 0, sizeof(attr));
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 // ------------------------------------------------------------------ attention
 // A KV head's G query heads: one tile of 8, or tiles of 16.
 int tiles_of(int group) { return group <= 8 ? 1 : (group + 15) / 16; }
@@ -190,31 +211,11 @@ int launch_attend(const AttendArgs& a, const nsa_cache_attend_plan_info& p, int 
       g_attr_done[dev] |= bit;
     }
   }
-  cudaLaunchAttribute attr;
-  memset(&attr, 0, sizeof(attr));
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)p.grid);
-  cfg.blockDim = dim3((unsigned)p.threads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, nsa::cache::attend_kernel<C>, a);
+  cudaError_t e = launch(&nsa::cache::attend_kernel<C>, dim3((unsigned)p.grid), p.threads, C::kSmem, p.cluster, st, a);
   if (e != cudaSuccess || p.merge == 0) return done(e, "cache attention launch");
   const int64_t units = (int64_t)a.b.n_rows * a.hq;
-  memset(&attr, 0, sizeof(attr));
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(p.merge == 1 ? (units + 7) / 8 : units));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  cfg.numAttrs = 1;
-  e = p.merge == 1 ? cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 1>, a)
-                   : cudaLaunchKernelEx(&cfg, nsa::cache::merge_kernel<C, 8>, a);
+  e = p.merge == 1 ? launch(&nsa::cache::merge_kernel<C, 1>, dim3((unsigned)((units + 7) / 8)), 256, 0, 1, st, a)
+                   : launch(&nsa::cache::merge_kernel<C, 8>, dim3((unsigned)units), 256, 0, 1, st, a);
   return done(e, "cache attention's merge launch");
 }
 
@@ -294,9 +295,9 @@ int nsa_cache_write(const nsa_cache_batch* b, const void* k, const void* v, int6
                                    static_cast<uint8_t*>(b->cache), page_stride_of(b), b->heads_kv, in_dtype == NSA_DTYPE_F16};
   const int64_t threads = (int64_t)b->n_rows * b->heads_kv * std::max(b->d_qk, b->d_v) / (2 * nsa::cache::kGroup);
   return for_dims(b->d_qk, b->d_v, [&](auto dqk, auto dv) {
-    nsa::cache::write_kernel<decltype(dqk)::value, decltype(dv)::value>
-        <<<dim3((unsigned)((threads + 255) / 256), 2), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-    return done(cudaGetLastError(), "cache write launch");
+    return done(launch(&nsa::cache::write_kernel<decltype(dqk)::value, decltype(dv)::value>, dim3((unsigned)((threads + 255) / 256), 2),
+                       256, 0, 1, reinterpret_cast<cudaStream_t>(stream), a),
+                "cache write launch");
   });
 }
 
@@ -315,9 +316,9 @@ int nsa_cache_read(const nsa_cache_batch* b, void* k, void* v, int32_t out_dtype
                                   out_dtype};
   const int64_t groups = (int64_t)b->n_rows * b->heads_kv * std::max(b->d_qk, b->d_v) / nsa::cache::kGroup;
   return for_dims(b->d_qk, b->d_v, [&](auto dqk, auto dv) {
-    nsa::cache::read_kernel<decltype(dqk)::value, decltype(dv)::value>
-        <<<dim3((unsigned)((groups + 255) / 256), 2), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-    return done(cudaGetLastError(), "cache read launch");
+    return done(launch(&nsa::cache::read_kernel<decltype(dqk)::value, decltype(dv)::value>, dim3((unsigned)((groups + 255) / 256), 2),
+                       256, 0, 1, reinterpret_cast<cudaStream_t>(stream), a),
+                "cache read launch");
   });
 }
 

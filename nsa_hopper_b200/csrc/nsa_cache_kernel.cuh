@@ -49,6 +49,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// Every kernel here is launched programmatically (while the stream's kernel before it still runs, if that one allows it):
+// it lets the next one be launched, and touches no memory before all earlier ones have ended.
+__device__ __forceinline__ void start_in_order() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ 4-bit conversions
 // Two codes of byte I of `w` as fp16 pair (low nibble in the low half).
 template <int I>
@@ -175,6 +182,7 @@ __device__ __forceinline__ void write_groups(const WriteArgs& a, uint32_t i) {
 
 template <int DQK, int DV>
 __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
+  start_in_order();
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (blockIdx.y == 0) write_groups<DQK, DV, 0>(a, i);
   else write_groups<DQK, DV, 1>(a, i);
@@ -233,6 +241,7 @@ __device__ __forceinline__ void read_group(const ReadArgs& a, uint32_t i) {
 
 template <int DQK, int DV>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
+  start_in_order();
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (blockIdx.y == 0) read_group<DQK, DV, 0>(a, i);
   else read_group<DQK, DV, 1>(a, i);
@@ -879,7 +888,9 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   int4* queue = reinterpret_cast<int4*>(join + C::NW * C::kJoin) + warp * C::kQueue;
   uint64_t* bars = reinterpret_cast<uint64_t*>(queue + (C::NW - warp) * C::kQueue) + warp * C::STAGES;
   uint32_t* starts = reinterpret_cast<uint32_t*>(smem + C::NW * C::kWarp);
-  asm volatile("griddepcontrol.launch_dependents;");  // (merge_kernel, whose blocks then wait for the end of this one)
+  if (lane < C::STAGES) ptx::mbar_init(bars + lane, 1);
+  ptx::fence_mbar_init();
+  start_in_order();
   const uint32_t rows_h = a.hkv * a.tiles, rows = a.b.n_rows * rows_h;
   uint32_t total = rows * a.slots;
   Split split = a.split;
@@ -962,8 +973,6 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   const bool cut_before = cur.j != 0;  // the first row's earlier slots are another team's
   cur.entered = false;
 
-  if (lane < C::STAGES) ptx::mbar_init(bars + lane, 1);
-  ptx::fence_mbar_init();
   __syncwarp();
   Worker<C> w;
   int head, tail = 0, issued = 0;
@@ -1024,14 +1033,13 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
 }
 
 // Joins the parts of the rows that were cut, in the order of the line.  WPH warps share a row's query head:
-// 1 where a row has a few parts, 8 where one row is cut over many teams.  Starts while attend_kernel still runs
-// (programmatic launch) and waits for its end before it reads anything.
+// 1 where a row has a few parts, 8 where one row is cut over many teams.
 template <class C, int WPH>
 __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a) {
   constexpr int DV = C::DV, V4 = DV / 4;
   __shared__ float shared_o[8][DV];
   __shared__ float shared_ml[8][2];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  start_in_order();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rows_h = a.hkv * a.tiles;
   const int64_t unit = WPH == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;  // (row, query head)

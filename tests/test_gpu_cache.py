@@ -569,6 +569,62 @@ def test_waits_are_bounded(n):
     assert err.item() == 0 and torch.equal(o, want[0]) and torch.equal(lse, want[1])
 
 
+def test_calls_in_a_row_keep_their_order():
+    """The kernels are launched before the ones ahead of them end; each must still see what those wrote, and write nothing
+    that they still read: a token overwritten and attended to a hundred times, without and with a wait after each call."""
+    q, cache, pages, lens = _small(25)
+    lens = torch.tensor([500, 64, 2100], dtype=torch.int32, device="cuda")
+    ks = torch.randn(100, 3, 2, 128, device="cuda").bfloat16()
+    results = []
+    for wait in (True, False):
+        c, outs = cache.clone(), []
+        x = torch.zeros_like(ks[0])
+        for k in ks:
+            x.copy_(k)                                   # (a copy, then a kernel of torch's, ahead of the first)
+            ops.cache_write(c, x, x.mul(2), pages, lens)
+            if wait:
+                torch.cuda.synchronize()
+            outs += ops.cache_attend(q, c, pages, lens)
+            if wait:
+                torch.cuda.synchronize()
+            outs += ops.cache_read(c, 128, pages, lens)
+            if wait:
+                torch.cuda.synchronize()
+        results.append(outs)
+    torch.cuda.synchronize()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_captured_behind_copies_and_other_streams():
+    q, cache, pages, lens = _small(26)
+    k = torch.randn(3, 2, 128, device="cuda").bfloat16()
+    c, x, l2 = cache.clone(), torch.zeros_like(q), lens.clone()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    buf = torch.empty(3, 16, 128, device="cuda")
+    with torch.cuda.graph(g):
+        x.copy_(q)                       # a copy node
+        c.copy_(cache)
+        buf.zero_()                      # a memset node
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            o1, _ = ops.cache_attend(x, c, pages, l2, window=100)
+        ops.cache_attend(x, c, pages, l2, out=buf, accumulate=True)
+        main.wait_stream(side)           # two nodes ahead of the next
+        ops.cache_write(c, k, k, pages, l2)
+        o2, _ = ops.cache_attend(x, c, pages, l2)
+    for _ in range(3):
+        q.mul_(-1.5)
+        g.replay()
+        torch.cuda.synchronize()
+        fresh = cache.clone()
+        assert torch.equal(o1, ops.cache_attend(q, fresh, pages, lens, window=100)[0])
+        assert torch.equal(buf, ops.cache_attend(q, fresh, pages, lens, out=torch.zeros_like(buf), accumulate=True)[0])
+        ops.cache_write(fresh, k, k, pages, lens)
+        assert torch.equal(o2, ops.cache_attend(q, fresh, pages, lens)[0])
+
+
 def test_side_stream():
     q, cache, pages, lens = _small(22)
     want = ops.cache_attend(q, cache, pages, lens)
