@@ -303,7 +303,7 @@ int nsa_cache_write(const nsa_cache_batch* batch, const void* k, const void* v, 
                     int64_t v_row_stride, int64_t v_head_stride, int32_t in_dtype, nsa_stream_t stream);
 
 /* Reads the rows back: k [heads_kv, n_rows, d_qk], v [heads_kv, n_rows, d_v] (the packed layout of the varlen forward),
-   contiguous, 16-byte aligned, dtype NSA_DTYPE_BF16, _F16 or _F32.  Absent tokens and rows of no sequence read as zeros.
+   contiguous, 32-byte aligned, dtype NSA_DTYPE_BF16, _F16 or _F32.  Absent tokens and rows of no sequence read as zeros.
    One launch. */
 int nsa_cache_read(const nsa_cache_batch* batch, void* k, void* v, int32_t out_dtype, nsa_stream_t stream);
 

@@ -308,7 +308,7 @@ int nsa_cache_read(const nsa_cache_batch* b, void* k, void* v, int32_t out_dtype
     return fail(NSA_ERR_INVALID_ARG, "out_dtype must be NSA_DTYPE_BF16, NSA_DTYPE_F16 or NSA_DTYPE_F32");
   if (b->n_rows == 0) return done(cudaSuccess, "");
   if (k == nullptr || v == nullptr) return fail(NSA_ERR_INVALID_ARG, "k and v must be non-NULL");
-  if (misaligned(k, 16) || misaligned(v, 16)) return fail(NSA_ERR_INVALID_ARG, "k and v must be 16-byte aligned");
+  if (misaligned(k, 32) || misaligned(v, 32)) return fail(NSA_ERR_INVALID_ARG, "k and v must be 32-byte aligned");
   int sm = 0, dev = 0;
   rc = nsa::host::current_sm_count(&sm, &dev);
   if (rc != NSA_OK) return rc;
@@ -316,8 +316,11 @@ int nsa_cache_read(const nsa_cache_batch* b, void* k, void* v, int32_t out_dtype
                                   out_dtype};
   const int64_t groups = (int64_t)b->n_rows * b->heads_kv * std::max(b->d_qk, b->d_v) / nsa::cache::kGroup;
   return for_dims(b->d_qk, b->d_v, [&](auto dqk, auto dv) {
-    return done(launch(&nsa::cache::read_kernel<decltype(dqk)::value, decltype(dv)::value>, dim3((unsigned)((groups + 255) / 256), 2),
-                       256, 0, 1, reinterpret_cast<cudaStream_t>(stream), a),
+    constexpr int kQk = decltype(dqk)::value, kV = decltype(dv)::value;
+    const int items = groups > 32ll * 256 * sm ? 2 : 1;  // (the border: 32 blocks an SM)
+    return done(launch(items == 2 ? &nsa::cache::read_kernel<kQk, kV, 2> : &nsa::cache::read_kernel<kQk, kV, 1>,
+                       dim3((unsigned)((groups + 256 * items - 1) / (256 * items)), 2), 256, 0, 1,
+                       reinterpret_cast<cudaStream_t>(stream), a),
                 "cache read launch");
   });
 }

@@ -277,6 +277,7 @@ def test_write_and_read_refusals(batch, kw, code):
     if "strides" not in kw and "dtype" not in kw:
         assert lib.nsa_cache_read(ctypes.byref(b), ptr(a["k"]), ptr(a["v"]), a["dtype"], None) == code
     assert lib.nsa_cache_read(ctypes.byref(_batch()), ptr(256), ptr(256), 7, None) == capi.NSA_ERR_INVALID_ARG
+    assert lib.nsa_cache_read(ctypes.byref(_batch()), ptr(256), ptr(272), 0, None) == capi.NSA_ERR_INVALID_ARG
 
 
 def test_struct_layout_matches_header(tmp_path):

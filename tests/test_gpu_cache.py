@@ -167,6 +167,25 @@ def test_write_takes_strided_rows_and_pages():
     assert torch.equal(again, k)
 
 
+@pytest.mark.parametrize("dims,hkv,lens", [((192, 128), 4, [9000, 0, 33001, 7]), ((64, 64), 2, [200001])])
+def test_long_inputs_come_back(dims, hkv, lens):
+    """Enough rows for the kernels' forms for long inputs, an odd number of them, and three rows of no sequence."""
+    gen = _gen(4)
+    n = sum(lens)
+    num_pages = sum((x + 63) // 64 for x in lens)
+    pages, lens, cu = _batch(lens, lens, num_pages, gen)
+    k, v = torch.randn(n + 3, hkv, dims[0], generator=gen).bfloat16(), torch.randn(n + 3, hkv, dims[1], generator=gen).bfloat16()
+    cache = ops.cache_alloc(num_pages, hkv, *dims)
+    kd, vd, pd, ld, cd = _cuda(k, v, pages, lens, cu)
+    ops.cache_write(cache, kd, vd, pd, ld, cd)
+    for dtype in (torch.bfloat16, torch.float32):
+        for x, y in zip(ops.cache_read(cache, dims[0], pd, ld, cd, n + 3, dtype), (k, v)):
+            assert not x[0, :, n:].any()
+            at = torch.cat((torch.arange(0, n, 997), torch.arange(n - 130, n)))
+            np.testing.assert_array_equal(x[0, :, :n].cpu()[:, at].double().numpy().transpose(1, 0, 2),
+                                          oc.values(*oc.quantise(y[at].double().numpy())))
+
+
 def test_absent_tokens_are_skipped():
     """Pages outside the cache, lengths behind the table, negative lengths, rows of no sequence."""
     gen = _gen(3)
