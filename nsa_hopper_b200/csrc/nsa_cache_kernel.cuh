@@ -272,16 +272,17 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 }
 
 // ------------------------------------------------------------------ attention
-// For a row n, KV head h and its G query heads (16 at a time, the M of one tensor-core tile):
+// For a row n, KV head h and its G query heads (8 or 16 at a time: a tile):
 //     z_j = scale * q . k_j,   O = sum_j exp(z_j - m) v_j / sum_j exp(z_j - m),   LSE = m + ln sum_j exp(z_j - m)
 // over the visible keys j, in one pass with the running maximum m (kept in powers of two).
 //
-// A key costs 9/16 (d_qk + d_v) bytes and 2 G (d_qk + d_v) operations: at d = 128 and G = 16 57 operations a
-// byte, so the floor is the cache's bytes from DRAM, provided that turning 4 bits into tensor-core operands keeps
-// up.  Hence the layout of the work: every warp is a worker of its own with a ring of page records in shared
-// memory (bulk copies), and codes go from there straight into the registers that the tensor core reads
-// (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  The cache is the A operand, S^T = K Q^T and
-// O^T = V^T P^T, so that 8 query heads (n) cost half of what 16 cost, and a decoded fragment serves both halves.  For that
+// A key costs 9/16 (d_qk + d_v) bytes and 2 G (d_qk + d_v) operations: at d = 128 and G = 16 57 operations a byte, so the floor
+// is the cache's bytes from DRAM, provided that turning 4 bits into tensor-core operands keeps up.  Hence every warp is
+// a worker of its own with a ring of page records in shared memory (bulk copies), and codes go from there straight into the
+// registers that the tensor core reads (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  (Operands in shared
+// memory, as tcgen05 wants them, would cost 64 KB of shared-memory traffic a page beside the 9 KB that are fetched.)
+// The cache is the A operand, S^T = K Q^T and O^T = V^T P^T, so that 8 query heads cost half the tensor instructions of 16,
+// and a decoded fragment serves both halves.  For that
 //   * the d axis of QK is permuted so that a thread's K fragments are d_qk / 4 consecutive codes of one key: one
 //     wide shared load, one conversion and one product with the scale for each pair, exact in fp16;
 //   * a thread's V fragments are d_v / 8 consecutive codes of four keys, which are interleaved two and two; P^T takes
@@ -292,10 +293,15 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 // largest to within 2^-25 of it).  P is rounded to fp16 (at most 2^-11 of each term): the sum of
 // its fp32 values is the divisor.  Scores, statistics and O are fp32.
 //
+// What binds: a page of 64 keys (d = 128) takes a scheduler 1800 cycles with 16 heads and two warps (2090 with one; 1310 and
+// 1560 with 8 heads), of which half are the issue of 128 tensor instructions, most of the rest 256 conversions and 256 products;
+// DRAM would deliver a page in 1550.  64 rows of up to 32768 keys, 616 MB: 165 us, 3.7 TB/s; 256 rows of 16 selected blocks,
+// 155 MB: 47 us, 3.3 TB/s; one row of 16 blocks: 10.3 us.
+//
 // All (row, page) slots of the call stand in one line that is shared out evenly (split_line): teams of 1 to 8 warps of a
 // block take turns at a row's pages and join their (m, sum, O) in shared memory; a row that is cut between teams leaves
-// partial results in the workspace, and merge_kernel joins them in the order of the line.  Results do not depend on
-// timing.
+// partial results in the workspace, and merge_kernel joins them in the order of the line.  Where rows are few and not
+// long, the blocks of a cluster share each and join through one another's shared memory.  Results do not depend on timing.
 struct AttendArgs {
   Batch b;
   const void* q;                 // [n_rows, Hq, DQK], bf16 or fp16, unit stride along d
