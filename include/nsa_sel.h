@@ -345,7 +345,7 @@ typedef struct nsa_cache_attend_plan_info {
   int32_t share;              /* whole rows of a team, or its slots where rows are cut (merge != 0) */
   int32_t grid, threads, smem_bytes;
   int32_t merge;              /* warps that join the parts of a cut row's head; 0 = no row is cut, one launch */
-  int32_t tiles;              /* 16-row tiles of a KV head's query heads */
+  int32_t tiles;              /* tiles of a KV head's query heads: one of up to 8, or as many of 16 as they need */
 } nsa_cache_attend_plan_info;
 int nsa_cache_attend_plan(const nsa_cache_attend_desc* desc, int32_t sm_count, nsa_cache_attend_plan_info* out);
 

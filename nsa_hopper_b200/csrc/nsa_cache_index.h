@@ -80,7 +80,7 @@ NSA_HD int first_key(int pos, int window) { return window > 0 && pos + 1 > windo
 NSA_HD int selected_sub(int entry, int part, int per, int first, int end) {
   if (entry < 0 || end <= 0 || entry > (end - 1) / (per * kPage)) return -1;  // (before the product can overflow)
   const int sub = entry * per + part;
-  return sub * kPage < end && (sub + 1) * kPage > first ? sub : -1;
+  return sub <= (end - 1) / kPage && sub >= first / kPage ? sub : -1;  // (the last one's end may be 2^31)
 }
 NSA_HD int running_sub(int j, int first, int end) {
   const int sub = first / kPage + j;

@@ -107,6 +107,21 @@ def test_sub_blocks(index):
     assert [index.first(p, w) for p, w in ((5, 0), (5, 1), (5, 6), (5, 7), (5, BIG), (BIG - 1, 3))] == [0, 5, 0, 0, 0, BIG - 3]
 
 
+def test_sub_blocks_of_the_longest_sequences(index):
+    """Positions up to 2^31 - 2: the last sub-block ends at 2^31, which no int holds."""
+    top = 2**31 - 1  # keys
+    for per in (1, 2, 4):
+        for first in (0, top - 1, top - 64, top - 100):
+            for entry in range((top - 1) // (64 * per) - 1, (top - 1) // (64 * per) + 2):
+                for part in range(per):
+                    sub = entry * per + part
+                    want = sub if sub * 64 < top and (sub + 1) * 64 > first else -1
+                    assert index.selected(entry, part, per, first, top) == want, (per, first, entry, part)
+    for first in (0, top - 64):
+        assert index.running((top - 1) // 64 - first // 64, first, top) == 2**25 - 1
+        assert index.running((top - 1) // 64 - first // 64 + 1, first, top) == -1
+
+
 def test_shares_cover_the_line(index):
     rng = np.random.default_rng(0)
     warps = 148 * 8
