@@ -242,21 +242,57 @@ def nsa_forward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, *, n_sel: int
     return O, sel
 
 
+COMPRESS_VALUES = 1 << 26  # fp32 values that cache_compress reads back at a time
+
+
 def cache_compress(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: torch.Tensor, cmp_cache: torch.Tensor,
-                   cmp_pages: torch.Tensor, cmp_block: int = 32, cmp_stride: int = 16) -> torch.Tensor:
-    """One decode step of :func:`compress_kv` on 4-bit caches: where a sequence's newest token completes a
-    compressed key (``lens[s]`` = cmp_block + i * cmp_stride), the mean of its last ``cmp_block`` keys and
-    values, read back from ``cache``, is written to place i of ``cmp_cache``.  Returns the number of
-    compressed keys of each sequence, int32 [S].  Nothing is read on the host."""
+                   cmp_pages: torch.Tensor, cmp_block: int = 32, cmp_stride: int = 16,
+                   cu_seqlens: Optional[torch.Tensor] = None, n_tokens: Optional[int] = None) -> torch.Tensor:
+    """:func:`compress_kv` on 4-bit caches, call by call: to be called after every ``ops.cache_write`` to ``cache``,
+    the prompt's included, with that call's ``pages``, ``lens`` and ``cu_seqlens`` (and ``n_tokens``, its rows, which are
+    needed with ``cu_seqlens``; without, every sequence has one).  Each compressed key i that one of the call's tokens
+    completes (position cmp_block - 1 + i * cmp_stride of a sequence), the mean of its ``cmp_block`` keys and values as
+    they are read back from ``cache``, is written to place i of ``cmp_cache``.  Returns the number of compressed keys of
+    each sequence, int32 [S]; those completed by earlier tokens are taken to be there.  Nothing is read on the host.
+
+    The means are rounded to bf16, as :func:`nsa_forward` does, whatever the type of the keys: 2^-8 of a value that the
+    cache then rounds to a 4-bit code."""
     from . import ops
 
-    S = lens.shape[0]
-    count = torch.where(lens >= cmp_block, (lens - cmp_block) // cmp_stride + 1, torch.zeros_like(lens))
-    complete = (lens >= cmp_block) & ((lens - cmp_block) % cmp_stride == 0)
-    cu = torch.arange(S + 1, device=lens.device, dtype=torch.int32) * cmp_block
-    K, V = ops.cache_read(cache, d_qk, pages, lens, cu, S * cmp_block, torch.float32)
-    Kc, Vc = (x[0].unflatten(1, (S, cmp_block)).mean(2).transpose(0, 1).to(torch.bfloat16) for x in (K, V))
-    ops.cache_write(cmp_cache, Kc.contiguous(), Vc.contiguous(), cmp_pages, torch.where(complete, count, torch.zeros_like(count)))
+    if cmp_block < 1 or cmp_stride < 1:
+        raise ValueError("cmp_block and cmp_stride must be positive")
+    S, dev = lens.shape[0], lens.device
+
+    def completed(n):  # compressed keys of the first n tokens
+        return torch.where(n >= cmp_block, (n - cmp_block) // cmp_stride + 1, torch.zeros_like(n))
+
+    def write(table, ends, places, where, cu):  # the means of the last cmp_block of `ends` tokens, to newest places
+        m = ends.shape[0]
+        K, V = ops.cache_read(cache, d_qk, table, ends, torch.arange(m + 1, device=dev, dtype=torch.int32) * cmp_block,
+                              m * cmp_block, torch.float32)
+        Kc, Vc = (x[0].unflatten(1, (m, cmp_block)).mean(2).transpose(0, 1).to(torch.bfloat16) for x in (K, V))
+        ops.cache_write(cmp_cache, Kc.contiguous(), Vc.contiguous(), places, where, cu)
+
+    count = completed(lens)
+    if cu_seqlens is None:
+        newest = (lens >= cmp_block) & ((lens - cmp_block) % cmp_stride == 0)
+        write(pages, lens, cmp_pages, torch.where(newest, count, torch.zeros_like(count)), None)
+        return count
+    if n_tokens is None or n_tokens < 0:
+        raise ValueError("n_tokens (the rows that cu_seqlens packs) is needed with cu_seqlens")
+    # rows first to last - 1 of the call are tokens begin to end - 1 of a sequence
+    first, last = (x.clamp(0, n_tokens) for x in (cu_seqlens[:-1].long(), cu_seqlens[1:].long()))
+    end = lens.long().clamp(min=0) - (cu_seqlens[1:].long() - last)
+    begin = end - (last - first).clamp(min=0)
+    upto = completed(end)
+    cmp_cu = torch.cat((upto.new_zeros(1), (upto - completed(begin)).cumsum(0))).int()  # the completed keys, packed
+    rows = min(n_tokens, n_tokens // cmp_stride + S) if S > 0 else 0  # (r tokens complete (r - 1) // stride + 1 at most)
+    step = max(1, COMPRESS_VALUES // (cmp_block * cache.shape[1] * (cache.shape[2] // 36)))
+    for r0 in range(0, rows, step):
+        row = torch.arange(r0, min(rows, r0 + step), device=dev, dtype=torch.int32)
+        seq = (torch.searchsorted(cmp_cu, row, right=True) - 1).clamp(0, S - 1)
+        key = upto[seq] - (cmp_cu[seq + 1] - row)  # (behind the last one: any; it is not written)
+        write(pages[seq], (key * cmp_stride + cmp_block).int(), cmp_pages, upto.int(), cmp_cu - r0)
     return count
 
 
@@ -267,8 +303,8 @@ def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: 
     """The three NSA branches and the gate of :func:`nsa_forward` for the newest token of every sequence of a
     4-bit cache (``ops.cache_write`` has put its K and V there): Q [S, Hq, d_qk] bf16 or fp16, sel int32
     [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  The compressed branch sees
-    every key of ``cmp_cache`` (kept by :func:`cache_compress`), as the newest token does in the forward;
-    without one it is left out.  Each branch adds its gated result into O."""
+    every key of ``cmp_cache`` (:func:`cache_compress` keeps it, called after every write), as the newest token does in
+    the forward; without one it is left out.  Each branch adds its gated result into O."""
     from . import ops
 
     g = gate_weights(gate_w, Q.device)

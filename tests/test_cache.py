@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from nsa_hopper_b200 import capi, ops
+from nsa_hopper_b200 import capi, nsa, ops
 from oracle import cache as oc
 
 CSRC = os.path.join(capi.PKG_DIR, "csrc")
@@ -335,3 +335,96 @@ def test_torch_ops_refuse_host_tensors():
         ops.cache_read(cache, 128, pages, lens, cu_seqlens=lens)
     with pytest.raises(RuntimeError, match="not one of"):
         ops.cache_alloc(4, 2, 96, 96, device="cpu")
+
+
+# ------------------------------------------------------------------ compressed keys as tokens come
+class _Model:
+    """cache_write and cache_read on fp32 places [pages, Hkv, 64, d_qk + d_v], row by row through the oracle's `place`."""
+
+    @staticmethod
+    def write(cache, K, V, pages, lens, cu_seqlens=None):
+        cu = None if cu_seqlens is None else cu_seqlens.numpy()
+        for r in range(K.shape[0]):
+            _, pos, page = oc.place(r, pages.numpy(), lens.numpy(), cu, cache.shape[0])
+            if page >= 0:
+                cache[page, :, pos % 64, :2] = torch.cat((K[r], V[r]), -1).float()
+
+    @staticmethod
+    def read(cache, d_qk, pages, lens, cu_seqlens, n_tokens, dtype):
+        out = torch.zeros(cache.shape[1], n_tokens, 2)
+        for r in range(n_tokens):
+            _, pos, page = oc.place(r, pages.numpy(), lens.numpy(), cu_seqlens.numpy(), cache.shape[0])
+            if page >= 0:
+                out[:, r] = cache[page, :, pos % 64, :2]
+        return out[None, ..., :1], out[None, ..., 1:]
+
+
+@pytest.mark.parametrize("block,stride", [(32, 16), (8, 8), (4, 6), (1, 1), (16, 5)])
+@pytest.mark.parametrize("chunk", [1, 10**9])
+def test_every_completed_key_is_compressed(monkeypatch, block, stride, chunk):
+    """Prompts, steps of one token and of several: every key that cache_compress counts is the mean of its tokens, all other
+    places keep what they held."""
+    monkeypatch.setattr(ops, "cache_write", _Model.write)
+    monkeypatch.setattr(ops, "cache_read", _Model.read)
+    monkeypatch.setattr(nsa, "COMPRESS_VALUES", chunk)
+    rng = np.random.default_rng(block * 100 + stride)
+    S, W, P = 4, 4, 20
+    i32 = dict(dtype=torch.int32)
+    pages = torch.from_numpy(rng.permutation(P)[:S * W].reshape(S, W)).int()
+    cmp_pages = torch.from_numpy(rng.permutation(P)[:S * W].reshape(S, W)).int()
+    cache, cmp_cache = torch.zeros(P, 1, 64, 36), torch.full((P, 1, 64, 36), -1000.0)  # (36: as wide as d = 1 in records)
+    tokens = torch.from_numpy(rng.integers(-8, 9, (S, W * 64, 2))).float()             # (sums of them are exact)
+    lens = torch.zeros(S, **i32)
+    while int(lens.min()) < W * 64 - 40:
+        if rng.random() < 0.3:   # one token each, no cu_seqlens
+            new, cu, n = np.ones(S, int), None, None
+        else:                    # several, or a prompt; rows of no sequence behind them
+            new = np.minimum(rng.choice([0, 1, 3, 17, 40]) * rng.integers(0, 2, S), W * 64 - lens.numpy())
+            cu, n = torch.tensor([0, *np.cumsum(new)], **i32), int(new.sum()) + int(rng.integers(0, 3))
+        old, lens = lens, (lens + torch.from_numpy(new).int()).clamp(max=W * 64)
+        rows = [tokens[s, int(old[s]):int(lens[s])] for s in range(S)] if cu is not None else \
+            [tokens[s, int(lens[s]) - 1:int(lens[s])] for s in range(S)]
+        flat = torch.cat(rows + [torch.full((0 if n is None else n - int(cu[-1]), 2), 77.0)])[:, None]
+        ops.cache_write(cache, flat[..., :1], flat[..., 1:], pages, lens, cu)
+        count = nsa.cache_compress(cache, 1, pages, lens, cmp_cache, cmp_pages, block, stride, cu, n)
+        assert count.dtype == torch.int32
+        want = torch.full_like(cmp_cache, -1000.0)
+        for s in range(S):
+            m = max(0, (int(lens[s]) - block) // stride + 1)
+            assert int(count[s]) == m
+            for i in range(min(m, W * 64)):
+                want[cmp_pages[s, i // 64], 0, i % 64, :2] = tokens[s, i * stride:i * stride + block].mean(0).bfloat16().float()
+        assert torch.equal(cmp_cache, want)
+
+
+def test_compress_takes_broken_batches(monkeypatch):
+    """More rows than tokens, rows before the first sequence, cu_seqlens behind the call's rows or out of order, negative and
+    huge lengths: what a call writes is the mean of tokens that its rows complete."""
+    monkeypatch.setattr(ops, "cache_write", _Model.write)
+    monkeypatch.setattr(ops, "cache_read", _Model.read)
+    i32 = dict(dtype=torch.int32)
+    pages = torch.tensor([[0, 1], [2, 3], [-1, 99]], **i32)
+    cache = torch.arange(4.0).view(4, 1, 1, 1) * 64 + torch.arange(64.0).view(1, 1, 64, 1) + torch.zeros(4, 1, 64, 36)
+    for lens, cu, n in (([40, 128, 70], [0, 60, 61, 70], 80), ([40, 50, 60], [5, 9, 30, 31], 33), ([40, BIG, -5], [0, 40, 60, 90], 50),
+                        ([33, 128, 64], [30, 3, 60, 10], 40), ([BIG, BIG, BIG], [0, BIG, BIG, BIG], 20),
+                        ([48, 64, 0], [-7, 9, 40, 40], 40)):
+        cmp_cache = torch.full((4, 1, 64, 36), -1000.0)
+        lens, cu = torch.tensor(lens, **i32), torch.tensor(cu, **i32)
+        count = nsa.cache_compress(cache, 1, pages, lens, cmp_cache, pages, 8, 4, cu, n)
+        assert count.tolist() == [(x - 8) // 4 + 1 if x >= 8 else 0 for x in lens.tolist()]
+        for p in range(4):
+            for t in range(64):
+                i, got = p % 2 * 64 + t, cmp_cache[p, 0, t, 0]
+                if got != -1000:  # key i of sequence p // 2, of tokens 4 i to 4 i + 7
+                    keys = [cache[pages[p // 2, x // 64], 0, x % 64, 0] if x < 128 else torch.tensor(0.0) for x in range(4 * i, 4 * i + 8)]
+                    assert got == torch.stack(keys).mean().bfloat16()
+        if (np.diff(cu.numpy()) >= 0).all():  # every key that a row completes is there
+            for r in range(n):
+                seq, pos, page = oc.place(r, pages.numpy(), lens.numpy(), cu.numpy(), 4)
+                if page >= 0 and pos >= 7 and (pos - 7) % 4 == 0:
+                    i = (pos - 7) // 4
+                    assert cmp_cache[pages[seq, i // 64], 0, i % 64, 0] != -1000
+    assert nsa.cache_compress(cache, 1, pages[:0], lens[:0], cmp_cache, pages[:0], 8, 4, torch.tensor([3], **i32), 9).shape == (0,)
+    for kw in (dict(cu_seqlens=cu), dict(cu_seqlens=cu, n_tokens=-1), dict(cmp_stride=0), dict(cmp_block=0)):
+        with pytest.raises(ValueError):
+            nsa.cache_compress(cache, 1, pages, lens, cmp_cache, pages, **kw)

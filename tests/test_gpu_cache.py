@@ -739,3 +739,35 @@ def test_decode_continues_a_prefill():
         Ks, _ = ops.cache_read(cache, d, pages[s:s + 1].contiguous(), torch.tensor([t], dtype=torch.int32, device="cuda"), one, 32, torch.float32)
         mean = Ks[0].mean(1).bfloat16()
         np.testing.assert_array_equal(Kc[0, :, s].double().cpu().numpy(), oc.values(*oc.quantise(mean.double().cpu().numpy())))
+
+
+def test_steps_of_several_tokens_lose_no_compressed_key():
+    """A prompt in pieces, then drafted tokens that pass the borders of compressed keys between two calls, on caches whose
+    empty places are NaN: after each write cache_compress gives every key that it counts, and the decode step is finite."""
+    gen = _gen(31)
+    hq, hkv, dims, S, W = 8, 2, (64, 64), 3, 6
+    cache = torch.full((S * W, hkv, 36 * 128), 0xFF, dtype=torch.uint8, device="cuda")
+    cmp_cache = torch.full((4, hkv, 36 * 128), 0xFF, dtype=torch.uint8, device="cuda")
+    pages = torch.randperm(S * W, generator=gen).view(S, W).int().cuda()
+    cmp_pages = torch.tensor([[3], [0], [2]], dtype=torch.int32, device="cuda")
+    lens = torch.zeros(S, dtype=torch.int32, device="cuda")
+    for new in ([200, 31, 0], [3, 1, 47], [14, 3, 1], [5, 17, 0], [0, 0, 0], [33, 16, 100]):
+        n = sum(new) + 2
+        cu = torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device="cuda")
+        lens = lens + torch.tensor(new, dtype=torch.int32, device="cuda")
+        k, v = (torch.randn(n, hkv, 64, generator=gen).bfloat16().cuda() for _ in range(2))
+        ops.cache_write(cache, k, v, pages, lens, cu)
+        count = nsa.cache_compress(cache, 64, pages, lens, cmp_cache, cmp_pages, cu_seqlens=cu, n_tokens=n)
+        assert count.tolist() == [max(0, (x - 32) // 16 + 1) for x in lens.tolist()]
+        whole = torch.tensor([0, *np.cumsum(lens.tolist())], dtype=torch.int32, device="cuda")
+        K, V = ops.cache_read(cache, 64, pages, lens, whole, int(whole[-1]), torch.float32)
+        cmp_cu = torch.tensor([0, *np.cumsum(count.tolist())], dtype=torch.int32, device="cuda")
+        Kc, Vc = ops.cache_read(cmp_cache, 64, cmp_pages, count, cmp_cu, int(cmp_cu[-1]), torch.float32)
+        for s in (x for x in range(S) if count[x] > 0):
+            at, to = slice(int(whole[s]), int(whole[s + 1])), slice(int(cmp_cu[s]), int(cmp_cu[s + 1]))
+            for got, mean in zip((Kc, Vc), nsa.compress_kv(K[:, :, at], V[:, :, at])):
+                np.testing.assert_array_equal(got[0, :, to].double().cpu().numpy(),
+                                              oc.values(*oc.quantise(mean[0].bfloat16().double().cpu().numpy())))
+        sel = torch.zeros(S, hkv, 1, dtype=torch.int32, device="cuda")
+        q = torch.randn(S, hq, 64, generator=gen).bfloat16().cuda()
+        assert nsa.nsa_decode(q, cache, pages, lens, sel, cmp_cache=cmp_cache, cmp_pages=cmp_pages, cmp_lens=count).isfinite().all()
