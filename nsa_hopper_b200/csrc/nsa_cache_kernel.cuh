@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 //   * the key axis is permuted (rows 2q, 2q + 1 of a tile of 8 are keys q, 4 + (q ^ 1)) so that neither K's nor V's
 //     shared loads collide more than two ways on the record as it is.
 // Q has up to 8 (bf16) or 11 significant bits, so a power of two per row puts it into fp16 (below 2^-14 of the row's
-// largest to within 2^-25 of it).  P is rounded to fp16 (at most 2^-11 of each term): the sum of
-// its fp32 values is the divisor.  Scores, statistics and O are fp32.
+// largest to within 2^-25 of it).  P is rounded to fp16 for the tensor core (2^-11 of each term, or 2^-32 of the largest where
+// that is more: see page()); the sum of its fp32 values is the divisor.  Scores, statistics and O are fp32.
 //
 // What binds: a page of 64 keys (d = 128) takes a scheduler 1800 cycles with 16 heads and two warps (2090 with one; 1310 and
 // 1560 with 8 heads), of which half are the issue of 128 tensor instructions, most of the rest 256 conversions and 256 products;
@@ -567,7 +567,7 @@ struct Worker {
   // ---- the consumer's side.  The thread's heads in tile h are 8 h + 2 c and 8 h + 2 c + 1 (c = lane % 4).
   float o[MT][NH][4];      // O^T: d = (DV / 8) r + 2 j + e / 2 (r = lane / 4) of head 8 h + 2 c + e % 2
   uint32_t q[NH][KS * 2];  // Q of head 8 h + r: d = c * DQK / 4 + 2 i, + 1
-  float2 f[NH], m[NH], l[NH];  // of the thread's heads: factor, maximum (a power of two), the thread's share of the sum
+  float2 f[NH], m[NH], l[NH];  // of the thread's heads: factor, reference m of the powers of two, the thread's share of the sum
 
   // A new row: its queries are asked for, then (when the copies of the first pages are under way) made ready.
   __device__ __forceinline__ void ask(const AttendArgs& a, uint32_t row, int lane) {
@@ -661,11 +661,13 @@ struct Worker {
       ptx::fence_proxy_async_smem();  // (before the record that is copied here next)
       __syncwarp();
     }
-    // Softmax, in powers of two, against a maximum m of the scores so far.  m is raised, and O and the sums with it, when a
-    // score is more than 2^kSlack above it: until then P is at most 2^kSlack, and neither its roundings nor the result depend
-    // on m.  So most pages need no exchange between the threads that share a head.  (The first m is so low that every number
-    // is above it, and it scales zeros, or NaN, which stays.)
-    constexpr float kSlack = 8.0f;
+    // Softmax, in powers of two, against m, kBelow less than a maximum of the scores so far.  m is raised, and O and the sums
+    // with it, when a score is more than 2^kMost above it, so most pages need no exchange between the threads that share a
+    // head.  The largest P is 2^kBelow to 2^kMost: as fp16, a P is off by 2^-11 of itself at most, or, where it is below 2^-14,
+    // by 2^-25, which is 2^-32 of the largest or less (with kBelow = 0 it would be 2^-25 of it, and a flat tail of many small
+    // weights would be lost from O).  (The first m is so low that every number is above it, and it scales zeros, or NaN, which
+    // stays.)
+    constexpr float kBelow = 7.0f, kMost = 15.0f;
     uint32_t p[4][NH][2];  // P^T as the tensor core takes it: fp16 pairs of keys (of rows 2c, 2c + 1, and 8 more) of head 8 h + r
     float2 y[4][NH][2];
     float most = -INFINITY;
@@ -678,7 +680,7 @@ struct Worker {
           y[t][h][x] = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-m[h].x, -m[h].y));
         most = max3(max3(most, y[t][h][0].x, y[t][h][0].y), y[t][h][1].x, y[t][h][1].y);
       }
-    if (__any_sync(0xFFFFFFFFu, most > kSlack)) {
+    if (__any_sync(0xFFFFFFFFu, most > kMost)) {
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         float2 top = make_float2(-INFINITY, -INFINITY);
@@ -690,7 +692,7 @@ struct Worker {
           top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, k));
           top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, k));
         }
-        top = make_float2(fmaxf(m[h].x, top.x * f[h].x), fmaxf(m[h].y, top.y * f[h].y));
+        top = make_float2(fmaxf(m[h].x, top.x * f[h].x - kBelow), fmaxf(m[h].y, top.y * f[h].y - kBelow));
         const float2 k = make_float2(exp2_fast(m[h].x - top.x), exp2_fast(m[h].y - top.y));
         l[h] = mul2(l[h], k);
 #pragma unroll

@@ -771,3 +771,59 @@ def test_steps_of_several_tokens_lose_no_compressed_key():
         sel = torch.zeros(S, hkv, 1, dtype=torch.int32, device="cuda")
         q = torch.randn(S, hq, 64, generator=gen).bfloat16().cuda()
         assert nsa.nsa_decode(q, cache, pages, lens, sel, cmp_cache=cmp_cache, cmp_pages=cmp_pages, cmp_lens=count).isfinite().all()
+
+
+def _one_group(values, d):
+    """Codes and scales of a token whose first group of 16 has `values` in front, all else 0."""
+    x = np.zeros((1, d))
+    x[0, :len(values)] = values
+    return [a[0] for a in oc.quantise(x)]
+
+
+def _records(tokens, hkv, d_qk, d_v):
+    """Pages uint8 [n, hkv, record] of (k values, v values) a token, the same for every head."""
+    num = (len(tokens) + 63) // 64
+    parts = [np.zeros((num, hkv, 64, w), np.uint8) for w in (d_qk // 2, d_qk // 16, d_v // 2, d_v // 16)]
+    for t, (k, v) in enumerate(tokens):
+        for i, (x, d) in enumerate(((k, d_qk), (v, d_v))):
+            code, byte = _one_group(x, d)
+            parts[2 * i][t // 64, :, t % 64] = code[0::2] + 16 * code[1::2]
+            parts[2 * i + 1][t // 64, :, t % 64] = byte
+    return np.concatenate([p.reshape(num, hkv, -1) for p in parts], -1)
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("n,length,hq,plan", [
+    (1000, 640, 1, dict(cluster=1)),                 # a warp for each row
+    (3, 640, 4, dict(cluster=2)),
+    (100, 1500, 16, dict(cluster=1)),                # teams
+    (1, 40000, 9, dict(merge=8)),                    # cut
+])
+def test_a_long_flat_tail_counts(dims, n, length, hq, plan):
+    """One key far above all others, whose values are zeros: O is what the tail adds up to, however small each of its
+    weights is.  P is in fp16 at 2^7 times the weight or more (the largest weight is 1), so 2^-25 of it are 2^-32 a key."""
+    got_plan = _plan(n, hq, 1, dims, (length + 63) // 64, 0, 64, 0)
+    assert {k: got_plan[k] for k in plan} == plan
+    num = (length + 63) // 64
+    pages3 = torch.from_numpy(_records([([6.0], [0.0])] + [([0.0], [6.0, -1.5, 4.0])] * 127, 1, *dims))
+    pages = torch.ones(n, num, dtype=torch.int32)    # (the tail's pages are one page)
+    pages[:, 0] = 0
+    lens = torch.full((n,), length, dtype=torch.int32)
+    q = torch.zeros(n, hq, dims[0])
+    q[:, :, 0] = torch.linspace(2, 33, n * hq).view(n, hq) * np.log(2.0) * dims[0]**0.5 / 6   # the tail's weights: 2^-2 to 2^-33
+    q = q.bfloat16()
+    qd, cd, pd, ld = _cuda(q, pages3, pages, lens)
+    out = torch.empty(n, hq, dims[1], device="cuda")
+    o, lse = ops.cache_attend(qd, cd, pd, ld, out=out)
+    z = q[:, :, 0].double().numpy() * 6 / dims[0]**0.5
+    p = np.exp(-z) * (length - 1)
+    v = np.zeros(dims[1])
+    v[:3] = 6.0, -1.5, 4.0
+    want = (p / (1 + p))[..., None] * v
+    u = 2.0**-24
+    dz = (3 * dims[0] + 8) * u * z                   # (the terms of _tolerances, with 2^-32 for 2^-25)
+    rel = 2.0**-11 + 2 * (2.0**-22 + dz) + 4 * length * u + 2.0**-22
+    tol = np.abs(want) * (rel[..., None] + u) + length * np.abs(v) * 2.0**-32
+    assert (np.abs(o.double().cpu().numpy() - want) <= tol).all()
+    ref = z + np.log1p(p)
+    assert (np.abs(lse.double().cpu().numpy() - ref) <= dz + 2.0**-22 + dz + 2 * length * u + 2.0**-22 + 8 * u * np.abs(ref)).all()
