@@ -692,8 +692,13 @@ struct Worker {
           top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, k));
           top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, k));
         }
-        top = make_float2(fmaxf(m[h].x, top.x * f[h].x - kBelow), fmaxf(m[h].y, top.y * f[h].y - kBelow));
-        const float2 k = make_float2(exp2_fast(m[h].x - top.x), exp2_fast(m[h].y - top.y));
+        // m is the largest score to within its last bit, but the scores below are not rounded before m is taken off: from 2^28
+        // on the difference is more than fp16 holds.  So what the largest has over kBelow, or lacks, is taken off as well.
+        const float2 was = m[h], z = top;
+        top = make_float2(fmaxf(was.x, z.x * f[h].x - kBelow), fmaxf(was.y, z.y * f[h].y - kBelow));
+        float2 over = make_float2(fmaf(z.x, f[h].x, -top.x) - kBelow, fmaf(z.y, f[h].y, -top.y) - kBelow);
+        over = make_float2(top.x > was.x ? over.x : fmaxf(over.x, 0.0f), top.y > was.y ? over.y : fmaxf(over.y, 0.0f));
+        const float2 k = make_float2(exp2_fast(was.x - top.x), exp2_fast(was.y - top.y));
         l[h] = mul2(l[h], k);
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][h][0] *= k.x, o[j][h][1] *= k.y, o[j][h][2] *= k.x, o[j][h][3] *= k.y;
@@ -702,7 +707,8 @@ struct Worker {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            y[t][h][x] = fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-top.x, -top.y));
+            y[t][h][x] = add2(fma2(make_float2(s[t][h][2 * x], s[t][h][2 * x + 1]), f[h], make_float2(-top.x, -top.y)),
+                              make_float2(-over.x, -over.y));
       }
     }
 #pragma unroll

@@ -827,3 +827,34 @@ def test_a_long_flat_tail_counts(dims, n, length, hq, plan):
     assert (np.abs(o.double().cpu().numpy() - want) <= tol).all()
     ref = z + np.log1p(p)
     assert (np.abs(lse.double().cpu().numpy() - ref) <= dz + 2.0**-22 + dz + 2 * length * u + 2.0**-22 + 8 * u * np.abs(ref)).all()
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq", [3, 16])
+@pytest.mark.parametrize("length,width", [(70, 2), (3000, 47), (3000, 1000)])
+def test_scores_beyond_a_sums_last_bit(dims, dtype, hq, length, width):
+    """Scores so large that half of their last bit is above fp16's range in powers of two: the key far above the others has
+    all of the weight, in its page and behind it, and two equal ones in one page have half of it each."""
+    gen = _gen(60)
+    top, twin, d = length // 2 // 64 * 64 + 5, length // 2 // 64 * 64 + 9, dims[0]
+    size = torch.exp2(torch.arange(hq).float() * 5 / hq + 10) * (1 + torch.rand(hq, generator=gen))   # scores of 2^28 to 2^35
+    q = size.view(hq, 1).expand(2, hq, d).to(dtype)
+    k, v = torch.zeros(2 * length, 1, d), torch.randn(2 * length, 1, dims[1], generator=gen)
+    for s in range(2):
+        k[s * length:(s + 1) * length, 0] = torch.rand(length, 1, generator=gen) * 20000
+        k[s * length + top] = 60000.0
+    k[length + twin] = 60000.0
+    pages, lens, cu = _batch([length] * 2, [length] * 2, 2 * ((length + 63) // 64), gen, width)
+    cache = ops.cache_alloc(2 * ((length + 63) // 64), 1, *dims)
+    kd, vd, pd, ld, cd, qd = _cuda(k.to(dtype), v.to(dtype), pages, lens, cu, q)
+    ops.cache_write(cache, kd, vd, pd, ld, cd)
+    K, V = (x[0, 0].double().cpu().numpy() for x in ops.cache_read(cache, d, pd, ld, cd, 2 * length, torch.float32))
+    assert (np.sort(K[:length, 0])[-2] < 0.5 * K[top, 0]) and K[length + top, 0] == K[length + twin, 0]
+    want = np.stack((V[top], (V[length + top] + V[length + twin]) / 2))
+    ref = q[:, :, 0].double().numpy() * K[top, 0] * d**0.5 + np.log([[1.0], [2.0]])
+    o, lse = ops.cache_attend(qd, cache, pd, ld, out=torch.empty(2, hq, dims[1], device="cuda"))
+    got = o.double().cpu().numpy()
+    # (every P is 0 or one power of two: 2^-22 for that in the sum, 2^-22 for the division and weight)
+    assert (np.abs(got - want[:, None]) <= np.abs(V).max() * 2.0**-21).all()
+    assert (np.abs(lse.double().cpu().numpy() - ref) <= (3 * d + 8) * 2.0**-24 * np.abs(ref)).all()
