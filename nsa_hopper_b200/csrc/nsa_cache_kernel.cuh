@@ -380,6 +380,13 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint64_t 
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t ns) {
   return ptx::mbar_try_wait(bar, parity) || wait_long(bar, parity, ns);
 }
+// Waits for the copies that are on their way (a bit of `flying` for each stage), `ns` at most for each: after one that did not
+// come in time, and before the ring is used for anything else or the block ends.
+__device__ __noinline__ void wait_all(uint64_t* bars, uint32_t phases, uint32_t flying, uint64_t ns) {
+  for (int i = 0; flying >> i != 0; ++i)
+    if (flying >> i & 1) wait_long(bars + i, phases >> i & 1, ns);
+  __syncwarp();
+}
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -1022,7 +1029,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
   Worker<C> w;
   int head, tail = 0, issued = 0;
   uint32_t phases = 0, flying = 0;  // each stage's parity of the next phase; copies on their way
-  bool lost = false;                // a copy did not come: rows from here on are NaN
+  bool lost = false;                // a copy did not come: no more are made, rows from here on are NaN
   bool fresh = true, first_row = true;
   // the ring holds STAGES records: STAGES - 1 on their way (the first of them before the loop's first page) while one is
   // worked on
@@ -1059,6 +1066,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
       }
     }
     if (fresh) {
+      if (lost) wait_all(bars, phases, flying, a.wait_ns), flying = 0;  // (before a part of the row goes where they end)
       // a row is whole here unless it began before this share, or goes on behind it
       const bool head_cut = first_row && cut_before;
       const bool tail_cut = head + 1 == tail && cur.next == cur.end && cur.j < cur.len;
@@ -1070,11 +1078,7 @@ __global__ void __launch_bounds__(C::NW * 32, 1) attend_kernel(const AttendArgs 
     __syncwarp();
   }
   if (a.cluster > 1) join_cluster<C>(a, row, reinterpret_cast<const float*>(smem), rank);
-  if (lost) {  // the block's memory is not given up under a copy (bounded, too)
-    if (a.err != nullptr && lane == 0) atomicOr(a.err, 1);
-    for (int i = 0; i < C::STAGES; ++i)
-      if (flying >> i & 1) wait_for(bars + i, phases >> i & 1, a.wait_ns);
-  }
+  if (lost && a.err != nullptr && lane == 0) atomicOr(a.err, 1);
 }
 
 // Joins the parts of the rows that were cut, in the order of the line.  WPH warps share a row's query head:

@@ -858,3 +858,41 @@ def test_scores_beyond_a_sums_last_bit(dims, dtype, hq, length, width):
     # (every P is 0 or one power of two: 2^-22 for that in the sum, 2^-22 for the division and weight)
     assert (np.abs(got - want[:, None]) <= np.abs(V).max() * 2.0**-21).all()
     assert (np.abs(lse.double().cpu().numpy() - ref) <= (3 * d + 8) * 2.0**-24 * np.abs(ref)).all()
+
+
+@pytest.mark.parametrize("case", [0, 4, 6, 7, 10, 12, 13, 14])
+def test_waits_are_bounded_however_the_work_is_shared(case):
+    """No copy comes: the launch ends by itself, every row that has a key is NaN through each kind of join, the error word is
+    set, and the next call is right."""
+    lens, width, n_sel, dims, (hq, hkv), want_plan = SHARING[case]
+    n = len(lens)
+    gen = _gen(70 + case)
+    num_pages = sum((x + 63) // 64 for x in lens)
+    pages, lens, _ = _batch(lens, None, num_pages, gen, width)
+    cache = _random_cache(num_pages, hkv, dims, gen)
+    q = torch.randn(n, hq, dims[0], generator=gen).bfloat16()
+    sel = torch.randint(-1, width, (n, hkv, n_sel), generator=gen, dtype=torch.int32) if n_sel else None
+    if n_sel:
+        sel[:, :, 0] = torch.clamp(lens - 1, min=0).view(-1, 1) // 64
+    qd, cd, pd, ld, sd = _cuda(q, cache, pages, lens, sel)
+    want = ops.cache_attend(qd, cd, pd, ld, sel=sd)
+    o, lse, err = torch.zeros_like(want[0]), torch.zeros_like(want[1]), torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = capi.make_cache_batch(cache=cd.data_ptr(), pages=pd.data_ptr(), lens=ld.data_ptr(), num_pages=num_pages, n_seqs=n,
+                                  width=width, n_rows=n, heads_kv=hkv, d_qk=dims[0], d_v=dims[1])
+    desc = capi.make_cache_attend_desc(batch=batch, q=qd.data_ptr(), o=o.data_ptr(), lse=lse.data_ptr(), heads_q=hq,
+                                       sel=sd.data_ptr() if n_sel else 0, n_sel=n_sel, block_size=64, err=err.data_ptr(),
+                                       timeout_ms=20, debug_flags=capi.NSA_DEBUG_STALL)
+    plan = capi.cache_attend_plan(desc, 0)
+    assert {k: plan[k] for k in want_plan} == want_plan
+    work = torch.empty(capi.cache_attend_workspace_bytes(desc), dtype=torch.uint8, device="cuda")
+    desc.workspace = work.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.cache_attend(desc, stream)
+    assert err.item() == capi.NSA_DEVERR_TIMEOUT
+    live = ld > 0
+    assert o[live].isnan().all() and lse[live].isnan().all()
+    assert not o[~live].any() and torch.isneginf(lse[~live]).all()
+    err.zero_()
+    desc.debug_flags = 0
+    capi.cache_attend(desc, stream)
+    assert err.item() == 0 and torch.equal(o, want[0]) and torch.equal(lse, want[1])
