@@ -386,7 +386,8 @@ std::vector<torch::Tensor> cache_read(torch::Tensor cache, int64_t d_qk, torch::
 
 std::vector<torch::Tensor> cache_attend(torch::Tensor Q, torch::Tensor cache, torch::Tensor pages, torch::Tensor lens,
                                         OptTensor sel, int64_t l_prime, int64_t window, OptTensor cu_seqlens, double scale,
-                                        OptTensor out, OptTensor weight, bool accumulate, bool with_lse) {
+                                        OptTensor out, OptTensor weight, bool accumulate, bool with_lse, OptTensor err,
+                                        int64_t timeout_ms, int64_t debug_flags) {
   TORCH_CHECK(Q.dim() == 3, "Q must be [N, Hq, d_qk]");
   const int32_t dtype = dtype_code(Q, "Q");
   TORCH_CHECK(cache.dim() == 3, "cache must be uint8 [num_pages, Hkv, record bytes]");
@@ -412,6 +413,11 @@ std::vector<torch::Tensor> cache_attend(torch::Tensor Q, torch::Tensor cache, to
                     weight->get_device() == cache.get_device(),
                 "weight must be an fp32 CUDA tensor (its first element is used) on Q's device");
     d.o_weight = weight->data_ptr<float>();
+  }
+  if (err.has_value()) {
+    TORCH_CHECK(err->is_cuda() && err->scalar_type() == at::kInt && err->numel() >= 1 && err->get_device() == cache.get_device(),
+                "err must be an int32 CUDA tensor (its first element is used) on Q's device");
+    d.err = err->data_ptr<int32_t>();
   }
   const c10::cuda::CUDAGuard guard(cache.device());
   torch::Tensor O, L;
@@ -448,6 +454,8 @@ std::vector<torch::Tensor> cache_attend(torch::Tensor Q, torch::Tensor cache, to
   d.o_accumulate = accumulate ? 1 : 0;
   d.keep_rows = keep ? 1 : 0;
   d.scale = static_cast<float>(scale);
+  d.timeout_ms = i32(timeout_ms, "timeout_ms");
+  d.debug_flags = i32(debug_flags, "debug_flags");
   const Api& a = api();
   const int64_t ws = a.cache_attend_ws(&d);
   if (ws < 0) TORCH_CHECK(false, format_msg("nsa_cache_attend failed: %s", a.last_error()));
@@ -499,11 +507,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "cache_read(cache, d_qk, pages, lens, cu_seqlens, n_tokens, dtype) -> [K, V]", py::arg("cache"), py::arg("d_qk"),
         py::arg("pages"), py::arg("lens"), py::arg("cu_seqlens"), py::arg("n_tokens"), py::arg("dtype"));
   m.def("cache_attend", &cache_attend,
-        "cache_attend(Q, cache, pages, lens, sel, l_prime, window, cu_seqlens, scale, out, weight, accumulate, with_lse) -> "
-        "[O, LSE]",
+        "cache_attend(Q, cache, pages, lens, sel, l_prime, window, cu_seqlens, scale, out, weight, accumulate, with_lse, err, "
+        "timeout_ms, debug_flags) -> [O, LSE]",
         py::arg("Q"), py::arg("cache"), py::arg("pages"), py::arg("lens"), py::arg("sel") = py::none(),
         py::arg("l_prime") = 64, py::arg("window") = 0, py::arg("cu_seqlens") = py::none(), py::arg("scale") = 0.0,
         py::arg("out") = py::none(), py::arg("weight") = py::none(), py::arg("accumulate") = false,
-        py::arg("with_lse") = true);
+        py::arg("with_lse") = true, py::arg("err") = py::none(), py::arg("timeout_ms") = 0, py::arg("debug_flags") = 0);
   m.def("library_version", &library_version);
 }

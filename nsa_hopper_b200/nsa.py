@@ -299,20 +299,21 @@ def cache_compress(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: to
 def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, sel: torch.Tensor, *,
                l_prime: int = 64, window: int = 512, cmp_cache: Optional[torch.Tensor] = None,
                cmp_pages: Optional[torch.Tensor] = None, cmp_lens: Optional[torch.Tensor] = None,
-               gate_w: Optional[torch.Tensor] = None) -> torch.Tensor:
+               gate_w: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The three NSA branches and the gate of :func:`nsa_forward` for the newest token of every sequence of a
     4-bit cache (``ops.cache_write`` has put its K and V there): Q [S, Hq, d_qk] bf16 or fp16, sel int32
     [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  The compressed branch sees
     every key of ``cmp_cache`` (:func:`cache_compress` keeps it, called after every write), as the newest token does in
-    the forward; without one it is left out.  Each branch adds its gated result into O."""
+    the forward; without one it is left out.  Each branch adds its gated result into O.  ``err``: as in
+    ``ops.cache_attend``, for all three."""
     from . import ops
 
     g = gate_weights(gate_w, Q.device)
     O = torch.empty(Q.shape[0], Q.shape[1], cache.shape[2] // 36 - Q.shape[2], dtype=torch.float32, device=Q.device)
-    ops.cache_attend(Q, cache, pages, lens, sel=sel, l_prime=l_prime, out=O, weight=g[1:2], with_lse=False)
+    ops.cache_attend(Q, cache, pages, lens, sel=sel, l_prime=l_prime, out=O, weight=g[1:2], with_lse=False, err=err)
     if cmp_cache is not None:
-        ops.cache_attend(Q, cmp_cache, cmp_pages, cmp_lens, out=O, weight=g[0:1], accumulate=True, with_lse=False)
-    ops.cache_attend(Q, cache, pages, lens, window=window, out=O, weight=g[2:3], accumulate=True, with_lse=False)
+        ops.cache_attend(Q, cmp_cache, cmp_pages, cmp_lens, out=O, weight=g[0:1], accumulate=True, with_lse=False, err=err)
+    ops.cache_attend(Q, cache, pages, lens, window=window, out=O, weight=g[2:3], accumulate=True, with_lse=False, err=err)
     return O
 
 

@@ -152,8 +152,8 @@ def cache_read(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: torch.
 def cache_attend(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
                  sel: Optional[torch.Tensor] = None, l_prime: int = 64, window: int = 0,
                  cu_seqlens: Optional[torch.Tensor] = None, scale: float = 0.0, out: Optional[torch.Tensor] = None,
-                 weight: Optional[torch.Tensor] = None, accumulate: bool = False,
-                 with_lse: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+                 weight: Optional[torch.Tensor] = None, accumulate: bool = False, with_lse: bool = True,
+                 err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Attention of the batch's newest tokens over the 4-bit cache (nsa_cache_attend): the decode step.
 
     Q [N, Hq, d_qk] (bf16 or fp16) has the rows of :func:`cache_write`; the row at position t sees
@@ -164,9 +164,13 @@ def cache_attend(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens
 
     ``out``, ``weight``, ``accumulate``: as in :func:`forward_ext`, the result times ``weight[0]`` is
     written to ``out`` (fp32 or Q's dtype) or added into it (fp32); rows of no sequence are then left
-    as they were.  ``with_lse=False`` skips the LSE (an empty tensor is returned).  No gradients."""
+    as they were.  ``with_lse=False`` skips the LSE (an empty tensor is returned).  No gradients.
+
+    ``err`` (int32 on the device, optional): 1 is ORed into its first element if a copy inside the kernel did not come within
+    2 seconds, which no correct program meets; rows that it belonged to are then NaN.  Nothing is raised, as the call does not
+    wait for the device."""
     o, lse = _C.cache_attend(Q, cache, pages, lens, sel, int(l_prime), int(window), cu_seqlens, float(scale), out, weight,
-                             bool(accumulate), bool(with_lse))
+                             bool(accumulate), bool(with_lse), err)
     return o, lse
 
 

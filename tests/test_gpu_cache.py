@@ -896,3 +896,19 @@ def test_waits_are_bounded_however_the_work_is_shared(case):
     desc.debug_flags = 0
     capi.cache_attend(desc, stream)
     assert err.item() == 0 and torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
+def test_a_wait_that_ran_out_is_told_through_torch():
+    q, cache, pages, lens = _small(27)
+    err = torch.tensor([4, 9], dtype=torch.int32, device="cuda")
+    want = ops.cache_attend(q, cache, pages, lens, err=err)
+    assert err.tolist() == [4, 9]
+    sel = torch.zeros(3, 2, 1, dtype=torch.int32, device="cuda")
+    nsa.nsa_decode(q, cache, pages, lens, sel, err=err)
+    assert err.tolist() == [4, 9]
+    o, _ = ops._C.cache_attend(q, cache, pages, lens, err=err, timeout_ms=20, debug_flags=capi.NSA_DEBUG_STALL)
+    assert o.isnan().all() and err.tolist() == [4 | capi.NSA_DEVERR_TIMEOUT, 9]
+    assert torch.equal(ops.cache_attend(q, cache, pages, lens)[0], want[0])
+    for bad in (err.long(), err.cpu(), err[:0]):
+        with pytest.raises(RuntimeError, match="err must be"):
+            ops.cache_attend(q, cache, pages, lens, err=bad)
