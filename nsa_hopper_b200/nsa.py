@@ -308,6 +308,10 @@ def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: 
     ``ops.cache_attend``, for all three."""
     from . import ops
 
+    if window < 1:
+        raise ValueError("window must be positive (the window branch of nothing has no keys)")
+    if cmp_cache is not None and (cmp_pages is None or cmp_lens is None):
+        raise ValueError("cmp_pages and cmp_lens are needed with cmp_cache")
     g = gate_weights(gate_w, Q.device)
     O = torch.empty(Q.shape[0], Q.shape[1], cache.shape[2] // 36 - Q.shape[2], dtype=torch.float32, device=Q.device)
     ops.cache_attend(Q, cache, pages, lens, sel=sel, l_prime=l_prime, out=O, weight=g[1:2], with_lse=False, err=err)

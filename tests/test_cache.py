@@ -428,3 +428,13 @@ def test_compress_takes_broken_batches(monkeypatch):
     for kw in (dict(cu_seqlens=cu), dict(cu_seqlens=cu, n_tokens=-1), dict(cmp_stride=0), dict(cmp_block=0)):
         with pytest.raises(ValueError):
             nsa.cache_compress(cache, 1, pages, lens, cmp_cache, pages, **kw)
+
+
+def test_decode_refuses_what_has_no_branch():
+    """A window of 0 is no window to cache_attend (every key), but the window branch of 0 keys has none."""
+    q, i32 = torch.zeros(2, 4, 64, dtype=torch.bfloat16), dict(dtype=torch.int32)
+    cache, pages, lens = ops.cache_alloc(2, 1, 64, 64, device="cpu"), torch.zeros(2, 1, **i32), torch.ones(2, **i32)
+    sel = torch.zeros(2, 1, 1, **i32)
+    for kw in (dict(window=0), dict(window=-3), dict(cmp_cache=cache), dict(cmp_cache=cache, cmp_pages=pages)):
+        with pytest.raises(ValueError, match="window|cmp_pages"):
+            nsa.nsa_decode(q, cache, pages, lens, sel, **kw)
