@@ -280,8 +280,9 @@ int nsa_sel_backward(const nsa_sel_bwd_desc* desc, nsa_stream_t stream);
    cu_seqlens[s + 1]) is the token at position lens[s] - (cu_seqlens[s + 1] - r), so a sequence's rows are its last tokens;
    without cu_seqlens row r is the last token of sequence r, and n_rows == n_seqs.  The device arrays are trusted for
    nothing: a token at a negative position, behind the page table's width or on a page outside [0, num_pages) is absent: it
-   is not written, reads back as zeros and is not attended to.  Two rows that name one place of the cache (two sequences
-   that write to a shared page) leave a mixture of both there. */
+   is not written, reads back as zeros and is not attended to.  (In a cu_seqlens that is out of order a row is of any one of
+   the sequences whose range holds it, or of none.)  Two rows that name one place of the cache (two sequences that write
+   to a shared page) leave a mixture of both there. */
 typedef struct nsa_cache_batch {
   void* cache;                /* see above; 16-byte aligned (only nsa_cache_write changes it) */
   const int32_t* pages;       /* int32 [n_seqs, width] */

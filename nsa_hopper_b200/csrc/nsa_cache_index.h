@@ -25,6 +25,15 @@ NSA_HD constexpr int k_scale_at(int d_qk) { return kPage * d_qk / 2; }
 NSA_HD constexpr int v_code_at(int d_qk) { return kPage * d_qk * 9 / 16; }
 NSA_HD constexpr int v_scale_at(int d_qk, int d_v) { return v_code_at(d_qk) + kPage * d_v / 2; }
 
+// Of a number that is not 0.
+NSA_HD int highest_bit(uint32_t x) {
+#ifdef __CUDA_ARCH__
+  return 31 - __clz(x);
+#else
+  return 31 - __builtin_clz(x);
+#endif
+}
+
 // The batch that all three calls describe: page table [n_seqs, width], lengths, packed rows.
 struct Batch {
   const int32_t* pages;
@@ -36,8 +45,8 @@ struct Batch {
   int32_t n_rows;
 };
 
-// The sequence of a row, -1 for a row of none (before cu[0], behind cu[n_seqs], or in a cu_seqlens that
-// is not in order).
+// The sequence of a row, -1 for a row of none (before cu[0] or behind cu[n_seqs]).  In a cu_seqlens that is out of order it is
+// one of those whose range holds the row, or -1, and the two forms need not agree.
 NSA_HD int sequence_of(const Batch& b, int row) {
   if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
   if (b.n_seqs <= 0 || row < b.cu[0]) return -1;
@@ -48,6 +57,21 @@ NSA_HD int sequence_of(const Batch& b, int row) {
     else hi = mid;
   }
   return row < b.cu[lo + 1] ? lo : -1;
+}
+// The same, 32 places of cu at a time: `below(lo, step, hi)` has bit i set where place lo + i * step is before hi and its cu not
+// above the row.  (A thread that searches by itself is faster with the form above: the reading kernel takes 64 us for 104448
+// tokens of 16 sequences, and 71 with this one's steps.)
+template <class Below>
+NSA_HD int sequence_by_32(const Batch& b, int row, Below&& below) {
+  if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
+  int lo = 0, hi = b.n_seqs;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int last = highest_bit(below(lo, step, hi) | 1);  // (lo stays a candidate)
+    lo += last * step;
+    hi = hi - lo > step ? lo + step : hi;
+  }
+  return b.n_seqs > 0 && b.cu[lo] <= row && row < b.cu[lo + 1] ? lo : -1;
 }
 
 // Position of a row in its sequence (from sequence_of, >= 0): the sequence's last rows are the call's.

@@ -402,21 +402,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// sequence_of by a whole warp: 32 places of cu at a time instead of one.
+// sequence_of by a whole warp.
 __device__ __forceinline__ int sequence_of_warp(const Batch& b, int row, int lane) {
-  if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
-  int lo = 0, hi = b.n_seqs;  // the last s with cu[s] <= row, if there is one, is in [lo, hi)
-#pragma unroll 1
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int at = lo + lane * step;
-    const unsigned below = __ballot_sync(0xFFFFFFFFu, at < hi && b.cu[at] <= row);
-    // (lane 0 counts as below: lo stays a candidate)
-    const int last = 31 - __clz(below | 1u);
-    lo += last * step;
-    hi = min(hi, lo + step);
-  }
-  return b.n_seqs > 0 && b.cu[lo] <= row && row < b.cu[lo + 1] ? lo : -1;
+  return sequence_by_32(b, row, [&](int lo, int step, int hi) {
+    return __ballot_sync(0xFFFFFFFFu, lane * step < hi - lo && b.cu[lo + lane * step] <= row);
+  });
 }
 
 // 2N consecutive values of one row of Q: as they are in memory, and as fp16 pairs; `factor` undoes the row's power of two.

@@ -438,3 +438,51 @@ def test_decode_refuses_what_has_no_branch():
     for kw in (dict(window=0), dict(window=-3), dict(cmp_cache=cache), dict(cmp_cache=cache, cmp_pages=pages)):
         with pytest.raises(ValueError, match="window|cmp_pages"):
             nsa.nsa_decode(q, cache, pages, lens, sel, **kw)
+
+
+# ------------------------------------------------------------------ the search that a warp does
+SHIM_32 = r"""
+#include "nsa_cache_index.h"
+using namespace nsa::cache;
+extern "C" void both(const int32_t* cu, int n_seqs, const int32_t* rows, int n, int32_t* out) {
+  const Batch b = {nullptr, nullptr, cu, 0, n_seqs, 0, 0, 0};
+  for (int i = 0; i < n; ++i) {
+    out[2 * i] = sequence_of(b, rows[i]);
+    out[2 * i + 1] = sequence_by_32(b, rows[i], [&](int lo, int step, int hi) {
+      uint32_t bits = 0;
+      for (int lane = 0; lane < 32; ++lane) bits |= (uint32_t)(lane * step < hi - lo && cu[lo + lane * step] <= rows[i]) << lane;
+      return bits;
+    });
+  }
+}
+"""
+
+
+def test_a_thread_and_a_warp_find_a_rows_sequence(tmp_path):
+    """The same in any cu_seqlens that is in order; out of order, one whose range holds the row, or none."""
+    (tmp_path / "both.cpp").write_text(SHIM_32)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-fPIC", "-shared", f"-I{CSRC}",
+                    "-o", str(tmp_path / "both.so"), str(tmp_path / "both.cpp")], check=True)
+    lib = ctypes.CDLL(str(tmp_path / "both.so"))
+    rng = np.random.default_rng(1)
+    ptr = lambda a: a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    for i in range(600):
+        S = int(rng.choice([0, 1, 2, 31, 32, 33, 40, 64, 65, 1000, 1024, 1025, 3000]))
+        if i % 3 == 0:
+            cu = np.concatenate(([rng.integers(0, 3)], rng.integers(0, 4, S))).cumsum()
+        elif i % 3 == 1:
+            cu = rng.integers(-5, S + 5, S + 1)                        # in no order
+        else:
+            cu = np.arange(S + 1) * 2
+            at = rng.integers(0, S + 1, 3)
+            cu[at] = rng.choice([-2**31, BIG, 0, S], 3)                # a few entries broken
+        cu = cu.astype(np.int32)
+        rows = np.concatenate((rng.integers(0, 2 * S + 4, 40), [0, BIG])).astype(np.int32)
+        out = np.zeros((len(rows), 2), np.int32)
+        lib.both(ptr(cu), S, ptr(rows), len(rows), ptr(out))
+        for r, found in zip(rows.tolist(), out.tolist()):
+            for s in found:
+                assert -1 <= s < S and (s < 0 or cu[s] <= r < cu[s + 1])
+                if i % 3 == 0:
+                    at = np.nonzero(cu[:-1] <= r)[0]
+                    assert s == (at[-1] if at.size and r < cu[at[-1] + 1] else -1)
