@@ -912,3 +912,35 @@ def test_a_wait_that_ran_out_is_told_through_torch():
     for bad in (err.long(), err.cpu(), err[:0]):
         with pytest.raises(RuntimeError, match="err must be"):
             ops.cache_attend(q, cache, pages, lens, err=bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_value_of_the_type_is_quantised_by_the_definition(dtype):
+    """Every finite value as the largest of a group, and for each scale every value that is not beyond its saturation and not
+    far below its first border, with either sign: the kernel's bytes are the oracle's."""
+    every = torch.arange(0x7F80 if dtype == torch.bfloat16 else 0x7C00, dtype=torch.int16).view(dtype)
+    groups = torch.zeros(len(every), 16, dtype=dtype)
+    groups[torch.arange(len(every)), torch.arange(len(every)) % 16] = every * (1 - 2 * (torch.arange(len(every)) // 16 % 2)).to(dtype)
+    parts, x = [groups], every.double().numpy()
+    taken = oc.quantise(np.concatenate((x[:, None], np.zeros((len(x), 15))), 1))[1][:, 0]   # the scale of each as the largest
+    for byte in range(1, 0xE3):
+        if not (taken == byte).any():
+            continue
+        lead = every[np.nonzero(taken == byte)[0].max() if byte < 0xE2 else int(np.searchsorted(x, 6 * 10240.0))]
+        below = every[torch.from_numpy((x >= 0.2 * oc._SCALES[byte]) & (x <= float(lead)))]
+        below = torch.cat((below, below.new_zeros(-len(below) % 15))).view(-1, 15)
+        parts.append(torch.cat((lead.expand(len(below), 1), below), 1))
+        parts.append(-parts[-1].flip(1))
+    x = torch.cat(parts)
+    x = torch.cat((x, x.new_zeros(-len(x) % 8, 16))).view(-1, 1, 128)
+    n = x.shape[0]
+    cache = ops.cache_alloc((n + 63) // 64, 1, 128, 128)
+    pages = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None]
+    lens, cu = torch.tensor([n], dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    ops.cache_write(cache, x.cuda(), x.flip(0).contiguous().cuda(), pages, lens, cu)
+    code, byte = oc.quantise(x[:, 0].double().numpy())
+    kc, ks, vc, vs = (p[:, 0].reshape(-1, p.shape[-1])[:n] for p in oc.split(cache.cpu().numpy(), 128, 128))
+    for codes, scales, c, b in ((kc, ks, code, byte), (vc, vs, code[::-1], byte[::-1])):
+        np.testing.assert_array_equal(scales, b)
+        got = np.stack((codes & 15, codes >> 4), -1).reshape(n, 128)
+        assert ((got == c) | ((got & 7 == 0) & (c & 7 == 0))).all()          # (the sign of a zero is free)
