@@ -310,7 +310,9 @@ int nsa_cache_read(const nsa_cache_batch* batch, void* k, void* v, int32_t out_d
 
 /* Attention of the rows over the cache: row n at position t sees key p iff p <= t, and t - p < window (if window > 0),
    and p lies in one of the blocks sel[n][kvh] (if sel is given; block_size keys each, a set as in the forward; entries < 0
-   or behind t select nothing).  A row that sees no key gets O = 0 and LSE = -inf.  Zero-initialise, then fill. */
+   or behind t select nothing; n_sel at most 1024).  n_rows * heads_kv * tiles * (pages that a row may see: n_sel * block_size /
+   64 with sel, else the table's width or the window's pages) is at most 2^31 - 1, where a KV head with up to 8 query heads is
+   one tile and one with more has a tile for each 16 of them.  Beyond either: NSA_ERR_UNSUPPORTED.  A row that sees no key gets O = 0 and LSE = -inf.  Zero-initialise, then fill. */
 typedef struct nsa_cache_attend_desc {
   nsa_cache_batch batch;
   const void* q;              /* [n_rows, heads_q, d_qk], dtype q_dtype, d has unit stride, 16-byte aligned */

@@ -159,7 +159,7 @@ def cache_attend(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens
     Q [N, Hq, d_qk] (bf16 or fp16) has the rows of :func:`cache_write`; the row at position t sees
     the keys p <= t, with ``window`` > 0 those with t - p < window, and with ``sel`` int32
     [N, Hkv, KSEL] those in its selected blocks of ``l_prime`` keys (a set; entries < 0 or behind t
-    select nothing).  Returns (O [N, Hq, d_v] of Q's dtype, LSE fp32 [N, Hq], natural log); a row that
+    select nothing; KSEL at most 1024).  Returns (O [N, Hq, d_v] of Q's dtype, LSE fp32 [N, Hq], natural log); a row that
     sees no key, or of no sequence, has O = 0 and LSE = -inf.
 
     ``out``, ``weight``, ``accumulate``: as in :func:`forward_ext`, the result times ``weight[0]`` is
