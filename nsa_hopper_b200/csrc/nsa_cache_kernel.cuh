@@ -280,7 +280,8 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 // is the cache's bytes from DRAM, provided that turning 4 bits into tensor-core operands keeps up.  Hence every warp is
 // a worker of its own with a ring of page records in shared memory (bulk copies), and codes go from there straight into the
 // registers that the tensor core reads (m16n8k16, fp16 in, fp32 out): no dequantised value is ever stored.  (Operands in shared
-// memory, as tcgen05 wants them, would cost 64 KB of shared-memory traffic a page beside the 9 KB that are fetched.)
+// memory, as tcgen05 could have them, would cost 64 KB of shared-memory traffic a page beside the 9 KB that are fetched.  The
+// decoded operand in tensor memory was not tried.)
 // The cache is the A operand, S^T = K Q^T and O^T = V^T P^T, so that 8 query heads cost half the tensor instructions of 16,
 // and a decoded fragment serves both halves.  For that
 //   * the d axis of QK is permuted so that a thread's K fragments are d_qk / 4 consecutive codes of one key: one
@@ -296,7 +297,8 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
 // What binds: a page of 64 keys (d = 128) takes a scheduler 1800 cycles with 16 heads and two warps (2090 with one; 1310 and
 // 1560 with 8 heads), of which half are the issue of 128 tensor instructions, most of the rest 256 conversions and 256 products;
 // DRAM would deliver a page in 1550.  64 rows of up to 32768 keys, 616 MB: 165 us, 3.7 TB/s; 256 rows of 16 selected blocks,
-// 155 MB: 47 us, 3.3 TB/s; one row of 16 blocks: 10.3 us.
+// 155 MB: 47 us, 3.3 TB/s; one row of 16 blocks: 10.2 us.  (In the kernel a warp's page takes 4400 cycles, 3270 of them in
+// page(), the rest in finding, copying and waiting for the next ones.)
 //
 // All (row, page) slots of the call stand in one line that is shared out evenly (split_line): teams of 1 to 8 warps of a
 // block take turns at a row's pages and join their (m, sum, O) in shared memory; a row that is cut between teams leaves
