@@ -944,3 +944,40 @@ def test_every_value_of_the_type_is_quantised_by_the_definition(dtype):
         np.testing.assert_array_equal(scales, b)
         got = np.stack((codes & 15, codes >> 4), -1).reshape(n, 128)
         assert ((got == c) | ((got & 7 == 0) & (c & 7 == 0))).all()          # (the sign of a zero is free)
+
+
+def test_a_captured_step_of_several_tokens_compresses_on_replay(monkeypatch):
+    """Write and compress captured once, replayed on other lengths, rows and keys, each a chunk of three compressed keys at a
+    time: the same caches as by calls that are not captured and take all at once."""
+    gen = _gen(32)
+    hkv, S, W, n = 2, 3, 8, 70
+    pages = torch.randperm(S * W, generator=gen).view(S, W).int().cuda()
+    cmp_pages = torch.tensor([[1], [2], [0]], dtype=torch.int32, device="cuda")
+    size = lambda p: torch.full((p, hkv, 36 * 192), 0xFF, dtype=torch.uint8, device="cuda")  # noqa: E731
+    caches, want = (size(S * W), size(3)), (size(S * W), size(3))
+    lens, cu = torch.zeros(S, dtype=torch.int32, device="cuda"), torch.zeros(S + 1, dtype=torch.int32, device="cuda")
+    k, v = torch.zeros(n, hkv, 128, device="cuda").half(), torch.zeros(n, hkv, 64, device="cuda").half()
+
+    def step(cache, cmp_cache):
+        ops.cache_write(cache, k, v, pages, lens, cu)
+        return nsa.cache_compress(cache, 128, pages, lens, cmp_cache, cmp_pages, cu_seqlens=cu, n_tokens=n)
+
+    monkeypatch.setattr(nsa, "COMPRESS_VALUES", 3 * 32 * hkv * 192)
+    step(*caches)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        count = step(*caches)
+    monkeypatch.undo()
+    for new in ([60, 0, 10], [1, 2, 3], [0, 0, 70], [16, 32, 8], [0, 0, 0], [15, 17, 33]):
+        cu.copy_(torch.tensor([0, *np.cumsum(new)], dtype=torch.int32))
+        lens += torch.tensor(new, dtype=torch.int32, device="cuda")
+        k.copy_(torch.randn(n, hkv, 128, generator=gen))
+        v.copy_(torch.randn(n, hkv, 64, generator=gen))
+        g.replay()
+        assert torch.equal(count, step(*want))
+        torch.cuda.synchronize()
+        assert torch.equal(caches[0], want[0]) and torch.equal(caches[1], want[1])
+    assert count.tolist() == [max(0, (x - 32) // 16 + 1) for x in lens.tolist()]
+    back, _ = ops.cache_read(caches[1], 128, cmp_pages, count, torch.tensor([0, *np.cumsum(count.tolist())], dtype=torch.int32,
+                                                                           device="cuda"), int(count.sum()))
+    assert back.isfinite().all()
