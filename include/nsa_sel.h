@@ -1,7 +1,8 @@
 /*
  * nsa_sel.h -- C ABI of the B200 (sm_100a) NSA selected-branch attention forward, with the
  * block selection that produces its index rows, and with the backward and the 4-bit KV cache
- * (writing, reading back, attention of single tokens) that the reference lacks.
+ * (writing, reading back, attention of single tokens, pages and block selection for them, rotary
+ * positions) that the reference lacks.
  *
  * This is the drop-in boundary for the one hot path of the nsa-hopper reference: the
  * selected-branch forward that its kernels expose through pybind as
@@ -358,6 +359,114 @@ int64_t nsa_cache_attend_workspace_bytes(const nsa_cache_attend_desc* desc);
 /* Queues the attention (one or two launches).  Results do not depend on timing: the parts of a row are joined in a
    fixed order. */
 int nsa_cache_attend(const nsa_cache_attend_desc* desc, nsa_stream_t stream);
+
+/* ------------------------------------------------------------------ around the cache: pages, selection, positions
+   What a decode step needs before it attends.  Nothing here has a counterpart in the reference. */
+
+/* Gives the sequences of a batch the pages for their next tokens, or takes pages back, and works out where the rows of the
+   call lie.  Sequence s holds held[s] tokens (below 0: none; more than the table has room for: as many as that).
+     rows[s] > 0   it asks for that many more.  It gets them if the table has room, and if the pages that it and all sequences
+                   before it still need are there (a sequence whose last page has room needs none, and gets its rows always).
+                   Otherwise it stays as it is and has no rows in this call.
+     rows[s] < 0   it gives its last -rows[s] tokens back (all of them if it has no more), and the pages that they alone filled.
+     rows[s] == 0  it has no part in this call.
+   `pool` holds the free pages, pool[0] to pool[n_free[0] - 1].  Pages that are given back are added behind them, in the order
+   of the sequences and of their pages, before any are taken (those that pool_size leaves no room for are lost); then the
+   last pages of the pool are taken, in its order, by the sequences in theirs.  The rows of `pages` get the pages that are taken;
+   what stood there for pages that are given back stays.  A page that two sequences share would come back twice: it must not be
+   given back here before the other one has ended.
+   Results:
+     held_out [n_seqs]      tokens after the call       (may be `held`)
+     n_free_out [1]         free pages after it         (may be `n_free`)
+     lens [n_seqs]          as nsa_cache_batch wants them: held_out for sequences that got rows, 0 for all others
+     cu_seqlens [n_seqs+1]  sums of the rows that were asked for, so that a caller's packed rows keep their places (those of
+                            a sequence that got none are absent: its lens is 0); at most 2^31 - 1.  NULL: row s is sequence
+                            s's last token, and n_rows == n_seqs
+     positions [n_rows]     optional: a row's position in its sequence, -1 for an absent row
+     slots [n_rows]         optional: 64 * page + position % 64, -1 for an absent row
+   With held_out and n_free_out apart from held and n_free nothing that counts is changed, so that a call can be tried, dropped
+   and made again.  n_seqs is at most 8192 and n_seqs * width below 2^31.  Device arrays are trusted for nothing but pages
+   (copied, never used as an index); one that is not aligned to its element size is refused, as are positions and slots that
+   are not aligned to 16 bytes.  One launch. */
+typedef struct nsa_cache_reserve_desc {
+  int32_t* pages;             /* int32 [n_seqs, width] */
+  const int32_t* held;
+  const int32_t* rows;
+  int32_t* pool;              /* int32 [pool_size] */
+  const int32_t* n_free;
+  int32_t* held_out;
+  int32_t* n_free_out;
+  int32_t* lens;
+  int32_t* cu_seqlens;
+  int32_t* positions;
+  int64_t* slots;
+  int64_t pages_stride;       /* entries from one row of `pages` to the next; 0 = width */
+  int32_t n_seqs, width, pool_size, n_rows;
+  int32_t reserved[4];
+} nsa_cache_reserve_desc;
+
+int nsa_cache_reserve(const nsa_cache_reserve_desc* desc, nsa_stream_t stream);
+
+/* Block selection for single tokens: nsa_sel_select's rows for the tokens of a batch, from the compressed keys that a 4-bit
+   cache holds.  batch.cache and batch.pages are the compressed cache's; batch.lens are the tokens of the sequences themselves,
+   so that the row at position t sees T = t + 1 tokens as nsa_sel_select sees a sequence of T: n_cmp = (T - cmp_block) /
+   cmp_stride + 1 compressed keys, key i (place i of the cache) in block floor(linspace(0, T-1, n_cmp)[i] / block_size), and
+       score(block) = sum over its keys of (sum of the query heads of the KV head) . key.
+   sel [n_rows, heads_kv, n_sel]: the min(n_sel, ceil(T / block_size)) best blocks, the best first, then -1.  Blocks are ranked
+   by sums in 64 bits; the lower block comes first where two are equal, and scores that are not finite come last.  Keys that the
+   page table does not hold count as zeros.  A row of no token, and one of more than 2^24 tokens or of more than
+   64 * width * cmp_stride + cmp_block - 1 (whose keys the table cannot hold), selects nothing: -1 throughout.
+   n_sel is at most 1024, heads_q / heads_kv at most 256.  Zero-initialise, then fill.  Two launches for each 8192 rows. */
+typedef struct nsa_cache_select_desc {
+  nsa_cache_batch batch;
+  const void* q;              /* [n_rows, heads_q, d_qk], dtype q_dtype, d has unit stride, 16-byte aligned */
+  int32_t* sel;               /* int32 [n_rows, heads_kv, n_sel] */
+  void* workspace;            /* nsa_cache_select_workspace_bytes() bytes, 16-byte aligned, of this call alone */
+  int64_t q_row_stride;       /* elements, multiples of 8; 0 = heads_q * d_qk */
+  int64_t q_head_stride;      /* 0 = d_qk */
+  int32_t heads_q;            /* a multiple of heads_kv */
+  int32_t n_sel;
+  int32_t block_size;         /* l_prime: 64, 128 or 256 */
+  int32_t cmp_block, cmp_stride;
+  int32_t q_dtype;            /* NSA_DTYPE_BF16 or NSA_DTYPE_F16 */
+  int32_t reserved[4];
+} nsa_cache_select_desc;
+
+/* Bytes of the workspace, or -1 if the description is invalid (see nsa_sel_last_error()). */
+int64_t nsa_cache_select_workspace_bytes(const nsa_cache_select_desc* desc);
+int nsa_cache_select(const nsa_cache_select_desc* desc, nsa_stream_t stream);
+
+/* Rotary positions of one to four axes (time, height, width): values a_i, b_i of a head become a_i cos w - b_i sin w and
+   b_i cos w + a_i sin w with w = position[axis[i]] * inv_freq[i], for the `pairs` pairs i of the rotary part, which begins at
+   value `offset`: values i and i + pairs of it, or 2 i and 2 i + 1 if `interleaved`.  The other values are copied.  `inverse`
+   turns by -w: the gradient.  inv_freq is given as turns[i] = round(inv_freq[i] / (2 pi) * 2^64) modulo 2^64, so that angles of
+   any int32 position are exact to 2^-32 of a turn.  One or two tensors (Q and K) with the same tokens, in any layout in which d
+   has unit stride; y may be x where their strides are equal.  turns and axis are host arrays, read before the call returns.  One
+   launch. */
+typedef struct nsa_rotary_tensor {
+  const void* x;              /* NULL: no second tensor */
+  void* y;
+  int64_t x_stride[3];        /* elements from one batch entry, head, token to the next */
+  int64_t y_stride[3];
+  int32_t heads;
+  int32_t reserved;
+} nsa_rotary_tensor;
+
+typedef struct nsa_rotary_desc {
+  nsa_rotary_tensor t[2];
+  const int32_t* positions;   /* device int32 */
+  int64_t pos_stride[3];      /* elements from one axis, batch entry, token to the next */
+  const uint64_t* turns;      /* host [pairs] */
+  const uint8_t* axis;        /* host [pairs], below axes; NULL: all 0 */
+  int32_t batch, tokens;      /* tokens of each batch entry */
+  int32_t d;                  /* values of a head, at most 256 */
+  int32_t offset, pairs, axes;
+  int32_t interleaved, inverse;
+  int32_t dtype;              /* NSA_DTYPE_BF16, _F16 or _F32, of x and y */
+  int32_t reserved[3];
+} nsa_rotary_desc;
+
+int nsa_rotary(const nsa_rotary_desc* desc, nsa_stream_t stream);
 
 /* Size in bytes of the static scratch used by nsa_sel_select_noalloc. */
 int64_t nsa_sel_select_static_scratch_bytes(void);

@@ -120,6 +120,47 @@ class NsaCacheAttendDesc(ctypes.Structure):
     ]
 
 
+class NsaCacheReserveDesc(ctypes.Structure):
+    """Mirror of ``nsa_cache_reserve_desc``."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("pages", "held", "rows", "pool", "n_free", "held_out", "n_free_out", "lens",
+                                               "cu_seqlens", "positions", "slots")),
+        ("pages_stride", ctypes.c_int64),
+        ("n_seqs", ctypes.c_int32), ("width", ctypes.c_int32), ("pool_size", ctypes.c_int32), ("n_rows", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+
+class NsaCacheSelectDesc(ctypes.Structure):
+    """Mirror of ``nsa_cache_select_desc``."""
+
+    _fields_ = [
+        ("batch", NsaCacheBatch), ("q", ctypes.c_void_p), ("sel", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        *((name, ctypes.c_int32) for name in ("heads_q", "n_sel", "block_size", "cmp_block", "cmp_stride", "q_dtype")),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+
+class NsaRotaryTensor(ctypes.Structure):
+    """Mirror of ``nsa_rotary_tensor``."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_stride", ctypes.c_int64 * 3),
+                ("y_stride", ctypes.c_int64 * 3), ("heads", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class NsaRotaryDesc(ctypes.Structure):
+    """Mirror of ``nsa_rotary_desc``."""
+
+    _fields_ = [
+        ("t", NsaRotaryTensor * 2), ("positions", ctypes.c_void_p), ("pos_stride", ctypes.c_int64 * 3),
+        ("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p),
+        *((name, ctypes.c_int32) for name in ("batch", "tokens", "d", "offset", "pairs", "axes", "interleaved", "inverse", "dtype")),
+        ("reserved", ctypes.c_int32 * 3),
+    ]
+
+
 class NsaCacheAttendPlanInfo(ctypes.Structure):
     """Mirror of ``nsa_cache_attend_plan_info``."""
 
@@ -192,6 +233,14 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
         lib.nsa_cache_attend_workspace_bytes.restype = i64
         lib.nsa_cache_attend_plan.argtypes = [ctypes.POINTER(NsaCacheAttendDesc), i32, ctypes.POINTER(NsaCacheAttendPlanInfo)]
         lib.nsa_cache_attend_plan.restype = ctypes.c_int
+    if hasattr(lib, "nsa_rotary"):
+        lib.nsa_cache_reserve.argtypes = [ctypes.POINTER(NsaCacheReserveDesc), vp]
+        lib.nsa_cache_select.argtypes = [ctypes.POINTER(NsaCacheSelectDesc), vp]
+        lib.nsa_cache_select_workspace_bytes.argtypes = [ctypes.POINTER(NsaCacheSelectDesc)]
+        lib.nsa_cache_select_workspace_bytes.restype = i64
+        lib.nsa_rotary.argtypes = [ctypes.POINTER(NsaRotaryDesc), vp]
+        for fn in (lib.nsa_cache_reserve, lib.nsa_cache_select, lib.nsa_rotary):
+            fn.restype = ctypes.c_int
     if path is None:
         _lib = lib
     return lib
@@ -344,3 +393,39 @@ def cache_attend_workspace_bytes(desc: NsaCacheAttendDesc) -> int:
 
 def cache_attend(desc: NsaCacheAttendDesc, stream: int = 0) -> None:
     check(load().nsa_cache_attend(ctypes.byref(desc), ctypes.c_void_p(stream)))
+
+
+# ------------------------------------------------------------------ pages, selection and positions of a step
+def make_cache_reserve_desc(**kw) -> NsaCacheReserveDesc:
+    return _filled(NsaCacheReserveDesc(), **kw)
+
+
+def cache_reserve(desc: NsaCacheReserveDesc, stream: int = 0) -> None:
+    """nsa_cache_reserve: pages, lengths, packing, positions and slots of a batch."""
+    check(load().nsa_cache_reserve(ctypes.byref(desc), ctypes.c_void_p(stream)))
+
+
+def make_cache_select_desc(**kw) -> NsaCacheSelectDesc:
+    return _filled(NsaCacheSelectDesc(), **kw)
+
+
+def cache_select_workspace_bytes(desc: NsaCacheSelectDesc) -> int:
+    """nsa_cache_select_workspace_bytes (raises on an invalid description)."""
+    n = int(load().nsa_cache_select_workspace_bytes(ctypes.byref(desc)))
+    if n < 0:
+        raise NsaSelError(NSA_ERR_INVALID_ARG, last_error())
+    return n
+
+
+def cache_select(desc: NsaCacheSelectDesc, stream: int = 0) -> None:
+    """nsa_cache_select: the best blocks of every row from the compressed keys of a 4-bit cache."""
+    check(load().nsa_cache_select(ctypes.byref(desc), ctypes.c_void_p(stream)))
+
+
+def make_rotary_desc(**kw) -> NsaRotaryDesc:
+    return _filled(NsaRotaryDesc(), **kw)
+
+
+def rotary(desc: NsaRotaryDesc, stream: int = 0) -> None:
+    """nsa_rotary: one or two tensors turned by positions of one to four axes."""
+    check(load().nsa_rotary(ctypes.byref(desc), ctypes.c_void_p(stream)))

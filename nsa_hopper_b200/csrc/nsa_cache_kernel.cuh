@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "nsa_cache_index.h"
+#include "nsa_programmatic.cuh"
 #include "ptx.cuh"
 
 namespace nsa {
@@ -49,13 +50,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Every kernel here is launched programmatically (while the stream's kernel before it still runs, if that one allows it):
-// it lets the next one be launched, and touches no memory before all earlier ones have ended.
-__device__ __forceinline__ void start_in_order() {
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // ------------------------------------------------------------------ 4-bit conversions
 // Two codes of byte I of `w` as fp16 pair (low nibble in the low half).
 template <int I>

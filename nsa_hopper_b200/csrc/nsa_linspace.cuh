@@ -12,12 +12,26 @@
 
 namespace nsa {
 
-__device__ __forceinline__ float linspace_f32(int i, int T, int n) {
+// (On the host, for the CPU tests, the compiler must not contract products into FMAs either.)
+#ifdef __CUDACC__
+#define NSA_LINSPACE __host__ __device__ __forceinline__
+#else
+#define NSA_LINSPACE inline
+#endif
+NSA_LINSPACE float linspace_f32(int i, int T, int n) {
   if (n == 1) return 0.f;
+#ifndef __CUDA_ARCH__
+  const float step = (float)(T - 1) / (float)(n - 1);
+  if (i < n / 2) return (float)((double)step * (double)i);
+  return (float)((double)(T - 1) - (double)step * (double)(n - 1 - i));
+#else
   const float step = __fdiv_rn((float)(T - 1), (float)(n - 1));
   if (i < n / 2) return (float)__dmul_rn((double)step, (double)i);
   return (float)__dsub_rn((double)(T - 1), __dmul_rn((double)step, (double)(n - 1 - i)));
+#endif
 }
+
+#ifdef __CUDACC__
 
 __device__ __forceinline__ float floor_div_f32(float a, float b) {
   const float mod = fmodf(a, b);
@@ -41,5 +55,6 @@ __device__ __forceinline__ int compressed_limit(int t, int T, int n) {
     if (linspace_f32(i, T, n) <= (float)t) best = i;
   return best;
 }
+#endif  // __CUDACC__
 
 }  // namespace nsa

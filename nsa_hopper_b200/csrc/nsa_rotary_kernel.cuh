@@ -1,0 +1,192 @@
+// Rotary positions of one or several axes: pairs of a head's values turned by angles that grow with the token's position.
+//
+//     (a_i, b_i) -> (a_i cos w_i - b_i sin w_i, b_i cos w_i + a_i sin w_i),   w_i = position[axis(i)] * inv_freq(i)
+//
+// for the pairs i of the rotary part of a head (values i and i + pairs, or 2 i and 2 i + 1), the rest is copied; the gradient is
+// the same with -w.  Angles are kept in turns, as 64-bit fixed point: position * round(inv_freq / 2 pi * 2^64) wraps around
+// at whole turns by itself, so far positions cost no bits (an fp32 product would be off by 0.06 radians at a position of a
+// million).  Its upper 32 bits give the quadrant and the rest of it, at most an eighth of a turn, whose sine and cosine are
+// taken in fp32.  Products and sums are fp32, rounded once to the output's type.
+//
+// What bounds it: DRAM, 2 bytes in and 2 out a value.  So a block takes a few tokens with all their heads, Q's and K's in
+// one launch: the angles of a token are computed once, in shared memory, where all heads read them.  Any strides come in and
+// go out, so that [B, T, H, d], as projections write it, becomes the [B, H, T, d] that the attention reads on the way.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "nsa_programmatic.cuh"
+
+namespace nsa {
+namespace rotary {
+
+constexpr int kMaxPairs = 128;  // of a head of 256 values
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 8;   // of a block
+constexpr int kAtOnce = 4;      // items of a thread whose loads are in flight together
+
+struct Tensor {
+  const void* x;
+  void* y;
+  int64_t xs[3], ys[3];  // strides of batch, head, token
+};
+struct Args {
+  Tensor t[2];
+  const int32_t* pos;
+  int64_t ps[3];                 // strides of axis, batch, token
+  int32_t heads, first;          // of both tensors together, of the first one
+  int32_t batch, tokens;         // tokens of a batch entry
+  int32_t offset, pairs, rest;   // first value and pairs of the rotary part; values beside it
+  int32_t per_block;             // tokens of a block: a power of two
+  int32_t heads_block;           // heads of a block
+  int32_t interleaved;
+  uint32_t flip;                 // sign bit of the sines
+  uint64_t turn[kMaxPairs];      // inv_freq / 2 pi in units of 2^-64
+  uint8_t axis[kMaxPairs];
+};
+
+// VEC neighbouring values as one word.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { using type = uint4; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<2> { using type = uint16_t; };
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Cosine and sine of an angle of `turns` 2^-64.
+__device__ __forceinline__ float2 cos_sin(uint64_t turns, uint32_t flip) {
+  const uint32_t t = (uint32_t)(turns >> 32);
+  const uint32_t quadrant = (t + 0x20000000u) >> 30;
+  const float half_turns = (float)(int32_t)(t - (quadrant << 30)) * 4.656612873077393e-10f;  // (2^-31) in [-1/4, 1/4]
+  float s, c;
+  sincospif(half_turns, &s, &c);
+  const float x = quadrant & 1 ? -s : c, y = quadrant & 1 ? c : s;
+  const uint32_t turned = (quadrant & 2) << 30;
+  return make_float2(__uint_as_float(__float_as_uint(x) ^ turned), __uint_as_float(__float_as_uint(y) ^ turned ^ flip));
+}
+
+// Places of the angles in shared memory: those that neighbouring items of a warp read at once lie side by side.
+template <int VEC>
+__device__ __forceinline__ int place(int pair, int items) {
+  if (VEC == 1) return pair;
+  const int k = pair / VEC, e = pair % VEC;
+  return ((e / 2) * items + k) * 2 + e % 2;
+}
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(kThreads) kernel(const __grid_constant__ Args a) {
+  using W = typename Word<VEC * (int)sizeof(T)>::type;
+  extern __shared__ float2 angles[];  // [per_block][pairs]
+  const int tid = threadIdx.x;
+  const int blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  const int b = blockIdx.x / blocks, t0 = (blockIdx.x - b * blocks) * a.per_block;
+  const int h0 = blockIdx.y * a.heads_block, heads = min(a.heads_block, a.heads - h0);
+  const int tokens = min(a.per_block, a.tokens - t0);
+  const int turning = a.pairs / VEC;                                // items of a head that turn 2 VEC values
+  const int items = turning + (a.rest + 2 * VEC - 1) / (2 * VEC);   // and those that copy as many
+  start_in_order();
+  for (int i = tid; i < a.pairs * tokens; i += kThreads) {
+    const int t = i / a.pairs, pair = i - t * a.pairs;
+    const int64_t pos = a.pos[a.axis[pair] * a.ps[0] + b * a.ps[1] + (t0 + t) * a.ps[2]];
+    angles[t * a.pairs + place<VEC>(pair, turning)] = cos_sin((uint64_t)pos * a.turn[pair], a.flip);
+  }
+  __syncthreads();
+
+  // item, token and head of a thread's next item, stepped without divisions
+  const int shift = 31 - __clz(a.per_block);
+  int item = tid % items, ht = tid / items;
+  const int step = kThreads % items, steps = kThreads / items;
+  while (ht >> shift < heads) {
+    W lo[kAtOnce], hi[kAtOnce];
+    int64_t out[kAtOnce];
+    int at[kAtOnce], second[kAtOnce], mine[kAtOnce];
+    bool in[kAtOnce], turns[kAtOnce], q[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int t = ht & (a.per_block - 1), h = ht >> shift;
+      in[k] = h < heads && t < tokens;
+      turns[k] = item < turning;
+      mine[k] = t * a.pairs + (VEC == 1 ? 1 : 2) * item;
+      if (turns[k]) {
+        at[k] = a.offset + item * VEC * (a.interleaved ? 2 : 1);
+        second[k] = a.interleaved ? VEC : a.pairs;
+      } else {
+        // (the values beside the rotary part stand in one line; a last half item has no second word)
+        const int c = (item - turning) * 2 * VEC, d = c + VEC;
+        at[k] = c < a.offset ? c : c + 2 * a.pairs;
+        second[k] = d >= a.rest ? 0 : (d < a.offset ? d : d + 2 * a.pairs) - at[k];
+      }
+      const int head = h0 + h;
+      q[k] = head < a.first;
+      if (in[k]) {
+        const Tensor& x = a.t[q[k] ? 0 : 1];
+        const int hh = q[k] ? head : head - a.first;
+        const T* src = static_cast<const T*>(x.x) + b * x.xs[0] + hh * x.xs[1] + (t0 + t) * x.xs[2] + at[k];
+        lo[k] = *reinterpret_cast<const W*>(src);
+        hi[k] = *reinterpret_cast<const W*>(src + second[k]);
+        out[k] = b * x.ys[0] + hh * x.ys[1] + (t0 + t) * x.ys[2] + at[k];
+      }
+      item += step, ht += steps;
+      if (item >= items) item -= items, ++ht;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (!in[k]) continue;
+      if (turns[k]) {
+        alignas(16) T x[2 * VEC];
+        *reinterpret_cast<W*>(x) = lo[k];
+        *reinterpret_cast<W*>(x + VEC) = hi[k];
+        float2 cs[VEC];
+        if constexpr (VEC == 1) {
+          cs[0] = angles[mine[k]];
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float4 two = *reinterpret_cast<const float4*>(angles + mine[k] + e * turning);
+            cs[e] = make_float2(two.x, two.y), cs[e + 1] = make_float2(two.z, two.w);
+          }
+        }
+        if (a.interleaved) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float u = to_float(x[2 * e]), v = to_float(x[2 * e + 1]);
+            x[2 * e] = from_float<T>(u * cs[e].x - v * cs[e].y);
+            x[2 * e + 1] = from_float<T>(v * cs[e].x + u * cs[e].y);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float u = to_float(x[e]), v = to_float(x[e + VEC]);
+            x[e] = from_float<T>(u * cs[e].x - v * cs[e].y);
+            x[e + VEC] = from_float<T>(v * cs[e].x + u * cs[e].y);
+          }
+        }
+        lo[k] = *reinterpret_cast<const W*>(x);
+        hi[k] = *reinterpret_cast<const W*>(x + VEC);
+      }
+      T* dst = static_cast<T*>(a.t[q[k] ? 0 : 1].y) + out[k];
+      *reinterpret_cast<W*>(dst) = lo[k];
+      if (second[k] != 0) *reinterpret_cast<W*>(dst + second[k]) = hi[k];
+    }
+  }
+}
+
+}  // namespace rotary
+}  // namespace nsa

@@ -51,6 +51,10 @@ struct Api {
   decltype(&nsa_cache_read) cache_read = nullptr;
   decltype(&nsa_cache_attend) cache_attend = nullptr;
   decltype(&nsa_cache_attend_workspace_bytes) cache_attend_ws = nullptr;
+  decltype(&nsa_cache_reserve) cache_reserve = nullptr;
+  decltype(&nsa_cache_select) cache_select = nullptr;
+  decltype(&nsa_cache_select_workspace_bytes) cache_select_ws = nullptr;
+  decltype(&nsa_rotary) rotary = nullptr;
 };
 
 std::string dir_of(const std::string& path) {
@@ -88,9 +92,13 @@ const Api& api() {
     a.cache_read = reinterpret_cast<decltype(a.cache_read)>(dlsym(h, "nsa_cache_read"));
     a.cache_attend = reinterpret_cast<decltype(a.cache_attend)>(dlsym(h, "nsa_cache_attend"));
     a.cache_attend_ws = reinterpret_cast<decltype(a.cache_attend_ws)>(dlsym(h, "nsa_cache_attend_workspace_bytes"));
+    a.cache_reserve = reinterpret_cast<decltype(a.cache_reserve)>(dlsym(h, "nsa_cache_reserve"));
+    a.cache_select = reinterpret_cast<decltype(a.cache_select)>(dlsym(h, "nsa_cache_select"));
+    a.cache_select_ws = reinterpret_cast<decltype(a.cache_select_ws)>(dlsym(h, "nsa_cache_select_workspace_bytes"));
+    a.rotary = reinterpret_cast<decltype(a.rotary)>(dlsym(h, "nsa_rotary"));
   });
   if (!(a.forward && a.run && a.last_error && a.version && a.select && a.select_ws && a.cache_record && a.cache_write &&
-        a.cache_read && a.cache_attend && a.cache_attend_ws))
+        a.cache_read && a.cache_attend && a.cache_attend_ws && a.cache_reserve && a.cache_select && a.cache_select_ws && a.rotary))
     TORCH_CHECK(false, format_msg("libnsa_sel.so could not be loaded (build it first): %s", error.c_str()));
   return a;
 }
@@ -477,6 +485,163 @@ int64_t cache_record_bytes(int64_t d_qk, int64_t d_v) {
   return n;
 }
 
+// ------------------------------------------------------------------ pages, selection and positions of a step
+// [lens, cu_seqlens (empty without n_tokens), positions, slots, held, n_free]
+std::vector<torch::Tensor> cache_reserve(torch::Tensor pages, torch::Tensor held, torch::Tensor rows, torch::Tensor pool,
+                                         torch::Tensor n_free, c10::optional<int64_t> n_tokens, bool update) {
+  TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kInt && pages.dim() == 2, "pages must be an int32 CUDA tensor [S, W]");
+  const int64_t n = pages.size(0);
+  for (const torch::Tensor* t : {&held, &rows, &pool, &n_free})
+    TORCH_CHECK(t->is_cuda() && t->get_device() == pages.get_device() && t->scalar_type() == at::kInt && t->dim() == 1 &&
+                    t->is_contiguous(),
+                "held, rows, pool and n_free must be contiguous int32 vectors on the device of pages");
+  TORCH_CHECK(held.size(0) == n && rows.size(0) == n, "held and rows must have one entry for each sequence of pages");
+  TORCH_CHECK(n_free.size(0) == 1, "n_free must have one element");
+  TORCH_CHECK((pages.size(1) <= 1 || pages.stride(1) == 1) && (n <= 1 || pages.stride(0) >= pages.size(1)),
+              "the rows of pages must be contiguous and must not overlap");
+  TORCH_CHECK(!n_tokens.has_value() || *n_tokens >= 0, "n_tokens must not be negative");
+  const c10::cuda::CUDAGuard guard(pages.device());
+  const int64_t n_rows = n_tokens.value_or(n);
+  const auto i32s = held.options();
+  auto lens = torch::empty({n}, i32s), cu = torch::empty({n_tokens.has_value() ? n + 1 : 0}, i32s);
+  auto positions = torch::empty({n_rows}, i32s), slots = torch::empty({n_rows}, i32s.dtype(torch::kLong));
+  auto held_out = update ? held : torch::empty({n}, i32s), n_free_out = update ? n_free : torch::empty({1}, i32s);
+  nsa_cache_reserve_desc d;
+  memset(&d, 0, sizeof(d));
+  d.pages = pages.data_ptr<int32_t>();
+  d.held = held.data_ptr<int32_t>();
+  d.rows = rows.data_ptr<int32_t>();
+  d.pool = pool.data_ptr<int32_t>();
+  d.n_free = n_free.data_ptr<int32_t>();
+  d.held_out = held_out.data_ptr<int32_t>();
+  d.n_free_out = n_free_out.data_ptr<int32_t>();
+  d.lens = lens.data_ptr<int32_t>();
+  d.cu_seqlens = n_tokens.has_value() ? cu.data_ptr<int32_t>() : nullptr;
+  d.positions = n_rows > 0 ? positions.data_ptr<int32_t>() : nullptr;
+  d.slots = n_rows > 0 ? slots.data_ptr<int64_t>() : nullptr;
+  d.pages_stride = n > 1 ? pages.stride(0) : 0;
+  d.n_seqs = i32(n, "n_seqs");
+  d.width = i32(pages.size(1), "width");
+  d.pool_size = i32(pool.size(0), "pool_size");
+  d.n_rows = i32(n_rows, "n_tokens");
+  const int rc = api().cache_reserve(&d, current_stream());
+  if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_cache_reserve failed (%d): %s", rc, api().last_error()));
+  return {lens, cu, positions, slots, held_out, n_free_out};
+}
+
+torch::Tensor cache_select(torch::Tensor Q, torch::Tensor cache, torch::Tensor pages, torch::Tensor lens, int64_t n_sel,
+                           int64_t l_prime, int64_t cmp_block, int64_t cmp_stride, OptTensor cu_seqlens) {
+  TORCH_CHECK(Q.dim() == 3, "Q must be [N, Hq, d_qk]");
+  const int32_t dtype = dtype_code(Q, "Q");
+  TORCH_CHECK(cache.dim() == 3, "cache must be uint8 [num_pages, Hkv, record bytes]");
+  const int64_t d_qk = Q.size(2), d_v = cache.size(2) / 36 - d_qk;
+  nsa_cache_select_desc d;
+  memset(&d, 0, sizeof(d));
+  d.batch = cache_batch(cache, pages, lens, cu_seqlens, Q.size(0), d_qk, std::max<int64_t>(d_v, 0));
+  TORCH_CHECK(Q.is_cuda() && Q.get_device() == cache.get_device(), "all tensors must be on one device");
+  TORCH_CHECK(Q.size(1) > 0 && Q.size(1) % cache.size(1) == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(n_sel >= 1 && cmp_block >= 1 && cmp_stride >= 1, "n_sel, cmp_block and cmp_stride must be positive");
+  const c10::cuda::CUDAGuard guard(cache.device());
+  auto sel = torch::empty({Q.size(0), cache.size(1), n_sel}, Q.options().dtype(torch::kInt));
+  if ((Q.size(0) > 1 && Q.stride(0) == 0) || (Q.size(1) > 1 && Q.stride(1) == 0)) Q = Q.contiguous();  // (0 means the default)
+  if (Q.size(0) > 0) {
+    check_rows(Q, "Q");
+    d.q = Q.data_ptr();
+    d.sel = sel.data_ptr<int32_t>();
+  }
+  d.q_row_stride = stride_of(Q, 0);
+  d.q_head_stride = stride_of(Q, 1);
+  d.heads_q = i32(Q.size(1), "Hq");
+  d.n_sel = i32(n_sel, "n_sel");
+  d.block_size = i32(l_prime, "l_prime");
+  d.cmp_block = i32(cmp_block, "cmp_block");
+  d.cmp_stride = i32(cmp_stride, "cmp_stride");
+  d.q_dtype = dtype;
+  const int64_t ws = api().cache_select_ws(&d);
+  if (ws < 0) TORCH_CHECK(false, format_msg("nsa_cache_select failed: %s", api().last_error()));
+  auto work = torch::empty({ws}, Q.options().dtype(torch::kByte));
+  d.workspace = work.data_ptr();
+  const int rc = api().cache_select(&d, current_stream());
+  if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_cache_select failed (%d): %s", rc, api().last_error()));
+  return sel;
+}
+
+// X [N, H, d] or [B, H, T, d]: strides of batch, head, token.
+void rotary_strides(const torch::Tensor& x, int64_t (&s)[3]) {
+  const bool rows = x.dim() == 3;
+  s[0] = rows ? 0 : stride_of(x, 0);
+  s[1] = stride_of(x, 1);
+  s[2] = stride_of(x, rows ? 0 : 2);
+}
+
+// [Q', K'] (K' empty without K).  `token_major` says of each whether [B, H, T, d] is laid out as [B, T, H, d].
+std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor turns, torch::Tensor axis,
+                                  int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
+                                  bool q_token_major, bool k_token_major) {
+  TORCH_CHECK(Q.is_cuda() && (Q.dim() == 3 || Q.dim() == 4), "Q must be a CUDA tensor [N, H, d] or [B, H, T, d]");
+  TORCH_CHECK(Q.scalar_type() == at::kBFloat16 || Q.scalar_type() == at::kHalf || Q.scalar_type() == at::kFloat,
+              "Q must be bfloat16, float16 or float32");
+  const bool rows = Q.dim() == 3;
+  const int64_t B = rows ? 1 : Q.size(0), T = Q.size(rows ? 0 : 2);
+  TORCH_CHECK(Q.size(-1) == d_head, "the plan is for heads of another size");
+  if (K.has_value()) {
+    TORCH_CHECK(K->is_cuda() && K->get_device() == Q.get_device() && K->scalar_type() == Q.scalar_type() && K->dim() == Q.dim(),
+                "K must be of Q's dtype and dims, on its device");
+    TORCH_CHECK((rows ? 1 : K->size(0)) == B && K->size(rows ? 0 : 2) == T && K->size(-1) == d_head,
+                "K must have Q's tokens and head size");
+  }
+  TORCH_CHECK(positions.is_cuda() && positions.get_device() == Q.get_device() && positions.scalar_type() == at::kInt,
+              "positions must be int32 on Q's device");
+  const int64_t lead = axes > 1 ? 1 : 0;
+  TORCH_CHECK(positions.dim() == lead + (rows ? 1 : 2) && (!lead || positions.size(0) == axes) &&
+                  (rows || positions.size(lead) == B) && positions.size(-1) == T,
+              "positions must be [N] or [B, T], one for each token of Q, with the axes before them if there are several");
+  TORCH_CHECK(!turns.is_cuda() && turns.scalar_type() == at::kLong && turns.is_contiguous() && !axis.is_cuda() &&
+                  axis.scalar_type() == at::kByte && axis.is_contiguous() && axis.numel() == turns.numel(),
+              "a plan's turns and axis are int64 and uint8 host vectors of one length");
+  const c10::cuda::CUDAGuard guard(Q.device());
+  nsa_rotary_desc d;
+  memset(&d, 0, sizeof(d));
+  torch::Tensor out[2];
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && !K.has_value()) {
+      out[1] = torch::empty({0}, Q.options());
+      continue;
+    }
+    torch::Tensor x = i == 0 ? Q : *K;
+    if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
+    if (!rows && (i == 0 ? q_token_major : k_token_major))
+      out[i] = torch::empty({B, T, x.size(1), d_head}, x.options()).transpose(1, 2);
+    else
+      out[i] = torch::empty(x.sizes(), x.options());
+    if (x.numel() == 0) continue;
+    d.t[i].x = x.data_ptr();
+    d.t[i].y = out[i].data_ptr();
+    rotary_strides(x, d.t[i].x_stride);
+    rotary_strides(out[i], d.t[i].y_stride);
+    d.t[i].heads = i32(x.size(1), "heads");
+    (i == 0 ? Q : *K) = x;  // (a copy lives until the launch)
+  }
+  if (B * T > 0) d.positions = positions.data_ptr<int32_t>();
+  d.pos_stride[0] = lead ? positions.stride(0) : 0;
+  d.pos_stride[1] = rows ? 0 : positions.stride(lead);
+  d.pos_stride[2] = positions.stride(-1);
+  d.turns = reinterpret_cast<const uint64_t*>(turns.data_ptr<int64_t>());
+  d.axis = axis.data_ptr<uint8_t>();
+  d.batch = i32(B, "batch");
+  d.tokens = i32(T, "tokens");
+  d.d = i32(d_head, "d");
+  d.offset = i32(offset, "offset");
+  d.pairs = i32(turns.numel(), "pairs");
+  d.axes = i32(axes, "axes");
+  d.interleaved = interleaved ? 1 : 0;
+  d.inverse = inverse ? 1 : 0;
+  d.dtype = Q.scalar_type() == at::kBFloat16 ? NSA_DTYPE_BF16 : Q.scalar_type() == at::kHalf ? NSA_DTYPE_F16 : NSA_DTYPE_F32;
+  const int rc = api().rotary(&d, current_stream());
+  if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_rotary failed (%d): %s", rc, api().last_error()));
+  return {out[0], out[1]};
+}
+
 int64_t library_version() { return api().version(); }
 
 }  // namespace
@@ -513,5 +678,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("l_prime") = 64, py::arg("window") = 0, py::arg("cu_seqlens") = py::none(), py::arg("scale") = 0.0,
         py::arg("out") = py::none(), py::arg("weight") = py::none(), py::arg("accumulate") = false,
         py::arg("with_lse") = true, py::arg("err") = py::none(), py::arg("timeout_ms") = 0, py::arg("debug_flags") = 0);
+  m.def("cache_reserve", &cache_reserve,
+        "cache_reserve(pages, held, rows, pool, n_free, n_tokens, update) -> [lens, cu_seqlens, positions, slots, held, n_free]",
+        py::arg("pages"), py::arg("held"), py::arg("rows"), py::arg("pool"), py::arg("n_free"), py::arg("n_tokens") = py::none(),
+        py::arg("update") = true);
+  m.def("cache_select", &cache_select,
+        "cache_select(Q, cache, pages, lens, n_sel, l_prime, cmp_block, cmp_stride, cu_seqlens) -> sel int32", py::arg("Q"),
+        py::arg("cache"), py::arg("pages"), py::arg("lens"), py::arg("n_sel"), py::arg("l_prime") = 64,
+        py::arg("cmp_block") = 32, py::arg("cmp_stride") = 16, py::arg("cu_seqlens") = py::none());
+  m.def("rotary", &rotary,
+        "rotary(Q, K, positions, turns, axis, axes, d, offset, interleaved, inverse, q_token_major, k_token_major) -> [Q', K']",
+        py::arg("Q"), py::arg("K"), py::arg("positions"), py::arg("turns"), py::arg("axis"), py::arg("axes"), py::arg("d"),
+        py::arg("offset"), py::arg("interleaved"), py::arg("inverse") = false, py::arg("q_token_major") = false,
+        py::arg("k_token_major") = false);
   m.def("library_version", &library_version);
 }

@@ -6,7 +6,9 @@ is missing, or the device is not a B200, the call raises.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import math
+from fractions import Fraction
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -172,6 +174,158 @@ def cache_attend(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens
     o, lse = _C.cache_attend(Q, cache, pages, lens, sel, int(l_prime), int(window), cu_seqlens, float(scale), out, weight,
                              bool(accumulate), bool(with_lse), err)
     return o, lse
+
+
+class CacheBatch(NamedTuple):
+    """A call's batch, as :func:`cache_reserve` works it out."""
+    lens: torch.Tensor                  # int32 [S] tokens of the sequences that got rows (these included), 0 for the others
+    cu_seqlens: Optional[torch.Tensor]  # int32 [S + 1] where the rows are packed (n_tokens), else None
+    positions: torch.Tensor             # int32 [N] a row's position in its sequence, -1 for an absent row
+    slots: torch.Tensor                 # int64 [N] PAGE * page + position % PAGE, -1 for an absent row
+    held: torch.Tensor                  # int32 [S] tokens of every sequence after the call
+    n_free: torch.Tensor                # int32 [1] free pages after the call
+
+
+def cache_reserve(pages: torch.Tensor, held: torch.Tensor, rows: torch.Tensor, pool: torch.Tensor, n_free: torch.Tensor,
+                  n_tokens: Optional[int] = None, update: bool = True) -> CacheBatch:
+    """Page table, lengths, packing, positions and slots of a call's batch, from the tokens that each request gets or gives
+    back (nsa_cache_reserve).  Everything is on the device: a step can be captured, and replayed with other ``rows``.
+
+    ``pages`` int32 [S, W] is the page table, ``held`` int32 [S] the tokens that the sequences hold, ``pool`` int32 [P] the
+    free pages, of which the first ``n_free`` (int32 [1]) count.  ``rows`` int32 [S]: > 0, the sequence asks for that many
+    more tokens; < 0, it gives its last ones back (rejected drafts, or all of a sequence that has ended: ``-held``), and the pages
+    with them; 0, it has no part in the call.  Pages that are given back come first, then those that are asked for are taken
+    from the end of the pool, by the sequences in their order.  A sequence that does not fit its row of the table, or for which
+    (it and those before it) the pool has too few pages, stays as it was and has no rows: its ``lens`` is 0, which the cache's
+    calls take as absent rows, and ``held`` tells the scheduler.
+
+    With ``n_tokens`` = N the call's rows are packed (``rows[s]`` for each sequence that asks, those of refused ones too, N at
+    least their sum); without, row s is sequence s's last token (``rows`` at most 1).  ``pages`` and ``pool`` are changed in
+    place, ``held`` and ``n_free`` too unless ``update`` is False: then new tensors are returned and nothing that counts has
+    changed, so the call can be made again.  A page that two sequences share must not be given back while the other uses it."""
+    lens, cu, positions, slots, held, n_free = _C.cache_reserve(pages, held, rows, pool, n_free,
+                                                                None if n_tokens is None else int(n_tokens), bool(update))
+    return CacheBatch(lens, None if n_tokens is None else cu, positions, slots, held, n_free)
+
+
+def cache_select(Q: torch.Tensor, cmp_cache: torch.Tensor, cmp_pages: torch.Tensor, lens: torch.Tensor, n_sel: int,
+                 l_prime: int = 64, cmp_block: int = 32, cmp_stride: int = 16,
+                 cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`select_blocks` for the batch's newest tokens, from the compressed keys of a 4-bit cache (nsa_cache_select;
+    ``nsa.cache_compress`` keeps them): int32 [N, Hkv, n_sel], the ``sel`` of :func:`cache_attend`.
+
+    Q [N, Hq, d_qk] (bf16 or fp16) has the rows of :func:`cache_attend`; ``lens`` int32 [S] are the tokens of the sequences (not
+    their compressed keys).  The row at position t gets what the last row of ``select_blocks`` gets for t + 1 tokens: the
+    blocks of ``l_prime`` tokens with the largest sums of (summed query heads) . (compressed key), the best first, -1 behind
+    the last.  Scores are compared as 64-bit sums, equal ones by the lower block; scores that are not finite come last.
+    ``n_sel`` at most 1024, Hq / Hkv at most 256, sequences of up to 2^24 tokens (longer ones, and those whose compressed keys
+    ``cmp_pages`` cannot hold, select nothing).  No gradients."""
+    return _C.cache_select(Q, cmp_cache, cmp_pages, lens, int(n_sel), int(l_prime), int(cmp_block), int(cmp_stride), cu_seqlens)
+
+
+class RotaryPlan(NamedTuple):
+    """Which values of a head :func:`rotary` turns, and how fast (made by :func:`rotary_plan`, kept for all calls)."""
+    d: int
+    offset: int
+    interleaved: bool
+    axes: int
+    turns: torch.Tensor  # int64 [pairs] on the host: inv_freq / 2 pi in units of 2^-64
+    axis: torch.Tensor   # uint8 [pairs] on the host
+
+
+# 2^192 / (2 pi)
+_TURN = round(2**192 / (2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640629")))
+
+
+def _turns(inv_freq: float) -> int:
+    """inv_freq / (2 pi) in units of 2^-64, modulo a turn, as int64."""
+    n, d = float(inv_freq).as_integer_ratio()
+    t = (2 * n * _TURN // (d << 128) + 1) // 2 % 2**64
+    return t - 2**64 if t >= 2**63 else t
+
+
+def rotary_plan(d: int, *, rotary_dim: Optional[int] = None, offset: int = 0, base: float = 10000.0,
+                sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                inv_freq: Optional[Sequence[float]] = None, axis: Optional[Sequence[int]] = None) -> RotaryPlan:
+    """How :func:`rotary` turns heads of ``d`` (at most 256) values: ``rotary_dim`` of them (all unless given) from ``offset``
+    on, value i with value i + rotary_dim / 2 of that part, or neighbours (``interleaved``).
+
+    Pair i turns by position * ``base`` ** (-2 i / rotary_dim), or position * ``inv_freq[i]`` (radians, taken in 64 bits).  With
+    several axes (time, height, width) each pair follows one: ``sections`` = (16, 24, 24) gives the first 16 pairs the first
+    axis and so on; ``axis`` names it pair by pair instead.  At most four axes."""
+    dim = d if rotary_dim is None else rotary_dim
+    if not 0 < d <= 256:
+        raise ValueError("d must be from 1 to 256")
+    if dim < 2 or dim % 2 or offset < 0 or offset + dim > d:
+        raise ValueError("rotary_dim must be even and positive, and lie in the head with its offset")
+    pairs = dim // 2
+    if inv_freq is None:
+        if not base > 0:
+            raise ValueError("base must be positive")
+        inv_freq = [float(base) ** (-i / pairs) for i in range(pairs)]
+    if axis is None:
+        sections = [pairs] if sections is None else list(sections)
+        if any(n < 0 for n in sections) or sum(sections) != pairs:
+            raise ValueError(f"sections must add up to the {pairs} pairs")
+        axis, axes = [a for a, n in enumerate(sections) for _ in range(n)], len(sections)
+    elif sections is not None:
+        raise ValueError("sections and axis exclude each other")
+    else:
+        axis = [int(a) for a in axis]
+        axes = max(axis, default=0) + 1
+    if len(axis) != pairs or len(inv_freq) != pairs:
+        raise ValueError(f"axis and inv_freq must have an entry for each of the {pairs} pairs")
+    if axes > 4 or min(axis) < 0:
+        raise ValueError("there are one to four axes")
+    if not all(math.isfinite(f) for f in inv_freq):
+        raise ValueError("inv_freq must be finite")
+    return RotaryPlan(d, offset, bool(interleaved), axes,
+                      torch.tensor([_turns(f) for f in inv_freq], dtype=torch.int64, device="cpu"),
+                      torch.tensor(axis, dtype=torch.uint8, device="cpu"))
+
+
+def _turned(Q, K, positions, plan: RotaryPlan, inverse: bool, token_major=(False, False)):
+    q, k = _C.rotary(Q, K, positions, plan.turns, plan.axis, plan.axes, plan.d, plan.offset, plan.interleaved, inverse,
+                     *token_major)
+    return q, None if K is None else k
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, Q, K, positions, plan, inverse):
+        ctx.save_for_backward(positions)
+        # gradients come back as the inputs lie: heads of [B, H, T, d] may be a view of [B, T, H, d]
+        ctx.token_major = [x is not None and x.dim() == 4 and not x.is_contiguous() and x.transpose(1, 2).is_contiguous()
+                           for x in (Q, K)]
+        ctx.plan, ctx.inverse = plan, inverse
+        ctx.set_materialize_grads(False)
+        return _turned(Q, K, positions, plan, inverse)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dQ, dK):
+        (positions,) = ctx.saved_tensors
+        dQ, dK = (g if need else None for g, need in zip((dQ, dK), ctx.needs_input_grad))
+        q_major, k_major = ctx.token_major
+        if dQ is None:
+            dK = None if dK is None else _turned(dK, None, positions, ctx.plan, not ctx.inverse, (k_major, False))[0]
+        else:
+            dQ, dK = _turned(dQ, dK, positions, ctx.plan, not ctx.inverse, (q_major, k_major))
+        return dQ, dK, None, None, None
+
+
+def rotary(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryPlan,
+           inverse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Turns Q and K (or Q alone: ``K`` None) by their tokens' positions (nsa_rotary).
+
+    Rows Q [N, Hq, d] and K [N, Hkv, d] as the cache's calls take them, or heads [B, Hq, T, d] and [B, Hkv, T, d] as the forward
+    does; bf16, fp16 or fp32, any strides (a projection's [B, T, H, d] is given as ``x.transpose(1, 2)``).  ``positions`` int32
+    [N] or [B, T] (any strides, e.g. expanded over the batch), with the axes of the plan before that if there are several.
+    The results are contiguous and of the inputs' dtype; angles are exact for all int32 positions, products are fp32.
+    Differentiable in Q and K; ``inverse`` turns back."""
+    if torch.is_grad_enabled() and (Q.requires_grad or (K is not None and K.requires_grad)):
+        return _Rotary.apply(Q, K, positions, plan, bool(inverse))
+    return _turned(Q, K, positions, plan, bool(inverse))
 
 
 def library_version() -> int:
