@@ -51,9 +51,9 @@ def build_kernel_lib(force: bool = False, extra: List[str] = ()) -> str:
     # one object for each translation unit: rebuilt when it or a header it may include is newer
     units = {"nsa_sel_api.cu": sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh") and "cache" not in f)
              + ["nsa_host.h"],
-             "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "nsa_cache_host.h", "nsa_programmatic.cuh",
-                                  "ptx.cuh", "nsa_host.h"],
-             "nsa_step_api.cu": ["nsa_cache_index.h", "nsa_cache_select_index.h", "nsa_cache_select_kernel.cuh",
+             "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "nsa_cache_decode.cuh", "nsa_cache_host.h",
+                                  "nsa_programmatic.cuh", "ptx.cuh", "nsa_host.h"],
+             "nsa_step_api.cu": ["nsa_cache_index.h", "nsa_cache_select_index.h", "nsa_cache_select_kernel.cuh", "nsa_cache_decode.cuh",
                                  "nsa_reserve_index.h", "nsa_reserve_kernel.cuh", "nsa_rotary_kernel.cuh", "nsa_linspace.cuh",
                                  "nsa_cache_host.h", "nsa_programmatic.cuh", "ptx.cuh", "nsa_host.h"]}
     objects = []

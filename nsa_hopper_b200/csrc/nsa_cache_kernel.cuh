@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "nsa_cache_decode.cuh"
 #include "nsa_cache_index.h"
 #include "nsa_programmatic.cuh"
 #include "ptx.cuh"
@@ -51,20 +52,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 // ------------------------------------------------------------------ 4-bit conversions
-// Two codes of byte I of `w` as fp16 pair (low nibble in the low half).
-template <int I>
-__device__ __forceinline__ uint32_t decode_byte(uint32_t w) {
-  uint32_t r;
-  if constexpr (I == 0)
-    asm("{.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;}" : "=r"(r) : "r"(w));
-  else if constexpr (I == 1)
-    asm("{.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b1;}" : "=r"(r) : "r"(w));
-  else if constexpr (I == 2)
-    asm("{.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b2;}" : "=r"(r) : "r"(w));
-  else
-    asm("{.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b3;}" : "=r"(r) : "r"(w));
-  return r;
-}
 // Codes of eight values, the first in the lowest nibble.
 __device__ __forceinline__ uint32_t encode8(const float* y) {
   uint32_t r;
@@ -78,11 +65,6 @@ __device__ __forceinline__ uint32_t encode8(const float* y) {
       : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return r;
 }
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t low2(uint32_t x) {  // (an operand's modifier, not an instruction)
   uint32_t r;
   asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {l, l};}" : "=r"(r) : "r"(x));
@@ -93,9 +75,6 @@ __device__ __forceinline__ uint32_t high2(uint32_t x) {
   asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {h, h};}" : "=r"(r) : "r"(x));
   return r;
 }
-// A scale byte in both halves of an fp16 pair.
-__device__ __forceinline__ uint32_t scale2(uint32_t byte) { return byte * 0x00800080u; }
-
 // The scale byte of a group with the largest value amax: the scale nearest to amax / 6, ties to even, at most 10240 (0xE2).
 // The product with 1/6 is off by 2^-23 of itself; rounded to 17 bits it is the quotient again where that has few bits (the
 // ties), and amax's 8 or 11 bits keep every other quotient 2^-12 of itself away from a tie.
@@ -385,12 +364,6 @@ __device__ __noinline__ void wait_all(uint64_t* bars, uint32_t phases, uint32_t 
 }
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float exp2_fast(float x) { return ptx::ex2(x); }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {

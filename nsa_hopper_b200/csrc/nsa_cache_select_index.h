@@ -31,19 +31,40 @@ NSA_HD int32_t tokens_of(const Batch& b, int row, int32_t most) {
 }
 NSA_HD int32_t blocks_of(int32_t tokens, int32_t shift) { return (int32_t)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
-// The block of compressed key i of n.
-NSA_LINSPACE int32_t block_of(int i, int32_t tokens, int32_t n, int32_t shift) {
-  const int32_t block = (int32_t)linspace_f32(i, tokens, n) >> shift, last = blocks_of(tokens, shift) - 1;
-  return block < last ? block : last;
+// The compressed keys of a row's tokens among the blocks.
+struct Places {
+  int32_t tokens, n;  // n: compressed keys
+  int32_t shift;      // of a block's tokens
+  float step;         // tokens from one key to the next
+  float per;          // and the reverse, about
+};
+NSA_LINSPACE Places places_of(int32_t tokens, int32_t block, int32_t stride, int32_t shift) {
+  Places p;
+  p.tokens = tokens, p.n = completed(tokens, block, stride), p.shift = shift;
+  p.step = p.n > 1 ? linspace_step(tokens, p.n) : 1.f;
+  p.per = 1.f / p.step;
+  return p;
 }
-// The first compressed key that is not in a block before `block`; n if there is none.
-NSA_LINSPACE int32_t first_key(int32_t block, int32_t tokens, int32_t n, int32_t shift) {
-  if (block <= 0 || n <= 1) return block <= 0 ? 0 : n;
-  int64_t i = (int64_t)((double)((int64_t)block << shift) * (double)(n - 1) / (double)(tokens - 1));
-  if (i > n) i = n;
-  while (i > 0 && block_of((int)i - 1, tokens, n, shift) >= block) --i;
-  while (i < n && block_of((int)i, tokens, n, shift) < block) ++i;
-  return (int32_t)i;
+// linspace_at with one rounding.  It has one too: a key and a position are below 2^24 and the step is at least 1, so that
+// products and differences have at most 48 bits and are exact in fp64 (the CPU tests compare the two).
+NSA_LINSPACE float place_of(const Places& p, int32_t i) {
+#ifdef __CUDA_ARCH__
+  return i < p.n / 2 ? __fmul_rn(p.step, (float)i) : __fmaf_rn(-p.step, (float)(p.n - 1 - i), (float)(p.tokens - 1));
+#else
+  return i < p.n / 2 ? p.step * (float)i : fmaf(-p.step, (float)(p.n - 1 - i), (float)(p.tokens - 1));
+#endif
+}
+// The block of key i of more than one.  (A place is at most that of the last token, so no block is behind the last one.)
+NSA_LINSPACE int32_t block_of(const Places& p, int32_t i) { return (int32_t)place_of(p, i) >> p.shift; }
+// The first key that is not in a block before `block`; n if there is none.
+NSA_LINSPACE int32_t first_key(const Places& p, int32_t block) {
+  if (block <= 0) return 0;
+  if (p.n <= 1) return p.n;
+  const float guess = (float)((int64_t)block << p.shift) * p.per;
+  int32_t i = guess < (float)p.n ? (int32_t)guess : p.n;
+  while (i > 0 && block_of(p, i - 1) >= block) --i;
+  while (i < p.n && block_of(p, i) < block) ++i;
+  return i;
 }
 
 }  // namespace cache_select

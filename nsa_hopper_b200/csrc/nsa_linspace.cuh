@@ -18,21 +18,26 @@ namespace nsa {
 #else
 #define NSA_LINSPACE inline
 #endif
-NSA_LINSPACE float linspace_f32(int i, int T, int n) {
-  if (n == 1) return 0.f;
-#ifndef __CUDA_ARCH__
-  const float step = (float)(T - 1) / (float)(n - 1);
-  if (i < n / 2) return (float)((double)step * (double)i);
-  return (float)((double)(T - 1) - (double)step * (double)(n - 1 - i));
+// The step of n > 1 positions, and position i of them.
+NSA_LINSPACE float linspace_step(int T, int n) {
+#ifdef __CUDA_ARCH__
+  return __fdiv_rn((float)(T - 1), (float)(n - 1));
 #else
-  const float step = __fdiv_rn((float)(T - 1), (float)(n - 1));
-  if (i < n / 2) return (float)__dmul_rn((double)step, (double)i);
-  return (float)__dsub_rn((double)(T - 1), __dmul_rn((double)step, (double)(n - 1 - i)));
+  return (float)(T - 1) / (float)(n - 1);
 #endif
 }
+NSA_LINSPACE float linspace_at(float step, int i, int T, int n) {
+#ifdef __CUDA_ARCH__
+  if (i < n / 2) return (float)__dmul_rn((double)step, (double)i);
+  return (float)__dsub_rn((double)(T - 1), __dmul_rn((double)step, (double)(n - 1 - i)));
+#else
+  if (i < n / 2) return (float)((double)step * (double)i);
+  return (float)((double)(T - 1) - (double)step * (double)(n - 1 - i));
+#endif
+}
+NSA_LINSPACE float linspace_f32(int i, int T, int n) { return n == 1 ? 0.f : linspace_at(linspace_step(T, n), i, T, n); }
 
 #ifdef __CUDACC__
-
 __device__ __forceinline__ float floor_div_f32(float a, float b) {
   const float mod = fmodf(a, b);
   float div = __fdiv_rn(__fsub_rn(a, mod), b);

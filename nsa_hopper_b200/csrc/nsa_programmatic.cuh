@@ -3,10 +3,14 @@
 
 namespace nsa {
 
+// Lets the next kernel be launched.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+// Until all earlier kernels have ended.
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next kernel be launched, and touches no memory before all earlier ones have ended.
 __device__ __forceinline__ void start_in_order() {
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  allow_next();
+  wait_for_earlier();
 }
 
 }  // namespace nsa

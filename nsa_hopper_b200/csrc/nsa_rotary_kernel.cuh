@@ -23,8 +23,6 @@ namespace rotary {
 
 constexpr int kMaxPairs = 128;  // of a head of 256 values
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;   // of a block
-constexpr int kAtOnce = 4;      // items of a thread whose loads are in flight together
 
 struct Tensor {
   const void* x;
@@ -38,7 +36,6 @@ struct Args {
   int32_t heads, first;          // of both tensors together, of the first one
   int32_t batch, tokens;         // tokens of a batch entry
   int32_t offset, pairs, rest;   // first value and pairs of the rotary part; values beside it
-  int32_t per_block;             // tokens of a block: a power of two
   int32_t heads_block;           // heads of a block
   int32_t interleaved;
   uint32_t flip;                 // sign bit of the sines
@@ -82,6 +79,13 @@ __device__ __forceinline__ float2 cos_sin(uint64_t turns, uint32_t flip) {
   return make_float2(__uint_as_float(__float_as_uint(x) ^ turned), __uint_as_float(__float_as_uint(y) ^ turned ^ flip));
 }
 
+template <class T>
+__device__ __forceinline__ void turn(T& a, T& b, float2 cs) {
+  const float u = to_float(a), v = to_float(b);
+  a = from_float<T>(u * cs.x - v * cs.y);
+  b = from_float<T>(v * cs.x + u * cs.y);
+}
+
 // Places of the angles in shared memory: those that neighbouring items of a warp read at once lie side by side.
 template <int VEC>
 __device__ __forceinline__ int place(int pair, int items) {
@@ -90,101 +94,75 @@ __device__ __forceinline__ int place(int pair, int items) {
   return ((e / 2) * items + k) * 2 + e % 2;
 }
 
+// A block turns a.heads_block heads of one token.
 template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads) kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 2048 / kThreads) kernel(const __grid_constant__ Args a) {
   using W = typename Word<VEC * (int)sizeof(T)>::type;
-  extern __shared__ float2 angles[];  // [per_block][pairs]
+  __shared__ __align__(16) float2 angles[kMaxPairs];
   const int tid = threadIdx.x;
-  const int blocks = (a.tokens + a.per_block - 1) / a.per_block;
-  const int b = blockIdx.x / blocks, t0 = (blockIdx.x - b * blocks) * a.per_block;
-  const int h0 = blockIdx.y * a.heads_block, heads = min(a.heads_block, a.heads - h0);
-  const int tokens = min(a.per_block, a.tokens - t0);
+  const int b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens;
+  const int h0 = blockIdx.y * a.heads_block, h1 = min(h0 + a.heads_block, a.heads);
   const int turning = a.pairs / VEC;                                // items of a head that turn 2 VEC values
   const int items = turning + (a.rest + 2 * VEC - 1) / (2 * VEC);   // and those that copy as many
   start_in_order();
-  for (int i = tid; i < a.pairs * tokens; i += kThreads) {
-    const int t = i / a.pairs, pair = i - t * a.pairs;
-    const int64_t pos = a.pos[a.axis[pair] * a.ps[0] + b * a.ps[1] + (t0 + t) * a.ps[2]];
-    angles[t * a.pairs + place<VEC>(pair, turning)] = cos_sin((uint64_t)pos * a.turn[pair], a.flip);
+  if (tid < a.pairs) {
+    const int64_t pos = a.pos[a.axis[tid] * a.ps[0] + b * a.ps[1] + t * a.ps[2]];
+    angles[place<VEC>(tid, turning)] = cos_sin((uint64_t)pos * a.turn[tid], a.flip);
   }
   __syncthreads();
 
-  // item, token and head of a thread's next item, stepped without divisions
-  const int shift = 31 - __clz(a.per_block);
-  int item = tid % items, ht = tid / items;
+  // item and head of a thread's next item, stepped without divisions
+  int item = tid % items, head = h0 + tid / items;
   const int step = kThreads % items, steps = kThreads / items;
-  while (ht >> shift < heads) {
-    W lo[kAtOnce], hi[kAtOnce];
-    int64_t out[kAtOnce];
-    int at[kAtOnce], second[kAtOnce], mine[kAtOnce];
-    bool in[kAtOnce], turns[kAtOnce], q[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int t = ht & (a.per_block - 1), h = ht >> shift;
-      in[k] = h < heads && t < tokens;
-      turns[k] = item < turning;
-      mine[k] = t * a.pairs + (VEC == 1 ? 1 : 2) * item;
-      if (turns[k]) {
-        at[k] = a.offset + item * VEC * (a.interleaved ? 2 : 1);
-        second[k] = a.interleaved ? VEC : a.pairs;
+  for (; head < h1; item += step, head += steps) {
+    if (item >= items) {
+      item -= items;
+      if (++head >= h1) break;
+    }
+    // two words, `second` values apart
+    int at, second;
+    if (item < turning) {
+      at = a.offset + item * VEC * (a.interleaved ? 2 : 1);
+      second = a.interleaved ? VEC : a.pairs;
+    } else {
+      // (the values beside the rotary part stand in one line; a last half item has no second word)
+      const int c = (item - turning) * 2 * VEC, d = c + VEC;
+      at = c < a.offset ? c : c + 2 * a.pairs;
+      second = d >= a.rest ? 0 : (d < a.offset ? d : d + 2 * a.pairs) - at;
+    }
+    const bool q = head < a.first;
+    const Tensor& x = a.t[q ? 0 : 1];
+    const int h = q ? head : head - a.first;
+    const T* src = static_cast<const T*>(x.x) + (b * x.xs[0] + h * x.xs[1] + t * x.xs[2]) + at;
+    W lo = *reinterpret_cast<const W*>(src), hi = *reinterpret_cast<const W*>(src + second);
+    if (item < turning) {
+      alignas(16) T v[2 * VEC];
+      *reinterpret_cast<W*>(v) = lo;
+      *reinterpret_cast<W*>(v + VEC) = hi;
+      float2 cs[VEC];
+      const float2* mine = angles + (VEC == 1 ? 1 : 2) * item;
+      if constexpr (VEC == 1) {
+        cs[0] = mine[0];
       } else {
-        // (the values beside the rotary part stand in one line; a last half item has no second word)
-        const int c = (item - turning) * 2 * VEC, d = c + VEC;
-        at[k] = c < a.offset ? c : c + 2 * a.pairs;
-        second[k] = d >= a.rest ? 0 : (d < a.offset ? d : d + 2 * a.pairs) - at[k];
-      }
-      const int head = h0 + h;
-      q[k] = head < a.first;
-      if (in[k]) {
-        const Tensor& x = a.t[q[k] ? 0 : 1];
-        const int hh = q[k] ? head : head - a.first;
-        const T* src = static_cast<const T*>(x.x) + b * x.xs[0] + hh * x.xs[1] + (t0 + t) * x.xs[2] + at[k];
-        lo[k] = *reinterpret_cast<const W*>(src);
-        hi[k] = *reinterpret_cast<const W*>(src + second[k]);
-        out[k] = b * x.ys[0] + hh * x.ys[1] + (t0 + t) * x.ys[2] + at[k];
-      }
-      item += step, ht += steps;
-      if (item >= items) item -= items, ++ht;
-    }
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      if (!in[k]) continue;
-      if (turns[k]) {
-        alignas(16) T x[2 * VEC];
-        *reinterpret_cast<W*>(x) = lo[k];
-        *reinterpret_cast<W*>(x + VEC) = hi[k];
-        float2 cs[VEC];
-        if constexpr (VEC == 1) {
-          cs[0] = angles[mine[k]];
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float4 two = *reinterpret_cast<const float4*>(angles + mine[k] + e * turning);
-            cs[e] = make_float2(two.x, two.y), cs[e + 1] = make_float2(two.z, two.w);
-          }
+        for (int e = 0; e < VEC; e += 2) {
+          const float4 two = *reinterpret_cast<const float4*>(mine + e * turning);
+          cs[e] = make_float2(two.x, two.y), cs[e + 1] = make_float2(two.z, two.w);
         }
-        if (a.interleaved) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float u = to_float(x[2 * e]), v = to_float(x[2 * e + 1]);
-            x[2 * e] = from_float<T>(u * cs[e].x - v * cs[e].y);
-            x[2 * e + 1] = from_float<T>(v * cs[e].x + u * cs[e].y);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float u = to_float(x[e]), v = to_float(x[e + VEC]);
-            x[e] = from_float<T>(u * cs[e].x - v * cs[e].y);
-            x[e + VEC] = from_float<T>(v * cs[e].x + u * cs[e].y);
-          }
-        }
-        lo[k] = *reinterpret_cast<const W*>(x);
-        hi[k] = *reinterpret_cast<const W*>(x + VEC);
       }
-      T* dst = static_cast<T*>(a.t[q[k] ? 0 : 1].y) + out[k];
-      *reinterpret_cast<W*>(dst) = lo[k];
-      if (second[k] != 0) *reinterpret_cast<W*>(dst + second[k]) = hi[k];
+      if (a.interleaved) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) turn(v[2 * e], v[2 * e + 1], cs[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) turn(v[e], v[e + VEC], cs[e]);
+      }
+      lo = *reinterpret_cast<const W*>(v);
+      hi = *reinterpret_cast<const W*>(v + VEC);
     }
+    T* dst = static_cast<T*>(x.y) + (b * x.ys[0] + h * x.ys[1] + t * x.ys[2]) + at;
+    *reinterpret_cast<W*>(dst) = lo;
+    if (second != 0) *reinterpret_cast<W*>(dst + second) = hi;
   }
 }
 

@@ -122,19 +122,19 @@ int32_t unit_of(const nsa_cache_select_desc* d) {
 
 template <int D>
 int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t st) {
-  const int fixed = (int)sizeof(select::Warp<D>) * select::kWarps;
-  const int rc = allow_smem(reinterpret_cast<const void*>(&select::score_kernel<D>), fixed + (select::kMaxRows + 1) * 4, dev,
-                            D == 64 ? 2u : D == 128 ? 4u : 8u);
+  const int list = select::list_bytes(a.n_sel);
+  const uint32_t bit = D == 64 ? 2u : D == 128 ? 4u : 8u;
+  const int rc = allow_smem(reinterpret_cast<const void*>(&select::pick_kernel<D>), select::list_bytes(select::kMaxSel), dev, bit);
   if (rc != NSA_OK) return rc;
   const int64_t units = (a.blocks + a.unit - 1) / a.unit;  // of a row and KV head
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(select::kMaxRows, kMaxIndex / (units * a.hkv)));
   for (int64_t row0 = 0; row0 < n_rows; row0 += most) {
     a.row0 = (int32_t)row0;
     a.rows = (int32_t)std::min(most, n_rows - row0);
-    const int64_t grid = std::min<int64_t>(2 * sm, (units * a.hkv * a.rows + select::kWarps - 1) / select::kWarps);
-    cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::kWarps * 32, fixed + (a.rows + 1) * 4, 1, st, a);
+    const int64_t grid = std::min<int64_t>(select::blocks_per_sm(D) * sm, units * a.hkv * a.rows);
+    cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::kWarps * 32, (a.rows + 1) * 4, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection's score launch");
-    e = launch(&select::pick_kernel, dim3((unsigned)(a.rows * a.hkv)), select::kPickThreads, 0, 1, st, a);
+    e = launch(&select::pick_kernel<D>, dim3((unsigned)(a.rows * a.hkv)), select::kPickThreads, list, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection launch");
   }
   return done(cudaSuccess, "");
@@ -158,7 +158,7 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.q_head = d->q_head_stride ? d->q_head_stride : b.d_qk;
   a.cache = static_cast<const uint8_t*>(b.cache);
   a.page_stride = cache::page_stride_of(&b);
-  a.score = static_cast<uint64_t*>(d->workspace);
+  a.bounds = static_cast<float2*>(d->workspace);
   a.sel = d->sel;
   a.hkv = b.heads_kv, a.group = d->heads_q / b.heads_kv, a.n_sel = d->n_sel;
   a.shift = shift_of(d->block_size);
@@ -212,7 +212,7 @@ int check_rotary(const nsa_rotary_desc* d) {
 
 template <class T, int VEC>
 cudaError_t launch_rotary(const rotary::Args& a, dim3 grid, cudaStream_t st) {
-  return launch(&rotary::kernel<T, VEC>, grid, rotary::kThreads, a.per_block * a.pairs * 8, 1, st, a);
+  return launch(&rotary::kernel<T, VEC>, grid, rotary::kThreads, 0, 1, st, a);
 }
 
 int run_rotary(const nsa_rotary_desc* d, cudaStream_t st) {
@@ -249,16 +249,12 @@ int run_rotary(const nsa_rotary_desc* d, cudaStream_t st) {
   a.flip = d->inverse ? 0x80000000u : 0u;
   memcpy(a.turn, d->turns, sizeof(uint64_t) * d->pairs);
   if (d->axis != nullptr) memcpy(a.axis, d->axis, d->pairs);
-  // Tokens of a block: as many as leave every SM several blocks; where even single tokens are few, their heads are shared out.
-  a.per_block = 1;
-  while (a.per_block < rotary::kMaxTokens && total >= (int64_t)a.per_block * 2 * 16 * sm) a.per_block *= 2;
+  // A block has a token; where tokens are few, its heads are shared out among blocks.
   const int items = a.pairs / vec + (a.rest + 2 * vec - 1) / (2 * vec);
-  int64_t parts = 1;
-  if (a.per_block == 1)
-    parts = std::min<int64_t>(std::max<int64_t>(1, 2 * sm / total), ((int64_t)a.heads * items + rotary::kThreads - 1) / rotary::kThreads);
+  const int64_t most = ((int64_t)a.heads * items + rotary::kThreads - 1) / rotary::kThreads;
+  const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * sm / total), most);
   a.heads_block = (int32_t)((a.heads + parts - 1) / parts);
-  const dim3 grid((unsigned)(((int64_t)d->tokens + a.per_block - 1) / a.per_block * d->batch),
-                  (unsigned)((a.heads + a.heads_block - 1) / a.heads_block));
+  const dim3 grid((unsigned)total, (unsigned)((a.heads + a.heads_block - 1) / a.heads_block));
   cudaError_t e;
   if (d->dtype == NSA_DTYPE_F32) {
     e = vec == 4   ? launch_rotary<float, 4>(a, grid, st)
