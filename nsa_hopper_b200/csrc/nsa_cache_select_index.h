@@ -60,10 +60,13 @@ NSA_LINSPACE int32_t block_of(const Places& p, int32_t i) { return (int32_t)plac
 NSA_LINSPACE int32_t first_key(const Places& p, int32_t block) {
   if (block <= 0) return 0;
   if (p.n <= 1) return p.n;
-  const float guess = (float)((int64_t)block << p.shift) * p.per;
+  const float guess = ceilf((float)((int64_t)block << p.shift) * p.per);
   int32_t i = guess < (float)p.n ? (int32_t)guess : p.n;
-  while (i > 0 && block_of(p, i - 1) >= block) --i;
-  while (i < p.n && block_of(p, i) < block) ++i;
+  const bool down = i > 0 && block_of(p, i - 1) >= block, up = i < p.n && block_of(p, i) < block;
+  if (down || up) {  // (the guess is off by a key where a block begins at one, about)
+    while (i > 0 && block_of(p, i - 1) >= block) --i;
+    while (i < p.n && block_of(p, i) < block) ++i;
+  }
   return i;
 }
 

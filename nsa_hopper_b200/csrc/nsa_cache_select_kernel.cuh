@@ -87,10 +87,11 @@ struct Quarter {
   uint32_t code[D / 32];  // eight codes each
   uint32_t scale;         // D / 64 bytes
 };
+// Place t of a record; its codes and its scales are counted from `codes` and `scales`, the record or as much before it.
 template <int D>
-__device__ __forceinline__ void load_quarter(Quarter<D>& k, const uint8_t* rec, int t, int q) {
-  const uint8_t* code = rec + t * (D / 2) + q * (D / 8);
-  const uint8_t* scale = rec + cache::k_scale_at(D) + t * (D / 16) + q * (D / 64);
+__device__ __forceinline__ void load_quarter(Quarter<D>& k, const uint8_t* codes, const uint8_t* scales, int t, int q) {
+  const uint8_t* code = codes + t * (D / 2) + q * (D / 8);
+  const uint8_t* scale = scales + cache::k_scale_at(D) + t * (D / 16) + q * (D / 64);
   if constexpr (D == 128) {
     const uint4 v = *reinterpret_cast<const uint4*>(code);
     k.code[0] = v.x, k.code[1] = v.y, k.code[2] = v.z, k.code[3] = v.w;
@@ -114,15 +115,23 @@ __device__ __forceinline__ float load_query(const Args& a, uint32_t (&bq)[D / 8]
   constexpr int N = D / 32;  // dims of a lane at first
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.group * a.q_head + lane * N;
   float sum[N] = {}, size = 0.0f;
-#pragma unroll 4
-  for (int g = 0; g < a.group; ++g)
+#pragma unroll 8
+  for (int g = 0; g < a.group; ++g) {
+    uint32_t two[N / 2];
+    if constexpr (N == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(q + g * a.q_head);
+      two[0] = v.x, two[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) two[i] = reinterpret_cast<const uint32_t*>(q + g * a.q_head)[i];
+    }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const uint32_t two = reinterpret_cast<const uint32_t*>(q + g * a.q_head)[i];
-      const float x = query_value(a, two & 0xFFFFu), y = query_value(a, two >> 16);
+      const float x = query_value(a, two[i] & 0xFFFFu), y = query_value(a, two[i] >> 16);
       sum[2 * i] += x, sum[2 * i + 1] += y;
       size += fabsf(x) + fabsf(y);
     }
+  }
   size *= (float)(a.group - 1) * 5.9604645e-08f;  // 2^-24
   uint32_t top = 0;
 #pragma unroll
@@ -230,23 +239,29 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(co
       const int32_t mine_end = __shfl_down_sync(0xFFFFFFFFu, mine_first, 1);
       const int32_t begin = __shfl_sync(0xFFFFFFFFu, mine_first, 0), end = __shfl_sync(0xFFFFFFFFu, mine_first, blocks);
       float score = 0.0f;
-      uint32_t top = 0;
+      uint32_t even = 0, odd = 0;
       for (int32_t base = begin; base < end; base += kUnitKeys) {
         // keys base + 8 j + g (tile j / 2, row g or g + 8), of the page of `base` or the next one
         const int page0 = cache::page_of(a.b, seq, base / kPage), page1 = cache::page_of(a.b, seq, base / kPage + 1);
         const uint8_t* rec0 = a.cache + (int64_t)page0 * a.page_stride + (int64_t)head * a.record;
         const uint8_t* rec1 = a.cache + (int64_t)page1 * a.page_stride + (int64_t)head * a.record;
-        const int t = base % kPage + g, last = page0 >= 0 ? end - base : 0, turn = kPage - t;
+        const int t = base % kPage + g, left = end - base - g;
+        const int here = page0 >= 0 ? left : 0, there = page1 >= 0 ? left : 0;
         Quarter<D> k[8];
+        if (end - base >= kUnitKeys && page0 >= 0 && page1 >= 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool next = 8 * j >= turn;
-          if (8 * j + g < (next && page1 < 0 ? 0 : next ? end - base : last)) {
-            load_quarter<D>(k[j], next ? rec1 : rec0, t + 8 * j - (next ? kPage : 0), quarter);
-          } else {
+          for (int j = 0; j < 8; ++j)
+            load_quarter<D>(k[j], t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 2), t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 16),
+                            t + 8 * j, quarter);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) k[j].code[c] = 0;
             k[j].scale = 0;
+            if (8 * j < (t + 8 * j < kPage ? here : there))
+              load_quarter<D>(k[j], t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 2),
+                              t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 16), t + 8 * j, quarter);
           }
         }
 #pragma unroll
@@ -268,9 +283,13 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(co
               const uint32_t s = k[2 * tile + h].scale;
               const float scale = group == 0 ? scale_value<0>(s) : group == 1 ? scale_value<1>(s) : scale_value<2>(s);
               sum[h] = fmaf(scale, c[2 * h] + c[2 * h + 1], sum[h]);
-              top = max(top, s >> 8 * group & 255u);
             }
           }
+          // the largest scales: lower bytes of halves, and upper ones (whatever is below them)
+          const uint32_t two = __byte_perm(k[2 * tile].scale, k[2 * tile + 1].scale, 0x5410);
+          even = __vmaxu2(even, two & 0x00FF00FFu);
+          if (D > 64) odd = __vmaxu2(odd, two);
+          if (D > 128) even = __vmaxu2(even, __byte_perm(k[2 * tile].scale, k[2 * tile + 1].scale, 0x7632));
           keys[warp][(16 * tile + g) * 4 + quarter] = sum[0];
           keys[warp][(16 * tile + 8 + g) * 4 + quarter] = sum[1];
         }
@@ -282,7 +301,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(co
           }
         __syncwarp();
       }
-      top = __reduce_max_sync(0xFFFFFFFFu, top);
+      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(even & 0xFFFFu, even >> 16), max(odd >> 8 & 0xFFu, odd >> 24)));
       if (lane < blocks) {
         const float error = size * (float)(mine_end - mine_first) * scale_value<0>(top);
         const float least = score - error, most = score + error;
@@ -399,15 +418,15 @@ __device__ __forceinline__ double dot(const Exact<D>& w, const Quarter<D>& k, in
 }
 
 // Scores of entries [from, to) of the list (blocks with the keys of `range`) by all threads: 16 of them for two blocks, four for
-// a key, up to 8 keys of either block on their way at once.
+// a key, up to 8 keys of either block on their way at once.  `part` is shared.
 template <int D>
 __device__ __forceinline__ void exact_scores(const Args& a, const Exact<D>& w, int limbs, int seq, int head, const int2* range,
-                                             uint64_t* rank, uint32_t from, uint32_t to) {
+                                             uint64_t* rank, uint32_t from, uint32_t to, double (&part)[kPickThreads / 16][2][8]) {
   constexpr uint32_t kHalves = kPickThreads / 16;
-  const int lane = threadIdx.x % 32, quarter = lane % 4, key = lane / 4 % 4;
-  for (uint32_t e0 = from + threadIdx.x / 16; e0 - threadIdx.x / 16 < to; e0 += 2 * kHalves) {
+  const int lane = threadIdx.x % 32, quarter = lane % 4, key = lane / 4 % 4, half = threadIdx.x / 16;
+  for (uint32_t e0 = from + half; e0 - half < to; e0 += 2 * kHalves) {
     int2 r[2];
-    double score[2] = {0.0, 0.0};
+    double score = 0.0;  // of block e0 + x kHalves, in lane x of the 16
 #pragma unroll
     for (int x = 0; x < 2; ++x) r[x] = e0 + x * kHalves < to ? range[e0 + x * kHalves] : make_int2(0, 0);
     for (int32_t at = 0; __any_sync(0xFFFFFFFFu, at < r[0].y - r[0].x || at < r[1].y - r[1].x); at += 8) {
@@ -418,21 +437,23 @@ __device__ __forceinline__ void exact_scores(const Args& a, const Exact<D>& w, i
         const int32_t i = r[x / 2].x + at + x % 2 * 4 + key;
         const int page = i < r[x / 2].y ? cache::page_of(a.b, seq, i / kPage) : -1;
         there[x] = page >= 0;
-        if (there[x]) load_quarter<D>(k[x], a.cache + (int64_t)page * a.page_stride + (int64_t)head * a.record, i % kPage, quarter);
+        const uint8_t* rec = a.cache + (int64_t)page * a.page_stride + (int64_t)head * a.record;
+        if (there[x]) load_quarter<D>(k[x], rec, rec, i % kPage, quarter);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        if (!__any_sync(0xFFFFFFFFu, there[x])) continue;
-        const double y = limbs == 4 ? dot<D, 4>(w, k[x], quarter) : dot<D, 6>(w, k[x], quarter);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          score[x / 2] += __shfl_sync(0xFFFFFFFFu, y, lane / 16 * 16 + 4 * j);  // (absent keys are zeros)
+        double y = 0.0;  // (also of keys that are not there)
+        if (__any_sync(0xFFFFFFFFu, there[x])) y = limbs == 4 ? dot<D, 4>(w, k[x], quarter) : dot<D, 6>(w, k[x], quarter);
+        if (quarter == 0) part[half][x / 2][x % 2 * 4 + key] = y;
       }
-    }
+      __syncwarp();
+      if (lane % 16 < 2)
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (lane % 16 == 0 && e0 + x * kHalves < to)
-        rank[e0 + x * kHalves] = rank_of(limbs == 0 ? __longlong_as_double(0x7FF8000000000000ll) : score[x]);
+        for (int j = 0; j < 8; ++j) score += part[half][lane % 16][j];  // (in the order of the keys)
+      __syncwarp();
+    }
+    const uint32_t e = e0 + lane % 16 * kHalves;
+    if (lane % 16 < 2 && e < to) rank[e] = rank_of(limbs == 0 ? __longlong_as_double(0x7FF8000000000000ll) : score);
   }
 }
 
@@ -460,6 +481,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Args a) {
   __shared__ float2 held[kHeldBounds];
   __shared__ __align__(16) uint32_t count[kBins];
   __shared__ uint32_t sums[kPickThreads / 32];
+  __shared__ double part[kPickThreads / 16][2][8];
   __shared__ uint32_t s_least, s_most, s_bin, s_total, s_n;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int size = list_size(a.n_sel);
@@ -535,22 +557,24 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Args a) {
   uint32_t scored = 0;
   const auto keep_best = [&](bool last) {
     const uint32_t in = s_n;
-    for (uint32_t e = scored + tid; e < in; e += kPickThreads) {
-      const int32_t block = (int32_t)list.index[e];
-      range[e] = make_int2(first_key(p, block), first_key(p, block + 1));
-    }
+    for (uint32_t x = 2 * scored + tid; x < 2 * in; x += kPickThreads)
+      (x % 2 == 0 ? range[x / 2].x : range[x / 2].y) = first_key(p, (int32_t)(list.index[x / 2] + x % 2));
     __syncthreads();
-    exact_scores<D>(a, w, limbs, seq, head, range, list.rank, scored, in);
+    exact_scores<D>(a, w, limbs, seq, head, range, list.rank, scored, in, part);
     __syncthreads();
-    for (uint32_t e = tid; e < in; e += kPickThreads) {
+    for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += kPickThreads / 8) {  // 8 threads for an entry
+      const uint32_t e = min(e0, in - 1);
       const uint64_t key = list.rank[e];
       const uint32_t block = list.index[e];
       uint32_t better = 0;
-      for (uint32_t j = 0; j < in; ++j) better += list.rank[j] > key || (list.rank[j] == key && list.index[j] < block);
-      if (better >= wanted) continue;
+      for (uint32_t j = tid % 8; j < in; j += 8) better += list.rank[j] > key || (list.rank[j] == key && list.index[j] < block);
+#pragma unroll
+      for (int by = 4; by > 0; by /= 2) better += __shfl_xor_sync(0xFFFFFFFFu, better, by);
+      if (tid % 8 != 0 || e0 >= in || better >= wanted) continue;
       if (last) sel[better] = (int32_t)block;
       else other.rank[better] = key, other.index[better] = block;
     }
+    if (last) return;
     scored = min(in, wanted);
     const List swap = list;
     list = other, other = swap;
@@ -563,26 +587,26 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < kChecked; ++j) {
       const int i = i0 + j * kPickThreads + tid;
-      mask |= (i < n && bin_of(of[i].y, low, per) >= edge ? 1u : 0u) << j;
+      if (i < n && bin_of(of[i].y, low, per) >= edge) mask |= 1u << j;
     }
-    const uint32_t found = __reduce_add_sync(0xFFFFFFFFu, __popc(mask));
-    if (lane == 0 && found != 0) atomicAdd(&s_total, found);
+    if (mask != 0) atomicAdd(&s_total, __popc(mask));
     __syncthreads();
     const bool room = s_n + s_total <= (uint32_t)size;
     __syncthreads();
     if (tid == 0) s_total = 0;
-    for (int j = 0; j < kChecked; ++j) {
-      const bool in = mask >> j & 1;
-      const uint32_t votes = __ballot_sync(0xFFFFFFFFu, in);
-      uint32_t at = 0;
-      if (lane == 0 && votes != 0) at = atomicAdd(&s_n, __popc(votes));
-      at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(votes & ((1u << lane) - 1));
-      if (in) list.index[at] = (uint32_t)(i0 + j * kPickThreads + tid);
-      if (room) continue;
-      __syncthreads();
-      const bool full = s_n + kPickThreads > (uint32_t)size;
-      __syncthreads();
-      if (full) keep_best(false);
+    if (room) {
+      if (mask != 0) {
+        uint32_t at = atomicAdd(&s_n, __popc(mask));
+        for (; mask != 0; mask &= mask - 1) list.index[at++] = (uint32_t)(i0 + (__ffs(mask) - 1) * kPickThreads + tid);
+      }
+    } else {
+      for (int j = 0; j < kChecked; ++j) {
+        if (mask >> j & 1) list.index[atomicAdd(&s_n, 1u)] = (uint32_t)(i0 + j * kPickThreads + tid);
+        __syncthreads();
+        const bool full = s_n + kPickThreads > (uint32_t)size;
+        __syncthreads();
+        if (full) keep_best(false);
+      }
     }
     __syncthreads();
   }
