@@ -416,7 +416,7 @@ int nsa_cache_reserve(const nsa_cache_reserve_desc* desc, nsa_stream_t stream);
    by sums in 64 bits; the lower block comes first where two are equal, and scores that are not finite come last.  Keys that the
    page table does not hold count as zeros.  A row of no token, and one of more than 2^24 tokens or of more than
    64 * width * cmp_stride + cmp_block - 1 (whose keys the table cannot hold), selects nothing: -1 throughout.
-   n_sel is at most 1024, heads_q / heads_kv at most 256.  Zero-initialise, then fill.  Two launches for each 8192 rows. */
+   n_sel is at most 1024, heads_q / heads_kv at most 256.  Zero-initialise, then fill.  Two launches for each 1024 rows. */
 typedef struct nsa_cache_select_desc {
   nsa_cache_batch batch;
   const void* q;              /* [n_rows, heads_q, d_qk], dtype q_dtype, d has unit stride, 16-byte aligned */

@@ -23,9 +23,8 @@ NSA_HD int32_t most_tokens(int32_t width, int32_t block, int32_t stride) {
   const int64_t t = (int64_t)width * kPage * stride + block - 1;
   return t < kMaxTokens ? (int32_t)t : kMaxTokens;
 }
-// Tokens that a row sees, 0 where it selects nothing (no such token, or more of them than the table or float32 can place).
-NSA_HD int32_t tokens_of(const Batch& b, int row, int32_t most) {
-  const int seq = cache::sequence_of(b, row);
+// Tokens that a row of sequence `seq` (from sequence_of) sees, 0 where it selects nothing (no such token, or more of them than the table or float32 can place).
+NSA_HD int32_t tokens_of(const Batch& b, int seq, int row, int32_t most) {
   const int pos = seq < 0 ? -1 : cache::position_of(b, seq, row);
   return pos >= 0 && pos < most ? pos + 1 : 0;
 }

@@ -29,24 +29,27 @@
 #include "nsa_cache_decode.cuh"
 #include "nsa_cache_select_index.h"
 #include "nsa_programmatic.cuh"
+#include "ptx.cuh"
 
 namespace nsa {
 namespace cache_select {
 
-constexpr int kWarps = 8;
-// Blocks of an SM: the codes of 64 keys in registers leave room for 24 warps, with d = 192 for 16.
-__host__ __device__ constexpr int blocks_per_sm(int d) { return d <= 128 ? 3 : 2; }
+constexpr int kStages = 2;        // units of a warp in shared memory: one that is scored and one that is on its way
+// Warps of score_kernel, one block of which fills an SM: shared memory holds 14 times two units of d = 192.  (20 warps with
+// d = 128 are 2 % faster for long calls and 12 % slower for short ones.)
+__host__ __device__ constexpr int warps_of(int d) { return d <= 128 ? 16 : 14; }
 constexpr int kLimbs = 6;
-constexpr int kMaxRows = 8192;    // of a launch: their units' places fill 32 KB of shared memory
+constexpr int kMaxRows = 1024;    // of a launch: what is kept of them fills 12 KB of shared memory
 constexpr int kUnitKeys = 64;     // keys of a unit, about
 constexpr int kUnitBlocks = 31;   // its blocks at most: a lane for each and one for the end
 constexpr int kMaxGroup = 256;    // query heads of a KV head
 constexpr int kMaxSel = 1024;
 constexpr int kPickThreads = 256;
-constexpr int kCandidates = 512;  // blocks whose exact scores are kept beside the n_sel best
-constexpr int kHeldBounds = 2048; // bounds that pick_kernel keeps in shared memory
 constexpr int kBins = 4 * kPickThreads;
-constexpr int kChecked = 8;       // blocks that a thread looks at between two meetings
+constexpr int kChecked = 2048;    // blocks that pick_kernel looks at between two meetings, and whose bounds it can hold
+constexpr int kAdded = 512;       // of them, those whose exact scores are compared with the best so far
+constexpr int kKeys = 512;        // places of keys that are scored between two meetings
+constexpr int kHeldPages = 256;   // first pages of a sequence, looked up beforehand
 constexpr float kHuge = 3.0e38f;  // bound of what has none
 
 struct Args {
@@ -66,6 +69,8 @@ struct Args {
   int32_t record;       // bytes
   int32_t q_half;
   int32_t bits;         // of a query head's value in the exact sum: its largest is below 2^bits
+  int32_t keys;         // of a block, at most
+  int32_t at_once;      // blocks that have kKeys places
   int32_t row0, rows;   // rows of this launch
 };
 
@@ -87,11 +92,11 @@ struct Quarter {
   uint32_t code[D / 32];  // eight codes each
   uint32_t scale;         // D / 64 bytes
 };
-// Place t of a record; its codes and its scales are counted from `codes` and `scales`, the record or as much before it.
+// Of key t, counted from the quarters of another one.
 template <int D>
-__device__ __forceinline__ void load_quarter(Quarter<D>& k, const uint8_t* codes, const uint8_t* scales, int t, int q) {
-  const uint8_t* code = codes + t * (D / 2) + q * (D / 8);
-  const uint8_t* scale = scales + cache::k_scale_at(D) + t * (D / 16) + q * (D / 64);
+__device__ __forceinline__ void load_quarter(Quarter<D>& k, const uint8_t* codes, const uint8_t* scales, int t) {
+  const uint8_t* code = codes + t * (D / 2);
+  const uint8_t* scale = scales + t * (D / 16);
   if constexpr (D == 128) {
     const uint4 v = *reinterpret_cast<const uint4*>(code);
     k.code[0] = v.x, k.code[1] = v.y, k.code[2] = v.z, k.code[3] = v.w;
@@ -166,19 +171,67 @@ __device__ __forceinline__ float load_query(const Args& a, uint32_t (&bq)[D / 8]
   return top >> 23 < 11u && size > 0.0f ? __uint_as_float(0x7F800000u) : 6.0f * size * factor;
 }
 
-// fp32 of scale byte I of `s` (a finite one of those that are no numbers: the caller looks for those).
+// fp32 of scale bytes 2 I and 2 I + 1 of `s`.
 template <int I>
-__device__ __forceinline__ float scale_value(uint32_t s) {
-  return __uint_as_float(s << (20 - 8 * I) & 0x0FF00000u) * 5.192296858534828e33f;  // 2^112
+__device__ __forceinline__ float2 scale_values(uint32_t s) {
+  const uint32_t two = __byte_perm(s, 0, I == 0 ? 0x4140 : 0x4342) * 128;  // (byte << 7 is the fp16)
+  return __half22float2(*reinterpret_cast<const __half2*>(&two));
+}
+
+// Keys of a unit as they are in the cache: codes [64][D / 2], scales [64][D / 16].
+template <int D>
+struct Stage {
+  static constexpr int kScaleAt = kUnitKeys * D / 2, kBytes = kUnitKeys * D * 9 / 16;
+};
+template <int D>
+struct ScoreWarp {
+  uint8_t stage[kStages][Stage<D>::kBytes];
+  float part[kUnitKeys * 4];  // score of every quarter of a key
+};
+__device__ __forceinline__ void copy16(void* to, const void* from, bool there) {  // zeros if it is not there
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+// Starts the copies of keys base to base + 63 of a sequence, zeros for those from `end` on and those of no page.
+template <int D>
+__device__ __forceinline__ void fetch(const Args& a, uint8_t* stage, int seq, int head, int32_t base, int32_t end, int lane) {
+  // (they are of the page of `base` and the next one)
+  const int page0 = cache::page_of(a.b, seq, base / kPage), page1 = cache::page_of(a.b, seq, base / kPage + 1);
+  const uint8_t* rec = a.cache + (int64_t)head * a.record;
+  const int t0 = base % kPage, left = end - base;
+  const int here = page0 >= 0 ? left : 0, there = page1 >= 0 ? left : 0, turn = kPage - t0;
+  // (where there is no page, an address that is never read)
+  const uint8_t* rec0 = rec + (int64_t)max(page0, 0) * a.page_stride;
+  const uint8_t* rec1 = rec + (int64_t)max(page1, 0) * a.page_stride;
+  const uint8_t *codes0 = rec0 + t0 * (D / 2), *codes1 = rec1 - turn * (D / 2);
+  const uint8_t *scales0 = rec0 + cache::k_scale_at(D) + t0 * (D / 16), *scales1 = rec1 + cache::k_scale_at(D) - turn * (D / 16);
+  codes0 += 16 * lane, codes1 += 16 * lane, scales0 += 4 * lane, scales1 += 4 * lane;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int key = (32 * i + lane) / (D / 32);
+    const bool first = key < turn;
+    copy16(stage + 16 * (32 * i + lane), (first ? codes0 : codes1) + 512 * i, key < (first ? here : there));
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const int key = (32 * i + lane) / (D / 64);
+    const bool first = key < turn;
+    copy4(stage + Stage<D>::kScaleAt + 4 * (32 * i + lane), (first ? scales0 : scales1) + 128 * i, key < (first ? here : there));
+  }
 }
 
 // Every unit of `unit` blocks of a row and KV head is a warp's work; the units of all rows stand in one line, head after head,
-// that is shared out evenly.
+// that is shared out evenly.  While a warp scores 64 keys in shared memory the next ones are on their way.
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(const Args a) {
-  extern __shared__ uint32_t line[];  // [rows + 1] units before every row
-  __shared__ __align__(16) float keys[kWarps][kUnitKeys * 4];  // score of every quarter of a key
+__global__ void __launch_bounds__(warps_of(D) * 32) score_kernel(const Args a) {
+  constexpr int kWarps = warps_of(D);
+  extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ uint32_t sums[kWarps];
+  ScoreWarp<D>* const all_warps = reinterpret_cast<ScoreWarp<D>*>(dynamic);
+  int2* const row_of = reinterpret_cast<int2*>(all_warps + kWarps);      // [rows] sequence and tokens
+  uint32_t* const line = reinterpret_cast<uint32_t*>(row_of + a.rows);  // [rows + 1] units before every row
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   // (pick_kernel is let go only after this wait, so that it may read what earlier kernels wrote without one of its own)
   wait_for_earlier();
@@ -186,8 +239,10 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(co
   const int each = (a.rows + kWarps * 32 - 1) / (kWarps * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
   uint32_t mine = 0;
   for (int r = r0; r < r1; ++r) {
+    const int seq = cache::sequence_of(a.b, a.row0 + r);
+    row_of[r] = make_int2(seq, tokens_of(a.b, seq, a.row0 + r, a.most));
     line[r] = mine;
-    mine += (uint32_t)(blocks_of(tokens_of(a.b, a.row0 + r, a.most), a.shift) + a.unit - 1) / (uint32_t)a.unit;
+    mine += (uint32_t)(blocks_of(row_of[r].y, a.shift) + a.unit - 1) / (uint32_t)a.unit;
   }
   uint32_t upto = mine;
 #pragma unroll
@@ -213,112 +268,137 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(D)) score_kernel(co
   const uint32_t share = all / workers, more = all % workers;
   uint32_t u = me * share + min(me, more);
   const uint32_t u1 = u + share + (me < more ? 1 : 0);
+  if (u >= u1) return;
+  ScoreWarp<D>& w = all_warps[warp];
   const int g = lane / 4, quarter = lane % 4;
-  while (u < u1) {
-    // the units of one (row, head)
-    const int head = (int)(u / total);
-    const uint32_t place = u - head * total;
-    int lo = 0, hi = a.rows;
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (line[mid] <= place) lo = mid;
-      else hi = mid;
-    }
-    const uint32_t stop = min(u1, u + (line[lo + 1] - place));
-    const int row = a.row0 + lo, seq = cache::sequence_of(a.b, row);
-    const Places p = places_of(tokens_of(a.b, row, a.most), a.cmp_block, a.cmp_stride, a.shift);
-    const int32_t n_blocks = blocks_of(p.tokens, a.shift);
-    float2* bounds = a.bounds + ((int64_t)row * a.hkv + head) * a.blocks;
-    uint32_t bq[D / 8];
-    const float size = load_query<D>(a, bq, row, head, lane);  // error
-    int32_t first = (int32_t)(place - line[lo]) * a.unit;
-    for (; u < stop; ++u, first += a.unit) {
-      const int32_t blocks = min(a.unit, n_blocks - first);
-      // lane j: the first key of block j of the unit
-      const int32_t mine_first = first_key(p, first + min(lane, blocks));
-      const int32_t mine_end = __shfl_down_sync(0xFFFFFFFFu, mine_first, 1);
-      const int32_t begin = __shfl_sync(0xFFFFFFFFu, mine_first, 0), end = __shfl_sync(0xFFFFFFFFu, mine_first, blocks);
-      float score = 0.0f;
-      uint32_t even = 0, odd = 0;
-      for (int32_t base = begin; base < end; base += kUnitKeys) {
-        // keys base + 8 j + g (tile j / 2, row g or g + 8), of the page of `base` or the next one
-        const int page0 = cache::page_of(a.b, seq, base / kPage), page1 = cache::page_of(a.b, seq, base / kPage + 1);
-        const uint8_t* rec0 = a.cache + (int64_t)page0 * a.page_stride + (int64_t)head * a.record;
-        const uint8_t* rec1 = a.cache + (int64_t)page1 * a.page_stride + (int64_t)head * a.record;
-        const int t = base % kPage + g, left = end - base - g;
-        const int here = page0 >= 0 ? left : 0, there = page1 >= 0 ? left : 0;
-        Quarter<D> k[8];
-        if (end - base >= kUnitKeys && page0 >= 0 && page1 >= 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            load_quarter<D>(k[j], t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 2), t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 16),
-                            t + 8 * j, quarter);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) k[j].code[c] = 0;
-            k[j].scale = 0;
-            if (8 * j < (t + 8 * j < kPage ? here : there))
-              load_quarter<D>(k[j], t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 2),
-                              t + 8 * j < kPage ? rec0 : rec1 - kPage * (D / 16), t + 8 * j, quarter);
-          }
-        }
-#pragma unroll
-        for (int tile = 0; tile < 4; ++tile) {
-          float sum[2] = {};
-#pragma unroll
-          for (int group = 0; group < D / 64; ++group) {
-            float c[4] = {};
-#pragma unroll
-            for (int w = 2 * group; w < 2 * group + 2; ++w) {  // eight codes of both keys: two steps of the tensor core
-              const uint32_t u = k[2 * tile].code[w], v = k[2 * tile + 1].code[w];
-              cache::mma(c, cache::decode_byte<0>(u), cache::decode_byte<0>(v), cache::decode_byte<1>(u), cache::decode_byte<1>(v),
-                         bq[4 * w], bq[4 * w + 1]);
-              cache::mma(c, cache::decode_byte<2>(u), cache::decode_byte<2>(v), cache::decode_byte<3>(u), cache::decode_byte<3>(v),
-                         bq[4 * w + 2], bq[4 * w + 3]);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t s = k[2 * tile + h].scale;
-              const float scale = group == 0 ? scale_value<0>(s) : group == 1 ? scale_value<1>(s) : scale_value<2>(s);
-              sum[h] = fmaf(scale, c[2 * h] + c[2 * h + 1], sum[h]);
-            }
-          }
-          // the largest scales: lower bytes of halves, and upper ones (whatever is below them)
-          const uint32_t two = __byte_perm(k[2 * tile].scale, k[2 * tile + 1].scale, 0x5410);
-          even = __vmaxu2(even, two & 0x00FF00FFu);
-          if (D > 64) odd = __vmaxu2(odd, two);
-          if (D > 128) even = __vmaxu2(even, __byte_perm(k[2 * tile].scale, k[2 * tile + 1].scale, 0x7632));
-          keys[warp][(16 * tile + g) * 4 + quarter] = sum[0];
-          keys[warp][(16 * tile + 8 + g) * 4 + quarter] = sum[1];
-        }
-        __syncwarp();
-        if (lane < blocks)
-          for (int32_t i = max(mine_first, base); i < min(mine_end, base + kUnitKeys); ++i) {
-            const float4 x = reinterpret_cast<const float4*>(keys[warp])[i - base];
-            score += (x.x + x.y) + (x.z + x.w);
-          }
-        __syncwarp();
+
+  // The unit whose keys are fetched: that of `u`, in the row whose units end with `stop`.
+  uint32_t stop = u;
+  int row = 0, head = 0, seq = 0;
+  int32_t first = 0, n_blocks = 0;
+  Places p;
+  struct Unit {
+    float2* bounds;       // of its first block
+    int32_t blocks;
+    int32_t first, end;   // keys of block `lane`
+    int32_t base, last;   // 64 keys from `base` on, of the unit's up to `last`
+    int row, head;
+  };
+  const auto begin = [&]() {
+    if (u == stop) {
+      head = (int)(u / total);
+      const uint32_t place = u - head * total;
+      int lo = 0, hi = a.rows;
+      while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        if (line[mid] <= place) lo = mid;
+        else hi = mid;
       }
+      stop = u + (line[lo + 1] - place);
+      row = a.row0 + lo, seq = row_of[lo].x;
+      p = places_of(row_of[lo].y, a.cmp_block, a.cmp_stride, a.shift);
+      n_blocks = blocks_of(p.tokens, a.shift);
+      first = (int32_t)(place - line[lo]) * a.unit;
+    }
+    Unit x;
+    x.bounds = a.bounds + ((int64_t)row * a.hkv + head) * a.blocks + first;
+    x.blocks = min(a.unit, n_blocks - first);
+    x.first = first_key(p, first + min(lane, x.blocks));
+    x.end = __shfl_down_sync(0xFFFFFFFFu, x.first, 1);
+    x.base = __shfl_sync(0xFFFFFFFFu, x.first, 0), x.last = __shfl_sync(0xFFFFFFFFu, x.first, x.blocks);
+    x.row = row, x.head = head;
+    ++u, first += a.unit;
+    return x;
+  };
+
+  Unit now = begin();
+  fetch<D>(a, w.stage[0], seq, head, now.base, now.last, lane);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  uint32_t bq[D / 8];
+  int of_row = -1, of_head = -1, stage = 0;
+  float size = 0.0f, score = 0.0f;  // error of a key's score in units of a scale; score of block `lane`
+  uint32_t even = 0, odd = 0;
+  while (true) {
+    const bool whole = now.base + kUnitKeys >= now.last, more = !whole || u < u1;
+    Unit next = now;
+    if (whole && more) next = begin();
+    else next.base += kUnitKeys;
+    if (more) fetch<D>(a, w.stage[stage ^ 1], seq, head, next.base, next.last, lane);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (now.row != of_row || now.head != of_head) {
+      size = load_query<D>(a, bq, now.row, now.head, lane);
+      of_row = now.row, of_head = now.head;
+    }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint8_t* codes = w.stage[stage] + quarter * (D / 8);
+    const uint8_t* scales = w.stage[stage] + Stage<D>::kScaleAt + quarter * (D / 64);
+#pragma unroll
+    for (int tile = 0; tile < 4; ++tile) {  // keys 16 tile + g and 8 more
+      Quarter<D> k[2];
+      load_quarter<D>(k[0], codes, scales, 16 * tile + g);
+      load_quarter<D>(k[1], codes, scales, 16 * tile + 8 + g);
+      float sum[2] = {}, scale[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 x = scale_values<0>(k[h].scale), y = D > 128 ? scale_values<1>(k[h].scale) : make_float2(0.0f, 0.0f);
+        scale[h][0] = x.x, scale[h][1] = x.y, scale[h][2] = y.x, scale[h][3] = y.y;
+      }
+#pragma unroll
+      for (int group = 0; group < D / 64; ++group) {
+        float c[4] = {};
+#pragma unroll
+        for (int i = 2 * group; i < 2 * group + 2; ++i) {  // eight codes of both keys: two steps of the tensor core
+          const uint32_t x = k[0].code[i], y = k[1].code[i];
+          cache::mma(c, cache::decode_byte<0>(x), cache::decode_byte<0>(y), cache::decode_byte<1>(x), cache::decode_byte<1>(y),
+                     bq[4 * i], bq[4 * i + 1]);
+          cache::mma(c, cache::decode_byte<2>(x), cache::decode_byte<2>(y), cache::decode_byte<3>(x), cache::decode_byte<3>(y),
+                     bq[4 * i + 2], bq[4 * i + 3]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          sum[h] = fmaf(scale[h][group], c[2 * h] + c[2 * h + 1], sum[h]);
+        }
+      }
+      // the largest scales: lower bytes of halves, and upper ones (whatever is below them)
+      const uint32_t two = __byte_perm(k[0].scale, k[1].scale, 0x5410);
+      even = __vmaxu2(even, two & 0x00FF00FFu);
+      if (D > 64) odd = __vmaxu2(odd, two);
+      if (D > 128) even = __vmaxu2(even, __byte_perm(k[0].scale, k[1].scale, 0x7632));
+      w.part[(16 * tile + g) * 4 + quarter] = sum[0];
+      w.part[(16 * tile + 8 + g) * 4 + quarter] = sum[1];
+    }
+    __syncwarp();
+    if (lane < now.blocks)
+      for (int32_t i = max(now.first, now.base); i < min(now.end, now.base + kUnitKeys); ++i) {
+        const float4 x = reinterpret_cast<const float4*>(w.part)[i - now.base];
+        score += (x.x + x.y) + (x.z + x.w);
+      }
+    if (whole) {
       const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(even & 0xFFFFu, even >> 16), max(odd >> 8 & 0xFFu, odd >> 24)));
-      if (lane < blocks) {
-        const float error = size * (float)(mine_end - mine_first) * scale_value<0>(top);
+      if (lane < now.blocks) {
+        const float error = size * (float)(now.end - now.first) * scale_values<0>(top).x;
         const float least = score - error, most = score + error;
         // (what may not be finite has to be looked at)
         const bool fine = top < 0xF8u && fabsf(least) < kHuge && fabsf(most) < kHuge;
-        bounds[first + lane] = fine ? make_float2(least, most) : make_float2(-kHuge, kHuge);
+        now.bounds[lane] = fine ? make_float2(least, most) : make_float2(-kHuge, kHuge);
       }
+      score = 0.0f, even = odd = 0;
     }
+    if (!more) break;
+    __syncwarp();
+    now = next, stage ^= 1;
   }
 }
 
 // ------------------------------------------------------------------ exact scores
 template <int D>
 struct Exact {
-  int4 limb[D / 16][kLimbs];   // bytes of the query, the lowest first, of the 16 dims of a group, four to a word
-  int32_t start[D / 16][8];    // what the sums of a group begin with: 12 of every code too many, taken off
-  uint32_t top, low;
+  int4 limb[D / 16][kLimbs + 1];  // bytes of the query, the lowest first, of the 16 dims of a group, four to a word (and room
+                                  // that puts what the threads of a key read at once into different banks)
+  int2 start[D / 16];             // what the sums of a group begin with: 12 of every code too many, taken off
+  int32_t sum[2][D];              // of the heads: whole parts and fractions
+  uint32_t top;
 };
 
 // fp64 of an integer, without a conversion: its bits in the mantissa of 2^52 + 2^31 + x.
@@ -341,178 +421,198 @@ __device__ __forceinline__ int decode4(uint32_t codes) {
 
 // The sum of a (row, head)'s query heads as whole numbers of a power of two, so that the largest stays below 2^46, cut into six
 // signed bytes: values down to 2^-33 of the largest are exact in bf16 (2^-30 in fp16) with 16 heads, smaller ones off by less
-// than 2^-40 of it.  The lower two bytes are mostly zero in every place.  By all threads; false if a value is not finite.
+// than 2^-40 of it.  By all threads: kParts of them share the heads of two dims.  False if a value is not finite.
 template <int D>
 __device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, int row, int head) {
-  const int d = threadIdx.x;
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.group * a.q_head + d;
+  constexpr int kParts = kPickThreads / (D / 2);
+  const int tid = threadIdx.x, pair = tid % (D / 2), part = tid / (D / 2);
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.group * a.q_head + 2 * pair;
+  const int heads = part < kParts ? a.group : 0;
   uint32_t top = 0;
-  if (d < D) {
-#pragma unroll 8
-    for (int g = 0; g < a.group; ++g) top = max(top, (uint32_t)q[g * a.q_head] & 0x7FFFu);
-  }
-  if (d == 0) w.top = w.low = 0;
+#pragma unroll 4
+  for (int g = part; g < heads; g += kParts) top = __vmaxu2(top, *reinterpret_cast<const uint32_t*>(q + g * a.q_head) & 0x7FFF7FFFu);
+  if (tid == 0) w.top = 0;
+  for (int i = tid; i < 2 * D; i += kPickThreads) w.sum[0][i] = 0;
   __syncthreads();
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if (d % 32 == 0) atomicMax(&w.top, top);
+  top = __reduce_max_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16));
+  if (tid % 32 == 0) atomicMax(&w.top, top);
   __syncthreads();
   top = w.top;
   if (top >= (a.q_half ? 0x7C00u : 0x7F80u)) return false;
   // x 2^up: below 2^(bits - 22), its fraction to 22 bits
   const int up = a.bits - 22 + 126 - max((int)(__float_as_uint(query_value(a, top)) >> 23), 1);
   const float up0 = __uint_as_float((uint32_t)(127 + up / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
-  if (d < D) {
-    int32_t upper = 0, lower = 0;
+  int32_t upper[2] = {}, lower[2] = {};
 #pragma unroll 4
-    for (int g = 0; g < a.group; ++g) {
-      const float x = query_value(a, q[g * a.q_head]) * up0 * up1, whole_part = rintf(x);
-      upper += (int)whole_part;
-      lower += __float2int_rn((x - whole_part) * 4194304.0f);
+  for (int g = part; g < heads; g += kParts) {
+    const uint32_t two = *reinterpret_cast<const uint32_t*>(q + g * a.q_head);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = query_value(a, i == 0 ? two & 0xFFFFu : two >> 16) * up0 * up1, whole_part = rintf(x);
+      upper[i] += (int)whole_part;
+      lower[i] += __float2int_rn((x - whole_part) * 4194304.0f);
     }
-    int64_t x = (int64_t)upper * 4194304 + lower;
-    uint32_t low = 0;
+  }
+  if (part < kParts)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) atomicAdd(&w.sum[0][2 * pair + i], upper[i]), atomicAdd(&w.sum[1][2 * pair + i], lower[i]);
+  __syncthreads();
+  if (tid < D) {
+    int64_t x = (int64_t)w.sum[0][tid] * 4194304 + w.sum[1][tid];
 #pragma unroll
     for (int l = 0; l < kLimbs; ++l) {
       const int8_t byte = (int8_t)x;
       x = (x - byte) >> 8;
-      reinterpret_cast<int8_t*>(&w.limb[d / 16][l])[d % 16] = byte;
-      if (l < 2) low |= (uint8_t)byte;
+      reinterpret_cast<int8_t*>(&w.limb[tid / 16][l])[tid % 16] = byte;
     }
-    if (low != 0) w.low = 1;
   }
   __syncthreads();
-  if (d < D / 16 * kLimbs) {
-    const int4 v = w.limb[d / kLimbs][d % kLimbs];
+  if (tid < D / 16) {
     const int ones = 0x01010101;
-    w.start[d / kLimbs][d % kLimbs] = -12 * __dp4a(v.x, ones, __dp4a(v.y, ones, __dp4a(v.z, ones, __dp4a(v.w, ones, 0))));
+    int32_t start[kLimbs];
+#pragma unroll
+    for (int l = 0; l < kLimbs; ++l) {
+      const int4 v = w.limb[tid][l];
+      start[l] = -12 * __dp4a(v.x, ones, __dp4a(v.y, ones, __dp4a(v.z, ones, __dp4a(v.w, ones, 0))));
+    }
+    w.start[tid] = make_int2((start[2] * 256 + start[1]) * 256 + start[0], (start[5] * 256 + start[4]) * 256 + start[3]);
   }
   return true;  // (the caller meets before the sums are read)
 }
 
-// Score of a key, by four threads, each with a quarter of it; all of them get it.
-template <int D, int LIMBS>
-__device__ __forceinline__ double dot(const Exact<D>& w, const Quarter<D>& k, int quarter) {
-  constexpr int L0 = kLimbs - LIMBS, HALF = LIMBS / 2;
-  double upper = 0.0, lower = 0.0;
+// Scores of two keys, by four threads, each with a quarter of both; all of them get them.
+template <int D>
+__device__ __forceinline__ void dot(const Exact<D>& w, const Quarter<D> (&k)[2], int quarter, double (&x)[2]) {
+  double upper[2] = {0.0, 0.0}, lower[2] = {0.0, 0.0};
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
     const int g = quarter * (D / 64) + j;
-    const int c[4] = {decode4(k.code[2 * j]), decode4(k.code[2 * j] >> 16), decode4(k.code[2 * j + 1]),
-                      decode4(k.code[2 * j + 1] >> 16)};
+    int c[2][4];
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[y][i] = decode4(k[y].code[2 * j + i / 2] >> i % 2 * 16);
     // (a sum is at most 128 * 12 * 16 in size, so that three of them, a byte apart, fit 32 bits)
-    int up = 0, lo = 0;
+    uint32_t up[2] = {}, lo[2] = {};  // (those with 12 of every code too many may wrap around)
 #pragma unroll
-    for (int l = LIMBS - 1; l >= 0; --l) {
-      const int4 q = w.limb[g][L0 + l];
-      const int sum = __dp4a(c[0], q.x, __dp4a(c[1], q.y, __dp4a(c[2], q.z, __dp4a(c[3], q.w, w.start[g][L0 + l]))));
-      if (l >= HALF) up = up * 256 + sum;
-      else lo = lo * 256 + sum;
+    for (int l = kLimbs - 1; l >= 0; --l) {
+      const int4 q = w.limb[g][l];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        uint32_t& sum = l >= kLimbs / 2 ? up[y] : lo[y];
+        sum = (uint32_t)__dp4a(c[y][0], q.x, __dp4a(c[y][1], q.y, __dp4a(c[y][2], q.z, __dp4a(c[y][3], q.w, (int)(sum * 256)))));
+      }
     }
-    const double s = scale_of(k.scale >> 8 * j & 255u);
-    upper = fma(s, whole(up), upper);
-    lower = fma(s, whole(lo), lower);
+    const int2 start = w.start[g];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const double s = scale_of(k[y].scale >> 8 * j & 255u);
+      upper[y] = fma(s, whole((int)(up[y] + (uint32_t)start.y)), upper[y]);
+      lower[y] = fma(s, whole((int)(lo[y] + (uint32_t)start.x)), lower[y]);
+    }
   }
-  double x = fma(upper, (double)(1 << 8 * HALF), lower);
-  x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
-  return x + __shfl_xor_sync(0xFFFFFFFFu, x, 2);
-}
-
-// Scores of entries [from, to) of the list (blocks with the keys of `range`) by all threads: 16 of them for two blocks, four for
-// a key, up to 8 keys of either block on their way at once.  `part` is shared.
-template <int D>
-__device__ __forceinline__ void exact_scores(const Args& a, const Exact<D>& w, int limbs, int seq, int head, const int2* range,
-                                             uint64_t* rank, uint32_t from, uint32_t to, double (&part)[kPickThreads / 16][2][8]) {
-  constexpr uint32_t kHalves = kPickThreads / 16;
-  const int lane = threadIdx.x % 32, quarter = lane % 4, key = lane / 4 % 4, half = threadIdx.x / 16;
-  for (uint32_t e0 = from + half; e0 - half < to; e0 += 2 * kHalves) {
-    int2 r[2];
-    double score = 0.0;  // of block e0 + x kHalves, in lane x of the 16
 #pragma unroll
-    for (int x = 0; x < 2; ++x) r[x] = e0 + x * kHalves < to ? range[e0 + x * kHalves] : make_int2(0, 0);
-    for (int32_t at = 0; __any_sync(0xFFFFFFFFu, at < r[0].y - r[0].x || at < r[1].y - r[1].x); at += 8) {
-      Quarter<D> k[4] = {};
-      bool there[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int32_t i = r[x / 2].x + at + x % 2 * 4 + key;
-        const int page = i < r[x / 2].y ? cache::page_of(a.b, seq, i / kPage) : -1;
-        there[x] = page >= 0;
-        const uint8_t* rec = a.cache + (int64_t)page * a.page_stride + (int64_t)head * a.record;
-        if (there[x]) load_quarter<D>(k[x], rec, rec, i % kPage, quarter);
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        double y = 0.0;  // (also of keys that are not there)
-        if (__any_sync(0xFFFFFFFFu, there[x])) y = limbs == 4 ? dot<D, 4>(w, k[x], quarter) : dot<D, 6>(w, k[x], quarter);
-        if (quarter == 0) part[half][x / 2][x % 2 * 4 + key] = y;
-      }
-      __syncwarp();
-      if (lane % 16 < 2)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) score += part[half][lane % 16][j];  // (in the order of the keys)
-      __syncwarp();
-    }
-    const uint32_t e = e0 + lane % 16 * kHalves;
-    if (lane % 16 < 2 && e < to) rank[e] = rank_of(limbs == 0 ? __longlong_as_double(0x7FF8000000000000ll) : score);
+  for (int y = 0; y < 2; ++y) {
+    x[y] = fma(upper[y], 16777216.0, lower[y]);
+    x[y] += __shfl_xor_sync(0xFFFFFFFFu, x[y], 1);
+    x[y] += __shfl_xor_sync(0xFFFFFFFFu, x[y], 2);
   }
 }
 
-// ------------------------------------------------------------------ the best of a row
+// Adds `n` blocks with their scores to a list, by all threads.  Each block has a.keys places, four threads score the keys of two
+// places, and one sums those of a block, in their order.
 struct List {
   uint64_t* rank;
   uint32_t* index;
 };
-// The bin of a bound: never a lower one for a larger bound.
-__device__ __forceinline__ int bin_of(float x, float low, float per) { return max(0, min(kBins - 1, (int)((x - low) * per))); }
-__host__ __device__ constexpr int list_size(int n_sel) { return n_sel + kCandidates; }
-__host__ __device__ constexpr int list_bytes(int n_sel) { return 32 * list_size(n_sel); }  // two lists and the keys of one
+template <int D>
+__device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, bool fine, const Places& p, int seq, int head,
+                                             const int32_t* pages, const uint16_t* blocks, int base, uint32_t n, const List& list,
+                                             uint32_t at, double* scores) {
+  const int tid = threadIdx.x, quarter = tid % 4;
+  for (uint32_t e0 = 0; e0 < n; e0 += a.at_once) {
+    const uint32_t some = min(n - e0, (uint32_t)a.at_once), places = some * a.keys;
+    for (uint32_t t0 = tid / 4; t0 - tid / 4 < places; t0 += kPickThreads / 2) {
+      Quarter<D> k[2] = {};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t t = t0 + x * (kPickThreads / 4), e = t / (uint32_t)a.keys;
+        // (two threads find where the block begins, two where it ends)
+        const int32_t block = t < places ? base + blocks[e0 + e] : 0;
+        const int32_t bound = first_key(p, block + quarter % 2);
+        const int32_t i = __shfl_sync(0xFFFFFFFFu, bound, tid % 32 / 4 * 4) + (int32_t)(t - e * a.keys);
+        const bool in = i < __shfl_sync(0xFFFFFFFFu, bound, tid % 32 / 4 * 4 + 1) && t < places;
+        const int page = !in ? -1 : i / kPage < kHeldPages ? pages[i / kPage] : cache::page_of(a.b, seq, i / kPage);
+        const uint8_t* rec = a.cache + (int64_t)page * a.page_stride + (int64_t)head * a.record;
+        if (page >= 0)
+          load_quarter<D>(k[x], rec + quarter * (D / 8), rec + cache::k_scale_at(D) + quarter * (D / 64), i % kPage);
+      }
+      double score[2];  // (0 of a place without a key, and of a key of no page)
+      dot<D>(w, k, quarter, score);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (quarter == x && t0 + x * (kPickThreads / 4) < places) scores[t0 + x * (kPickThreads / 4)] = score[x];
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < some; e += kPickThreads) {
+      double score = 0.0;
+      for (int j = 0; j < a.keys; ++j) score += scores[e * a.keys + j];
+      list.rank[at + e0 + e] = rank_of(fine ? score : __longlong_as_double(0x7FF8000000000000ll));
+      list.index[at + e0 + e] = (uint32_t)(base + blocks[e0 + e]);
+    }
+    __syncthreads();
+  }
+}
 
+// ------------------------------------------------------------------ the best of a row
+__host__ __device__ constexpr int list_size(int n_sel) { return n_sel + kAdded; }
+__host__ __device__ constexpr int list_bytes(int n_sel) { return 24 * list_size(n_sel); }  // two lists
 // Numbers that compare like fp32, and back.
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
+// The bin of a bound: never a lower one for a larger bound.
+__device__ __forceinline__ int bin_of(float x, float low, float per) { return max(0, min(kBins - 1, (int)((x - low) * per))); }
 
 template <int D>
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const Args a) {
+__global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Exact<D> w;
-  __shared__ float2 held[kHeldBounds];
+  __shared__ double scores[kKeys];
+  __shared__ float2 held[kChecked];
+  __shared__ uint16_t found[kChecked];
+  __shared__ int32_t pages[kHeldPages];
   __shared__ __align__(16) uint32_t count[kBins];
   __shared__ uint32_t sums[kPickThreads / 32];
-  __shared__ double part[kPickThreads / 16][2][8];
-  __shared__ uint32_t s_least, s_most, s_bin, s_total, s_n;
+  __shared__ uint32_t s_least, s_most, s_bin, s_found;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int size = list_size(a.n_sel);
   List list = {reinterpret_cast<uint64_t*>(dynamic), reinterpret_cast<uint32_t*>(dynamic + 16 * size)};
   List other = {list.rank + size, list.index + size};
-  int2* range = reinterpret_cast<int2*>(dynamic + 24 * size);
   allow_next();
   // What earlier kernels wrote is read before score_kernel has ended (see there).
   const int64_t unit = blockIdx.x;
   const int row = a.row0 + (int)(unit / a.hkv), head = (int)(unit % a.hkv);
   const float2* bounds = a.bounds + ((int64_t)a.row0 * a.hkv + unit) * a.blocks;
   int32_t* sel = a.sel + ((int64_t)a.row0 * a.hkv + unit) * a.n_sel;
-  const int32_t tokens = tokens_of(a.b, row, a.most), n = blocks_of(tokens, a.shift);
+  reinterpret_cast<uint4*>(count)[tid] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s_least = 0xFFFFFFFFu, s_most = 0, s_found = 0;
+  const bool finite = prepare_exact<D>(a, w, row, head);
+  const int seq = cache::sequence_of(a.b, row);
+  const int32_t tokens = tokens_of(a.b, seq, row, a.most), n = blocks_of(tokens, a.shift);
   const uint32_t wanted = min((uint32_t)a.n_sel, (uint32_t)n);
   for (int i = (int)wanted + tid; i < a.n_sel; i += kPickThreads) sel[i] = -1;
-  if (n == 0) {
-    wait_for_earlier();
-    return;
-  }
-  const int seq = cache::sequence_of(a.b, row);
   const Places p = places_of(tokens, a.cmp_block, a.cmp_stride, a.shift);
-  reinterpret_cast<uint4*>(count)[tid] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) s_least = 0xFFFFFFFFu, s_most = 0, s_total = 0, s_n = 0;
-  int limbs = prepare_exact<D>(a, w, row, head) ? 4 : 0;
+  for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += kPickThreads) pages[i] = cache::page_of(a.b, seq, i);
   __syncthreads();
-  if (limbs != 0 && w.low != 0) limbs = 6;
   wait_for_earlier();
+  if (n == 0) return;
 
   // The lower bounds are counted in bins; the n_sel-th largest lies in bin `edge`, so a block whose upper bound is in a bin
   // below that is none of the best.
-  const bool fits = n <= kHeldBounds;
+  const bool fits = n <= kChecked;
   uint32_t least = 0xFFFFFFFFu, most = 0;
 #pragma unroll 4
   for (int i = tid; i < n; i += kPickThreads) {
@@ -553,64 +653,43 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Args a) {
     edge = (int)s_bin;
   }
 
-  // Exact scores of the blocks that are left; where they are too many, only the best so far are kept.
-  uint32_t scored = 0;
-  const auto keep_best = [&](bool last) {
-    const uint32_t in = s_n;
-    for (uint32_t x = 2 * scored + tid; x < 2 * in; x += kPickThreads)
-      (x % 2 == 0 ? range[x / 2].x : range[x / 2].y) = first_key(p, (int32_t)(list.index[x / 2] + x % 2));
-    __syncthreads();
-    exact_scores<D>(a, w, limbs, seq, head, range, list.rank, scored, in, part);
-    __syncthreads();
-    for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += kPickThreads / 8) {  // 8 threads for an entry
-      const uint32_t e = min(e0, in - 1);
-      const uint64_t key = list.rank[e];
-      const uint32_t block = list.index[e];
-      uint32_t better = 0;
-      for (uint32_t j = tid % 8; j < in; j += 8) better += list.rank[j] > key || (list.rank[j] == key && list.index[j] < block);
+  // Exact scores of the blocks that are left; where they are many, only the best so far are kept.
+  uint32_t kept = 0;
+  for (int i0 = 0;; i0 += kChecked) {
 #pragma unroll
-      for (int by = 4; by > 0; by /= 2) better += __shfl_xor_sync(0xFFFFFFFFu, better, by);
-      if (tid % 8 != 0 || e0 >= in || better >= wanted) continue;
-      if (last) sel[better] = (int32_t)block;
-      else other.rank[better] = key, other.index[better] = block;
+    for (int j = 0; j < kChecked / kPickThreads; ++j) {
+      const int i = j * kPickThreads + tid;
+      if (i0 + i < n && bin_of(of[i0 + i].y, low, per) >= edge) found[atomicAdd(&s_found, 1u)] = (uint16_t)i;
     }
-    if (last) return;
-    scored = min(in, wanted);
-    const List swap = list;
-    list = other, other = swap;
     __syncthreads();
-    if (tid == 0) s_n = scored;
-    __syncthreads();
-  };
-  for (int i0 = 0; i0 < n; i0 += kChecked * kPickThreads) {
-    uint32_t mask = 0;
+    const uint32_t n_found = s_found;
+    for (uint32_t f0 = 0;;) {
+      const uint32_t some = min(n_found - f0, (uint32_t)kAdded), in = kept + some;
+      score_blocks<D>(a, w, finite, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
+      f0 += some;
+      const bool whole = f0 == n_found, last = whole && i0 + kChecked >= n;
+      for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += kPickThreads / 8) {  // 8 threads for an entry
+        const uint32_t e = min(e0, in - 1);
+        const uint64_t key = list.rank[e];
+        const uint32_t block = list.index[e];
+        uint32_t better = 0;
+        for (uint32_t j = tid % 8; j < in; j += 8) better += list.rank[j] > key || (list.rank[j] == key && list.index[j] < block);
 #pragma unroll
-    for (int j = 0; j < kChecked; ++j) {
-      const int i = i0 + j * kPickThreads + tid;
-      if (i < n && bin_of(of[i].y, low, per) >= edge) mask |= 1u << j;
-    }
-    if (mask != 0) atomicAdd(&s_total, __popc(mask));
-    __syncthreads();
-    const bool room = s_n + s_total <= (uint32_t)size;
-    __syncthreads();
-    if (tid == 0) s_total = 0;
-    if (room) {
-      if (mask != 0) {
-        uint32_t at = atomicAdd(&s_n, __popc(mask));
-        for (; mask != 0; mask &= mask - 1) list.index[at++] = (uint32_t)(i0 + (__ffs(mask) - 1) * kPickThreads + tid);
+        for (int by = 4; by > 0; by /= 2) better += __shfl_xor_sync(0xFFFFFFFFu, better, by);
+        if (tid % 8 != 0 || e0 >= in || better >= wanted) continue;
+        if (last) sel[better] = (int32_t)block;
+        else other.rank[better] = key, other.index[better] = block;
       }
-    } else {
-      for (int j = 0; j < kChecked; ++j) {
-        if (mask >> j & 1) list.index[atomicAdd(&s_n, 1u)] = (uint32_t)(i0 + j * kPickThreads + tid);
-        __syncthreads();
-        const bool full = s_n + kPickThreads > (uint32_t)size;
-        __syncthreads();
-        if (full) keep_best(false);
-      }
+      if (last) return;
+      kept = min(in, wanted);
+      const List swap = list;
+      list = other, other = swap;
+      __syncthreads();
+      if (whole) break;
     }
+    if (tid == 0) s_found = 0;
     __syncthreads();
   }
-  keep_best(true);
 }
 
 }  // namespace cache_select

@@ -122,17 +122,19 @@ int32_t unit_of(const nsa_cache_select_desc* d) {
 
 template <int D>
 int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t st) {
-  const int list = select::list_bytes(a.n_sel);
-  const uint32_t bit = D == 64 ? 2u : D == 128 ? 4u : 8u;
-  const int rc = allow_smem(reinterpret_cast<const void*>(&select::pick_kernel<D>), select::list_bytes(select::kMaxSel), dev, bit);
+  const int list = select::list_bytes(a.n_sel), fixed = (int)sizeof(select::ScoreWarp<D>) * select::warps_of(D);
+  const uint32_t bit = D == 64 ? 2u : D == 128 ? 8u : 32u;
+  int rc = allow_smem(reinterpret_cast<const void*>(&select::score_kernel<D>), fixed + select::kMaxRows * 12 + 4, dev, bit);
+  if (rc == NSA_OK)
+    rc = allow_smem(reinterpret_cast<const void*>(&select::pick_kernel<D>), select::list_bytes(select::kMaxSel), dev, 2 * bit);
   if (rc != NSA_OK) return rc;
   const int64_t units = (a.blocks + a.unit - 1) / a.unit;  // of a row and KV head
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(select::kMaxRows, kMaxIndex / (units * a.hkv)));
   for (int64_t row0 = 0; row0 < n_rows; row0 += most) {
     a.row0 = (int32_t)row0;
     a.rows = (int32_t)std::min(most, n_rows - row0);
-    const int64_t grid = std::min<int64_t>(select::blocks_per_sm(D) * sm, units * a.hkv * a.rows);
-    cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::kWarps * 32, (a.rows + 1) * 4, 1, st, a);
+    const int64_t grid = std::min<int64_t>(sm, units * a.hkv * a.rows);
+    cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::warps_of(D) * 32, fixed + a.rows * 12 + 4, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection's score launch");
     e = launch(&select::pick_kernel<D>, dim3((unsigned)(a.rows * a.hkv)), select::kPickThreads, list, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection launch");
@@ -170,6 +172,8 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.q_half = d->q_dtype == NSA_DTYPE_F16;
   a.bits = 46;  // (the sum of the heads, in six signed bytes)
   while ((1 << (46 - a.bits)) < a.group) --a.bits;
+a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
+  a.at_once = select::kKeys / a.keys;
   if (b.d_qk == 64) return launch_select<64>(a, b.n_rows, sm, dev, st);
   if (b.d_qk == 128) return launch_select<128>(a, b.n_rows, sm, dev, st);
   return launch_select<192>(a, b.n_rows, sm, dev, st);
