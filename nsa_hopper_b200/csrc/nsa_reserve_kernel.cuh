@@ -21,7 +21,7 @@ namespace reserve {
 constexpr int kMaxSeqs = 8192;  // their six sums and lengths fill 196 KB of shared memory
 constexpr int kMaxThreads = 1024;
 constexpr int kCluster = 8;
-constexpr int kRows = 4;        // rows of a thread at a time
+constexpr int kRowsInside = 16384;  // packed rows from which on a second kernel is faster (2999 sequences with 8500: see below)
 
 struct Args {
   int32_t* pages;
@@ -37,6 +37,7 @@ struct Args {
   int64_t* slots;       // may be nullptr
   int64_t page_row;
   int32_t n_seqs, width, pool_size, n_rows;
+  int32_t rows_apart;   // packed rows are left to rows_kernel
 };
 
 __host__ __device__ constexpr int smem_bytes(int n_seqs) { return (6 * n_seqs + 3) * 4; }
@@ -82,6 +83,19 @@ __device__ __forceinline__ Sums sum_before(const Sums& mine, Sums* warps) {
   return s;
 }
 
+// Moves n pages by a warp, four of a lane on their way at once.
+template <class From, class To>
+__device__ __forceinline__ void move_pages(uint32_t n, uint32_t lane, From&& from, To&& to) {
+  for (uint32_t j0 = lane; j0 - lane < n; j0 += 128) {
+    int32_t page[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) page[k] = j0 + 32 * k < n ? from(j0 + 32 * k) : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (j0 + 32 * k < n) to(j0 + 32 * k, page[k]);
+  }
+}
+
 __global__ void __launch_bounds__(kMaxThreads) kernel(const Args a) {
   extern __shared__ uint32_t sm[];
   __shared__ Sums warps[32];
@@ -95,6 +109,7 @@ __global__ void __launch_bounds__(kMaxThreads) kernel(const Args a) {
   int32_t* held = lens + n;
   start_in_order();
   const int32_t free = clamp_free(a.n_free[0], a.pool_size);
+#pragma unroll 4
   for (int s = tid; s < n; s += blockDim.x) lens[s] = a.rows[s], held[s] = a.held[s];
   if (tid == 0) s_taken = 0;
   __syncthreads();
@@ -138,51 +153,53 @@ __global__ void __launch_bounds__(kMaxThreads) kernel(const Args a) {
   if (a.cu != nullptr)
     for (uint32_t s = me; s <= (uint32_t)n; s += threads) a.cu[s] = (int32_t)cu[s];
   // Pages that are given back are read from the rows of shrinking sequences and those taken are written to the rows of growing
-  // ones; the pool is read below `free` and written from there on.  So nothing that is read here is written here.
-  for (uint32_t j = me; j < taken; j += threads) {
-    const int s = range_of(need, n, j);
-    a.pages[(int64_t)s * a.page_row + from[s] + (int32_t)(j - need[s])] = taken_page(p, j);
+  // ones; the pool is read below `free` and written from there on.  So nothing that is read here is written here.  A warp has
+  // some neighbouring sequences: a lane takes the one page of its sequence, and for more they work together.
+  const uint32_t lane = tid % 32, crew = threads / 32;
+  uint32_t some = 1;
+  while (some < 32 && 4 * some * crew < (uint32_t)n) some *= 2;
+  for (uint32_t s0 = me / 32 * some; s0 < (uint32_t)n; s0 += crew * some) {
+    const uint32_t s = s0 + lane;
+    const bool mine = lane < some && s < (uint32_t)n;
+    const uint32_t takes = mine ? min(need[s + 1], taken) - min(need[s], taken) : 0;
+    if (takes == 1) a.pages[(int64_t)s * a.page_row + from[s]] = taken_page(p, need[s]);
+    uint32_t many = __ballot_sync(0xFFFFFFFFu, takes > 1 || (mine && give[s + 1] > give[s]));
+    for (; many != 0; many &= many - 1) {
+      const uint32_t x = s0 + __ffs(many) - 1, n0 = need[x], g0 = give[x];
+      int32_t* table = a.pages + (int64_t)x * a.page_row + from[x];
+      move_pages(min(need[x + 1], taken) - min(n0, taken), lane, [&](uint32_t j) { return taken_page(p, n0 + j); },
+                 [&](uint32_t j, int32_t page) { table[j] = page; });
+      const int64_t at = free + (int64_t)g0;
+      move_pages((uint32_t)max((int64_t)0, min((int64_t)(give[x + 1] - g0), a.pool_size - at)), lane,
+                 [&](uint32_t j) { return table[j]; }, [&](uint32_t j, int32_t page) { a.pool[at + j] = page; });
+    }
   }
-  for (uint32_t j = me; j < all.give && free + (int64_t)j < a.pool_size; j += threads) a.pool[free + (int64_t)j] = given_page(p, j);
-
   if (a.cu == nullptr) {
     for (uint32_t s = me; s < (uint32_t)n; s += threads) {
       const int32_t pos = lens[s] - 1;
       if (a.positions != nullptr) a.positions[s] = pos;
       if (a.slots != nullptr) a.slots[s] = pos < 0 ? -1 : slot_of(page_after(p, (int)s, pos / kPage), pos);
     }
-    return;
-  }
-  // kRows neighbouring rows of a thread are mostly of one page
-  for (uint32_t r0 = me * kRows; r0 < (uint32_t)a.n_rows; r0 += threads * kRows) {
-    int s = n > 0 ? range_of(cu, n, r0) : -1;
-    int32_t page = -1, page_sub = -1;
-    int32_t pos[kRows];
-    int64_t slot[kRows];
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const uint32_t r = r0 + k;
-      pos[k] = -1, slot[k] = -1;
-      if (s < 0 || r >= cu[n]) continue;
-      if (r >= cu[s + 1]) s = range_of(cu, n, r), page_sub = -1;
-      if (lens[s] == 0) continue;
-      pos[k] = lens[s] - (int32_t)(cu[s + 1] - r);
-      if (pos[k] / kPage != page_sub) page_sub = pos[k] / kPage, page = page_after(p, s, page_sub);
-      slot[k] = slot_of(page, pos[k]);
-    }
-    if (r0 + kRows <= (uint32_t)a.n_rows) {
-      if (a.positions != nullptr) reinterpret_cast<int4*>(a.positions + r0)[0] = make_int4(pos[0], pos[1], pos[2], pos[3]);
-      if (a.slots != nullptr) {
-        reinterpret_cast<longlong2*>(a.slots + r0)[0] = make_longlong2(slot[0], slot[1]);
-        reinterpret_cast<longlong2*>(a.slots + r0)[1] = make_longlong2(slot[2], slot[3]);
-      }
-    } else {
-      for (int k = 0; k < kRows && r0 + k < (uint32_t)a.n_rows; ++k) {
-        if (a.positions != nullptr) a.positions[r0 + k] = pos[k];
-        if (a.slots != nullptr) a.slots[r0 + k] = slot[k];
-      }
+  } else if (!a.rows_apart) {
+    for (uint32_t r = me; r < (uint32_t)a.n_rows; r += threads) {
+      const int s = n > 0 && r < cu[n] ? range_of(cu, n, r) : -1;
+      const int32_t pos = s >= 0 && lens[s] > 0 ? lens[s] - (int32_t)(cu[s + 1] - r) : -1;
+      if (a.positions != nullptr) a.positions[r] = pos;
+      if (a.slots != nullptr) a.slots[r] = pos < 0 ? -1 : slot_of(page_after(p, s, pos / kPage), pos);
     }
   }
+}
+
+// Positions and slots of packed rows, a thread each, from what `kernel` has written.
+__global__ void __launch_bounds__(256) rows_kernel(const Args a) {
+  start_in_order();
+  const int32_t r = (int32_t)(blockIdx.x * 256u + threadIdx.x);
+  if (r >= a.n_rows) return;
+  const cache::Batch b = {a.pages, a.lens, a.cu, a.page_row, a.n_seqs, a.width, 0x7FFFFFFF, a.n_rows};
+  const int s = cache::sequence_of(b, r);
+  const int32_t pos = s >= 0 && a.lens[s] > 0 ? cache::position_of(b, s, r) : -1;
+  if (a.positions != nullptr) a.positions[r] = pos;
+  if (a.slots != nullptr) a.slots[r] = pos < 0 ? -1 : slot_of(cache::page_of(b, s, pos / kPage), pos);
 }
 
 }  // namespace reserve

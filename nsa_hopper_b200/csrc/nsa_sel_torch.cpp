@@ -13,12 +13,14 @@
 // from the directory of this extension, or from the package directory next to this source.
 #include <dlfcn.h>
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <limits>
 #include <mutex>
 #include <string>
 
@@ -486,6 +488,19 @@ int64_t cache_record_bytes(int64_t d_qk, int64_t d_v) {
 }
 
 // ------------------------------------------------------------------ pages, selection and positions of a step
+// torch::empty on the current device without its dispatch: a step's small calls take less time than that.
+torch::Tensor empty_like_on(const torch::Tensor& t, c10::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt);
+}
+// `n` elements of a buffer, from byte `at` on, as a tensor of its own.
+torch::Tensor part_of(const torch::Tensor& buffer, at::ScalarType dtype, int64_t at, int64_t n) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                    c10::scalarTypeToTypeMeta(dtype));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(dtype)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // [lens, cu_seqlens (empty without n_tokens), positions, slots, held, n_free]
 std::vector<torch::Tensor> cache_reserve(torch::Tensor pages, torch::Tensor held, torch::Tensor rows, torch::Tensor pool,
                                          torch::Tensor n_free, c10::optional<int64_t> n_tokens, bool update) {
@@ -502,10 +517,22 @@ std::vector<torch::Tensor> cache_reserve(torch::Tensor pages, torch::Tensor held
   TORCH_CHECK(!n_tokens.has_value() || *n_tokens >= 0, "n_tokens must not be negative");
   const c10::cuda::CUDAGuard guard(pages.device());
   const int64_t n_rows = n_tokens.value_or(n);
-  const auto i32s = held.options();
-  auto lens = torch::empty({n}, i32s), cu = torch::empty({n_tokens.has_value() ? n + 1 : 0}, i32s);
-  auto positions = torch::empty({n_rows}, i32s), slots = torch::empty({n_rows}, i32s.dtype(torch::kLong));
-  auto held_out = update ? held : torch::empty({n}, i32s), n_free_out = update ? n_free : torch::empty({1}, i32s);
+  // one buffer for all results, each at a multiple of 16 bytes
+  int64_t bytes = 0;
+  const auto place = [&](int64_t size) {
+    const int64_t at = bytes;
+    bytes += (size + 15) / 16 * 16;
+    return at;
+  };
+  const int64_t n_cu = n_tokens.has_value() ? n + 1 : 0;
+  TORCH_CHECK(n_rows <= std::numeric_limits<int32_t>::max(), "n_tokens out of int32 range");
+  const int64_t at_slots = place(8 * n_rows), at_positions = place(4 * n_rows), at_lens = place(4 * n), at_cu = place(4 * n_cu);
+  const int64_t at_held = place(update ? 0 : 4 * n), at_free = place(update ? 0 : 4);
+  const auto buffer = empty_like_on(pages, {std::max<int64_t>(bytes, 16)}, at::kByte);
+  const auto lens = part_of(buffer, at::kInt, at_lens, n), cu = part_of(buffer, at::kInt, at_cu, n_cu);
+  const auto positions = part_of(buffer, at::kInt, at_positions, n_rows), slots = part_of(buffer, at::kLong, at_slots, n_rows);
+  const auto held_out = update ? held : part_of(buffer, at::kInt, at_held, n);
+  const auto n_free_out = update ? n_free : part_of(buffer, at::kInt, at_free, 1);
   nsa_cache_reserve_desc d;
   memset(&d, 0, sizeof(d));
   d.pages = pages.data_ptr<int32_t>();
@@ -542,7 +569,7 @@ torch::Tensor cache_select(torch::Tensor Q, torch::Tensor cache, torch::Tensor p
   TORCH_CHECK(Q.size(1) > 0 && Q.size(1) % cache.size(1) == 0, "Hq must be a multiple of Hkv");
   TORCH_CHECK(n_sel >= 1 && cmp_block >= 1 && cmp_stride >= 1, "n_sel, cmp_block and cmp_stride must be positive");
   const c10::cuda::CUDAGuard guard(cache.device());
-  auto sel = torch::empty({Q.size(0), cache.size(1), n_sel}, Q.options().dtype(torch::kInt));
+  auto sel = empty_like_on(Q, {Q.size(0), cache.size(1), n_sel}, at::kInt);
   if ((Q.size(0) > 1 && Q.stride(0) == 0) || (Q.size(1) > 1 && Q.stride(1) == 0)) Q = Q.contiguous();  // (0 means the default)
   if (Q.size(0) > 0) {
     check_rows(Q, "Q");
@@ -559,7 +586,7 @@ torch::Tensor cache_select(torch::Tensor Q, torch::Tensor cache, torch::Tensor p
   d.q_dtype = dtype;
   const int64_t ws = api().cache_select_ws(&d);
   if (ws < 0) TORCH_CHECK(false, format_msg("nsa_cache_select failed: %s", api().last_error()));
-  auto work = torch::empty({ws}, Q.options().dtype(torch::kByte));
+  const auto work = empty_like_on(Q, {ws}, at::kByte);
   d.workspace = work.data_ptr();
   const int rc = api().cache_select(&d, current_stream());
   if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_cache_select failed (%d): %s", rc, api().last_error()));
@@ -574,10 +601,10 @@ void rotary_strides(const torch::Tensor& x, int64_t (&s)[3]) {
   s[2] = stride_of(x, rows ? 0 : 2);
 }
 
-// [Q', K'] (K' empty without K).  `token_major` says of each whether [B, H, T, d] is laid out as [B, T, H, d].
-std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor turns, torch::Tensor axis,
-                                  int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
-                                  bool q_token_major, bool k_token_major) {
+// [Q', K'] (K' undefined without K).  `token_major` says of each whether [B, H, T, d] is laid out as [B, T, H, d].
+std::vector<torch::Tensor> turned(torch::Tensor Q, OptTensor K, const torch::Tensor& positions, const torch::Tensor& turns,
+                                  const torch::Tensor& axis, int64_t axes, int64_t d_head, int64_t offset, bool interleaved,
+                                  bool inverse, bool q_token_major, bool k_token_major) {
   TORCH_CHECK(Q.is_cuda() && (Q.dim() == 3 || Q.dim() == 4), "Q must be a CUDA tensor [N, H, d] or [B, H, T, d]");
   TORCH_CHECK(Q.scalar_type() == at::kBFloat16 || Q.scalar_type() == at::kHalf || Q.scalar_type() == at::kFloat,
               "Q must be bfloat16, float16 or float32");
@@ -605,15 +632,14 @@ std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor po
   torch::Tensor out[2];
   for (int i = 0; i < 2; ++i) {
     if (i == 1 && !K.has_value()) {
-      out[1] = torch::empty({0}, Q.options());
       continue;
     }
     torch::Tensor x = i == 0 ? Q : *K;
     if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
     if (!rows && (i == 0 ? q_token_major : k_token_major))
-      out[i] = torch::empty({B, T, x.size(1), d_head}, x.options()).transpose(1, 2);
+      out[i] = empty_like_on(x, {B, T, x.size(1), d_head}, x.scalar_type()).transpose(1, 2);
     else
-      out[i] = torch::empty(x.sizes(), x.options());
+      out[i] = empty_like_on(x, x.sizes(), x.scalar_type());
     if (x.numel() == 0) continue;
     d.t[i].x = x.data_ptr();
     d.t[i].y = out[i].data_ptr();
@@ -640,6 +666,67 @@ std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor po
   const int rc = api().rotary(&d, current_stream());
   if (rc != NSA_OK) TORCH_CHECK(false, format_msg("nsa_rotary failed (%d): %s", rc, api().last_error()));
   return {out[0], out[1]};
+}
+
+std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor turns, torch::Tensor axis,
+                                  int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
+                                  bool q_token_major, bool k_token_major);
+
+// The turn is linear and its transpose the turn back, so the gradient is a call of the same kind, and has gradients too.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor Q, torch::Tensor K,
+                                                torch::Tensor positions, torch::Tensor turns, torch::Tensor axis, int64_t axes,
+                                                int64_t d_head, int64_t offset, bool interleaved, bool inverse, bool q_token_major,
+                                                bool k_token_major) {
+    const bool both = K.defined();
+    ctx->save_for_backward({positions, turns, axis});
+    ctx->set_materialize_grads(false);
+    // gradients come back as the inputs lie: heads of [B, H, T, d] may be a view of [B, T, H, d]
+    const auto as_view = [](const torch::Tensor& x) {
+      return x.dim() == 4 && !x.is_contiguous() && x.transpose(1, 2).is_contiguous();
+    };
+    const int64_t flags = (both ? 1 : 0) | (interleaved ? 2 : 0) | (inverse ? 4 : 0) | (as_view(Q) ? 8 : 0) |
+                          (both && as_view(K) ? 16 : 0);
+    ctx->saved_data["flags"] = flags;
+    ctx->saved_data["axes"] = axes;
+    ctx->saved_data["d"] = d_head;
+    ctx->saved_data["offset"] = offset;
+    auto out = turned(Q, both ? OptTensor(K) : OptTensor(), positions, turns, axis, axes, d_head, offset, interleaved, inverse,
+                      q_token_major, k_token_major);
+    if (!both) out.pop_back();
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const auto back = [&](const torch::Tensor& q, const OptTensor& k, bool q_major, bool k_major) {
+      return rotary(q, k, saved[0], saved[1], saved[2], ctx->saved_data["axes"].toInt(), ctx->saved_data["d"].toInt(),
+                    ctx->saved_data["offset"].toInt(), (flags & 2) != 0, (flags & 4) == 0, q_major, k_major);
+    };
+    torch::autograd::variable_list result(12);
+    const bool q = grads[0].defined() && ctx->needs_input_grad(0);
+    const bool k = (flags & 1) != 0 && grads[1].defined() && ctx->needs_input_grad(1);
+    if (q) {
+      const auto d = back(grads[0], k ? OptTensor(grads[1]) : OptTensor(), (flags & 8) != 0, (flags & 16) != 0);
+      result[0] = d[0];
+      if (k) result[1] = d[1];
+    } else if (k) {
+      result[1] = back(grads[1], OptTensor(), (flags & 16) != 0, false)[0];
+    }
+    return result;
+  }
+};
+
+std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor turns, torch::Tensor axis,
+                                  int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
+                                  bool q_token_major, bool k_token_major) {
+  if (torch::GradMode::is_enabled() && (Q.requires_grad() || (K.has_value() && K->requires_grad()))) {
+    auto out = RotaryFunction::apply(Q, K.has_value() ? *K : torch::Tensor(), positions, turns, axis, axes, d_head, offset,
+                                     interleaved, inverse, q_token_major, k_token_major);
+    if (!K.has_value()) out.push_back(torch::Tensor());
+    return out;
+  }
+  return turned(Q, K, positions, turns, axis, axes, d_head, offset, interleaved, inverse, q_token_major, k_token_major);
 }
 
 int64_t library_version() { return api().version(); }

@@ -78,11 +78,15 @@ int run_reserve(const nsa_cache_reserve_desc* d, cudaStream_t st) {
   a.positions = d->positions, a.slots = d->slots;
   a.page_row = d->pages_stride ? d->pages_stride : d->width;
   a.n_seqs = d->n_seqs, a.width = d->width, a.pool_size = d->pool_size, a.n_rows = d->n_rows;
-  const int64_t items = std::max<int64_t>(d->n_seqs, d->n_rows / reserve::kRows);
-  const int threads = items <= 256 ? 256 : items <= 512 ? 512 : reserve::kMaxThreads;
-  const int blocks = items <= 2 * reserve::kMaxThreads ? 1 : reserve::kCluster;
-  return done(launch(&reserve::kernel, dim3((unsigned)blocks), threads, reserve::smem_bytes(d->n_seqs), blocks, st, a),
-              "cache reserve launch");
+  a.rows_apart = d->cu_seqlens != nullptr && (d->positions != nullptr || d->slots != nullptr) && d->n_rows > reserve::kRowsInside;
+  // One block where there is little to share out, else a cluster; threads for all sequences at once, or many.
+  const int inside = a.rows_apart ? 0 : d->n_rows;
+  const int blocks = std::max(d->n_seqs, inside / 8) <= 64 ? 1 : reserve::kCluster;
+  const int threads = blocks == 1 ? 256 : reserve::kMaxThreads;
+  cudaError_t e = launch(&reserve::kernel, dim3((unsigned)blocks), threads, reserve::smem_bytes(d->n_seqs), blocks, st, a);
+  if (e == cudaSuccess && a.rows_apart)
+    e = launch(&reserve::rows_kernel, dim3((unsigned)(((int64_t)d->n_rows + 255) / 256)), 256, 0, 1, st, a);
+  return done(e, "cache reserve launch");
 }
 
 // ------------------------------------------------------------------ block selection

@@ -284,36 +284,6 @@ def rotary_plan(d: int, *, rotary_dim: Optional[int] = None, offset: int = 0, ba
                       torch.tensor(axis, dtype=torch.uint8, device="cpu"))
 
 
-def _turned(Q, K, positions, plan: RotaryPlan, inverse: bool, token_major=(False, False)):
-    q, k = _C.rotary(Q, K, positions, plan.turns, plan.axis, plan.axes, plan.d, plan.offset, plan.interleaved, inverse,
-                     *token_major)
-    return q, None if K is None else k
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, Q, K, positions, plan, inverse):
-        ctx.save_for_backward(positions)
-        # gradients come back as the inputs lie: heads of [B, H, T, d] may be a view of [B, T, H, d]
-        ctx.token_major = [x is not None and x.dim() == 4 and not x.is_contiguous() and x.transpose(1, 2).is_contiguous()
-                           for x in (Q, K)]
-        ctx.plan, ctx.inverse = plan, inverse
-        ctx.set_materialize_grads(False)
-        return _turned(Q, K, positions, plan, inverse)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dQ, dK):
-        (positions,) = ctx.saved_tensors
-        dQ, dK = (g if need else None for g, need in zip((dQ, dK), ctx.needs_input_grad))
-        q_major, k_major = ctx.token_major
-        if dQ is None:
-            dK = None if dK is None else _turned(dK, None, positions, ctx.plan, not ctx.inverse, (k_major, False))[0]
-        else:
-            dQ, dK = _turned(dQ, dK, positions, ctx.plan, not ctx.inverse, (q_major, k_major))
-        return dQ, dK, None, None, None
-
-
 def rotary(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryPlan,
            inverse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Turns Q and K (or Q alone: ``K`` None) by their tokens' positions (nsa_rotary).
@@ -322,10 +292,9 @@ def rotary(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, 
     does; bf16, fp16 or fp32, any strides (a projection's [B, T, H, d] is given as ``x.transpose(1, 2)``).  ``positions`` int32
     [N] or [B, T] (any strides, e.g. expanded over the batch), with the axes of the plan before that if there are several.
     The results are contiguous and of the inputs' dtype; angles are exact for all int32 positions, products are fp32.
-    Differentiable in Q and K; ``inverse`` turns back."""
-    if torch.is_grad_enabled() and (Q.requires_grad or (K is not None and K.requires_grad)):
-        return _Rotary.apply(Q, K, positions, plan, bool(inverse))
-    return _turned(Q, K, positions, plan, bool(inverse))
+    Differentiable in Q and K, any number of times; ``inverse`` turns back."""
+    q, k = _C.rotary(Q, K, positions, plan.turns, plan.axis, plan.axes, plan.d, plan.offset, plan.interleaved, bool(inverse))
+    return q, k
 
 
 def library_version() -> int:
