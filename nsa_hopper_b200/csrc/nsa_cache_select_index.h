@@ -20,7 +20,7 @@ NSA_HD int32_t completed(int32_t tokens, int32_t block, int32_t stride) {
 }
 // Tokens of the longest sequence whose compressed keys a table of `width` pages holds.
 NSA_HD int32_t most_tokens(int32_t width, int32_t block, int32_t stride) {
-  const int64_t t = (int64_t)width * kPage * stride + block - 1;
+  const int64_t keys = (int64_t)width * kPage, t = (keys < kMaxTokens ? keys : kMaxTokens) * stride + block - 1;
   return t < kMaxTokens ? (int32_t)t : kMaxTokens;
 }
 // Tokens that a row of sequence `seq` (from sequence_of) sees, 0 where it selects nothing (no such token, or more of them than the table or float32 can place).

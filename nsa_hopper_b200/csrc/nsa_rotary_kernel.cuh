@@ -79,11 +79,12 @@ __device__ __forceinline__ float2 cos_sin(uint64_t turns, uint32_t flip) {
   return make_float2(__uint_as_float(__float_as_uint(x) ^ turned), __uint_as_float(__float_as_uint(y) ^ turned ^ flip));
 }
 
+// (The same roundings in every instance, so that results do not depend on strides and alignment.)
 template <class T>
 __device__ __forceinline__ void turn(T& a, T& b, float2 cs) {
   const float u = to_float(a), v = to_float(b);
-  a = from_float<T>(u * cs.x - v * cs.y);
-  b = from_float<T>(v * cs.x + u * cs.y);
+  a = from_float<T>(__fmaf_rn(u, cs.x, -__fmul_rn(v, cs.y)));
+  b = from_float<T>(__fmaf_rn(v, cs.x, __fmul_rn(u, cs.y)));
 }
 
 // Places of the angles in shared memory: those that neighbouring items of a warp read at once lie side by side.

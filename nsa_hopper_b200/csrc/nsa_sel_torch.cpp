@@ -674,11 +674,11 @@ std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor po
 
 // The turn is linear and its transpose the turn back, so the gradient is a call of the same kind, and has gradients too.
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor Q, torch::Tensor K,
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor Q, OptTensor K,
                                                 torch::Tensor positions, torch::Tensor turns, torch::Tensor axis, int64_t axes,
                                                 int64_t d_head, int64_t offset, bool interleaved, bool inverse, bool q_token_major,
                                                 bool k_token_major) {
-    const bool both = K.defined();
+    const bool both = K.has_value();
     ctx->save_for_backward({positions, turns, axis});
     ctx->set_materialize_grads(false);
     // gradients come back as the inputs lie: heads of [B, H, T, d] may be a view of [B, T, H, d]
@@ -686,12 +686,12 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
       return x.dim() == 4 && !x.is_contiguous() && x.transpose(1, 2).is_contiguous();
     };
     const int64_t flags = (both ? 1 : 0) | (interleaved ? 2 : 0) | (inverse ? 4 : 0) | (as_view(Q) ? 8 : 0) |
-                          (both && as_view(K) ? 16 : 0);
+                          (both && as_view(*K) ? 16 : 0);
     ctx->saved_data["flags"] = flags;
     ctx->saved_data["axes"] = axes;
     ctx->saved_data["d"] = d_head;
     ctx->saved_data["offset"] = offset;
-    auto out = turned(Q, both ? OptTensor(K) : OptTensor(), positions, turns, axis, axes, d_head, offset, interleaved, inverse,
+    auto out = turned(Q, K, positions, turns, axis, axes, d_head, offset, interleaved, inverse,
                       q_token_major, k_token_major);
     if (!both) out.pop_back();
     return out;
@@ -721,7 +721,7 @@ std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor po
                                   int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
                                   bool q_token_major, bool k_token_major) {
   if (torch::GradMode::is_enabled() && (Q.requires_grad() || (K.has_value() && K->requires_grad()))) {
-    auto out = RotaryFunction::apply(Q, K.has_value() ? *K : torch::Tensor(), positions, turns, axis, axes, d_head, offset,
+    auto out = RotaryFunction::apply(Q, K, positions, turns, axis, axes, d_head, offset,
                                      interleaved, inverse, q_token_major, k_token_major);
     if (!K.has_value()) out.push_back(torch::Tensor());
     return out;

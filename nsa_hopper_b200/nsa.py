@@ -296,13 +296,15 @@ def cache_compress(cache: torch.Tensor, d_qk: int, pages: torch.Tensor, lens: to
     return count
 
 
-def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, sel: torch.Tensor, *,
-               l_prime: int = 64, window: int = 512, cmp_cache: Optional[torch.Tensor] = None,
-               cmp_pages: Optional[torch.Tensor] = None, cmp_lens: Optional[torch.Tensor] = None,
-               gate_w: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor,
+               sel: Optional[torch.Tensor] = None, *, l_prime: int = 64, window: int = 512,
+               cmp_cache: Optional[torch.Tensor] = None, cmp_pages: Optional[torch.Tensor] = None,
+               cmp_lens: Optional[torch.Tensor] = None, gate_w: Optional[torch.Tensor] = None,
+               err: Optional[torch.Tensor] = None, n_sel: int = 16, cmp_block: int = 32, cmp_stride: int = 16) -> torch.Tensor:
     """The three NSA branches and the gate of :func:`nsa_forward` for the newest token of every sequence of a
     4-bit cache (``ops.cache_write`` has put its K and V there): Q [S, Hq, d_qk] bf16 or fp16, sel int32
-    [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  The compressed branch sees
+    [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  Without ``sel`` the ``n_sel`` best blocks are
+    taken (``ops.cache_select``; ``cmp_block`` and ``cmp_stride`` as :func:`cache_compress` was called with).  The compressed branch sees
     every key of ``cmp_cache`` (:func:`cache_compress` keeps it, called after every write), as the newest token does in
     the forward; without one it is left out.  Each branch adds its gated result into O.  ``err``: as in
     ``ops.cache_attend``, for all three."""
@@ -312,6 +314,10 @@ def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: 
         raise ValueError("window must be positive (the window branch of nothing has no keys)")
     if cmp_cache is not None and (cmp_pages is None or cmp_lens is None):
         raise ValueError("cmp_pages and cmp_lens are needed with cmp_cache")
+    if sel is None:
+        if cmp_cache is None:
+            raise ValueError("cmp_cache is needed to select blocks (or give sel)")
+        sel = ops.cache_select(Q, cmp_cache, cmp_pages, lens, n_sel, l_prime, cmp_block, cmp_stride)
     g = gate_weights(gate_w, Q.device)
     O = torch.empty(Q.shape[0], Q.shape[1], cache.shape[2] // 36 - Q.shape[2], dtype=torch.float32, device=Q.device)
     ops.cache_attend(Q, cache, pages, lens, sel=sel, l_prime=l_prime, out=O, weight=g[1:2], with_lse=False, err=err)
