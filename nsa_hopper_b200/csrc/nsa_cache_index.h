@@ -45,24 +45,30 @@ struct Batch {
   int32_t n_rows;
 };
 
+// How the batch's arrays are read.
+struct Load {
+  NSA_HD int32_t operator()(const int32_t* p) const { return *p; }
+};
+
 // The sequence of a row, -1 for a row of none (before cu[0] or behind cu[n_seqs]).  In a cu_seqlens that is out of order it is
 // one of those whose range holds the row, or -1, and the two forms need not agree.
-NSA_HD int sequence_of(const Batch& b, int row) {
+template <class L = Load>
+NSA_HD int sequence_of(const Batch& b, int row, L load = L()) {
   if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
-  if (b.n_seqs <= 0 || row < b.cu[0]) return -1;
+  if (b.n_seqs <= 0 || row < load(b.cu)) return -1;
   int lo = 0, hi = b.n_seqs;  // the last s with cu[s] <= row is in [lo, hi)
   while (hi - lo > 1) {
     const int mid = lo + (hi - lo) / 2;
-    if (b.cu[mid] <= row) lo = mid;
+    if (load(b.cu + mid) <= row) lo = mid;
     else hi = mid;
   }
-  return row < b.cu[lo + 1] ? lo : -1;
+  return row < load(b.cu + lo + 1) ? lo : -1;
 }
 // The same, 32 places of cu at a time: `below(lo, step, hi)` has bit i set where place lo + i * step is before hi and its cu not
 // above the row.  (A thread that searches by itself is faster with the form above: the reading kernel takes 64 us for 104448
 // tokens of 16 sequences, and 71 with this one's steps.)
-template <class Below>
-NSA_HD int sequence_by_32(const Batch& b, int row, Below&& below) {
+template <class Below, class L = Load>
+NSA_HD int sequence_by_32(const Batch& b, int row, Below&& below, L load = L()) {
   if (b.cu == nullptr) return row < b.n_seqs ? row : -1;
   int lo = 0, hi = b.n_seqs;
   while (hi - lo > 1) {
@@ -71,14 +77,15 @@ NSA_HD int sequence_by_32(const Batch& b, int row, Below&& below) {
     lo += last * step;
     hi = hi - lo > step ? lo + step : hi;
   }
-  return b.n_seqs > 0 && b.cu[lo] <= row && row < b.cu[lo + 1] ? lo : -1;
+  return b.n_seqs > 0 && load(b.cu + lo) <= row && row < load(b.cu + lo + 1) ? lo : -1;
 }
 
 // Position of a row in its sequence (from sequence_of, >= 0): the sequence's last rows are the call's.
 // Negative where the sequence has no such token.
-NSA_HD int position_of(const Batch& b, int seq, int row) {
-  const int len = b.lens[seq] > 0 ? b.lens[seq] : 0;
-  const int behind = b.cu == nullptr ? 1 : b.cu[seq + 1] - row;  // >= 1
+template <class L = Load>
+NSA_HD int position_of(const Batch& b, int seq, int row, L load = L()) {
+  const int held = load(b.lens + seq), len = held > 0 ? held : 0;
+  const int behind = b.cu == nullptr ? 1 : load(b.cu + seq + 1) - row;  // >= 1
   return len - behind;
 }
 
@@ -90,9 +97,10 @@ NSA_HD int keys_up_to(const Batch& b, int pos) {
 }
 
 // The cache page of 64-key sub-block `sub` of a sequence, -1 where there is none.
-NSA_HD int page_of(const Batch& b, int seq, int sub) {
+template <class L = Load>
+NSA_HD int page_of(const Batch& b, int seq, int sub, L load = L()) {
   if (sub < 0 || sub >= b.width) return -1;
-  const int p = b.pages[(int64_t)seq * b.page_row + sub];
+  const int p = load(b.pages + (int64_t)seq * b.page_row + sub);
   return p >= 0 && p < b.num_pages ? p : -1;
 }
 

@@ -24,8 +24,9 @@ NSA_HD int32_t most_tokens(int32_t width, int32_t block, int32_t stride) {
   return t < kMaxTokens ? (int32_t)t : kMaxTokens;
 }
 // Tokens that a row of sequence `seq` (from sequence_of) sees, 0 where it selects nothing (no such token, or more of them than the table or float32 can place).
-NSA_HD int32_t tokens_of(const Batch& b, int seq, int row, int32_t most) {
-  const int pos = seq < 0 ? -1 : cache::position_of(b, seq, row);
+template <class L = cache::Load>
+NSA_HD int32_t tokens_of(const Batch& b, int seq, int row, int32_t most, L load = L()) {
+  const int pos = seq < 0 ? -1 : cache::position_of(b, seq, row, load);
   return pos >= 0 && pos < most ? pos + 1 : 0;
 }
 NSA_HD int32_t blocks_of(int32_t tokens, int32_t shift) { return (int32_t)(((int64_t)tokens + (1 << shift) - 1) >> shift); }

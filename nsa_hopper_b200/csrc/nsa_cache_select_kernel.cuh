@@ -14,13 +14,18 @@
 //     is cut into whole numbers too (prepare_exact), the 16 products of a group that share a scale are added as integers
 //     (dot products of four bytes), and only scale times group sum is rounded, in fp64.
 //
-// Error of the approximation of a key's score, in units of max|k| (six times the largest scale of the unit's keys), with
+// Error of the approximation, in units of max|k| (six times the largest scale of a unit's keys) times the keys of a block, with
 // S = sum over d and heads of |q| and Q = sum over d of |sum of the heads|: the fp32 sum of G heads (G - 1) 2^-24 S; the two
-// fp16 parts of the query 2^-22 Q; the sums of d products (the tensor core cuts each term off below 2^-23 of the largest, twice
-// that is allowed for; a running sum is half of Q on average) and of up to 12 group sums, d 2^-22.9 Q together; taken as
-// d 2^-22 Q, with room for the sums over keys.
+// fp16 parts of the query 2^-22 Q; a group's products, added to the sum so far four at a time, four times (the tensor core cuts
+// each term off below 2^-23 of the largest, twice that is allowed for), 20 2^-22 Q; the sums of groups and quarters in fp32
+// 8 2^-24 Q; that of up to 258 keys 258 2^-24 Q.  All but the first are less than 90 2^-22 Q, and taken as 2^-15 Q.
 //
-// What bounds it: a key costs 9/16 d bytes, 72 at d = 128, and half as many instructions of a thread: DRAM, for large calls.
+// What bounds it.  A key costs 9/16 d bytes.  256 sequences of up to 65536 tokens, 4 heads of 128: 151 MB, which DRAM would
+// deliver in 24 us, take 64.  46 of them are score_kernel's: the ALU pipe, which converts codes (128 of its 400 instructions for
+// 64 keys), is its busiest unit at 59 %, tensor cores 19 %.  The others are pick_kernel's, 1024 blocks that are chains of
+// 9000 cycles (reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks 900).  One sequence of 65536 tokens:
+// 9.3 us; 64 of up to 32768: 17 us.  Tried: exact scores of all blocks with dot products of four bytes (select of the 256 above 102 us);
+// the bin from the threads' largest bounds instead of counts (2000 cycles and half as many candidates again).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,8 +50,8 @@ constexpr int kUnitBlocks = 31;   // its blocks at most: a lane for each and one
 constexpr int kMaxGroup = 256;    // query heads of a KV head
 constexpr int kMaxSel = 1024;
 constexpr int kPickThreads = 256;
+constexpr int kChecked = 8 * kPickThreads;  // blocks that pick_kernel looks at at a time
 constexpr int kBins = 4 * kPickThreads;
-constexpr int kChecked = 2048;    // blocks that pick_kernel looks at between two meetings, and whose bounds it can hold
 constexpr int kAdded = 512;       // of them, those whose exact scores are compared with the best so far
 constexpr int kKeys = 512;        // places of keys that are scored between two meetings
 constexpr int kHeldPages = 256;   // first pages of a sequence, looked up beforehand
@@ -70,6 +75,7 @@ struct Args {
   int32_t q_half;
   int32_t bits;         // of a query head's value in the exact sum: its largest is below 2^bits
   int32_t keys;         // of a block, at most
+  uint32_t per_key;     // 2^20 / keys, rounded up: exact for the kKeys places
   int32_t at_once;      // blocks that have kKeys places
   int32_t row0, rows;   // rows of this launch
 };
@@ -142,7 +148,7 @@ __device__ __forceinline__ float load_query(const Args& a, uint32_t (&bq)[D / 8]
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     top = max(top, __float_as_uint(sum[i]) & 0x7FFFFFFFu);
-    size += fabsf(sum[i]) * ((float)D * 2.3841858e-07f);  // 2^-22
+    size += fabsf(sum[i]) * 3.0517578e-05f;  // 2^-15
   }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
 #pragma unroll
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32) score_kernel(const Args a) {
   int2* const row_of = reinterpret_cast<int2*>(all_warps + kWarps);      // [rows] sequence and tokens
   uint32_t* const line = reinterpret_cast<uint32_t*>(row_of + a.rows);  // [rows + 1] units before every row
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  // (pick_kernel is let go only after this wait, so that it may read what earlier kernels wrote without one of its own)
+  // (pick_kernel is let go only after this wait, so that it may read what earlier kernels wrote before its own)
   wait_for_earlier();
   allow_next();
   const int each = (a.rows + kWarps * 32 - 1) / (kWarps * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
@@ -421,16 +427,37 @@ __device__ __forceinline__ int decode4(uint32_t codes) {
 
 // The sum of a (row, head)'s query heads as whole numbers of a power of two, so that the largest stays below 2^46, cut into six
 // signed bytes: values down to 2^-33 of the largest are exact in bf16 (2^-30 in fp16) with 16 heads, smaller ones off by less
-// than 2^-40 of it.  By all threads: kParts of them share the heads of two dims.  False if a value is not finite.
+// than 2^-40 of it.  By all threads: kParts of them share the heads of two dims; the first kAhead of each are loaded beforehand.
+constexpr int kAhead = 4;
 template <int D>
-__device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, int row, int head) {
-  constexpr int kParts = kPickThreads / (D / 2);
-  const int tid = threadIdx.x, pair = tid % (D / 2), part = tid / (D / 2);
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.group * a.q_head + 2 * pair;
-  const int heads = part < kParts ? a.group : 0;
+struct Heads {
+  static constexpr int kParts = kPickThreads / (D / 2);
+  const uint16_t* q;
+  int64_t step;
+  int pair, part, n;  // n: heads of this thread
+  uint32_t first[kAhead];
+  __device__ __forceinline__ Heads(const Args& a, int row, int head) {
+    pair = threadIdx.x % (D / 2), part = threadIdx.x / (D / 2);
+    q = static_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_row + ((int64_t)head * a.group + part) * a.q_head + 2 * pair;
+    step = kParts * a.q_head;
+    n = part < kParts && part < a.group ? (a.group - part + kParts - 1) / kParts : 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) first[i] = i < n ? __ldcg(reinterpret_cast<const uint32_t*>(q + i * step)) : 0;
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f(first[i]);  // (zeros behind the last)
+#pragma unroll 1
+    for (int i = kAhead; i < n; ++i) f(__ldcg(reinterpret_cast<const uint32_t*>(q + i * step)));
+  }
+};
+template <int D>
+__device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const Heads<D>& heads) {
+  constexpr int kParts = Heads<D>::kParts;
+  const int tid = threadIdx.x, pair = heads.pair, part = heads.part;
   uint32_t top = 0;
-#pragma unroll 4
-  for (int g = part; g < heads; g += kParts) top = __vmaxu2(top, *reinterpret_cast<const uint32_t*>(q + g * a.q_head) & 0x7FFF7FFFu);
+  heads.each([&](uint32_t two) { top = __vmaxu2(top, two & 0x7FFF7FFFu); });
   if (tid == 0) w.top = 0;
   for (int i = tid; i < 2 * D; i += kPickThreads) w.sum[0][i] = 0;
   __syncthreads();
@@ -443,16 +470,14 @@ __device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, int ro
   const int up = a.bits - 22 + 126 - max((int)(__float_as_uint(query_value(a, top)) >> 23), 1);
   const float up0 = __uint_as_float((uint32_t)(127 + up / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
   int32_t upper[2] = {}, lower[2] = {};
-#pragma unroll 4
-  for (int g = part; g < heads; g += kParts) {
-    const uint32_t two = *reinterpret_cast<const uint32_t*>(q + g * a.q_head);
+  heads.each([&](uint32_t two) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float x = query_value(a, i == 0 ? two & 0xFFFFu : two >> 16) * up0 * up1, whole_part = rintf(x);
       upper[i] += (int)whole_part;
       lower[i] += __float2int_rn((x - whole_part) * 4194304.0f);
     }
-  }
+  });
   if (part < kParts)
 #pragma unroll
     for (int i = 0; i < 2; ++i) atomicAdd(&w.sum[0][2 * pair + i], upper[i]), atomicAdd(&w.sum[1][2 * pair + i], lower[i]);
@@ -536,7 +561,7 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, b
       Quarter<D> k[2] = {};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t t = t0 + x * (kPickThreads / 4), e = t / (uint32_t)a.keys;
+        const uint32_t t = t0 + x * (kPickThreads / 4), e = t * a.per_key >> 20;  // t / a.keys
         // (two threads find where the block begins, two where it ends)
         const int32_t block = t < places ? base + blocks[e0 + e] : 0;
         const int32_t bound = first_key(p, block + quarter % 2);
@@ -565,6 +590,16 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, b
 }
 
 // ------------------------------------------------------------------ the best of a row
+// From the L2: what is read while score_kernel still runs, since an L1 may hold what the kernels before that one have replaced.
+struct LoadPastL1 {
+  NSA_HD int32_t operator()(const int32_t* p) const {
+#ifdef __CUDA_ARCH__
+    return __ldcg(p);
+#else
+    return *p;
+#endif
+  }
+};
 __host__ __device__ constexpr int list_size(int n_sel) { return n_sel + kAdded; }
 __host__ __device__ constexpr int list_bytes(int n_sel) { return 24 * list_size(n_sel); }  // two lists
 // Numbers that compare like fp32, and back.
@@ -581,87 +616,101 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Exact<D> w;
   __shared__ double scores[kKeys];
-  __shared__ float2 held[kChecked];
   __shared__ uint16_t found[kChecked];
   __shared__ int32_t pages[kHeldPages];
   __shared__ __align__(16) uint32_t count[kBins];
-  __shared__ uint32_t sums[kPickThreads / 32];
-  __shared__ uint32_t s_least, s_most, s_bin, s_found;
+  __shared__ uint32_t s_least[kPickThreads / 32], s_most[kPickThreads / 32], sums[kPickThreads / 32], s_bin, s_found;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int size = list_size(a.n_sel);
   List list = {reinterpret_cast<uint64_t*>(dynamic), reinterpret_cast<uint32_t*>(dynamic + 16 * size)};
   List other = {list.rank + size, list.index + size};
   allow_next();
-  // What earlier kernels wrote is read before score_kernel has ended (see there).
+  // What earlier kernels wrote is read before score_kernel has ended: it has waited for them before this one could begin.
   const int64_t unit = blockIdx.x;
   const int row = a.row0 + (int)(unit / a.hkv), head = (int)(unit % a.hkv);
   const float2* bounds = a.bounds + ((int64_t)a.row0 * a.hkv + unit) * a.blocks;
   int32_t* sel = a.sel + ((int64_t)a.row0 * a.hkv + unit) * a.n_sel;
-  reinterpret_cast<uint4*>(count)[tid] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) s_least = 0xFFFFFFFFu, s_most = 0, s_found = 0;
-  const bool finite = prepare_exact<D>(a, w, row, head);
-  const int seq = cache::sequence_of(a.b, row);
-  const int32_t tokens = tokens_of(a.b, seq, row, a.most), n = blocks_of(tokens, a.shift);
+  const Heads<D> heads(a, row, head);
+  const int seq = cache::sequence_by_32(
+      a.b, row,
+      [&](int lo, int step, int hi) {
+        return __ballot_sync(0xFFFFFFFFu, lane * step < hi - lo && LoadPastL1()(a.b.cu + lo + lane * step) <= row);
+      },
+      LoadPastL1());
+  const int32_t tokens = tokens_of(a.b, seq, row, a.most, LoadPastL1()), n = blocks_of(tokens, a.shift);
   const uint32_t wanted = min((uint32_t)a.n_sel, (uint32_t)n);
-  for (int i = (int)wanted + tid; i < a.n_sel; i += kPickThreads) sel[i] = -1;
   const Places p = places_of(tokens, a.cmp_block, a.cmp_stride, a.shift);
-  for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += kPickThreads) pages[i] = cache::page_of(a.b, seq, i);
+  for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += kPickThreads) pages[i] = cache::page_of(a.b, seq, i, LoadPastL1());
+  if (tid == 0) s_found = 0;
+  const bool finite = prepare_exact<D>(a, w, heads);
   __syncthreads();
   wait_for_earlier();
+  // (all of them: in a cu_seqlens out of order score_kernel may have taken the row for another sequence's)
+  for (int i = tid; i < a.n_sel; i += kPickThreads) sel[i] = -1;
   if (n == 0) return;
 
-  // The lower bounds are counted in bins; the n_sel-th largest lies in bin `edge`, so a block whose upper bound is in a bin
-  // below that is none of the best.
-  const bool fits = n <= kChecked;
-  uint32_t least = 0xFFFFFFFFu, most = 0;
-#pragma unroll 4
-  for (int i = tid; i < n; i += kPickThreads) {
-    const float2 x = bounds[i];
-    if (fits) held[i] = x;
-    if (x.x > -kHuge) least = min(least, ordered(x.x)), most = max(most, ordered(x.x));
-  }
-  const float2* of = fits ? held : bounds;
-  least = __reduce_min_sync(0xFFFFFFFFu, least), most = __reduce_max_sync(0xFFFFFFFFu, most);
-  if (lane == 0) atomicMin(&s_least, least), atomicMax(&s_most, most);
-  __syncthreads();
-  float low = 0.0f, per = 0.0f;
-  int edge = 0;
-  if (n > (int)wanted && s_most > s_least) {
-    low = unordered(s_least);
-    per = (float)kBins / (unordered(s_most) - low);  // (0 if that is beyond fp32: one bin)
-    for (int i = tid; i < n; i += kPickThreads) atomicAdd(&count[bin_of(of[i].x, low, per)], 1u);
-    __syncthreads();
-    // four bins of a thread, the largest first
-    const uint4 c = reinterpret_cast<const uint4*>(count)[kPickThreads - 1 - tid];
-    const uint32_t mine = c.x + c.y + c.z + c.w;
-    uint32_t upto = mine;
-#pragma unroll
-    for (int by = 1; by < 32; by *= 2) {
-      const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, upto, by);
-      if (lane >= by) upto += before;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    uint32_t at = upto - mine;
-#pragma unroll
-    for (int i = 0; i < kPickThreads / 32; ++i) at += i < warp ? sums[i] : 0;
-    if (at < wanted && wanted <= at + mine) {
-      const int bin = 4 * (kPickThreads - 1 - tid);
-      s_bin = wanted <= at + c.w ? bin + 3 : wanted <= at + c.w + c.z ? bin + 2 : wanted <= at + c.w + c.z + c.y ? bin + 1 : bin;
-    }
-    __syncthreads();
-    edge = (int)s_bin;
-  }
-
-  // Exact scores of the blocks that are left; where they are many, only the best so far are kept.
   uint32_t kept = 0;
   for (int i0 = 0;; i0 += kChecked) {
+    // The lower bounds are counted in bins; the n_sel-th largest lies in bin `edge`, so a block whose upper bound is in a bin
+    // below that is none of the best.  (1024 bins: mostly one or two blocks too many.)
+    constexpr int kEach = kChecked / kPickThreads;
+    const int here = min(n - i0, kChecked);
+    float2 x[kEach];
+    uint32_t least = 0xFFFFFFFFu, most = 0;
 #pragma unroll
-    for (int j = 0; j < kChecked / kPickThreads; ++j) {
+    for (int j = 0; j < kEach; ++j) {
       const int i = j * kPickThreads + tid;
-      if (i0 + i < n && bin_of(of[i0 + i].y, low, per) >= edge) found[atomicAdd(&s_found, 1u)] = (uint16_t)i;
+      x[j] = i < here ? bounds[i0 + i] : make_float2(-kHuge, -kHuge);
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (x[j].x > -kHuge) least = min(least, ordered(x[j].x)), most = max(most, ordered(x[j].x));
+    float low = 0.0f, per = 0.0f;
+    int edge = 0;
+    if (here > (int)wanted) {
+      least = __reduce_min_sync(0xFFFFFFFFu, least), most = __reduce_max_sync(0xFFFFFFFFu, most);
+      if (lane == 0) s_least[warp] = least, s_most[warp] = most;
+      reinterpret_cast<uint4*>(count)[tid] = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPickThreads / 32; ++i) least = min(least, s_least[i]), most = max(most, s_most[i]);
+      if (least < most) {
+        low = unordered(least);
+        per = (float)kBins / (unordered(most) - low);  // (0 if that is beyond fp32: one bin)
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (j * kPickThreads + tid < here) atomicAdd(&count[bin_of(x[j].x, low, per)], 1u);
+      __syncthreads();
+      // four bins of a thread, the largest first
+      const uint4 c = reinterpret_cast<const uint4*>(count)[kPickThreads - 1 - tid];
+      const uint32_t mine = c.x + c.y + c.z + c.w;
+      uint32_t upto = mine;
+#pragma unroll
+      for (int by = 1; by < 32; by *= 2) {
+        const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, upto, by);
+        if (lane >= by) upto += before;
+      }
+      if (lane == 31) sums[warp] = upto;
+      __syncthreads();
+      uint32_t at = upto - mine;
+#pragma unroll
+      for (int i = 0; i < kPickThreads / 32; ++i) at += i < warp ? sums[i] : 0;
+      if (at < wanted && wanted <= at + mine) {
+        const int bin = 4 * (kPickThreads - 1 - tid);
+        s_bin = wanted <= at + c.w ? bin + 3 : wanted <= at + c.w + c.z ? bin + 2 : wanted <= at + c.w + c.z + c.y ? bin + 1 : bin;
+      }
+      __syncthreads();
+      edge = (int)s_bin;
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = j * kPickThreads + tid;
+      if (i < here && bin_of(x[j].y, low, per) >= edge) found[atomicAdd(&s_found, 1u)] = (uint16_t)i;
     }
     __syncthreads();
+
+    // Exact scores of the blocks that are left; where they are many, only the best so far are kept.
     const uint32_t n_found = s_found;
     for (uint32_t f0 = 0;;) {
       const uint32_t some = min(n_found - f0, (uint32_t)kAdded), in = kept + some;

@@ -18,7 +18,7 @@
 namespace nsa {
 namespace reserve {
 
-constexpr int kMaxSeqs = 8192;  // their six sums and lengths fill 196 KB of shared memory
+constexpr int kMaxSeqs = 8192;  // their six sums and lengths fill 192 KB of shared memory
 constexpr int kMaxThreads = 1024;
 constexpr int kCluster = 8;
 constexpr int kRowsInside = 16384;  // packed rows from which on a second kernel is faster (2999 sequences with 8500: see below)

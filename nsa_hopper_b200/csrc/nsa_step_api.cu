@@ -137,7 +137,9 @@ int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t 
   for (int64_t row0 = 0; row0 < n_rows; row0 += most) {
     a.row0 = (int32_t)row0;
     a.rows = (int32_t)std::min(most, n_rows - row0);
-    const int64_t grid = std::min<int64_t>(sm, units * a.hkv * a.rows);
+    // (two units for a block at least, so that where there are few some SMs are left for pick_kernel, which begins before this
+    // one has ended: one sequence of 65536 tokens 11.8 us, and 9.4 so)
+    const int64_t grid = std::min<int64_t>(sm, (units * a.hkv * a.rows + 1) / 2);
     cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::warps_of(D) * 32, fixed + a.rows * 12 + 4, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection's score launch");
     e = launch(&select::pick_kernel<D>, dim3((unsigned)(a.rows * a.hkv)), select::kPickThreads, list, 1, st, a);
@@ -177,6 +179,7 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.bits = 46;  // (the sum of the heads, in six signed bytes)
   while ((1 << (46 - a.bits)) < a.group) --a.bits;
 a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
+  a.per_key = ((1u << 20) + a.keys - 1) / a.keys;
   a.at_once = select::kKeys / a.keys;
   if (b.d_qk == 64) return launch_select<64>(a, b.n_rows, sm, dev, st);
   if (b.d_qk == 128) return launch_select<128>(a, b.n_rows, sm, dev, st);
