@@ -69,7 +69,7 @@ int run_reserve(const nsa_cache_reserve_desc* d, cudaStream_t st) {
   int sm = 0, dev = 0;
   rc = nsa::host::current_sm_count(&sm, &dev);
   if (rc != NSA_OK) return rc;
-  rc = allow_smem(reinterpret_cast<const void*>(&reserve::kernel), reserve::smem_bytes(reserve::kMaxSeqs), dev, 1u);
+  rc = allow_smem(reinterpret_cast<const void*>(&reserve::reserve_kernel), reserve::smem_bytes(reserve::kMaxSeqs), dev, 1u);
   if (rc != NSA_OK) return rc;
   reserve::Args a;
   memset(&a, 0, sizeof(a));
@@ -83,7 +83,7 @@ int run_reserve(const nsa_cache_reserve_desc* d, cudaStream_t st) {
   const int inside = a.rows_apart ? 0 : d->n_rows;
   const int blocks = std::max(d->n_seqs, inside / 8) <= 64 ? 1 : reserve::kCluster;
   const int threads = blocks == 1 ? 256 : reserve::kMaxThreads;
-  cudaError_t e = launch(&reserve::kernel, dim3((unsigned)blocks), threads, reserve::smem_bytes(d->n_seqs), blocks, st, a);
+  cudaError_t e = launch(&reserve::reserve_kernel, dim3((unsigned)blocks), threads, reserve::smem_bytes(d->n_seqs), blocks, st, a);
   if (e == cudaSuccess && a.rows_apart)
     e = launch(&reserve::rows_kernel, dim3((unsigned)(((int64_t)d->n_rows + 255) / 256)), 256, 0, 1, st, a);
   return done(e, "cache reserve launch");
@@ -223,7 +223,7 @@ int check_rotary(const nsa_rotary_desc* d) {
 
 template <class T, int VEC>
 cudaError_t launch_rotary(const rotary::Args& a, dim3 grid, cudaStream_t st) {
-  return launch(&rotary::kernel<T, VEC>, grid, rotary::kThreads, 0, 1, st, a);
+  return launch(&rotary::rotary_kernel<T, VEC>, grid, rotary::kThreads, 0, 1, st, a);
 }
 
 int run_rotary(const nsa_rotary_desc* d, cudaStream_t st) {
