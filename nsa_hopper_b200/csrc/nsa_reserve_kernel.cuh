@@ -197,11 +197,12 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
   start_in_order();
   const int32_t r = (int32_t)(blockIdx.x * 256u + threadIdx.x);
   if (r >= a.n_rows) return;
-  const cache::Batch b = {a.pages, a.lens, a.cu, a.page_row, a.n_seqs, a.width, 0x7FFFFFFF, a.n_rows};
+  const cache::Batch b = {a.pages, a.lens, a.cu, a.page_row, a.n_seqs, a.width, 0, a.n_rows};
   const int s = cache::sequence_of(b, r);
   const int32_t pos = s >= 0 && a.lens[s] > 0 ? cache::position_of(b, s, r) : -1;
   if (a.positions != nullptr) a.positions[r] = pos;
-  if (a.slots != nullptr) a.slots[r] = pos < 0 ? -1 : slot_of(cache::page_of(b, s, pos / kPage), pos);
+  if (a.slots != nullptr)  // (a length that the first kernel has written lies in the table)
+    a.slots[r] = pos < 0 ? -1 : slot_of(a.pages[(int64_t)s * a.page_row + pos / kPage], pos);
 }
 
 }  // namespace reserve

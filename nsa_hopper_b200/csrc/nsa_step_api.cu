@@ -90,6 +90,18 @@ int run_reserve(const nsa_cache_reserve_desc* d, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ block selection
+int shift_of(int32_t block_size) { return block_size == 64 ? 6 : block_size == 128 ? 7 : 8; }
+// Tokens and blocks of a row, at most.
+int32_t most_tokens(const nsa_cache_select_desc* d) { return select::most_tokens(d->batch.width, d->cmp_block, d->cmp_stride); }
+int32_t most_blocks(const nsa_cache_select_desc* d) { return std::max(1, select::blocks_of(most_tokens(d), shift_of(d->block_size))); }
+// Blocks of a warp's unit: those of about 64 keys.
+int32_t unit_of(const nsa_cache_select_desc* d) {
+  const int64_t blocks = (int64_t)select::kUnitKeys * d->cmp_stride / d->block_size;
+  return (int32_t)std::min<int64_t>(std::max<int64_t>(blocks, 1), select::kUnitBlocks);
+}
+// Units of a row and KV head, at most.
+int64_t units_of(const nsa_cache_select_desc* d) { return ((int64_t)most_blocks(d) + unit_of(d) - 1) / unit_of(d); }
+
 int check_select(const nsa_cache_select_desc* d) {
   if (d == nullptr) return fail(NSA_ERR_INVALID_ARG, "desc is NULL");
   const int rc = cache::check_batch(&d->batch);
@@ -106,22 +118,14 @@ int check_select(const nsa_cache_select_desc* d) {
   if (d->block_size != 64 && d->block_size != 128 && d->block_size != 256)
     return fail(NSA_ERR_UNSUPPORTED, "block_size must be 64, 128 or 256");
   if (d->cmp_block <= 0 || d->cmp_stride <= 0) return fail(NSA_ERR_INVALID_ARG, "cmp_block and cmp_stride must be positive");
+  if (units_of(d) * b.heads_kv > kMaxIndex)
+    return fail(NSA_ERR_UNSUPPORTED, "heads_kv * (blocks of the longest sequence that the table holds) is too large");
   if (b.n_rows == 0) return NSA_OK;
   if (d->q == nullptr || d->sel == nullptr) return fail(NSA_ERR_INVALID_ARG, "q and sel must be non-NULL");
   if (misaligned(d->q, 16) || d->q_row_stride % 8 != 0 || d->q_head_stride % 8 != 0)
     return fail(NSA_ERR_INVALID_ARG, "q must be 16-byte aligned and its strides multiples of 8");
   if (misaligned(d->sel, 4)) return fail(NSA_ERR_INVALID_ARG, "sel must be aligned to its element size");
   return NSA_OK;
-}
-
-int shift_of(int32_t block_size) { return block_size == 64 ? 6 : block_size == 128 ? 7 : 8; }
-// Tokens and blocks of a row, at most.
-int32_t most_tokens(const nsa_cache_select_desc* d) { return select::most_tokens(d->batch.width, d->cmp_block, d->cmp_stride); }
-int32_t most_blocks(const nsa_cache_select_desc* d) { return std::max(1, select::blocks_of(most_tokens(d), shift_of(d->block_size))); }
-// Blocks of a warp's unit: those of about 64 keys.
-int32_t unit_of(const nsa_cache_select_desc* d) {
-  const int64_t blocks = (int64_t)select::kUnitKeys * d->cmp_stride / d->block_size;
-  return (int32_t)std::min<int64_t>(std::max<int64_t>(blocks, 1), select::kUnitBlocks);
 }
 
 template <int D>

@@ -311,7 +311,8 @@ def _select_desc(batch=None, **kw):
     ({}, dict(heads_q=0), -1), ({}, dict(heads_q=514), -2), ({}, dict(q_dtype=1), -1), ({}, dict(n_sel=0), -1), ({}, dict(n_sel=1025), -2),
     ({}, dict(block_size=96), -2), ({}, dict(cmp_block=0), -1), ({}, dict(cmp_stride=0), -1), ({}, dict(q=None), -1), ({}, dict(sel=None), -1),
     ({}, dict(q=P + 8), -1), ({}, dict(q_row_stride=4), -1), ({}, dict(q_head_stride=12), -1), ({}, dict(sel=P + 2), -1),
-    ({}, dict(workspace=None), -1), ({}, dict(workspace=P + 8), -1)])
+    ({}, dict(workspace=None), -1), ({}, dict(workspace=P + 8), -1),
+    (dict(heads_kv=16384, width=2**31 - 1, n_rows=1, n_seqs=1, d_qk=64, d_v=64), dict(heads_q=16384, cmp_stride=1), -2)])
 def test_select_refusals(batch, kw, code):
     assert _code("nsa_cache_select", _select_desc(batch, **kw)) == code and capi.last_error()
 
