@@ -21,11 +21,12 @@
 // 8 2^-24 Q; that of up to 258 keys 258 2^-24 Q.  All but the first are less than 90 2^-22 Q, and taken as 2^-15 Q.
 //
 // What bounds it.  A key costs 9/16 d bytes.  256 sequences of up to 65536 tokens, 4 heads of 128: 151 MB, which DRAM would
-// deliver in 24 us, take 64.  46 of them are score_kernel's: the ALU pipe, which converts codes (128 of its 400 instructions for
+// deliver in 24 us, take 56.  46 of them are score_kernel's: the ALU pipe, which converts codes (128 of its 400 instructions for
 // 64 keys), is its busiest unit at 59 %, tensor cores 19 %.  The others are pick_kernel's, 1024 blocks that are chains of
-// 9000 cycles (reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks 900).  One sequence of 65536 tokens:
-// 9.3 us; 64 of up to 32768: 17 us.  Tried: exact scores of all blocks with dot products of four bytes (select of the 256 above 102 us);
-// the bin from the threads' largest bounds instead of counts (2000 cycles and half as many candidates again).
+// steps (9000 cycles with 256 threads: reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks 900; 128
+// threads take longer, but 8 of their blocks fit an SM).  One sequence of 65536 tokens: 9.3 us; 64 of up to 32768: 17 us.  Tried:
+// exact scores of all blocks with dot products of four bytes (the 256 above 102 us); the bin from the threads' largest bounds
+// instead of counts (2000 cycles and half as many candidates again).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -49,9 +50,7 @@ constexpr int kUnitKeys = 64;     // keys of a unit, about
 constexpr int kUnitBlocks = 31;   // its blocks at most: a lane for each and one for the end
 constexpr int kMaxGroup = 256;    // query heads of a KV head
 constexpr int kMaxSel = 1024;
-constexpr int kPickThreads = 256;
-constexpr int kChecked = 8 * kPickThreads;  // blocks that pick_kernel looks at at a time
-constexpr int kBins = 4 * kPickThreads;
+__host__ __device__ constexpr int checked(int threads) { return 8 * threads; }  // blocks that pick_kernel looks at at a time
 constexpr int kAdded = 512;       // of them, those whose exact scores are compared with the best so far
 constexpr int kKeys = 512;        // places of keys that are scored between two meetings
 constexpr int kHeldPages = 256;   // first pages of a sequence, looked up beforehand
@@ -428,10 +427,9 @@ __device__ __forceinline__ int decode4(uint32_t codes) {
 // The sum of a (row, head)'s query heads as whole numbers of a power of two, so that the largest stays below 2^46, cut into six
 // signed bytes: values down to 2^-33 of the largest are exact in bf16 (2^-30 in fp16) with 16 heads, smaller ones off by less
 // than 2^-40 of it.  By all threads: kParts of them share the heads of two dims; the first kAhead of each are loaded beforehand.
-constexpr int kAhead = 4;
-template <int D>
+template <int D, int THREADS>
 struct Heads {
-  static constexpr int kParts = kPickThreads / (D / 2);
+  static constexpr int kParts = THREADS / (D / 2), kAhead = 1024 / THREADS;
   const uint16_t* q;
   int64_t step;
   int pair, part, n;  // n: heads of this thread
@@ -452,14 +450,14 @@ struct Heads {
     for (int i = kAhead; i < n; ++i) f(__ldcg(reinterpret_cast<const uint32_t*>(q + i * step)));
   }
 };
-template <int D>
-__device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const Heads<D>& heads) {
-  constexpr int kParts = Heads<D>::kParts;
+template <int D, int THREADS>
+__device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const Heads<D, THREADS>& heads) {
+  constexpr int kParts = Heads<D, THREADS>::kParts;
   const int tid = threadIdx.x, pair = heads.pair, part = heads.part;
   uint32_t top = 0;
   heads.each([&](uint32_t two) { top = __vmaxu2(top, two & 0x7FFF7FFFu); });
   if (tid == 0) w.top = 0;
-  for (int i = tid; i < 2 * D; i += kPickThreads) w.sum[0][i] = 0;
+  for (int i = tid; i < 2 * D; i += THREADS) w.sum[0][i] = 0;
   __syncthreads();
   top = __reduce_max_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16));
   if (tid % 32 == 0) atomicMax(&w.top, top);
@@ -482,13 +480,13 @@ __device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const 
 #pragma unroll
     for (int i = 0; i < 2; ++i) atomicAdd(&w.sum[0][2 * pair + i], upper[i]), atomicAdd(&w.sum[1][2 * pair + i], lower[i]);
   __syncthreads();
-  if (tid < D) {
-    int64_t x = (int64_t)w.sum[0][tid] * 4194304 + w.sum[1][tid];
+  for (int d = tid; d < D; d += THREADS) {
+    int64_t x = (int64_t)w.sum[0][d] * 4194304 + w.sum[1][d];
 #pragma unroll
     for (int l = 0; l < kLimbs; ++l) {
       const int8_t byte = (int8_t)x;
       x = (x - byte) >> 8;
-      reinterpret_cast<int8_t*>(&w.limb[tid / 16][l])[tid % 16] = byte;
+      reinterpret_cast<int8_t*>(&w.limb[d / 16][l])[d % 16] = byte;
     }
   }
   __syncthreads();
@@ -550,18 +548,18 @@ struct List {
   uint64_t* rank;
   uint32_t* index;
 };
-template <int D>
+template <int D, int THREADS>
 __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, bool fine, const Places& p, int seq, int head,
                                              const int32_t* pages, const uint16_t* blocks, int base, uint32_t n, const List& list,
                                              uint32_t at, double* scores) {
   const int tid = threadIdx.x, quarter = tid % 4;
   for (uint32_t e0 = 0; e0 < n; e0 += a.at_once) {
     const uint32_t some = min(n - e0, (uint32_t)a.at_once), places = some * a.keys;
-    for (uint32_t t0 = tid / 4; t0 - tid / 4 < places; t0 += kPickThreads / 2) {
+    for (uint32_t t0 = tid / 4; t0 - tid / 4 < places; t0 += THREADS / 2) {
       Quarter<D> k[2] = {};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t t = t0 + x * (kPickThreads / 4), e = t * a.per_key >> 20;  // t / a.keys
+        const uint32_t t = t0 + x * (THREADS / 4), e = t * a.per_key >> 20;  // t / a.keys
         // (two threads find where the block begins, two where it ends)
         const int32_t block = t < places ? base + blocks[e0 + e] : 0;
         const int32_t bound = first_key(p, block + quarter % 2);
@@ -576,10 +574,10 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, b
       dot<D>(w, k, quarter, score);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (quarter == x && t0 + x * (kPickThreads / 4) < places) scores[t0 + x * (kPickThreads / 4)] = score[x];
+        if (quarter == x && t0 + x * (THREADS / 4) < places) scores[t0 + x * (THREADS / 4)] = score[x];
     }
     __syncthreads();
-    for (uint32_t e = tid; e < some; e += kPickThreads) {
+    for (uint32_t e = tid; e < some; e += THREADS) {
       double score = 0.0;
       for (int j = 0; j < a.keys; ++j) score += scores[e * a.keys + j];
       list.rank[at + e0 + e] = rank_of(fine ? score : __longlong_as_double(0x7FF8000000000000ll));
@@ -609,17 +607,18 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
 // The bin of a bound: never a lower one for a larger bound.
-__device__ __forceinline__ int bin_of(float x, float low, float per) { return max(0, min(kBins - 1, (int)((x - low) * per))); }
+__device__ __forceinline__ int bin_of(float x, float low, float per, int bins) { return max(0, min(bins - 1, (int)((x - low) * per))); }
 
-template <int D>
-__global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
+template <int D, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
+  constexpr int kChecked = checked(THREADS), kBins = 4 * THREADS;
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Exact<D> w;
   __shared__ double scores[kKeys];
   __shared__ uint16_t found[kChecked];
   __shared__ int32_t pages[kHeldPages];
   __shared__ __align__(16) uint32_t count[kBins];
-  __shared__ uint32_t s_least[kPickThreads / 32], s_most[kPickThreads / 32], sums[kPickThreads / 32], s_bin, s_found;
+  __shared__ uint32_t s_least[THREADS / 32], s_most[THREADS / 32], sums[THREADS / 32], s_bin, s_found;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int size = list_size(a.n_sel);
   List list = {reinterpret_cast<uint64_t*>(dynamic), reinterpret_cast<uint32_t*>(dynamic + 16 * size)};
@@ -630,7 +629,7 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
   const int row = a.row0 + (int)(unit / a.hkv), head = (int)(unit % a.hkv);
   const float2* bounds = a.bounds + ((int64_t)a.row0 * a.hkv + unit) * a.blocks;
   int32_t* sel = a.sel + ((int64_t)a.row0 * a.hkv + unit) * a.n_sel;
-  const Heads<D> heads(a, row, head);
+  const Heads<D, THREADS> heads(a, row, head);
   const int seq = cache::sequence_by_32(
       a.b, row,
       [&](int lo, int step, int hi) {
@@ -640,26 +639,26 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
   const int32_t tokens = tokens_of(a.b, seq, row, a.most, LoadPastL1()), n = blocks_of(tokens, a.shift);
   const uint32_t wanted = min((uint32_t)a.n_sel, (uint32_t)n);
   const Places p = places_of(tokens, a.cmp_block, a.cmp_stride, a.shift);
-  for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += kPickThreads) pages[i] = cache::page_of(a.b, seq, i, LoadPastL1());
+  for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += THREADS) pages[i] = cache::page_of(a.b, seq, i, LoadPastL1());
   if (tid == 0) s_found = 0;
-  const bool finite = prepare_exact<D>(a, w, heads);
+  const bool finite = prepare_exact<D, THREADS>(a, w, heads);
   __syncthreads();
   wait_for_earlier();
   // (all of them: in a cu_seqlens out of order score_kernel may have taken the row for another sequence's)
-  for (int i = tid; i < a.n_sel; i += kPickThreads) sel[i] = -1;
+  for (int i = tid; i < a.n_sel; i += THREADS) sel[i] = -1;
   if (n == 0) return;
 
   uint32_t kept = 0;
   for (int i0 = 0;; i0 += kChecked) {
     // The lower bounds are counted in bins; the n_sel-th largest lies in bin `edge`, so a block whose upper bound is in a bin
-    // below that is none of the best.  (1024 bins: mostly one or two blocks too many.)
-    constexpr int kEach = kChecked / kPickThreads;
+    // below that is none of the best.  (256 threads have 1024 bins: mostly one or two blocks too many.)
+    constexpr int kEach = kChecked / THREADS;
     const int here = min(n - i0, kChecked);
     float2 x[kEach];
     uint32_t least = 0xFFFFFFFFu, most = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int i = j * kPickThreads + tid;
+      const int i = j * THREADS + tid;
       x[j] = i < here ? bounds[i0 + i] : make_float2(-kHuge, -kHuge);
     }
 #pragma unroll
@@ -673,17 +672,17 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
       reinterpret_cast<uint4*>(count)[tid] = make_uint4(0, 0, 0, 0);
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kPickThreads / 32; ++i) least = min(least, s_least[i]), most = max(most, s_most[i]);
+      for (int i = 0; i < THREADS / 32; ++i) least = min(least, s_least[i]), most = max(most, s_most[i]);
       if (least < most) {
         low = unordered(least);
         per = (float)kBins / (unordered(most) - low);  // (0 if that is beyond fp32: one bin)
       }
 #pragma unroll
       for (int j = 0; j < kEach; ++j)
-        if (j * kPickThreads + tid < here) atomicAdd(&count[bin_of(x[j].x, low, per)], 1u);
+        if (j * THREADS + tid < here) atomicAdd(&count[bin_of(x[j].x, low, per, kBins)], 1u);
       __syncthreads();
       // four bins of a thread, the largest first
-      const uint4 c = reinterpret_cast<const uint4*>(count)[kPickThreads - 1 - tid];
+      const uint4 c = reinterpret_cast<const uint4*>(count)[THREADS - 1 - tid];
       const uint32_t mine = c.x + c.y + c.z + c.w;
       uint32_t upto = mine;
 #pragma unroll
@@ -695,9 +694,9 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
       __syncthreads();
       uint32_t at = upto - mine;
 #pragma unroll
-      for (int i = 0; i < kPickThreads / 32; ++i) at += i < warp ? sums[i] : 0;
+      for (int i = 0; i < THREADS / 32; ++i) at += i < warp ? sums[i] : 0;
       if (at < wanted && wanted <= at + mine) {
-        const int bin = 4 * (kPickThreads - 1 - tid);
+        const int bin = 4 * (THREADS - 1 - tid);
         s_bin = wanted <= at + c.w ? bin + 3 : wanted <= at + c.w + c.z ? bin + 2 : wanted <= at + c.w + c.z + c.y ? bin + 1 : bin;
       }
       __syncthreads();
@@ -705,8 +704,8 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
     }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int i = j * kPickThreads + tid;
-      if (i < here && bin_of(x[j].y, low, per) >= edge) found[atomicAdd(&s_found, 1u)] = (uint16_t)i;
+      const int i = j * THREADS + tid;
+      if (i < here && bin_of(x[j].y, low, per, kBins) >= edge) found[atomicAdd(&s_found, 1u)] = (uint16_t)i;
     }
     __syncthreads();
 
@@ -714,10 +713,10 @@ __global__ void __launch_bounds__(kPickThreads, 3) pick_kernel(const Args a) {
     const uint32_t n_found = s_found;
     for (uint32_t f0 = 0;;) {
       const uint32_t some = min(n_found - f0, (uint32_t)kAdded), in = kept + some;
-      score_blocks<D>(a, w, finite, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
+      score_blocks<D, THREADS>(a, w, finite, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
       f0 += some;
       const bool whole = f0 == n_found, last = whole && i0 + kChecked >= n;
-      for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += kPickThreads / 8) {  // 8 threads for an entry
+      for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += THREADS / 8) {  // 8 threads for an entry
         const uint32_t e = min(e0, in - 1);
         const uint64_t key = list.rank[e];
         const uint32_t block = list.index[e];

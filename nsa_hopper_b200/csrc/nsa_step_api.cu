@@ -128,13 +128,20 @@ int check_select(const nsa_cache_select_desc* d) {
   return NSA_OK;
 }
 
+template <int D, int THREADS, int PER_SM>
+int launch_pick(const select::Args& a, int dev, uint32_t bit, cudaStream_t st) {
+  const auto kernel = &select::pick_kernel<D, THREADS, PER_SM>;
+  const int rc = allow_smem(reinterpret_cast<const void*>(kernel), select::list_bytes(select::kMaxSel), dev, bit);
+  if (rc != NSA_OK) return rc;
+  const cudaError_t e = launch(kernel, dim3((unsigned)(a.rows * a.hkv)), THREADS, select::list_bytes(a.n_sel), 1, st, a);
+  return e == cudaSuccess ? NSA_OK : done(e, "cache selection launch");
+}
+
 template <int D>
 int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t st) {
-  const int list = select::list_bytes(a.n_sel), fixed = (int)sizeof(select::ScoreWarp<D>) * select::warps_of(D);
-  const uint32_t bit = D == 64 ? 2u : D == 128 ? 8u : 32u;
+  const int fixed = (int)sizeof(select::ScoreWarp<D>) * select::warps_of(D);
+  const uint32_t bit = D == 64 ? 2u : D == 128 ? 16u : 128u;  // (three kernels each)
   int rc = allow_smem(reinterpret_cast<const void*>(&select::score_kernel<D>), fixed + select::kMaxRows * 12 + 4, dev, bit);
-  if (rc == NSA_OK)
-    rc = allow_smem(reinterpret_cast<const void*>(&select::pick_kernel<D>), select::list_bytes(select::kMaxSel), dev, 2 * bit);
   if (rc != NSA_OK) return rc;
   const int64_t units = (a.blocks + a.unit - 1) / a.unit;  // of a row and KV head
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(select::kMaxRows, kMaxIndex / (units * a.hkv)));
@@ -146,8 +153,15 @@ int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t 
     const int64_t grid = std::min<int64_t>(sm, (units * a.hkv * a.rows + 1) / 2);
     cudaError_t e = launch(&select::score_kernel<D>, dim3((unsigned)grid), select::warps_of(D) * 32, fixed + a.rows * 12 + 4, 1, st, a);
     if (e != cudaSuccess) return done(e, "cache selection's score launch");
-    e = launch(&select::pick_kernel<D>, dim3((unsigned)(a.rows * a.hkv)), select::kPickThreads, list, 1, st, a);
-    if (e != cudaSuccess) return done(e, "cache selection launch");
+    // A block's chain of steps takes longer with 128 threads than with 256, but less of it is spent in waiting for one another: where
+    // the blocks are more than fit at once, 8 small ones an SM win (256 sequences of up to 65536 tokens, 4 heads: 56 us
+    // against 64; 400 of up to 8192: 34 against 41), else 3 large ones (64 of up to 32768: 17 against 23).  They are even at
+    // 4 to 6 an SM.  The small ones look at 1024 of a row's blocks at a time, and a second look costs more than they gain (200
+    // sequences of up to 131072: 84 against 75).
+    const int32_t covered = (a.most - a.cmp_block + 1) >> a.shift;  // (by whole pages of keys; a.blocks may be one or a few more)
+    const bool many = (int64_t)a.rows * a.hkv > 5 * (int64_t)sm && covered <= select::checked(128);
+    rc = many ? launch_pick<D, 128, 8>(a, dev, 4 * bit, st) : launch_pick<D, 256, 3>(a, dev, 2 * bit, st);
+    if (rc != NSA_OK) return rc;
   }
   return done(cudaSuccess, "");
 }
@@ -182,7 +196,7 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.q_half = d->q_dtype == NSA_DTYPE_F16;
   a.bits = 46;  // (the sum of the heads, in six signed bytes)
   while ((1 << (46 - a.bits)) < a.group) --a.bits;
-a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
+  a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
   a.per_key = ((1u << 20) + a.keys - 1) / a.keys;
   a.at_once = select::kKeys / a.keys;
   if (b.d_qk == 64) return launch_select<64>(a, b.n_rows, sm, dev, st);

@@ -449,6 +449,22 @@ def test_select_most_blocks_and_heads():
     _check_select(torch.randn(rows, 2, 64, generator=g).to(torch.bfloat16), cache, pages, lens, 6)
 
 
+@pytest.mark.parametrize("dims", DIMS[:3])
+@pytest.mark.parametrize("hq,n_sel,l_prime", [(8, 16, 64), (24, 700, 64), (40, 5, 128)])
+def test_select_of_many_rows(dims, hq, n_sel, l_prime):
+    """More rows and KV heads than fit the GPU at once, up to 1024 blocks a row, of them equal ones and some of no number."""
+    rng, g = np.random.default_rng(dims[0] + hq), torch.Generator().manual_seed(dims[0] + hq)
+    lens = np.concatenate([rng.integers(0, 3000, 127), [65536 if l_prime == 64 else 40001, 0]])
+    pages, count = _tables(lens[-2:], 32, 16, rng)
+    pages = np.stack([np.roll(pages[0], r) for r in range(len(lens))])
+    x = torch.randn(count, 8, 64, dims[0], generator=g)
+    x[:, 6] = x[:1, 6, :1]
+    x[1, 7, 5, 3] = math.nan
+    q = torch.randn(len(lens), hq, dims[0], generator=g).to(torch.bfloat16)
+    q[3, 0, 0] = math.inf
+    _check_select(q, _records(x, dims[1]), pages, lens, n_sel, l_prime)
+
+
 def test_select_strides_streams_and_refusals():
     g = torch.Generator().manual_seed(10)
     lens = [3000, 2500]
