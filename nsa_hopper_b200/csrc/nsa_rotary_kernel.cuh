@@ -9,11 +9,14 @@
 // taken in fp32.  Products and sums are fp32, rounded once to the output's type.
 //
 // What bounds it: DRAM, 2 bytes in and 2 out a value of 16 bits.  A block has a token with all its heads, Q's and K's in one
-// launch: its angles are computed once, in shared memory, where all heads read them.  Any strides come in and go out, so that
-// [B, T, H, d], as projections write it, becomes the [B, H, T, d] that the attention reads on the way.  65536 tokens of 64 + 4 heads
-// of 128 in bf16: 362 us, 6.3 TB/s, 0.98 of the measured copy rate.  What brought it there was few registers: with four words a
-// thread in flight and 127 registers it took 574 us, with two and 64 430, with one and 32 (8 blocks an SM) 358.  Tokens
-// together in a block (2, 4, 8, 16) gave nothing, streaming loads took 398, streaming stores 379.
+// launch: its angles are computed once, in shared memory, where all heads read them; of few heads, which have no work for a block,
+// it has several tokens.  Any strides come in and go out, so that [B, T, H, d], as projections write it, becomes the
+// [B, H, T, d] that the attention reads on the way.  65536 tokens of 64 + 4 heads of 128 in bf16: 347 us, 6.6 TB/s, the measured
+// copy rate.  What brought it there was few registers: with four words a thread in flight and 127 registers it took 574 us,
+// with two and 64 430, with one and 32 (8 blocks an SM) 358, and with the outgoing address computed before the words are loaded
+// 347.  There tokens together in a block (2, 4, 8, 16) gave nothing, streaming loads took 398, streaming stores 379.  Rotary parts
+// that no words of 8 bytes fit are bound by instructions (36 of 128 values in bf16: 170 us for 88 us of copying; wider words for
+// the values beside them alone gave nothing).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -25,7 +28,8 @@ namespace nsa {
 namespace rotary {
 
 constexpr int kMaxPairs = 128;  // of a head of 256 values
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // of a block, at most
+constexpr int kAngles = 1024;   // of a block of several tokens, at most: they fill 8 KB of shared memory
 
 struct Tensor {
   const void* x;
@@ -39,7 +43,9 @@ struct Args {
   int32_t heads, first;          // of both tensors together, of the first one
   int32_t batch, tokens;         // tokens of a batch entry
   int32_t offset, pairs, rest;   // first value and pairs of the rotary part; values beside it
+  int32_t total;                 // tokens of all batch entries
   int32_t heads_block;           // heads of a block
+  int32_t tokens_block;          // tokens of a block
   int32_t interleaved;
   uint32_t flip;                 // sign bit of the sines
   uint64_t turn[kMaxPairs];      // inv_freq / 2 pi in units of 2^-64
@@ -98,26 +104,52 @@ __device__ __forceinline__ int place(int pair, int items) {
   return ((e / 2) * items + k) * 2 + e % 2;
 }
 
-// A block turns a.heads_block heads of one token.
-template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads, 2048 / kThreads) rotary_kernel(const __grid_constant__ Args a) {
+// What lies in the parameters, as memory: the constant cache serves one address of a warp at a time.
+template <class T>
+__device__ __forceinline__ const T* as_memory(const T* p) {
+  asm("mov.b64 %0, %0;" : "+l"(p));
+  return p;
+}
+
+// A block turns a.heads_block heads of one token, or (SEVERAL) all heads of a.tokens_block tokens, an item each thread.
+template <class T, int VEC, bool SEVERAL>
+__global__ void __launch_bounds__(kThreads, SEVERAL ? 6 : 8) rotary_kernel(const __grid_constant__ Args a) {
   using W = typename Word<VEC * (int)sizeof(T)>::type;
-  __shared__ __align__(16) float2 angles[kMaxPairs];
+  extern __shared__ __align__(16) float2 angles[];  // [a.tokens_block, a.pairs]
   const int tid = threadIdx.x;
-  const int b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens;
-  const int h0 = blockIdx.y * a.heads_block, h1 = min(h0 + a.heads_block, a.heads);
+  const int h0 = SEVERAL ? 0 : blockIdx.y * a.heads_block, h1 = SEVERAL ? a.heads : min(h0 + a.heads_block, a.heads);
   const int turning = a.pairs / VEC;                                // items of a head that turn 2 VEC values
   const int items = turning + (a.rest + 2 * VEC - 1) / (2 * VEC);   // and those that copy as many
-  start_in_order();
-  if (tid < a.pairs) {
-    const int64_t pos = a.pos[a.axis[tid] * a.ps[0] + b * a.ps[1] + t * a.ps[2]];
-    angles[place<VEC>(tid, turning)] = cos_sin((uint64_t)pos * a.turn[tid], a.flip);
+  const int first = blockIdx.x * (SEVERAL ? a.tokens_block : 1);
+  if constexpr (!SEVERAL) {
+    const uint64_t turn = tid < a.pairs ? a.turn[tid] : 0;
+    start_in_order();
+    if (tid < a.pairs) {
+      const int b = first / a.tokens, t = first - b * a.tokens;
+      const int64_t pos = a.pos[a.axis[tid] * a.ps[0] + b * a.ps[1] + t * a.ps[2]];
+      angles[place<VEC>(tid, turning)] = cos_sin((uint64_t)pos * turn, a.flip);
+    }
+  } else {
+    // (a thread keeps its pair; q and k of one head, 65536 tokens: 28 us, and 35 with the pairs from the constant cache)
+    const int at_once = blockDim.x / a.pairs, pair = tid % a.pairs;
+    const uint64_t turn = as_memory(a.turn)[pair];
+    const int axis = as_memory(a.axis)[pair];
+    start_in_order();
+    for (int token = tid / a.pairs; token < a.tokens_block && tid < at_once * a.pairs; token += at_once) {
+      const int g = min(first + token, a.total - 1), b = g / a.tokens, t = g - b * a.tokens;
+      const int64_t pos = a.pos[axis * a.ps[0] + b * a.ps[1] + t * a.ps[2]];
+      angles[token * a.pairs + place<VEC>(pair, turning)] = cos_sin((uint64_t)pos * turn, a.flip);
+    }
   }
   __syncthreads();
 
   // item and head of a thread's next item, stepped without divisions
-  int item = tid % items, head = h0 + tid / items;
-  const int step = kThreads % items, steps = kThreads / items;
+  const int token = SEVERAL ? tid / (items * a.heads) : 0;
+  if (SEVERAL && (token >= a.tokens_block || first + token >= a.total)) return;
+  const int of_token = SEVERAL ? tid - token * (items * a.heads) : tid;
+  const int b = (first + token) / a.tokens, t = first + token - b * a.tokens;
+  int item = of_token % items, head = h0 + of_token / items;
+  const int step = SEVERAL ? 0 : blockDim.x % items, steps = SEVERAL ? a.heads : blockDim.x / items;
   for (; head < h1; item += step, head += steps) {
     if (item >= items) {
       item -= items;
@@ -138,13 +170,14 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) rotary_kernel(const
     const Tensor& x = a.t[q ? 0 : 1];
     const int h = q ? head : head - a.first;
     const T* src = static_cast<const T*>(x.x) + (b * x.xs[0] + h * x.xs[1] + t * x.xs[2]) + at;
+    T* dst = static_cast<T*>(x.y) + (b * x.ys[0] + h * x.ys[1] + t * x.ys[2]) + at;
     W lo = *reinterpret_cast<const W*>(src), hi = *reinterpret_cast<const W*>(src + second);
     if (item < turning) {
       alignas(16) T v[2 * VEC];
       *reinterpret_cast<W*>(v) = lo;
       *reinterpret_cast<W*>(v + VEC) = hi;
       float2 cs[VEC];
-      const float2* mine = angles + (VEC == 1 ? 1 : 2) * item;
+      const float2* mine = angles + token * a.pairs + (VEC == 1 ? 1 : 2) * item;
       if constexpr (VEC == 1) {
         cs[0] = mine[0];
       } else {
@@ -164,7 +197,6 @@ __global__ void __launch_bounds__(kThreads, 2048 / kThreads) rotary_kernel(const
       lo = *reinterpret_cast<const W*>(v);
       hi = *reinterpret_cast<const W*>(v + VEC);
     }
-    T* dst = static_cast<T*>(x.y) + (b * x.ys[0] + h * x.ys[1] + t * x.ys[2]) + at;
     *reinterpret_cast<W*>(dst) = lo;
     if (second != 0) *reinterpret_cast<W*>(dst + second) = hi;
   }

@@ -240,8 +240,9 @@ int check_rotary(const nsa_rotary_desc* d) {
 }
 
 template <class T, int VEC>
-cudaError_t launch_rotary(const rotary::Args& a, dim3 grid, cudaStream_t st) {
-  return launch(&rotary::rotary_kernel<T, VEC>, grid, rotary::kThreads, 0, 1, st, a);
+cudaError_t launch_rotary(const rotary::Args& a, dim3 grid, int threads, int smem, cudaStream_t st) {
+  if (a.tokens_block > 1) return launch(&rotary::rotary_kernel<T, VEC, true>, grid, threads, smem, 1, st, a);
+  return launch(&rotary::rotary_kernel<T, VEC, false>, grid, threads, smem, 1, st, a);
 }
 
 int run_rotary(const nsa_rotary_desc* d, cudaStream_t st) {
@@ -278,27 +279,37 @@ int run_rotary(const nsa_rotary_desc* d, cudaStream_t st) {
   a.flip = d->inverse ? 0x80000000u : 0u;
   memcpy(a.turn, d->turns, sizeof(uint64_t) * d->pairs);
   if (d->axis != nullptr) memcpy(a.axis, d->axis, d->pairs);
-  // A block has a token; where tokens are few, its heads are shared out among blocks.
+  // A block has a token; where tokens are few, its heads are shared out among blocks.  Where they are more than are turned at once,
+  // a block has as many threads as its turns need (16384 tokens of 32 + 8 heads of 128 in bf16: 56 us, and 61 with 256), and as
+  // many tokens as they have room for (10 heads of 64: 12 us, and 24 with one; 2 of 128 and 65536 tokens: 28 and 90).  Where all
+  // are turned at once more threads are faster (1024 tokens of 68 heads: 7.4 us with 256, 8.2 with the 192 that they need).
   const int items = a.pairs / vec + (a.rest + 2 * vec - 1) / (2 * vec);
   const int64_t most = ((int64_t)a.heads * items + rotary::kThreads - 1) / rotary::kThreads;
   const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * sm / total), most);
   a.heads_block = (int32_t)((a.heads + parts - 1) / parts);
-  const dim3 grid((unsigned)total, (unsigned)((a.heads + a.heads_block - 1) / a.heads_block));
+  a.total = (int32_t)total;
+  const int64_t work = (int64_t)a.heads_block * items, turns = (work + rotary::kThreads - 1) / rotary::kThreads;
+  const bool many = total > 8 * sm;
+  a.tokens_block = (int32_t)std::max<int64_t>(1, std::min({rotary::kThreads / work, rotary::kAngles / (int64_t)a.pairs, total / (2 * sm)}));
+  const int64_t needed = std::max<int64_t>((work * a.tokens_block + turns - 1) / turns, a.pairs);
+  const int threads = many || a.tokens_block > 1 ? (int)((needed + 31) / 32 * 32) : rotary::kThreads;
+  const int smem = a.tokens_block * a.pairs * (int)sizeof(float2);
+  const dim3 grid((unsigned)((total + a.tokens_block - 1) / a.tokens_block), (unsigned)((a.heads + a.heads_block - 1) / a.heads_block));
   cudaError_t e;
   if (d->dtype == NSA_DTYPE_F32) {
-    e = vec == 4   ? launch_rotary<float, 4>(a, grid, st)
-        : vec == 2 ? launch_rotary<float, 2>(a, grid, st)
-                   : launch_rotary<float, 1>(a, grid, st);
+    e = vec == 4   ? launch_rotary<float, 4>(a, grid, threads, smem, st)
+        : vec == 2 ? launch_rotary<float, 2>(a, grid, threads, smem, st)
+                   : launch_rotary<float, 1>(a, grid, threads, smem, st);
   } else if (d->dtype == NSA_DTYPE_F16) {
-    e = vec == 8   ? launch_rotary<__half, 8>(a, grid, st)
-        : vec == 4 ? launch_rotary<__half, 4>(a, grid, st)
-        : vec == 2 ? launch_rotary<__half, 2>(a, grid, st)
-                   : launch_rotary<__half, 1>(a, grid, st);
+    e = vec == 8   ? launch_rotary<__half, 8>(a, grid, threads, smem, st)
+        : vec == 4 ? launch_rotary<__half, 4>(a, grid, threads, smem, st)
+        : vec == 2 ? launch_rotary<__half, 2>(a, grid, threads, smem, st)
+                   : launch_rotary<__half, 1>(a, grid, threads, smem, st);
   } else {
-    e = vec == 8   ? launch_rotary<__nv_bfloat16, 8>(a, grid, st)
-        : vec == 4 ? launch_rotary<__nv_bfloat16, 4>(a, grid, st)
-        : vec == 2 ? launch_rotary<__nv_bfloat16, 2>(a, grid, st)
-                   : launch_rotary<__nv_bfloat16, 1>(a, grid, st);
+    e = vec == 8   ? launch_rotary<__nv_bfloat16, 8>(a, grid, threads, smem, st)
+        : vec == 4 ? launch_rotary<__nv_bfloat16, 4>(a, grid, threads, smem, st)
+        : vec == 2 ? launch_rotary<__nv_bfloat16, 2>(a, grid, threads, smem, st)
+                   : launch_rotary<__nv_bfloat16, 1>(a, grid, threads, smem, st);
   }
   return done(e, "rotary launch");
 }

@@ -197,6 +197,24 @@ def test_rotary_heads_of_any_strides(batch, tokens, dtype):
     assert torch.equal(shared, want[:, :1].expand(batch, 5, tokens, 64))
 
 
+@pytest.mark.parametrize("hq,hkv", [(1, 0), (2, 1), (7, 1)])
+@pytest.mark.parametrize("d,dim,offset,dtype", [(64, 64, 0, torch.bfloat16), (72, 36, 36, torch.float32), (128, 14, 2, torch.float16),
+                                                (256, 256, 0, torch.bfloat16)])
+def test_rotary_few_heads_and_many_tokens(hq, hkv, d, dim, offset, dtype):
+    """Several tokens a block: bit for bit what calls of a few tokens give, with a last block that is not full."""
+    g = torch.Generator(device="cuda").manual_seed(d + hq)
+    plan = ops.rotary_plan(d, rotary_dim=dim, offset=offset, sections=(dim // 2 - 2, 2))
+    for batch, tokens in [(1, 593), (3, 1999), (2, 9001)]:
+        q, k = (torch.randn(batch, tokens, h, d, generator=g, device="cuda").to(dtype).transpose(1, 2) if h else None for h in (hq, hkv))
+        pos = torch.randint(-2**31, 2**31 - 1, (2, batch, tokens), generator=g, device="cuda", dtype=torch.int32)
+        got = ops.rotary(q, k, pos, plan)
+        for b in range(batch):
+            for t in range(0, tokens, 290):
+                part = [None if x is None else x[b:b + 1, :, t:t + 290] for x in (q, k)]
+                for x, y in zip(got, ops.rotary(*part, pos[:, b:b + 1, t:t + 290], plan)):
+                    assert (x is None and y is None) or torch.equal(x[b:b + 1, :, t:t + 290], y)
+
+
 def test_rotary_empty_and_refusals():
     plan, p = ops.rotary_plan(64), torch.zeros(0, **I32)
     q = torch.zeros(0, 4, 64, device="cuda")
