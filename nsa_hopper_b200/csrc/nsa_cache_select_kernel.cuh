@@ -188,6 +188,7 @@ template <int D>
 struct Stage {
   static constexpr int kScaleAt = kUnitKeys * D / 2, kBytes = kUnitKeys * D * 9 / 16;
 };
+static_assert(kUnitKeys == 64 && kUnitKeys == kPage, "fetch copies, and score_kernel's four tiles read, 64 keys of two pages at most");
 template <int D>
 struct ScoreWarp {
   uint8_t stage[kStages][Stage<D>::kBytes];

@@ -483,6 +483,20 @@ def test_select_of_many_rows(dims, hq, n_sel, l_prime):
     _check_select(q, _records(x, dims[1]), pages, lens, n_sel, l_prime)
 
 
+def test_select_of_many_rows_whose_last_block_has_no_page():
+    """1024 blocks of whole pages and the tokens behind them, which the last compressed key covers, in one block more."""
+    rng, g = np.random.default_rng(12), torch.Generator().manual_seed(12)
+    lens = np.concatenate([[65567, 65537, 65568, 65536], rng.integers(0, 900, 200)])
+    pages, count = _tables([65536], 32, 16, rng)
+    pages = np.repeat(pages, len(lens), 0)
+    assert pages.shape[1] == 64
+    cache = _records(torch.randn(count, 4, 64, 64, generator=g), 64)
+    q = torch.randn(len(lens), 4, 64, generator=g).to(torch.float16)
+    for n_sel in (16, 600):
+        want = _check_select(q, cache, pages, lens, n_sel)
+        assert (want[:2, :, :n_sel] >= 0).all() and (want[2] == -1).all()
+
+
 def test_select_strides_streams_and_refusals():
     g = torch.Generator().manual_seed(10)
     lens = [3000, 2500]
