@@ -12,7 +12,8 @@
 //   * pick_kernel finds a bound that n_sel blocks are certain to reach, and computes the scores of all blocks that may reach
 //     it, mostly n_sel and one or two more, in 64 bits from exact parts: codes (doubled) are whole numbers up to 12, the query
 //     is cut into whole numbers too (prepare_exact), the 16 products of a group that share a scale are added as integers
-//     (dot products of four bytes), and only scale times group sum is rounded, in fp64.
+//     (dot products of four bytes), and only scale times group sum is rounded, in fp64.  A query whose channels are too far apart
+//     for that keeps its sums in fp64, and so are its products.
 //
 // Error of the approximation, in units of max|k| (six times the largest scale of a unit's keys) times the keys of a block, with
 // S = sum over d and heads of |q| and Q = sum over d of |sum of the heads|: the fp32 sum of G heads (G - 1) 2^-24 S; the two
@@ -403,9 +404,14 @@ struct Exact {
   int4 limb[D / 16][kLimbs + 1];  // bytes of the query, the lowest first, of the 16 dims of a group, four to a word (and room
                                   // that puts what the threads of a key read at once into different banks)
   int2 start[D / 16];             // what the sums of a group begin with: 12 of every code too many, taken off
-  int32_t sum[2][D];              // of the heads: whole parts and fractions
+  union {
+    int32_t sum[2][D];            // of the heads: whole parts and fractions
+    double wide[D];               // the sum itself, where the bytes do not hold it
+  };
   uint32_t top;
 };
+// What a (row, head)'s exact scores are made from: nothing (a value of the query is no number), whole numbers, fp64.
+enum class Query { kNone, kWhole, kWide };
 
 // fp64 of an integer, without a conversion: its bits in the mantissa of 2^52 + 2^31 + x.
 __device__ __forceinline__ double whole(int32_t x) {
@@ -426,8 +432,9 @@ __device__ __forceinline__ int decode4(uint32_t codes) {
 }
 
 // The sum of a (row, head)'s query heads as whole numbers of a power of two, so that the largest stays below 2^46, cut into six
-// signed bytes: values down to 2^-33 of the largest are exact in bf16 (2^-30 in fp16) with 16 heads, smaller ones off by less
-// than 2^-40 of it.  By all threads: kParts of them share the heads of two dims; the first kAhead of each are loaded beforehand.
+// signed bytes.  With 16 heads that holds all values from 2^-34 of the largest on in bf16 (8 bits of 42), and every fp16 number.
+// Where a value does not fit (channels that are further apart), the sum is kept in fp64 instead.  By all threads: kParts of them
+// share the heads of two dims; the first kAhead of each are loaded beforehand.
 template <int D, int THREADS>
 struct Heads {
   static constexpr int kParts = THREADS / (D / 2), kAhead = 1024 / THREADS;
@@ -452,7 +459,7 @@ struct Heads {
   }
 };
 template <int D, int THREADS>
-__device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const Heads<D, THREADS>& heads) {
+__device__ __forceinline__ Query prepare_exact(const Args& a, Exact<D>& w, const Heads<D, THREADS>& heads) {
   constexpr int kParts = Heads<D, THREADS>::kParts;
   const int tid = threadIdx.x, pair = heads.pair, part = heads.part;
   uint32_t top = 0;
@@ -464,23 +471,38 @@ __device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const 
   if (tid % 32 == 0) atomicMax(&w.top, top);
   __syncthreads();
   top = w.top;
-  if (top >= (a.q_half ? 0x7C00u : 0x7F80u)) return false;
+  if (top >= (a.q_half ? 0x7C00u : 0x7F80u)) return Query::kNone;
   // x 2^up: below 2^(bits - 22), its fraction to 22 bits
   const int up = a.bits - 22 + 126 - max((int)(__float_as_uint(query_value(a, top)) >> 23), 1);
   const float up0 = __uint_as_float((uint32_t)(127 + up / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
   int32_t upper[2] = {}, lower[2] = {};
+  bool fits = true;
   heads.each([&](uint32_t two) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float x = query_value(a, i == 0 ? two & 0xFFFFu : two >> 16) * up0 * up1, whole_part = rintf(x);
+      const float value = query_value(a, i == 0 ? two & 0xFFFFu : two >> 16);
+      const float x = value * up0 * up1, whole_part = rintf(x), rest = (x - whole_part) * 4194304.0f;
+      const int fraction = __float2int_rn(rest);
       upper[i] += (int)whole_part;
-      lower[i] += __float2int_rn((x - whole_part) * 4194304.0f);
+      lower[i] += fraction;
+      fits = fits && (float)fraction == rest && (x != 0.0f || value == 0.0f);
     }
   });
   if (part < kParts)
 #pragma unroll
     for (int i = 0; i < 2; ++i) atomicAdd(&w.sum[0][2 * pair + i], upper[i]), atomicAdd(&w.sum[1][2 * pair + i], lower[i]);
-  __syncthreads();
+  if (__syncthreads_or(!fits)) {
+    if (part == 0) {  // (one thread for two dims, so that the heads are added in their order)
+      double sum[2] = {0.0, 0.0};
+#pragma unroll 1
+      for (int g = 0; g < a.group; ++g) {
+        const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(heads.q + g * a.q_head));
+        sum[0] += (double)query_value(a, two & 0xFFFFu), sum[1] += (double)query_value(a, two >> 16);
+      }
+      w.wide[2 * pair] = sum[0], w.wide[2 * pair + 1] = sum[1];
+    }
+    return Query::kWide;
+  }
   for (int d = tid; d < D; d += THREADS) {
     int64_t x = (int64_t)w.sum[0][d] * 4194304 + w.sum[1][d];
 #pragma unroll
@@ -501,7 +523,7 @@ __device__ __forceinline__ bool prepare_exact(const Args& a, Exact<D>& w, const 
     }
     w.start[tid] = make_int2((start[2] * 256 + start[1]) * 256 + start[0], (start[5] * 256 + start[4]) * 256 + start[3]);
   }
-  return true;  // (the caller meets before the sums are read)
+  return Query::kWhole;  // (the caller meets before the sums are read)
 }
 
 // Scores of two keys, by four threads, each with a quarter of both; all of them get them.
@@ -543,6 +565,32 @@ __device__ __forceinline__ void dot(const Exact<D>& w, const Quarter<D> (&k)[2],
   }
 }
 
+// The same from the sums in fp64.
+template <int D>
+__device__ __forceinline__ void dot_wide(const Exact<D>& w, const Quarter<D> (&k)[2], int quarter, double (&x)[2]) {
+  x[0] = x[1] = 0.0;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) {
+    const double* q = w.wide + (quarter * (D / 64) + j) * 16;
+    double sum[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int four = decode4(k[y].code[2 * j + i / 2] >> i % 2 * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[y] = fma(q[4 * i + e], whole((four >> 8 * e & 255) - 12), sum[y]);
+      }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) x[y] = fma(scale_of(k[y].scale >> 8 * j & 255u), sum[y], x[y]);
+  }
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    x[y] += __shfl_xor_sync(0xFFFFFFFFu, x[y], 1);
+    x[y] += __shfl_xor_sync(0xFFFFFFFFu, x[y], 2);
+  }
+}
+
 // Adds `n` blocks with their scores to a list, by all threads.  Each block has a.keys places, four threads score the keys of two
 // places, and one sums those of a block, in their order.
 struct List {
@@ -550,7 +598,7 @@ struct List {
   uint32_t* index;
 };
 template <int D, int THREADS>
-__device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, bool fine, const Places& p, int seq, int head,
+__device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, Query query, const Places& p, int seq, int head,
                                              const int32_t* pages, const uint16_t* blocks, int base, uint32_t n, const List& list,
                                              uint32_t at, double* scores) {
   const int tid = threadIdx.x, quarter = tid % 4;
@@ -572,7 +620,8 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, b
           load_quarter<D>(k[x], rec + quarter * (D / 8), rec + cache::k_scale_at(D) + quarter * (D / 64), i % kPage);
       }
       double score[2];  // (0 of a place without a key, and of a key of no page)
-      dot<D>(w, k, quarter, score);
+      if (query == Query::kWide) dot_wide<D>(w, k, quarter, score);
+      else dot<D>(w, k, quarter, score);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
         if (quarter == x && t0 + x * (THREADS / 4) < places) scores[t0 + x * (THREADS / 4)] = score[x];
@@ -581,7 +630,7 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, b
     for (uint32_t e = tid; e < some; e += THREADS) {
       double score = 0.0;
       for (int j = 0; j < a.keys; ++j) score += scores[e * a.keys + j];
-      list.rank[at + e0 + e] = rank_of(fine ? score : __longlong_as_double(0x7FF8000000000000ll));
+      list.rank[at + e0 + e] = rank_of(query != Query::kNone ? score : __longlong_as_double(0x7FF8000000000000ll));
       list.index[at + e0 + e] = (uint32_t)(base + blocks[e0 + e]);
     }
     __syncthreads();
@@ -642,7 +691,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
   const Places p = places_of(tokens, a.cmp_block, a.cmp_stride, a.shift);
   for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += THREADS) pages[i] = cache::page_of(a.b, seq, i, LoadPastL1());
   if (tid == 0) s_found = 0;
-  const bool finite = prepare_exact<D, THREADS>(a, w, heads);
+  const Query query = prepare_exact<D, THREADS>(a, w, heads);
   __syncthreads();
   wait_for_earlier();
   // (all of them: in a cu_seqlens out of order score_kernel may have taken the row for another sequence's)
@@ -714,7 +763,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
     const uint32_t n_found = s_found;
     for (uint32_t f0 = 0;;) {
       const uint32_t some = min(n_found - f0, (uint32_t)kAdded), in = kept + some;
-      score_blocks<D, THREADS>(a, w, finite, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
+      score_blocks<D, THREADS>(a, w, query, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
       f0 += some;
       const bool whole = f0 == n_found, last = whole && i0 + kChecked >= n;
       for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += THREADS / 8) {  // 8 threads for an entry
