@@ -54,8 +54,8 @@ def build_kernel_lib(force: bool = False, extra: List[str] = ()) -> str:
              "nsa_cache_api.cu": ["nsa_cache_index.h", "nsa_cache_kernel.cuh", "nsa_cache_decode.cuh", "nsa_cache_host.h",
                                   "nsa_programmatic.cuh", "ptx.cuh", "nsa_host.h"],
              "nsa_step_api.cu": ["nsa_cache_index.h", "nsa_cache_select_index.h", "nsa_cache_select_kernel.cuh", "nsa_cache_decode.cuh",
-                                 "nsa_reserve_index.h", "nsa_reserve_kernel.cuh", "nsa_rotary_kernel.cuh", "nsa_linspace.cuh",
-                                 "nsa_cache_host.h", "nsa_programmatic.cuh", "ptx.cuh", "nsa_host.h"]}
+                                 "nsa_reserve_index.h", "nsa_reserve_kernel.cuh", "nsa_rotary_kernel.cuh", "nsa_rotary_index.h",
+                                 "nsa_linspace.cuh", "nsa_cache_host.h", "nsa_programmatic.cuh", "ptx.cuh", "nsa_host.h"]}
     objects = []
     for unit, headers in units.items():
         obj = os.path.join(PKG, unit[:-3] + ".o")

@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include "nsa_programmatic.cuh"
+#include "nsa_rotary_index.h"
 
 namespace nsa {
 namespace rotary {
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, SEVERAL ? 6 : 8) rotary_kernel(const
   const int h0 = SEVERAL ? 0 : blockIdx.y * a.heads_block, h1 = SEVERAL ? a.heads : min(h0 + a.heads_block, a.heads);
   const int turning = a.pairs / VEC;                                // items of a head that turn 2 VEC values
   const int items = turning + (a.rest + 2 * VEC - 1) / (2 * VEC);   // and those that copy as many
-  const int first = blockIdx.x * (SEVERAL ? a.tokens_block : 1);
+  const int first = first_token(blockIdx.x, SEVERAL ? a.tokens_block : 1);
   if constexpr (!SEVERAL) {
     const uint64_t turn = tid < a.pairs ? a.turn[tid] : 0;
     start_in_order();
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, SEVERAL ? 6 : 8) rotary_kernel(const
     const int axis = as_memory(a.axis)[pair];
     start_in_order();
     for (int token = tid / a.pairs; token < a.tokens_block && tid < at_once * a.pairs; token += at_once) {
-      const int g = min(first + token, a.total - 1), b = g / a.tokens, t = g - b * a.tokens;
+      const int g = token_or_last(first, token, a.total), b = g / a.tokens, t = g - b * a.tokens;
       const int64_t pos = a.pos[axis * a.ps[0] + b * a.ps[1] + t * a.ps[2]];
       angles[token * a.pairs + place<VEC>(pair, turning)] = cos_sin((uint64_t)pos * turn, a.flip);
     }
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, SEVERAL ? 6 : 8) rotary_kernel(const
 
   // item and head of a thread's next item, stepped without divisions
   const int token = SEVERAL ? tid / (items * a.heads) : 0;
-  if (SEVERAL && (token >= a.tokens_block || first + token >= a.total)) return;
+  if (SEVERAL && !has_token(first, token, a.tokens_block, a.total)) return;
   const int of_token = SEVERAL ? tid - token * (items * a.heads) : tid;
   const int b = (first + token) / a.tokens, t = first + token - b * a.tokens;
   int item = of_token % items, head = h0 + of_token / items;
