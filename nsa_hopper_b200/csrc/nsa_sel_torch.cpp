@@ -717,9 +717,35 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
 };
 
+// Whether forward mode has a tangent for x that is not zero.
+bool has_tangent(const torch::Tensor& x) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return false;
+  const torch::Tensor& t = x._fw_grad(0);
+  return t.defined() && !t._is_zerotensor();
+}
+
 std::vector<torch::Tensor> rotary(torch::Tensor Q, OptTensor K, torch::Tensor positions, torch::Tensor turns, torch::Tensor axis,
                                   int64_t axes, int64_t d_head, int64_t offset, bool interleaved, bool inverse,
                                   bool q_token_major, bool k_token_major) {
+  const bool q_moves = has_tangent(Q), k_moves = K.has_value() && has_tangent(*K);
+  if (q_moves || k_moves) {
+    // forward mode: an output's tangent is the turned tangent of its input
+    const auto turn = [&](const torch::Tensor& q, const OptTensor& k, bool q_major) {
+      return rotary(q, k, positions, turns, axis, axes, d_head, offset, interleaved, inverse, q_major, k_token_major);
+    };
+    const auto primal = [](const torch::Tensor& x) { return std::get<0>(at::_unpack_dual(x, 0)); };
+    auto out = turn(primal(Q), K.has_value() ? OptTensor(primal(*K)) : OptTensor(), q_token_major);
+    torch::Tensor dq, dk;
+    if (q_moves) {
+      const auto d = turn(Q._fw_grad(0), k_moves ? OptTensor(K->_fw_grad(0)) : OptTensor(), q_token_major);
+      dq = d[0], dk = d[1];
+    } else {
+      dk = turn(K->_fw_grad(0), OptTensor(), k_token_major)[0];
+    }
+    if (q_moves) out[0] = at::_make_dual(out[0], dq, 0);
+    if (k_moves) out[1] = at::_make_dual(out[1], dk, 0);
+    return out;
+  }
   if (torch::GradMode::is_enabled() && (Q.requires_grad() || (K.has_value() && K->requires_grad()))) {
     auto out = RotaryFunction::apply(Q, K, positions, turns, axis, axes, d_head, offset,
                                      interleaved, inverse, q_token_major, k_token_major);

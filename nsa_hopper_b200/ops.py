@@ -292,7 +292,8 @@ def rotary(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, 
     does; bf16, fp16 or fp32, any strides (a projection's [B, T, H, d] is given as ``x.transpose(1, 2)``).  ``positions`` int32
     [N] or [B, T] (any strides, e.g. expanded over the batch), with the axes of the plan before that if there are several.
     The results are contiguous and of the inputs' dtype; angles are exact for all int32 positions, products are fp32.
-    Differentiable in Q and K, any number of times; ``inverse`` turns back."""
+    Differentiable in Q and K, any number of times, in reverse and in forward mode (``torch.autograd.forward_ad``; the transforms
+    of ``torch.func`` are refused); ``inverse`` turns back."""
     q, k = _C.rotary(Q, K, positions, plan.turns, plan.axis, plan.axes, plan.d, plan.offset, plan.interleaved, bool(inverse))
     return q, k
 

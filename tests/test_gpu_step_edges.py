@@ -1,8 +1,11 @@
-"""Edges of a decode step's preparation on the GPU: queries whose channels are far apart, against the oracle's exact sums."""
+"""Edges of a decode step's preparation on the GPU: queries whose channels are far apart, against the oracle's exact sums;
+forward-mode derivatives of the rotary positions."""
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+from nsa_hopper_b200 import ops
 from tests.test_gpu_step import DIMS, _check_select, _records, _tables
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +53,53 @@ def test_select_of_fp16_numbers_from_the_smallest_to_the_largest():
     q = torch.randint(-3, 4, (2, 256, 64), generator=g) * 2.0**-24
     q[:, 17, 63] = 65504.0
     _check_select(q.to(torch.float16), _records(x, 64), pages, lens, 12)
+
+
+# ------------------------------------------------------------------ rotary positions
+@pytest.mark.parametrize("layout", ["rows", "tokens"])
+@pytest.mark.parametrize("leaves", [False, True])
+def test_rotary_in_forward_mode(layout, leaves):
+    """The turn is linear: an output's tangent is the turned tangent, bit for bit what a call with it gives."""
+    g = torch.Generator().manual_seed(6)
+    plan = ops.rotary_plan(24, rotary_dim=16, offset=4)
+    shape = (6, 3, 24) if layout == "rows" else (2, 6, 3, 24)
+    pos = torch.randint(0, 5000, shape[:-2], generator=g).int().cuda()
+    view = (lambda t: t.transpose(1, 2)) if layout == "tokens" else (lambda t: t)
+    x, dx, y, dy = (view(torch.randn(shape, generator=g).cuda()) for _ in range(4))
+    want, moved = ops.rotary(x, y, pos, plan), ops.rotary(dx, dy, pos, plan)
+    if leaves:
+        x, y = x.requires_grad_(), y.requires_grad_()
+    with forward_ad.dual_level():
+        a, b = forward_ad.make_dual(x, dx), forward_ad.make_dual(y, dy)
+
+        def same(got, value, tangent):
+            u = forward_ad.unpack_dual(got)
+            assert torch.equal(u.primal, value) and (u.tangent is None) == (tangent is None)
+            assert tangent is None or torch.equal(u.tangent, tangent)
+            assert got.requires_grad == leaves
+
+        for q, k in ((a, b), (a, y), (x, b)):
+            u, v = ops.rotary(q, k, pos, plan)
+            same(u, want[0], moved[0] if q is a else None)
+            same(v, want[1], moved[1] if k is b else None)
+        alone, none = ops.rotary(a, None, pos, plan)
+        assert none is None
+        same(alone, want[0], moved[0])
+        if leaves:  # reverse over forward: the gradient of what the tangent does not depend on, and of the primal
+            (grad,) = torch.autograd.grad(forward_ad.unpack_dual(alone).primal, x, dx)
+            assert torch.equal(grad, ops.rotary(dx, None, pos, plan, inverse=True)[0])
+    assert forward_ad.unpack_dual(ops.rotary(x, y, pos, plan)[0]).tangent is None
+
+
+def test_rotary_gradients_in_forward_mode():
+    """Forward over reverse: the tangent of a gradient is the turn back of the incoming gradient's tangent."""
+    g = torch.Generator().manual_seed(7)
+    plan, pos = ops.rotary_plan(16), torch.arange(5, dtype=torch.int32, device="cuda")
+    x = torch.randn(5, 2, 16, generator=g).cuda().requires_grad_()
+    d, t = (torch.randn(5, 2, 16, generator=g).cuda() for _ in range(2))
+    y, _ = ops.rotary(x, None, pos, plan)
+    with forward_ad.dual_level():
+        (grad,) = torch.autograd.grad(y, x, forward_ad.make_dual(d, t))
+        u = forward_ad.unpack_dual(grad)
+        assert torch.equal(u.primal, ops.rotary(d, None, pos, plan, inverse=True)[0])
+        assert torch.equal(u.tangent, ops.rotary(t, None, pos, plan, inverse=True)[0])
