@@ -681,9 +681,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     const bool both = K.has_value();
     ctx->save_for_backward({positions, turns, axis});
     ctx->set_materialize_grads(false);
-    // gradients come back as the inputs lie: heads of [B, H, T, d] may be a view of [B, T, H, d]
+    // gradients come back as the inputs lie: [B, H, T, d] may be a view of [B, T, H, d], or of a part of a fused projection
     const auto as_view = [](const torch::Tensor& x) {
-      return x.dim() == 4 && !x.is_contiguous() && x.transpose(1, 2).is_contiguous();
+      return x.dim() == 4 && x.size(1) > 1 && x.size(2) > 1 && x.stride(1) > 0 && x.stride(1) < x.stride(2);
     };
     const int64_t flags = (both ? 1 : 0) | (interleaved ? 2 : 0) | (inverse ? 4 : 0) | (as_view(Q) ? 8 : 0) |
                           (both && as_view(*K) ? 16 : 0);

@@ -1,5 +1,5 @@
 """Edges of a decode step's preparation on the GPU: queries whose channels are far apart, against the oracle's exact sums;
-forward-mode derivatives of the rotary positions."""
+forward-mode derivatives of the rotary positions, and where their gradients lie."""
 import numpy as np
 import pytest
 import torch
@@ -103,3 +103,24 @@ def test_rotary_gradients_in_forward_mode():
         u = forward_ad.unpack_dual(grad)
         assert torch.equal(u.primal, ops.rotary(d, None, pos, plan, inverse=True)[0])
         assert torch.equal(u.tangent, ops.rotary(t, None, pos, plan, inverse=True)[0])
+
+
+@pytest.mark.parametrize("parts", [(4, 2, 2), (1, 1, 1), (3, 0, 5)])
+def test_rotary_gradients_lie_as_a_fused_projection(parts):
+    """Heads cut out of a fused projection: gradients have its order of tokens and heads, and the values of whole tensors."""
+    g = torch.Generator().manual_seed(sum(parts))
+    B, T, d, (hq, hk, _) = 2, 6, 16, parts
+    plan, pos = ops.rotary_plan(d), torch.arange(T, dtype=torch.int32, device="cuda").expand(B, T)
+    fused = torch.randn(B, T, sum(parts), d, generator=g).cuda().requires_grad_()
+    q, k = fused[:, :, :hq].transpose(1, 2), fused[:, :, hq:hq + hk].transpose(1, 2) if hk else None
+    out = [x for x in ops.rotary(q, k, pos, plan) if x is not None]
+    grads = [torch.randn(x.shape, generator=g).cuda() for x in out]
+    views = [x for x in (q, k) if x is not None]
+    back = torch.autograd.grad(out, views, grads, retain_graph=True)
+    for x, y, dy in zip(views, back, grads):
+        assert y.transpose(1, 2).is_contiguous() and torch.equal(y, ops.rotary(dy, None, pos, plan, inverse=True)[0])
+    (whole,) = torch.autograd.grad(out, fused, grads)
+    assert torch.equal(whole[:, :, :hq], back[0].transpose(1, 2)) and (whole[:, :, hq + hk:] == 0).all()
+    x = q.detach().contiguous().requires_grad_()  # (heads one after the other)
+    (y,) = torch.autograd.grad(ops.rotary(x, None, pos, plan)[0], x, grads[0])
+    assert y.is_contiguous() and torch.equal(y, back[0])
