@@ -432,7 +432,8 @@ typedef struct nsa_cache_select_desc {
   int32_t reserved[4];
 } nsa_cache_select_desc;
 
-/* Bytes of the workspace, or -1 if the description is invalid (see nsa_sel_last_error()). */
+/* Bytes of the workspace, or -1 if the description is invalid (see nsa_sel_last_error()): 8 for each block of the longest
+   sequence that the table can hold, KV head and row of a launch, however long the sequences are. */
 int64_t nsa_cache_select_workspace_bytes(const nsa_cache_select_desc* desc);
 int nsa_cache_select(const nsa_cache_select_desc* desc, nsa_stream_t stream);
 

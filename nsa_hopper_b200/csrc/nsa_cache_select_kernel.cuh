@@ -63,7 +63,7 @@ struct Args {
   int64_t q_row, q_head;
   const uint8_t* cache;
   int64_t page_stride;
-  float2* bounds;       // [n_rows, Hkv, blocks] lower and upper bound of a block's score
+  float2* bounds;       // [rows, Hkv, blocks] lower and upper bound of a block's score
   int32_t* sel;         // [n_rows, Hkv, n_sel]
   int32_t hkv, group, n_sel;
   int32_t shift;        // of a block's tokens
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(warps_of(D) * 32) score_kernel(const Args a) {
       first = (int32_t)(place - line[lo]) * a.unit;
     }
     Unit x;
-    x.bounds = a.bounds + ((int64_t)row * a.hkv + head) * a.blocks + first;
+    x.bounds = a.bounds + ((int64_t)(row - a.row0) * a.hkv + head) * a.blocks + first;
     x.blocks = min(a.unit, n_blocks - first);
     x.first = first_key(p, first + min(lane, x.blocks));
     x.end = __shfl_down_sync(0xFFFFFFFFu, x.first, 1);
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
   // What earlier kernels wrote is read before score_kernel has ended: it has waited for them before this one could begin.
   const int64_t unit = blockIdx.x;
   const int row = a.row0 + (int)(unit / a.hkv), head = (int)(unit % a.hkv);
-  const float2* bounds = a.bounds + ((int64_t)a.row0 * a.hkv + unit) * a.blocks;
+  const float2* bounds = a.bounds + unit * a.blocks;
   int32_t* sel = a.sel + ((int64_t)a.row0 * a.hkv + unit) * a.n_sel;
   const Heads<D, THREADS> heads(a, row, head);
   const int seq = cache::sequence_by_32(

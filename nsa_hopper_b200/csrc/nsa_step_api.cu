@@ -101,6 +101,10 @@ int32_t unit_of(const nsa_cache_select_desc* d) {
 }
 // Units of a row and KV head, at most.
 int64_t units_of(const nsa_cache_select_desc* d) { return ((int64_t)most_blocks(d) + unit_of(d) - 1) / unit_of(d); }
+// Rows of a launch, at most: their units have numbers of 31 bits.
+int64_t rows_of_launch(const nsa_cache_select_desc* d) {
+  return std::max<int64_t>(1, std::min<int64_t>(select::kMaxRows, kMaxIndex / (units_of(d) * d->batch.heads_kv)));
+}
 
 int check_select(const nsa_cache_select_desc* d) {
   if (d == nullptr) return fail(NSA_ERR_INVALID_ARG, "desc is NULL");
@@ -138,13 +142,12 @@ int launch_pick(const select::Args& a, int dev, uint32_t bit, cudaStream_t st) {
 }
 
 template <int D>
-int launch_select(select::Args a, int32_t n_rows, int sm, int dev, cudaStream_t st) {
+int launch_select(select::Args a, int32_t n_rows, int64_t most, int sm, int dev, cudaStream_t st) {
   const int fixed = (int)sizeof(select::ScoreWarp<D>) * select::warps_of(D);
   const uint32_t bit = D == 64 ? 2u : D == 128 ? 16u : 128u;  // (three kernels each)
   int rc = allow_smem(reinterpret_cast<const void*>(&select::score_kernel<D>), fixed + select::kMaxRows * 12 + 4, dev, bit);
   if (rc != NSA_OK) return rc;
   const int64_t units = (a.blocks + a.unit - 1) / a.unit;  // of a row and KV head
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(select::kMaxRows, kMaxIndex / (units * a.hkv)));
   for (int64_t row0 = 0; row0 < n_rows; row0 += most) {
     a.row0 = (int32_t)row0;
     a.rows = (int32_t)std::min(most, n_rows - row0);
@@ -199,9 +202,10 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
   a.per_key = ((1u << 20) + a.keys - 1) / a.keys;
   a.at_once = select::kKeys / a.keys;
-  if (b.d_qk == 64) return launch_select<64>(a, b.n_rows, sm, dev, st);
-  if (b.d_qk == 128) return launch_select<128>(a, b.n_rows, sm, dev, st);
-  return launch_select<192>(a, b.n_rows, sm, dev, st);
+  const int64_t most = rows_of_launch(d);
+  if (b.d_qk == 64) return launch_select<64>(a, b.n_rows, most, sm, dev, st);
+  if (b.d_qk == 128) return launch_select<128>(a, b.n_rows, most, sm, dev, st);
+  return launch_select<192>(a, b.n_rows, most, sm, dev, st);
 }
 
 // ------------------------------------------------------------------ rotary positions
@@ -325,7 +329,9 @@ int nsa_cache_reserve(const nsa_cache_reserve_desc* desc, nsa_stream_t stream) {
 int64_t nsa_cache_select_workspace_bytes(const nsa_cache_select_desc* desc) {
   if (check_select(desc) != NSA_OK) return -1;
   done(cudaSuccess, "");
-  return std::max<int64_t>(16, (int64_t)desc->batch.n_rows * desc->batch.heads_kv * most_blocks(desc) * 8);
+  // (the rows of one launch: the next one's bounds are written when the last one's have been read)
+  const int64_t rows = std::min<int64_t>(desc->batch.n_rows, rows_of_launch(desc));
+  return std::max<int64_t>(16, rows * desc->batch.heads_kv * most_blocks(desc) * 8);
 }
 int nsa_cache_select(const nsa_cache_select_desc* desc, nsa_stream_t stream) {
   return run_select(desc, reinterpret_cast<cudaStream_t>(stream));

@@ -5,8 +5,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from nsa_hopper_b200 import ops
-from tests.test_gpu_step import DIMS, _check_select, _records, _tables
+from nsa_hopper_b200 import capi, ops
+from tests.test_gpu_step import DIMS, _check_select, _records, _t, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -53,6 +53,28 @@ def test_select_of_fp16_numbers_from_the_smallest_to_the_largest():
     q = torch.randint(-3, 4, (2, 256, 64), generator=g) * 2.0**-24
     q[:, 17, 63] = 65504.0
     _check_select(q.to(torch.float16), _records(x, 64), pages, lens, 12)
+
+
+def test_select_of_many_launches_in_the_workspace_of_one():
+    """2300 rows with the workspace that is asked for and not a byte more, against calls of few rows."""
+    g = torch.Generator().manual_seed(14)
+    rows, count = 2300, 5
+    lens = np.random.default_rng(14).integers(0, 900, rows)
+    pages = _t(np.random.default_rng(15).integers(0, count, (rows, 1)))
+    cache = torch.from_numpy(_records(torch.randn(count, 2, 64, 64, generator=g), 64)).cuda()
+    q, lens = torch.randn(rows, 4, 64, generator=g).to("cuda", torch.bfloat16), _t(lens)
+    batch = capi.make_cache_batch(cache=cache.data_ptr(), pages=pages.data_ptr(), lens=lens.data_ptr(), num_pages=count, n_seqs=rows,
+                                  width=1, n_rows=rows, heads_kv=2, d_qk=64, d_v=64)
+    sel = torch.full((rows, 2, 6), 7, dtype=torch.int32, device="cuda")
+    desc = capi.make_cache_select_desc(batch=batch, q=q.data_ptr(), sel=sel.data_ptr(), heads_q=4, n_sel=6, block_size=64, cmp_block=32,
+                                       cmp_stride=16, q_dtype=capi.DTYPE_BF16)
+    size = capi.cache_select_workspace_bytes(desc)
+    assert size == 1024 * 2 * 17 * 8  # (T up to 64 * 16 + 31 = 1055 tokens, 17 blocks)
+    work = torch.full((size + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    desc.workspace = work.data_ptr()
+    capi.cache_select(desc, torch.cuda.current_stream().cuda_stream)
+    want = torch.cat([ops.cache_select(q[r:r + 500], cache, pages[r:r + 500], lens[r:r + 500], 6) for r in range(0, rows, 500)])
+    assert torch.equal(sel, want) and (work[size:] == 0xAB).all()
 
 
 # ------------------------------------------------------------------ rotary positions

@@ -58,3 +58,21 @@ def test_rotary_blocks_end_with_the_last_token(rotary_lib, total):
             assert angles.tolist() == [min(at * each + i, total - 1) for i in range(each)]
         passed += (last + 1) * each > BIG + 1
     assert (passed > 100) == (total == BIG)
+
+
+# ------------------------------------------------------------------ block selection
+def _select_desc(**batch):
+    b = capi.make_cache_batch(**{**dict(cache=1 << 20, pages=1 << 20, lens=1 << 20, num_pages=8, n_seqs=3, width=4, n_rows=3, heads_kv=2,
+                                        d_qk=128, d_v=128), **batch})
+    return capi.make_cache_select_desc(batch=b, q=1 << 20, sel=1 << 20, heads_q=b.heads_kv, n_sel=16, block_size=64, cmp_block=32,
+                                       cmp_stride=16, q_dtype=capi.DTYPE_BF16)
+
+
+def test_select_workspace_is_that_of_a_launch():
+    """65 blocks of 64 in a table of 4 pages; rows of a launch are 1024 at most, and fewer where units of a row are many."""
+    for rows, counted in ((1, 1), (1023, 1023), (1024, 1024), (1025, 1024), (100000, 1024)):
+        assert capi.cache_select_workspace_bytes(_select_desc(n_rows=rows, n_seqs=rows)) == counted * 2 * 65 * 8
+    # 2^18 blocks, a unit for 16 of them, 2048 heads: 2^25 units a row, 63 rows below 2^31
+    wide = dict(width=2**31 - 1, heads_kv=2048)
+    assert capi.cache_select_workspace_bytes(_select_desc(n_rows=500, n_seqs=500, **wide)) == 63 * 2048 * 2**18 * 8
+    assert capi.cache_select_workspace_bytes(_select_desc(n_rows=5, n_seqs=5, **wide)) == 5 * 2048 * 2**18 * 8
