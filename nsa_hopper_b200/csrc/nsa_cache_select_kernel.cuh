@@ -476,16 +476,18 @@ __device__ __forceinline__ Query prepare_exact(const Args& a, Exact<D>& w, const
   const int up = a.bits - 22 + 126 - max((int)(__float_as_uint(query_value(a, top)) >> 23), 1);
   const float up0 = __uint_as_float((uint32_t)(127 + up / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
   int32_t upper[2] = {}, lower[2] = {};
-  bool fits = true;
+  // (1.5 2^23: what it is added to, below 2^22, is rounded to a whole number, which the lowest bits then are)
+  constexpr float kRound = 12582912.0f;
+  bool fits = up >= -16;  // (below that the smallest numbers of bf16 could become 0)
   heads.each([&](uint32_t two) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float value = query_value(a, i == 0 ? two & 0xFFFFu : two >> 16);
-      const float x = value * up0 * up1, whole_part = rintf(x), rest = (x - whole_part) * 4194304.0f;
-      const int fraction = __float2int_rn(rest);
-      upper[i] += (int)whole_part;
-      lower[i] += fraction;
-      fits = fits && (float)fraction == rest && (x != 0.0f || value == 0.0f);
+      const float x = value * up0 * up1, w0 = __fadd_rn(x, kRound);
+      const float rest = __fmul_rn(__fsub_rn(x, __fsub_rn(w0, kRound)), 4194304.0f), w1 = __fadd_rn(rest, kRound);
+      upper[i] += __float_as_int(w0) - __float_as_int(kRound);
+      lower[i] += __float_as_int(w1) - __float_as_int(kRound);
+      fits = fits && __fsub_rn(w1, kRound) == rest;
     }
   });
   if (part < kParts)
@@ -565,7 +567,8 @@ __device__ __forceinline__ void dot(const Exact<D>& w, const Quarter<D> (&k)[2],
   }
 }
 
-// The same from the sums in fp64.
+// The same from the sums in fp64.  (In a loop: unrolled it is seldom run code between that which always is, and took 41
+// sequences with drafts 1 % more.)
 template <int D>
 __device__ __forceinline__ void dot_wide(const Exact<D>& w, const Quarter<D> (&k)[2], int quarter, double (&x)[2]) {
   x[0] = x[1] = 0.0;
@@ -573,11 +576,11 @@ __device__ __forceinline__ void dot_wide(const Exact<D>& w, const Quarter<D> (&k
   for (int j = 0; j < D / 64; ++j) {
     const double* q = w.wide + (quarter * (D / 64) + j) * 16;
     double sum[2] = {0.0, 0.0};
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int four = decode4(k[y].code[2 * j + i / 2] >> i % 2 * 16);
+        const int four = decode4((i < 2 ? k[y].code[2 * j] : k[y].code[2 * j + 1]) >> i % 2 * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[y] = fma(q[4 * i + e], whole((four >> 8 * e & 255) - 12), sum[y]);
       }

@@ -197,7 +197,7 @@ int run_select(const nsa_cache_select_desc* d, cudaStream_t st) {
   a.cmp_block = d->cmp_block, a.cmp_stride = d->cmp_stride;
   a.record = cache::record_bytes(b.d_qk, b.d_v);
   a.q_half = d->q_dtype == NSA_DTYPE_F16;
-  a.bits = 46;  // (the sum of the heads, in six signed bytes)
+  a.bits = 44;  // (the sum of the heads, below 2^46, in six signed bytes; a value's whole part is below 2^22)
   while ((1 << (46 - a.bits)) < a.group) --a.bits;
   a.keys = d->block_size / d->cmp_stride + 2;  // (keys are at least cmp_stride apart, but for a rounding; at most 258)
   a.per_key = ((1u << 20) + a.keys - 1) / a.keys;
