@@ -1,4 +1,5 @@
-// Where the compressed keys of a 4-bit cache stand among the selection blocks, for the block selection of single tokens.  A
+// Where the compressed keys of a 4-bit cache stand among the selection blocks, for the block selection of single tokens, and the
+// whole numbers of its exact scores.  Plain C++, which the CPU tests compile.  A
 // row at position t sees the first T = t + 1 tokens of its sequence as block selection sees a prompt of T: n compressed keys,
 // key i in the block of the float32 linspace(0, T - 1, n)[i] (see nsa_linspace.cuh).
 #pragma once
@@ -69,6 +70,58 @@ NSA_LINSPACE int32_t first_key(const Places& p, int32_t block) {
   }
   return i;
 }
+
+// ------------------------------------------------------------------ whole numbers
+// Four bytes of a and b (places 4 to 7), by the lower three bits of the nibbles of `select`; with the fourth bit the sign of that
+// byte in all its bits.
+NSA_HD uint32_t pick_bytes(uint32_t a, uint32_t b, uint32_t select) {
+#ifdef __CUDA_ARCH__
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(select));
+  return r;
+#else
+  uint32_t r = 0;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t s = select >> 4 * i & 15, at = s & 7, byte = (at < 4 ? a >> 8 * at : b >> 8 * (at - 4)) & 255;
+    r |= (s < 8 ? byte : byte >> 7 != 0 ? 255u : 0u) << 8 * i;
+  }
+  return r;
+#endif
+}
+// sum + the four products of signed bytes, modulo 2^32.
+NSA_HD uint32_t add_products(uint32_t a, uint32_t b, uint32_t sum) {
+#ifdef __CUDA_ARCH__
+  return (uint32_t)__dp4a((int)a, (int)b, (int)sum);
+#else
+  for (int i = 0; i < 4; ++i) sum += (uint32_t)((int32_t)(int8_t)(a >> 8 * i & 255) * (int8_t)(b >> 8 * i & 255));
+  return sum;
+#endif
+}
+constexpr int kCodeZero = 12;  // of decode4
+// Four codes, doubled and 12 more: whole numbers 0 to 24 in four bytes.
+NSA_HD uint32_t decode4(uint32_t codes) {
+  // (for negative codes the first gives the sign, 0, of a byte of the table; for the others the second does)
+  const uint32_t plus = pick_bytes(0x03020100u, 0x0C080604u, codes), minus = pick_bytes(0x03020100u, 0x0C080604u, codes ^ 0x8888u);
+  return 0x0C0C0C0Cu + plus - minus;
+}
+// The lowest signed byte of x, which is taken off; the next ones follow.
+NSA_HD int8_t next_byte(int64_t& x) {
+  const int8_t byte = (int8_t)(x & 255);
+  x = (x - byte) >> 8;
+  return byte;
+}
+// Adds 16 codes (from decode4) times 16 bytes of the query to the sum of the higher bytes.
+NSA_HD uint32_t add_group(uint32_t higher, const uint32_t (&codes)[4], const uint32_t (&bytes)[4]) {
+  return add_products(codes[0], bytes[0],
+                      add_products(codes[1], bytes[1], add_products(codes[2], bytes[2], add_products(codes[3], bytes[3], higher * 256))));
+}
+// What three bytes' sums are too large by, negative: 12 of every code.
+NSA_HD uint32_t too_many(const uint32_t (&low)[4], const uint32_t (&middle)[4], const uint32_t (&high)[4]) {
+  const uint32_t twelve[4] = {0x0C0C0C0Cu, 0x0C0C0C0Cu, 0x0C0C0C0Cu, 0x0C0C0C0Cu};
+  return 0u - add_group(add_group(add_group(0, twelve, high), twelve, middle), twelve, low);
+}
+// Upper half of the fp64 of a scale byte of at least 8 (a quiet NaN's for those that stand for no number); its lower half is 0.
+NSA_HD uint32_t scale_high(uint32_t byte) { return byte < 0xF8 ? (byte << 17) + (1008u << 20) : 0x7FF80000u; }
 
 }  // namespace cache_select
 }  // namespace nsa

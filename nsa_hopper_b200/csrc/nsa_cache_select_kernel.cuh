@@ -399,11 +399,14 @@ __global__ void __launch_bounds__(warps_of(D) * 32) score_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------ exact scores
+struct alignas(16) Bytes {
+  uint32_t x[4];
+};
 template <int D>
 struct Exact {
-  int4 limb[D / 16][kLimbs + 1];  // bytes of the query, the lowest first, of the 16 dims of a group, four to a word (and room
+  Bytes limb[D / 16][kLimbs + 1];  // bytes of the query, the lowest first, of the 16 dims of a group, four to a word (and room
                                   // that puts what the threads of a key read at once into different banks)
-  int2 start[D / 16];             // what the sums of a group begin with: 12 of every code too many, taken off
+  uint2 start[D / 16];             // what the sums of a group begin with: 12 of every code too many, taken off
   union {
     int32_t sum[2][D];            // of the heads: whole parts and fractions
     double wide[D];               // the sum itself, where the bytes do not hold it
@@ -420,15 +423,7 @@ __device__ __forceinline__ double whole(int32_t x) {
 // fp64 of a scale byte (NaN for those that stand for no number).
 __device__ __forceinline__ double scale_of(uint32_t byte) {
   if (byte < 8) return (double)byte * 7.62939453125e-06;  // (below the smallest normal scale: eighths of 2^-14)
-  return __hiloint2double(byte < 0xF8 ? (int)((byte << 17) + (1008u << 20)) : 0x7FF80000, 0);
-}
-// Four codes, doubled and 12 more: whole numbers 0 to 24 in four bytes.
-__device__ __forceinline__ int decode4(uint32_t codes) {
-  // (a selector whose upper bit is set gives the sign of the byte in all its bits, which is 0 for these)
-  uint32_t plus, minus;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(plus) : "r"(0x03020100u), "r"(0x0C080604u), "r"(codes));
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(minus) : "r"(0x03020100u), "r"(0x0C080604u), "r"(codes ^ 0x8888u));
-  return (int)(0x0C0C0C0Cu + plus - minus);
+  return __hiloint2double((int)scale_high(byte), 0);
 }
 
 // The sum of a (row, head)'s query heads as whole numbers of a power of two, so that the largest stays below 2^46, cut into six
@@ -508,22 +503,12 @@ __device__ __forceinline__ Query prepare_exact(const Args& a, Exact<D>& w, const
   for (int d = tid; d < D; d += THREADS) {
     int64_t x = (int64_t)w.sum[0][d] * 4194304 + w.sum[1][d];
 #pragma unroll
-    for (int l = 0; l < kLimbs; ++l) {
-      const int8_t byte = (int8_t)x;
-      x = (x - byte) >> 8;
-      reinterpret_cast<int8_t*>(&w.limb[d / 16][l])[d % 16] = byte;
-    }
+    for (int l = 0; l < kLimbs; ++l) reinterpret_cast<int8_t*>(&w.limb[d / 16][l])[d % 16] = next_byte(x);
   }
   __syncthreads();
   if (tid < D / 16) {
-    const int ones = 0x01010101;
-    int32_t start[kLimbs];
-#pragma unroll
-    for (int l = 0; l < kLimbs; ++l) {
-      const int4 v = w.limb[tid][l];
-      start[l] = -12 * __dp4a(v.x, ones, __dp4a(v.y, ones, __dp4a(v.z, ones, __dp4a(v.w, ones, 0))));
-    }
-    w.start[tid] = make_int2((start[2] * 256 + start[1]) * 256 + start[0], (start[5] * 256 + start[4]) * 256 + start[3]);
+    const auto limb = w.limb[tid];
+    w.start[tid] = make_uint2(too_many(limb[0].x, limb[1].x, limb[2].x), too_many(limb[3].x, limb[4].x, limb[5].x));
   }
   return Query::kWhole;  // (the caller meets before the sums are read)
 }
@@ -535,7 +520,7 @@ __device__ __forceinline__ void dot(const Exact<D>& w, const Quarter<D> (&k)[2],
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
     const int g = quarter * (D / 64) + j;
-    int c[2][4];
+    uint32_t c[2][4];
 #pragma unroll
     for (int y = 0; y < 2; ++y)
 #pragma unroll
@@ -544,19 +529,19 @@ __device__ __forceinline__ void dot(const Exact<D>& w, const Quarter<D> (&k)[2],
     uint32_t up[2] = {}, lo[2] = {};  // (those with 12 of every code too many may wrap around)
 #pragma unroll
     for (int l = kLimbs - 1; l >= 0; --l) {
-      const int4 q = w.limb[g][l];
+      const Bytes q = w.limb[g][l];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         uint32_t& sum = l >= kLimbs / 2 ? up[y] : lo[y];
-        sum = (uint32_t)__dp4a(c[y][0], q.x, __dp4a(c[y][1], q.y, __dp4a(c[y][2], q.z, __dp4a(c[y][3], q.w, (int)(sum * 256)))));
+        sum = add_group(sum, c[y], q.x);
       }
     }
-    const int2 start = w.start[g];
+    const uint2 start = w.start[g];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       const double s = scale_of(k[y].scale >> 8 * j & 255u);
-      upper[y] = fma(s, whole((int)(up[y] + (uint32_t)start.y)), upper[y]);
-      lower[y] = fma(s, whole((int)(lo[y] + (uint32_t)start.x)), lower[y]);
+      upper[y] = fma(s, whole((int)(up[y] + start.y)), upper[y]);
+      lower[y] = fma(s, whole((int)(lo[y] + start.x)), lower[y]);
     }
   }
 #pragma unroll
@@ -580,9 +565,9 @@ __device__ __forceinline__ void dot_wide(const Exact<D>& w, const Quarter<D> (&k
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int four = decode4((i < 2 ? k[y].code[2 * j] : k[y].code[2 * j + 1]) >> i % 2 * 16);
+        const uint32_t four = decode4((i < 2 ? k[y].code[2 * j] : k[y].code[2 * j + 1]) >> i % 2 * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[y] = fma(q[4 * i + e], whole((four >> 8 * e & 255) - 12), sum[y]);
+        for (int e = 0; e < 4; ++e) sum[y] = fma(q[4 * i + e], whole((int)(four >> 8 * e & 255) - kCodeZero), sum[y]);
       }
 #pragma unroll
     for (int y = 0; y < 2; ++y) x[y] = fma(scale_of(k[y].scale >> 8 * j & 255u), sum[y], x[y]);

@@ -1,4 +1,5 @@
-"""Edges of a decode step's preparation without a GPU: the largest calls' index arithmetic, compiled for the host."""
+"""Edges of a decode step's preparation without a GPU: the largest calls' index arithmetic and the whole numbers of the exact
+scores, compiled for the host; sizes of workspaces."""
 import ctypes
 import os
 import subprocess
@@ -76,3 +77,77 @@ def test_select_workspace_is_that_of_a_launch():
     wide = dict(width=2**31 - 1, heads_kv=2048)
     assert capi.cache_select_workspace_bytes(_select_desc(n_rows=500, n_seqs=500, **wide)) == 63 * 2048 * 2**18 * 8
     assert capi.cache_select_workspace_bytes(_select_desc(n_rows=5, n_seqs=5, **wide)) == 5 * 2048 * 2**18 * 8
+
+
+SELECT = r"""
+#include <string.h>
+#include "nsa_cache_select_index.h"
+using namespace nsa::cache_select;
+extern "C" {
+uint32_t decode(uint32_t codes) { return decode4(codes); }
+uint32_t scale(uint32_t byte) { return scale_high(byte); }
+void bytes(int64_t x, int8_t* out) { for (int i = 0; i < 6; ++i) out[i] = next_byte(x); }
+// The sum of 16 products, from the query's bytes and codes in words of eight: what the kernel's threads do.
+int64_t group(const int64_t* q, const uint32_t* words) {
+  uint32_t limb[6][4], codes[4], up = 0, lo = 0;
+  for (int d = 0; d < 16; ++d) {
+    int64_t x = q[d];
+    for (int l = 0; l < 6; ++l) reinterpret_cast<int8_t*>(limb[l])[d] = next_byte(x);
+  }
+  for (int i = 0; i < 4; ++i) codes[i] = decode4(words[i / 2] >> i % 2 * 16);
+  for (int l = 5; l >= 3; --l) up = add_group(up, codes, limb[l]);
+  for (int l = 2; l >= 0; --l) lo = add_group(lo, codes, limb[l]);
+  up += too_many(limb[3], limb[4], limb[5]), lo += too_many(limb[0], limb[1], limb[2]);
+  return (int64_t)(int32_t)up * 16777216 + (int32_t)lo;
+}
+}
+"""
+DOUBLED = [0, 1, 2, 3, 4, 6, 8, 12, 0, -1, -2, -3, -4, -6, -8, -12]
+
+
+@pytest.fixture(scope="module")
+def select_lib(tmp_path_factory):
+    lib = _build(tmp_path_factory, "select", SELECT)
+    lib.decode.restype = lib.scale.restype = ctypes.c_uint32
+    lib.group.restype = ctypes.c_int64
+    return lib
+
+
+def test_codes_become_whole_numbers(select_lib):
+    for word in range(1 << 16):
+        got = select_lib.decode(ctypes.c_uint32(word))
+        assert all((got >> 8 * i & 255) - 12 == DOUBLED[word >> 4 * i & 15] for i in range(4))
+        if word % 251 == 0:  # (what stands above four codes is not looked at)
+            assert select_lib.decode(ctypes.c_uint32(word | 0xABCD0000)) == got
+
+
+def test_scale_bytes_become_fp64(select_lib):
+    """Every byte of a normal number: the fp16 of which it is the upper part, in the upper half of an fp64."""
+    for byte in range(8, 256):
+        want = np.float64(np.array([byte << 7], np.uint16).view(np.float16)[0])
+        got = np.array([select_lib.scale(byte) << 32], np.uint64).view(np.float64)[0]
+        assert got == want or not (np.isfinite(want) or np.isfinite(got)), byte
+
+
+def test_signed_bytes_of_sums(select_lib):
+    rng = np.random.default_rng(11)
+    for x in [0, 1, -1, 127, 128, -128, -129, 2**46, -2**46, 2**46 - 1] + [int(v) for v in rng.integers(-2**46, 2**46, 500)]:
+        out = np.zeros(6, np.int8)
+        select_lib.bytes(ctypes.c_int64(x), out.ctypes.data_as(ctypes.c_void_p))
+        assert sum(int(b) << 8 * i for i, b in enumerate(out)) == x
+
+
+def test_sums_of_a_group_are_exact(select_lib):
+    """Queries up to 2^46 in size (the bytes' largest sums among them) times all codes; 256 sequences of codes each."""
+    rng = np.random.default_rng(12)
+    worst = sum(127 << 8 * i for i in range(5)) + (63 << 40)  # (every byte as large as it gets below 2^46)
+    queries = [np.full(16, s * x, np.int64) for x in (2**46, 2**46 - 1, worst, 1, 0) for s in (1, -1)]
+    queries += [np.where(rng.random(16) < 0.5, worst, -worst), *rng.integers(-2**46, 2**46, (20, 16)), *rng.integers(-300, 300, (5, 16))]
+    for q in queries:
+        q = np.ascontiguousarray(q, np.int64)
+        words = rng.integers(0, 2**32, (256, 2), dtype=np.uint32)
+        words[:4] = [[0x77777777] * 2, [0xFFFFFFFF] * 2, [0, 0], [0x89ABCDEF, 0x76543210]]
+        for w in words:
+            codes = [DOUBLED[int(w[i // 8]) >> 4 * (i % 8) & 15] for i in range(16)]
+            got = select_lib.group(q.ctypes.data_as(ctypes.c_void_p), w.ctypes.data_as(ctypes.c_void_p))
+            assert got == sum(int(a) * b for a, b in zip(q, codes))
