@@ -1,4 +1,5 @@
-"""Edges of a decode step's preparation on the GPU: queries whose channels are far apart, against the oracle's exact sums;
+"""Edges of a decode step's preparation on the GPU: block selection from queries whose channels are far apart and
+from the longest sequences, against the oracle's exact sums;
 forward-mode derivatives of the rotary positions, and where their gradients lie."""
 import numpy as np
 import pytest
@@ -6,6 +7,8 @@ import torch
 from torch.autograd import forward_ad
 
 from nsa_hopper_b200 import capi, ops
+from oracle import cache as oc
+from oracle import step as oracle
 from tests.test_gpu_step import DIMS, _check_select, _records, _t, _tables
 
 pytestmark = pytest.mark.gpu
@@ -75,6 +78,60 @@ def test_select_of_many_launches_in_the_workspace_of_one():
     capi.cache_select(desc, torch.cuda.current_stream().cuda_stream)
     want = torch.cat([ops.cache_select(q[r:r + 500], cache, pages[r:r + 500], lens[r:r + 500], 6) for r in range(0, rows, 500)])
     assert torch.equal(sel, want) and (work[size:] == 0xAB).all()
+
+
+def test_select_of_several_passes():
+    """300000 tokens: 4688 blocks in three passes of 2048, 293 pages of keys, more than are looked up beforehand.  Pages of equal
+    keys stand at the first pass's end and the next one's beginning, in the middle and at the end, so that equal scores meet
+    across passes; a row of other keys throughout; lengths that end with a pass and behind it."""
+    rng, g = np.random.default_rng(16), torch.Generator().manual_seed(16)
+    lens = [300000, 300000, 131072, 131073, 262144 + 31]
+    pages, _ = _tables(lens, 32, 16, rng)
+    assert pages.shape[1] == 293
+    x = torch.randn(24, 1, 64, 64, generator=g)
+    x[:4] = x[:4, :, :1]  # (pages of one key 64 times)
+    q = torch.randn(5, 4, 64, generator=g).to(torch.bfloat16)
+    x[2] = (q[0].float().sum(0) / 8).expand(64, 64)  # (what row 0 looks for)
+    for r in (0, 2, 3, 4):
+        pages[r] = np.where(pages[r] >= 0, rng.integers(0, 2, pages.shape[1]), -1)
+    pages[0, [3, 127, 128, 150, 200, 255, 256, 257, 291, 292]] = 2
+    pages[1] = rng.integers(4, 24, pages.shape[1])
+    cache = _records(x, 64)
+    want = oracle.select(q.double().numpy(), cache, pages, np.array(lens), 1024)
+    passes = {int(b) // 2048 for b in want[0, 0, :100]}
+    assert passes == {0, 1, 2} and {int(b) // 2048 for b in want[1, 0]} == passes and (want >= 0).all()
+    args = q.cuda(), torch.from_numpy(cache).cuda(), _t(pages), _t(lens)
+    for n_sel in (1, 16, 100, 1024):
+        assert np.array_equal(ops.cache_select(*args, n_sel).cpu().numpy(), want[..., :n_sel])
+
+
+def test_select_of_the_longest_sequences():
+    """2^24 tokens, the most that float32 places: a million keys, mostly zeros, of whole numbers; one token more selects nothing."""
+    rng, g = np.random.default_rng(17), torch.Generator().manual_seed(17)
+    most, width, n_sel = 2**24, 16384, 40
+    lens = [most, most + 1, most - 5, 31]
+    x = torch.zeros(6, 1, 64, 64)
+    x[1:] = torch.randint(-6, 7, (5, 1, 64, 64), generator=g).clamp(-4, 4)
+    x[1:, ..., ::16] = 6  # (so that every scale is 1)
+    cache = _records(x, 64)
+    keys, _ = oc.decode(cache[:, 0], 64, 64)
+    assert np.array_equal(keys, x[:, 0].numpy())
+    pages = np.where(rng.random((4, width)) < 0.01, rng.integers(1, 6, (4, width)), 0).astype(np.int32)
+    pages[:, [0, 127, 128, 8191, 16383]] = 5
+    q = torch.randint(-9, 10, (4, 3, 64), generator=g).to(torch.bfloat16)
+    got = ops.cache_select(q.cuda(), torch.from_numpy(cache).cuda(), _t(pages), _t(lens), n_sel).cpu().numpy()
+    for r, tokens in enumerate(lens):
+        if tokens > most:
+            assert (got[r] == -1).all()
+            continue
+        n, blocks = oracle.completed(tokens, 32, 16), -(-tokens // 64)
+        score = np.zeros(blocks)
+        if n:
+            where = np.floor(torch.linspace(0, tokens - 1, n, dtype=torch.float32).numpy() / 64).astype(np.int64)
+            np.add.at(score, np.minimum(where, blocks - 1), (keys @ q[r].double().sum(0).numpy())[pages[r]].ravel()[:n])
+        want = np.argsort(-score, kind="stable")[:n_sel]
+        assert got[r, 0].tolist() == want.tolist() + [-1] * (n_sel - len(want))
+        assert r == 1 or n == 0 or {int(b) // 2048 for b in want} > {int(want[0]) // 2048}
 
 
 # ------------------------------------------------------------------ rotary positions
