@@ -200,9 +200,10 @@ def cache_reserve(pages: torch.Tensor, held: torch.Tensor, rows: torch.Tensor, p
     calls take as absent rows, and ``held`` tells the scheduler.
 
     With ``n_tokens`` = N the call's rows are packed (``rows[s]`` for each sequence that asks, those of refused ones too, N at
-    least their sum); without, row s is sequence s's last token (``rows`` at most 1).  ``pages`` and ``pool`` are changed in
-    place, ``held`` and ``n_free`` too unless ``update`` is False: then new tensors are returned and nothing that counts has
-    changed, so the call can be made again.  A page that two sequences share must not be given back while the other uses it."""
+    least their sum); without, row s is sequence s's last token.  Tokens that a sequence gives back and tokens that it asks for
+    (rejected drafts, then new ones) take two calls.  ``pages`` and ``pool`` are changed in place, ``held`` and ``n_free`` too
+    unless ``update`` is False: then new tensors are returned and nothing that counts has changed, so the call can be made
+    again.  A page that two sequences share must not be given back while the other uses it."""
     lens, cu, positions, slots, held, n_free = _C.cache_reserve(pages, held, rows, pool, n_free,
                                                                 None if n_tokens is None else int(n_tokens), bool(update))
     return CacheBatch(lens, None if n_tokens is None else cu, positions, slots, held, n_free)

@@ -1,12 +1,12 @@
 """Edges of a decode step's preparation on the GPU: block selection from queries whose channels are far apart and
 from the longest sequences, against the oracle's exact sums;
-forward-mode derivatives of the rotary positions, and where their gradients lie."""
+forward-mode derivatives of the rotary positions, and where their gradients lie; pages of the compressed cache."""
 import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from nsa_hopper_b200 import capi, ops
+from nsa_hopper_b200 import capi, nsa, ops
 from oracle import cache as oc
 from oracle import step as oracle
 from tests.test_gpu_step import DIMS, _check_select, _records, _t, _tables
@@ -203,3 +203,81 @@ def test_rotary_gradients_lie_as_a_fused_projection(parts):
     x = q.detach().contiguous().requires_grad_()  # (heads one after the other)
     (y,) = torch.autograd.grad(ops.rotary(x, None, pos, plan)[0], x, grads[0])
     assert y.is_contiguous() and torch.equal(y, back[0])
+
+
+# ------------------------------------------------------------------ whole steps
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_whose_compressed_pages_come_from_a_pool(captured):
+    """The second pool runs out: the sequence that completes a key has no rows until another one has ended, no page is in two
+    rows of a table, and outputs are those of a fixed table for the compressed keys.  Rejected drafts are given back in a
+    call of their own."""
+    g = torch.Generator().manual_seed(31)
+    S, hq, hk, d, width, wide, n_sel = 4, 4, 2, 64, 36, 3, 3
+    i32 = dict(dtype=torch.int32, device="cuda")
+    prompt = [1055, 500, 2075, 31]  # 64, 30, 128 and 0 compressed keys: 4 pages
+    plan, total, cmp_count = ops.rotary_plan(d), sum(prompt), 5
+    pages, held, pool, n_free = torch.full((S, width), -1, **i32), torch.zeros(S, **i32), torch.randperm(S * width, generator=g).int().cuda(), _t([S * width])
+    cmp_pages, cmp_held, cmp_pool, cmp_free = (torch.full((S, wide), -1, **i32), torch.zeros(S, **i32),
+                                               torch.randperm(cmp_count, generator=g).int().cuda(), _t([cmp_count]))
+    fixed = torch.arange(S * wide, **i32).view(S, wide)
+    cache, cmp_cache, cmp_fixed = ops.cache_alloc(S * width, hk, d, d), ops.cache_alloc(cmp_count, hk, d, d), ops.cache_alloc(S * wide, hk, d, d)
+    rows = _t(prompt)
+
+    def reserve(n_tokens=None):
+        batch = ops.cache_reserve(pages, held, rows, pool, n_free, n_tokens=n_tokens)
+        want = torch.where(held >= 32, (held - 32) // 16 + 1, 0)
+        ops.cache_reserve(cmp_pages, cmp_held, want - cmp_held, cmp_pool, cmp_free)
+        short = cmp_held != want
+        ops.cache_reserve(pages, held, torch.where(short, -rows, 0), pool, n_free)
+        return batch._replace(lens=torch.where(short, 0, batch.lens))
+
+    batch = reserve(total)
+    assert batch.lens.tolist() == prompt == held.tolist() and cmp_held.tolist() == [64, 30, 128, 0] and int(cmp_free) == 1
+    k, v = (torch.randn(total, hk, d, generator=g).to("cuda", torch.bfloat16) for _ in range(2))
+    _, k = ops.rotary(k[:, :1], k, batch.positions, plan)
+    ops.cache_write(cache, k, v, pages, batch.lens, cu_seqlens=batch.cu_seqlens)
+    for c, p in ((cmp_cache, cmp_pages), (cmp_fixed, fixed)):
+        nsa.cache_compress(cache, d, pages, batch.lens, c, p, cu_seqlens=batch.cu_seqlens, n_tokens=total)
+    q, k, v = (torch.randn(S, h, d, generator=g).to("cuda", torch.bfloat16) for h in (hq, hk, hk))
+
+    def step():
+        batch = reserve()
+        a, b = ops.rotary(q, k, batch.positions, plan)
+        ops.cache_write(cache, b, v, pages, batch.lens)
+        out = []
+        for c, p in ((cmp_cache, cmp_pages), (cmp_fixed, fixed)):
+            cmp_lens = nsa.cache_compress(cache, d, pages, batch.lens, c, p)
+            out.append(nsa.nsa_decode(a, cache, pages, batch.lens, window=64, cmp_cache=c, cmp_pages=p, cmp_lens=cmp_lens, n_sel=n_sel))
+            out.append(ops.cache_select(a, c, p, batch.lens, n_sel))
+        return batch, out
+
+    graph, results = torch.cuda.CUDAGraph(), None
+    if captured:
+        state = [pages, held, pool, n_free, cmp_pages, cmp_held, cmp_pool, cmp_free, cache, cmp_cache, cmp_fixed]
+        saved = [t.clone() for t in state]
+        rows.copy_(_t([1, 1, 1, 0]))
+        step()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            results = step()
+        for t, old in zip(state, saved):
+            t.copy_(old)
+    have = list(prompt)
+    # rows of each step, and the sequences whose rows are refused: sequence 0's key 64 and sequence 3's key 0 want the last page
+    for asked, refused in (([0, 1, 1, 1], []), ([1, 1, 1, 1], [0]), ([1, 0, 0, 1], [0]), ([0, -502, 1, 0], []), ([1, 0, 1, 1], []),
+                           ([0, 0, -1030, 0], []), ([1, 1, 1, 0], [])):
+        rows.copy_(_t(asked))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        if captured:
+            graph.replay()
+        batch, (out, sel, want, want_sel) = results if captured else step()
+        have = [max(0, n + r) if s not in refused else n for s, (n, r) in enumerate(zip(have, asked))]
+        assert held.tolist() == have and cmp_held.tolist() == [oracle.completed(n, 32, 16) for n in have]
+        assert batch.lens.tolist() == [n if r > 0 and s not in refused else 0 for s, (n, r) in enumerate(zip(have, asked))]
+        for table, h, p, n in ((pages, held, pool, n_free), (cmp_pages, cmp_held, cmp_pool, cmp_free)):
+            ids = [i for s in range(S) for i in table[s, :-(-int(h[s]) // 64)].tolist()] + p[:int(n)].tolist()
+            assert sorted(ids) == list(range(len(p)))
+        # (the same keys at other places, and the same shares of the work: equal, but for what fp32 sums may differ by)
+        assert torch.equal(sel, want_sel) and float((out - want).abs().max()) <= 2.0**-10 * float(want.abs().max())
+        assert ((out != 0).flatten(1).any(1) == (batch.lens > 0)).all()
