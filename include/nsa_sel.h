@@ -413,8 +413,8 @@ int nsa_cache_reserve(const nsa_cache_reserve_desc* desc, nsa_stream_t stream);
    cmp_stride + 1 compressed keys, key i (place i of the cache) in block floor(linspace(0, T-1, n_cmp)[i] / block_size), and
        score(block) = sum over its keys of (sum of the query heads of the KV head) . key.
    sel [n_rows, heads_kv, n_sel]: the min(n_sel, ceil(T / block_size)) best blocks, the best first, then -1.  Blocks are ranked
-   by sums in 64 bits; the lower block comes first where two are equal, and scores that are not finite come last.  Keys that the
-   page table does not hold count as zeros.  A row of no token, and one of more than 2^24 tokens or of more than
+   by sums in 64 bits; the lower block comes first where two are equal, and scores that are not finite come last: all of them where
+   the query is not finite, so that the lowest blocks are selected.  Keys that the page table does not hold count as zeros.  A row of no token, and one of more than 2^24 tokens or of more than
    64 * width * cmp_stride + cmp_block - 1 (whose keys the table cannot hold), selects nothing: -1 throughout.
    n_sel is at most 1024, heads_q / heads_kv at most 256.  Zero-initialise, then fill.  Two launches for each 1024 rows. */
 typedef struct nsa_cache_select_desc {
@@ -441,7 +441,8 @@ int nsa_cache_select(const nsa_cache_select_desc* desc, nsa_stream_t stream);
    b_i cos w + a_i sin w with w = position[axis[i]] * inv_freq[i], for the `pairs` pairs i of the rotary part, which begins at
    value `offset`: values i and i + pairs of it, or 2 i and 2 i + 1 if `interleaved`.  The other values are copied.  `inverse`
    turns by -w: the gradient.  inv_freq is given as turns[i] = round(inv_freq[i] / (2 pi) * 2^64) modulo 2^64, so that angles of
-   any int32 position are exact to 2^-32 of a turn.  One or two tensors (Q and K) with the same tokens, in any layout in which d
+   any int32 position are reduced to an eighth of a turn with an error below 2^-32 of a turn; that angle is then rounded to fp32 (2^-28
+   of a turn at most), and so are its sine and cosine.  One or two tensors (Q and K) with the same tokens, in any layout in which d
    has unit stride; y may be x where their strides are equal.  turns and axis are host arrays, read before the call returns.  One
    launch. */
 typedef struct nsa_rotary_tensor {

@@ -21,13 +21,15 @@
 // each term off below 2^-23 of the largest, twice that is allowed for), 20 2^-22 Q; the sums of groups and quarters in fp32
 // 8 2^-24 Q; that of up to 258 keys 258 2^-24 Q.  All but the first are less than 90 2^-22 Q, and taken as 2^-15 Q.
 //
-// What bounds it.  A key costs 9/16 d bytes.  256 sequences of up to 65536 tokens, 4 heads of 128: 151 MB, which DRAM would
-// deliver in 24 us, take 56.  46 of them are score_kernel's: the ALU pipe, which converts codes (128 of its 400 instructions for
-// 64 keys), is its busiest unit at 59 %, tensor cores 19 %.  The others are pick_kernel's, 1024 blocks that are chains of
-// steps (9000 cycles with 256 threads: reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks 900; 128
-// threads take longer, but 8 of their blocks fit an SM).  One sequence of 65536 tokens: 9.3 us; 64 of up to 32768: 17 us.  Tried:
-// exact scores of all blocks with dot products of four bytes (the 256 above 102 us); the bin from the threads' largest bounds
-// instead of counts (2000 cycles and half as many candidates again).
+// What bounds it.  A key costs 9/16 d bytes.  256 sequences of up to 65536 tokens, 4 heads of 128: 156 MB with queries and results,
+// which DRAM would deliver in 24 us, take 56.  46 of them are score_kernel's: the ALU pipe, which converts codes (128 of its 400
+// instructions for 64 keys), is its busiest unit at 59 %, tensor cores 19 %.  The others are pick_kernel's, 1024 blocks that are
+// chains of steps (9000 cycles with 256 threads: reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks
+// 900; 128 threads take longer, but 8 of their blocks fit an SM).  One sequence of 65536 tokens: 9.2 us; 64 of up to 32768: 17 us.
+// Where all rows are scored in fp64 these are 64, 12 and 23 us.  Where the bounds tell nothing apart (blocks that are all alike,
+// query heads that cancel) every block is summed exactly: 0.77, 0.28 and 0.17 ms.  Tried: exact scores of all blocks with dot
+// products of four bytes (the 256 above 102 us); the bin from the threads' largest bounds instead of counts (2000 cycles and half
+// as many candidates again).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

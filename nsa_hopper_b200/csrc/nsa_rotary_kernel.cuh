@@ -14,9 +14,13 @@
 // [B, H, T, d] that the attention reads on the way.  65536 tokens of 64 + 4 heads of 128 in bf16: 347 us, 6.6 TB/s, the measured
 // copy rate.  What brought it there was few registers: with four words a thread in flight and 127 registers it took 574 us,
 // with two and 64 430, with one and 32 (8 blocks an SM) 358, and with the outgoing address computed before the words are loaded
-// 347.  There tokens together in a block (2, 4, 8, 16) gave nothing, streaming loads took 398, streaming stores 379.  Rotary parts
-// that no words of 8 bytes fit are bound by instructions (36 of 128 values in bf16, 16384 tokens of 68 heads: 172 us for 88 us of
-// copying, issue slots 75 %; two or four words of an item at once took 163 and 153, and whole heads 2 % longer).
+// 347.  There tokens together in a block (2, 4, 8, 16) gave nothing, streaming loads took 398, streaming stores 379.
+//
+// Two forms are far from the copy rate.  Rotary parts that no words of 8 bytes fit are bound by instructions (36 of 128 values in
+// bf16, 16384 tokens of 68 heads: 171 us for 88 us of copying, issue slots 75 %; two or four words of an item at once took 163
+// and 153 in a kernel whose wide words they made 2 % slower, and have not been built for narrow words alone).  Few heads, several
+// tokens a block, are bound by latency (65536 tokens of 2 heads of 128: 28 us for 10): a thread loads a position, makes an
+// angle, meets the others, and only then loads the one item that it has.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

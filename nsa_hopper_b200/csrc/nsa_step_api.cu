@@ -160,7 +160,8 @@ int launch_select(select::Args a, int32_t n_rows, int64_t most, int sm, int dev,
     // the blocks are more than fit at once, 8 small ones an SM win (256 sequences of up to 65536 tokens, 4 heads: 56 us
     // against 64; 400 of up to 8192: 34 against 41), else 3 large ones (64 of up to 32768: 17 against 23).  They are even at
     // 4 to 6 an SM.  The small ones look at 1024 of a row's blocks at a time, and a second look costs more than they gain (200
-    // sequences of up to 131072: 84 against 75).
+    // sequences of up to 131072: 84 against 75).  The host sees the table's width, not the lengths: where short sequences
+    // have a table for more than 1024 blocks the large ones are taken.
     const int32_t covered = (a.most - a.cmp_block + 1) >> a.shift;  // (by whole pages of keys; a.blocks may be one or a few more)
     const bool many = (int64_t)a.rows * a.hkv > 5 * (int64_t)sm && covered <= select::checked(128);
     rc = many ? launch_pick<D, 128, 8>(a, dev, 4 * bit, st) : launch_pick<D, 256, 3>(a, dev, 2 * bit, st);

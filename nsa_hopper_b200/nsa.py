@@ -304,9 +304,10 @@ def nsa_decode(Q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lens: 
     """The three NSA branches and the gate of :func:`nsa_forward` for the newest token of every sequence of a
     4-bit cache (``ops.cache_write`` has put its K and V there): Q [S, Hq, d_qk] bf16 or fp16, sel int32
     [S, Hkv, KSEL] the token's selected blocks; returns O fp32 [S, Hq, d_v].  Without ``sel`` the ``n_sel`` best blocks are
-    taken (``ops.cache_select``; ``cmp_block`` and ``cmp_stride`` as :func:`cache_compress` was called with).  The compressed branch sees
-    every key of ``cmp_cache`` (:func:`cache_compress` keeps it, called after every write), as the newest token does in
-    the forward; without one it is left out.  Each branch adds its gated result into O.  ``err``: as in
+    taken (``ops.cache_select``; ``cmp_block`` and ``cmp_stride`` as :func:`cache_compress` was called with; none of a sequence
+    whose compressed keys ``cmp_pages`` cannot hold).  The compressed branch sees every key of ``cmp_cache``
+    (:func:`cache_compress` keeps it, called after every write), as the newest token does in the forward; without one it is
+    left out.  Each branch adds its gated result into O.  ``err``: as in
     ``ops.cache_attend``, for all three."""
     from . import ops
 

@@ -218,7 +218,8 @@ def cache_select(Q: torch.Tensor, cmp_cache: torch.Tensor, cmp_pages: torch.Tens
     Q [N, Hq, d_qk] (bf16 or fp16) has the rows of :func:`cache_attend`; ``lens`` int32 [S] are the tokens of the sequences (not
     their compressed keys).  The row at position t gets what the last row of ``select_blocks`` gets for t + 1 tokens: the
     blocks of ``l_prime`` tokens with the largest sums of (summed query heads) . (compressed key), the best first, -1 behind
-    the last.  Scores are compared as 64-bit sums, equal ones by the lower block; scores that are not finite come last.
+    the last.  Scores are compared as 64-bit sums, equal ones by the lower block; scores that are not finite come last (of a
+    query that is not finite all are, so that the lowest blocks are selected).
     ``n_sel`` at most 1024, Hq / Hkv at most 256, sequences of up to 2^24 tokens (longer ones, and those whose compressed keys
     ``cmp_pages`` cannot hold, select nothing).  No gradients."""
     return _C.cache_select(Q, cmp_cache, cmp_pages, lens, int(n_sel), int(l_prime), int(cmp_block), int(cmp_stride), cu_seqlens)
@@ -292,7 +293,8 @@ def rotary(Q: torch.Tensor, K: Optional[torch.Tensor], positions: torch.Tensor, 
     Rows Q [N, Hq, d] and K [N, Hkv, d] as the cache's calls take them, or heads [B, Hq, T, d] and [B, Hkv, T, d] as the forward
     does; bf16, fp16 or fp32, any strides (a projection's [B, T, H, d] is given as ``x.transpose(1, 2)``).  ``positions`` int32
     [N] or [B, T] (any strides, e.g. expanded over the batch), with the axes of the plan before that if there are several.
-    The results are contiguous and of the inputs' dtype; angles are exact for all int32 positions, products are fp32.
+    The results are contiguous and of the inputs' dtype.  Angles of all int32 positions are reduced to an eighth of a turn with an
+    error below 2^-32 of a turn, and then rounded to fp32; sines, cosines and products are fp32.
     Differentiable in Q and K, any number of times, in reverse and in forward mode (``torch.autograd.forward_ad``; the transforms
     of ``torch.func`` are refused); ``inverse`` turns back."""
     q, k = _C.rotary(Q, K, positions, plan.turns, plan.axis, plan.axes, plan.d, plan.offset, plan.interleaved, bool(inverse))
