@@ -26,7 +26,7 @@
 // instructions for 64 keys), is its busiest unit at 59 %, tensor cores 19 %.  The others are pick_kernel's, 1024 blocks that are
 // chains of steps (9000 cycles with 256 threads: reading the bounds 1100, the bin 1450, candidates 650, exact scores 3900, ranks
 // 900; 128 threads take longer, but 8 of their blocks fit an SM).  One sequence of 65536 tokens: 9.2 us; 64 of up to 32768: 17 us.
-// Where all rows are scored in fp64 these are 64, 12 and 23 us.  Where the bounds tell nothing apart (blocks that are all alike,
+// Where all rows are scored in fp64 these are 63, 12 and 23 us.  Where the bounds tell nothing apart (blocks that are all alike,
 // query heads that cancel) every block is summed exactly: 0.77, 0.28 and 0.17 ms.  Tried: exact scores of all blocks with dot
 // products of four bytes (the 256 above 102 us); the bin from the threads' largest bounds instead of counts (2000 cycles and half
 // as many candidates again).
@@ -401,6 +401,8 @@ __global__ void __launch_bounds__(warps_of(D) * 32) score_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------ exact scores
+// What a (row, head)'s exact scores are made from: nothing (a value of the query is no number), whole numbers, fp64.
+enum class Query { kNone, kWhole, kWide };
 struct alignas(16) Bytes {
   uint32_t x[4];
 };
@@ -414,9 +416,8 @@ struct Exact {
     double wide[D];               // the sum itself, where the bytes do not hold it
   };
   uint32_t top;
+  Query query;                    // (here and not in a register, of which the small blocks have none left)
 };
-// What a (row, head)'s exact scores are made from: nothing (a value of the query is no number), whole numbers, fp64.
-enum class Query { kNone, kWhole, kWide };
 
 // fp64 of an integer, without a conversion: its bits in the mantissa of 2^52 + 2^31 + x.
 __device__ __forceinline__ double whole(int32_t x) {
@@ -588,7 +589,7 @@ struct List {
   uint32_t* index;
 };
 template <int D, int THREADS>
-__device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, Query query, const Places& p, int seq, int head,
+__device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, const Places& p, int seq, int head,
                                              const int32_t* pages, const uint16_t* blocks, int base, uint32_t n, const List& list,
                                              uint32_t at, double* scores) {
   const int tid = threadIdx.x, quarter = tid % 4;
@@ -610,7 +611,7 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, Q
           load_quarter<D>(k[x], rec + quarter * (D / 8), rec + cache::k_scale_at(D) + quarter * (D / 64), i % kPage);
       }
       double score[2];  // (0 of a place without a key, and of a key of no page)
-      if (query == Query::kWide) dot_wide<D>(w, k, quarter, score);
+      if (w.query == Query::kWide) dot_wide<D>(w, k, quarter, score);
       else dot<D>(w, k, quarter, score);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -620,7 +621,7 @@ __device__ __forceinline__ void score_blocks(const Args& a, const Exact<D>& w, Q
     for (uint32_t e = tid; e < some; e += THREADS) {
       double score = 0.0;
       for (int j = 0; j < a.keys; ++j) score += scores[e * a.keys + j];
-      list.rank[at + e0 + e] = rank_of(query != Query::kNone ? score : __longlong_as_double(0x7FF8000000000000ll));
+      list.rank[at + e0 + e] = rank_of(w.query != Query::kNone ? score : __longlong_as_double(0x7FF8000000000000ll));
       list.index[at + e0 + e] = (uint32_t)(base + blocks[e0 + e]);
     }
     __syncthreads();
@@ -682,6 +683,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
   for (int i = tid; i < min(kHeldPages, (p.n + kPage - 1) / kPage); i += THREADS) pages[i] = cache::page_of(a.b, seq, i, LoadPastL1());
   if (tid == 0) s_found = 0;
   const Query query = prepare_exact<D, THREADS>(a, w, heads);
+  if (tid == 0) w.query = query;
   __syncthreads();
   wait_for_earlier();
   // (all of them: in a cu_seqlens out of order score_kernel may have taken the row for another sequence's)
@@ -753,7 +755,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) pick_kernel(const Args a) {
     const uint32_t n_found = s_found;
     for (uint32_t f0 = 0;;) {
       const uint32_t some = min(n_found - f0, (uint32_t)kAdded), in = kept + some;
-      score_blocks<D, THREADS>(a, w, query, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
+      score_blocks<D, THREADS>(a, w, p, seq, head, pages, found + f0, i0, some, list, kept, scores);
       f0 += some;
       const bool whole = f0 == n_found, last = whole && i0 + kChecked >= n;
       for (uint32_t e0 = tid / 8; e0 - tid / 8 < in; e0 += THREADS / 8) {  // 8 threads for an entry
